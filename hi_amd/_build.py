@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhi_rocm.so")
 SOURCES = ["sampler_rows.hip", "sampler_select.hip", "sampler_fused.hip", "sampler_chunked.hip", "lm_head.hip", "sampler_debug.hip",
            "index_select.hip", "sampler_api.hip", "sampler_host.hip", "decode_step.hip",
-           "moe_router.hip", "spec_verify.hip"]
+           "moe_router.hip", "spec_verify.hip", "beam.hip", "w4.hip", "moe_experts.hip"]
 
 # -ffp-contract=off: every f32/f64 operation that decides a token is a
 # separate IEEE rounding (fused operations are written out explicitly).

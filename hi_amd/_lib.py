@@ -33,6 +33,7 @@ OK, ERR_ARGS, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 DTYPE_F32, DTYPE_BF16 = 0, 1
 FLAG_REP_ONCE = 1
 MAX_LOGPROBS = 1024
+BEAM_MAX, BEAM_MAX_OUT, BEAM_NO_EOS = 32, 64, 0xFFFFFFFF
 
 # Every function include/*.h declares, with its ctypes signature.
 _vp, _i, _f, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64, ctypes.c_size_t
@@ -75,6 +76,16 @@ SIGNATURES = {
     "hi_rocm_debug_fold": (_i, [_vp, _vp, _i, ctypes.c_float, _vp, _vp, _vp]),
     "hi_rocm_debug_wide_paths": (_i, [_vp, _sz, _i, _i, _vp, _vp]),
     "hi_rocm_debug_wide_totals": (_i, [_vp, _sz, _i, _i, _vp, _vp]),
+    "hi_rocm_beam_workspace_bytes": (_i, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
+    "hi_rocm_beam_select": (_i, [_vp, _i, _i, _i, _i, _i64, _vp, _vp, ctypes.c_uint32, _vp, _i, _vp, _vp, _vp, _vp, _vp,
+                                 _sz, _vp]),
+    "hi_rocm_beam_reorder": (_i, [_vp, _vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "hi_rocm_w4_packed_bytes": (_i, [_i, _i, _i, _i, _i, ctypes.POINTER(_sz)]),
+    "hi_rocm_w4_pack": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "hi_rocm_w4_linear": (_i, [_vp, _i, _i64, _vp, _sz, _i, _i, _i, _i, _i, _vp, _vp, _i, _i64, _vp]),
+    "hi_rocm_moe_group": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "hi_rocm_moe_grouped_product": (_i, [_vp, _i, _i64, _vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _vp, _i, _i64, _vp]),
+    "hi_rocm_moe_combine": (_i, [_vp, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _i, _i64, _vp]),
     "hi_rocm_last_error": (ctypes.c_char_p, []),
     "hi_rocm_version": (ctypes.c_char_p, []),
     # include/hi_rocm_host.h

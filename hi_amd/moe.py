@@ -1,0 +1,144 @@
+"""The expert layer behind the MoE router: the router's pairs grouped by
+expert, products over the groups, and the weighted sum of a token's experts
+(``hi_rocm_moe_group``, ``hi_rocm_moe_grouped_product``,
+``hi_rocm_moe_combine``)."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import check, load
+from .beam import _empty, _same_device
+from .sampler import _stream_ptr
+
+_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+class RowGroups:
+    """The (token, slot) pairs p = token * top_k + slot sorted by expert:
+    ``order`` (the pair in each place), ``slots`` (each pair's place) and
+    ``offsets`` (expert e's places are offsets[e] .. offsets[e + 1])."""
+
+    def __init__(self, tokens: int, top_k: int, experts: int, device="cuda"):
+        self.tokens, self.top_k, self.experts = tokens, top_k, experts
+        self.order = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
+        self.slots = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
+        self.offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
+
+    @property
+    def places(self) -> int:
+        return self.tokens * self.top_k
+
+
+def group_rows(ids: torch.Tensor, experts: int, out: Optional[RowGroups] = None,
+               stream: Optional[torch.cuda.Stream] = None) -> RowGroups:
+    """Groups the router's ``ids`` (int32 [tokens][top_k]) by expert, stably.
+    Pairs whose id names no expert come behind the groups."""
+    what = "group rows"
+    if ids.dim() != 2 or ids.dtype != torch.int32 or not ids.is_contiguous() or ids.numel() == 0:
+        raise ValueError(f"{what}: ids must be a contiguous int32 [tokens][top_k] tensor")
+    if out is None:
+        out = RowGroups(ids.shape[0], ids.shape[1], experts, device=ids.device)
+    if (out.tokens, out.top_k, out.experts) != (ids.shape[0], ids.shape[1], experts):
+        raise ValueError(f"{what}: out is for {out.tokens} tokens, top {out.top_k} of {out.experts} experts")
+    _same_device(what, ids.device, out=out.order)
+    check(load().hi_rocm_moe_group(ids.data_ptr(), out.tokens, out.top_k, experts, out.order.data_ptr(),
+                                   out.slots.data_ptr(), out.offsets.data_ptr(), _stream_ptr(stream)))
+    return out
+
+
+def grouped_product(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, gather: bool = True,
+                    swiglu: bool = False, out: Optional[torch.Tensor] = None, dtype=torch.bfloat16,
+                    stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """out[i] = x[row(i)] weight[e]^T for place i of expert e; row(i) is the
+    pair's token (``gather``) or i.  ``x`` bfloat16 [.][k], ``weight`` bfloat16
+    [experts][cols][k]; with ``swiglu`` the columns are gate and up halves and
+    out is silu(gate) * up, cols / 2 wide."""
+    what = "grouped product"
+    if weight.dim() != 3 or weight.dtype != torch.bfloat16 or not weight.is_contiguous():
+        raise ValueError(f"{what}: weight must be a contiguous bfloat16 [experts][cols][k] tensor")
+    experts, cols, k = weight.shape
+    if experts != groups.experts:
+        raise ValueError(f"{what}: weight has {experts} experts, the groups {groups.experts}")
+    rows = groups.tokens if gather else groups.places
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape != (rows, k) or x.stride(1) != 1:
+        raise ValueError(f"{what}: x must be a bfloat16 [{rows}][{k}] tensor, inputs contiguous")
+    if swiglu and cols % 2:
+        raise ValueError(f"{what}: gate and up columns: an even number")
+    wide = cols // 2 if swiglu else cols
+    if out is None:
+        out = _empty((groups.places, wide), dtype, x.device, stream)
+    if out.shape != (groups.places, wide) or out.dtype not in _CODES or out.stride(1) != 1:
+        raise ValueError(f"{what}: out must be a float32 or bfloat16 [{groups.places}][{wide}] tensor")
+    _same_device(what, x.device, weight=weight, groups=groups.order, out=out)
+    check(load().hi_rocm_moe_grouped_product(
+        x.data_ptr(), rows, x.stride(0) if rows > 1 else k, groups.order.data_ptr() if gather else 0, groups.top_k,
+        groups.offsets.data_ptr(), groups.places, experts, weight.data_ptr(), cols, k, int(swiglu), out.data_ptr(),
+        _CODES[out.dtype], out.stride(0) if groups.places > 1 else wide, _stream_ptr(stream)))
+    return out
+
+
+def combine(y: torch.Tensor, groups: RowGroups, weights: torch.Tensor, out: Optional[torch.Tensor] = None,
+            dtype=torch.bfloat16, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """out[t] = sum_s weights[t][s] y[place of (t, s)], in slot order."""
+    what = "combine"
+    if y.dim() != 2 or y.shape[0] != groups.places or y.dtype not in _CODES or y.stride(1) != 1:
+        raise ValueError(f"{what}: y must be a float32 or bfloat16 [{groups.places}][cols] tensor")
+    if weights.shape != (groups.tokens, groups.top_k) or weights.dtype != torch.float32 or not weights.is_contiguous():
+        raise ValueError(f"{what}: weights must be a contiguous float32 [tokens][top_k] tensor")
+    if out is None:
+        out = _empty((groups.tokens, y.shape[1]), dtype, y.device, stream)
+    if out.shape != (groups.tokens, y.shape[1]) or out.dtype not in _CODES or out.stride(1) != 1:
+        raise ValueError(f"{what}: out must be a float32 or bfloat16 [{groups.tokens}][{y.shape[1]}] tensor")
+    _same_device(what, y.device, groups=groups.order, weights=weights, out=out)
+    check(load().hi_rocm_moe_combine(
+        y.data_ptr(), _CODES[y.dtype], y.stride(0) if groups.places > 1 else y.shape[1], groups.slots.data_ptr(),
+        groups.offsets.data_ptr(), groups.experts, weights.data_ptr(), groups.tokens, groups.top_k, y.shape[1],
+        out.data_ptr(), _CODES[out.dtype], out.stride(0) if groups.tokens > 1 else y.shape[1], _stream_ptr(stream)))
+    return out
+
+
+class MoeExperts:
+    """The expert layer: y[t] = sum_s w[t][s] down_e (silu(gate_e x[t]) * (up_e
+    x[t])), e = ids[t][s].  ``w_up`` bfloat16 [experts][2 * inter][hidden]
+    (gate rows, then up rows), ``w_down`` bfloat16 [experts][hidden][inter].
+    Buffers for up to ``max_tokens`` tokens are allocated once; calls allocate
+    nothing when ``out`` is given."""
+
+    def __init__(self, w_up: torch.Tensor, w_down: torch.Tensor, max_tokens: int, top_k: int):
+        if (w_up.dim() != 3 or w_down.dim() != 3 or w_up.shape[1] % 2 or
+                w_down.shape != (w_up.shape[0], w_up.shape[2], w_up.shape[1] // 2)):
+            raise ValueError("moe experts: w_up [experts][2 * inter][hidden], w_down [experts][hidden][inter]")
+        self.w_up, self.w_down, self.max_tokens, self.top_k = w_up, w_down, max_tokens, top_k
+        self.experts, self.hidden, self.inter = w_up.shape[0], w_up.shape[2], w_down.shape[2]
+        dev = w_up.device
+        # The activations between the products are what the second product
+        # reads, bf16; its results stay f32 until they are summed.
+        self._h = torch.empty(max_tokens * top_k, self.inter, dtype=torch.bfloat16, device=dev)
+        self._y = torch.empty(max_tokens * top_k, self.hidden, dtype=torch.float32, device=dev)
+        self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev)
+
+    def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, out: Optional[torch.Tensor] = None,
+                 stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """x bfloat16 [tokens][hidden], ids int32 and weights float32
+        [tokens][top_k] from the router; returns [tokens][hidden] (bfloat16,
+        or out's type)."""
+        tokens = x.shape[0]
+        if ids.dim() != 2 or ids.shape != (tokens, self.top_k) or not 0 < tokens <= self.max_tokens:
+            raise ValueError(f"moe experts: ids must be [tokens][{self.top_k}], at most {self.max_tokens} tokens")
+        g = self._groups
+        if tokens != self.max_tokens:
+            g = RowGroups.__new__(RowGroups)
+            g.tokens, g.top_k, g.experts = tokens, self.top_k, self.experts
+            n = tokens * self.top_k
+            g.order, g.slots, g.offsets = self._groups.order[:n], self._groups.slots[:n], self._groups.offsets
+        h, y = self._h[:g.places], self._y[:g.places]
+        group_rows(ids, self.experts, out=g, stream=stream)
+        grouped_product(x, self.w_up, g, gather=True, swiglu=True, out=h, stream=stream)
+        grouped_product(h, self.w_down, g, gather=False, out=y, stream=stream)
+        return combine(y, g, weights, out=out, stream=stream)
+
+
+__all__ = ["RowGroups", "group_rows", "grouped_product", "combine", "MoeExperts"]

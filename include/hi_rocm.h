@@ -374,6 +374,114 @@ int hi_rocm_debug_expf(const float* x, float* y, int64_t n, void* stream);
 int hi_rocm_profile_begin(int max_calls);
 int hi_rocm_profile_end(double* pass_ms, double* finish_ms, int* calls);
 
+/* ---- beam search (no reference counterpart: the reference decodes without
+ *      beams) ---- */
+
+/* Most beams of a request, and most candidates kept of one. */
+#define HI_ROCM_BEAM_MAX 32
+#define HI_ROCM_BEAM_MAX_OUT 64
+/* No token ends a beam. */
+#define HI_ROCM_BEAM_NO_EOS 0xffffffffu
+
+/* Workspace bytes hi_rocm_beam_select needs for up to max_batch requests of
+ * `beams` beams (at most 65536 rows in all). */
+int hi_rocm_beam_workspace_bytes(int max_batch, int beams, int vocab, int n_out, size_t* out_bytes);
+
+/* One step of beam search: the first n_out candidates of each request over
+ * its beams and the vocabulary.
+ *   logits     [batch * beams][row_stride] of `dtype` (f32 or bf16), rows at
+ *              any alignment of their type
+ *   scores     f32[batch * beams] cumulative log-probabilities; a beam whose
+ *              score is not finite has no candidates (-inf: unused, as all
+ *              beams but one of a request's first step)
+ *   finished   u8[batch * beams] or NULL: a finished beam's only candidate is
+ *              eos_id at its own score (its logits are not read)
+ *   eos_id     the token that ends a beam, or HI_ROCM_BEAM_NO_EOS
+ *   mask_words as hi_rocm_sample's, one row a beam, or NULL
+ * A candidate's score is c + (l - lse), lse = m + log sum exp(l - m) over the
+ * beam's allowed tokens, each step in f32.  NaN logits count as masked, -inf
+ * logits and scores are no candidates, and a beam with a +inf logit or no
+ * allowed token has none.  Order: score descending, then the lower beam, the
+ * larger logit, the lower token.
+ *   out_scores f32[batch][n_out], out_tokens u32, out_parents i32 (the beam
+ *   within its request), out_finished u8 (the parent was finished, or the
+ *   token is eos_id).  Places without a candidate: score -inf, token eos_id
+ *   (0 without one), parent j % beams, finished.
+ * The workspace needs no initial value; one stream at a time.  No allocation
+ * and no host synchronisation: graph-capturable. */
+int hi_rocm_beam_select(const void* logits, int dtype, int batch, int beams, int vocab, int64_t row_stride,
+                        const float* scores, const uint8_t* finished, uint32_t eos_id, const uint32_t* mask_words,
+                        int n_out, float* out_scores, uint32_t* out_tokens, int32_t* out_parents,
+                        uint8_t* out_finished, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Moves the beams' states (caches, histories, page tables) to where
+ * hi_rocm_beam_select's parents put them: row b * beams + j of dst becomes row
+ * b * beams + parents[b * beams + j] of src (i32; a parent outside [0, beams)
+ * leaves the row its own).  A state is [outer][batch * beams][mid][positions]
+ * [pos_bytes], with strides in bytes for the first three and contiguous
+ * positions; of request b only positions [0, lengths[b]) move (i32[batch], or
+ * NULL: all), the rest of dst stays.  dst may be src (in place, rows that keep
+ * their own state untouched) or must not overlap it; both have the same
+ * strides, which must keep rows apart.  No allocation: graph-capturable. */
+int hi_rocm_beam_reorder(const void* src, void* dst, const int32_t* parents, int batch, int beams, int64_t outer,
+                         int64_t outer_stride, int64_t row_stride, int64_t mid, int64_t mid_stride, int64_t positions,
+                         int64_t pos_bytes, const int32_t* lengths, void* stream);
+
+/* ---- products with 4-bit weights and group scales ---- */
+
+/* Bytes of a weight [n][k] laid out by hi_rocm_w4_pack.  group: 32, 64 or 128
+ * inputs share a scale (k a multiple of it); scale_dtype: f32 or bf16. */
+int hi_rocm_w4_packed_bytes(int n, int k, int group, int scale_dtype, int has_zeros, size_t* out_bytes);
+
+/* Lays a quantised weight out for hi_rocm_w4_linear, once: q u8[n][k / 2]
+ * (input 2 j in the low, 2 j + 1 in the high nibble of byte j), scales
+ * [n][k / group] and zeros (the same, or NULL: 8) of scale_dtype, into packed
+ * (16-byte aligned).  The weight is (q - zero) * scale. */
+int hi_rocm_w4_pack(const void* q, const void* scales, const void* zeros, int scale_dtype, int n, int k, int group,
+                    void* packed, size_t packed_bytes, void* stream);
+
+/* out[m][c] = sum_k x[m][k] * w[c][k] + bias[c] for the packed weight w: x
+ * bf16[rows][x_stride] (rows start on 16 bytes), bias f32[n] or NULL, out f32
+ * or bf16 [rows][out_stride].  scale_dtype, has_zeros, n, k and group as
+ * packed.  Made for the rows of a decode step (1 to 64; more take the weights
+ * again for every 64).  A row's result does not depend on the other rows'
+ * values; a row of x that holds inf or NaN gives NaN.  With f32 out it writes
+ * the logits that hi_rocm_sample and hi_rocm_beam_select read.  No
+ * allocation: graph-capturable. */
+int hi_rocm_w4_linear(const void* x, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
+                      int scale_dtype, int has_zeros, int n, int k, int group, const float* bias, void* out,
+                      int out_dtype, int64_t out_stride, void* stream);
+
+/* ---- the experts behind hi_rocm_launch_moe_topk_router ---- */
+
+/* Sorts the router's pairs p = token * top_k + slot by expert, stably: ids
+ * u32[tokens][top_k] (the router's output_ids) -> order i32[tokens * top_k]
+ * (the pair in each place), slots i32[tokens * top_k] (each pair's place) and
+ * offsets i32[experts + 1] (expert e has places offsets[e] .. offsets[e + 1]).
+ * Pairs with an id outside [0, experts) come last, behind offsets[experts].
+ * experts <= 2048, at most 2^22 pairs.  No allocation: graph-capturable. */
+int hi_rocm_moe_group(const uint32_t* ids, int tokens, int top_k, int experts, int32_t* order, int32_t* slots,
+                      int32_t* offsets, void* stream);
+
+/* out[i][c] = sum_k x[row(i)][k] * weight[e][c][k] for every place i of every
+ * expert e: x bf16[x_rows][x_stride], weight bf16[experts][cols][k]
+ * contiguous, row(i) = order[i] / top_k, or i with order NULL (x in the
+ * groups' order); out f32 or bf16 [places][out_stride].  With swiglu the
+ * columns are gate and up halves and out[i][c] = silu(gate c) * (up c), cols /
+ * 2 wide.  k a multiple of 8, rows on 16 bytes.  Places behind
+ * offsets[experts] are not written.  Sums in f32, one rounding to out's type.
+ * No allocation: graph-capturable. */
+int hi_rocm_moe_grouped_product(const void* x, int x_rows, int64_t x_stride, const int32_t* order, int top_k,
+                                const int32_t* offsets, int places, int experts, const void* weight, int cols, int k,
+                                int swiglu, void* out, int out_dtype, int64_t out_stride, void* stream);
+
+/* out[t][c] = sum_s weights[t][s] * y[slots[t * top_k + s]][c] in slot order
+ * (f32 sums), for y [tokens * top_k][y_stride] in the groups' order.  Pairs
+ * behind offsets[experts] (an id that names no expert) add nothing. */
+int hi_rocm_moe_combine(const void* y, int y_dtype, int64_t y_stride, const int32_t* slots, const int32_t* offsets,
+                        int experts, const float* weights, int tokens, int top_k, int cols, void* out, int out_dtype,
+                        int64_t out_stride, void* stream);
+
 /* Thread-local message for the last non-zero status. */
 const char* hi_rocm_last_error(void);
 

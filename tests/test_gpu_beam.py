@@ -1,0 +1,342 @@
+"""Beam selection and state reordering against the definitions in 64 bits.
+
+A score is three f32 roundings (lse, l - lse, + c) beside lse's own error:
+the sum of up to 64 terms a thread, a tree over the workgroup and the row's
+parts, each term's exponential within a few units of its last place, and a
+logarithm.  SUM_EPS bounds that sum's relative error, which is lse's absolute
+one."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from hi_amd import _lib
+from hi_amd.beam import BeamSearch, reorder_states
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+SUM_EPS = (64 + 6 + 4 + 16 + 6 + 8) * EPS
+
+
+def definition(x, c, finished, eos, mask, K, n):
+    """All candidates of each request: (score64, beam, logit, token), in the
+    order (score, beam, logit, token) of the exact scores, and the tolerance."""
+    x = x.astype(np.float64)
+    out, tol = [], 0.0
+    for b in range(x.shape[0] // K):
+        cand = []
+        for k in range(K):
+            r = b * K + k
+            if not np.isfinite(c[r]):
+                continue
+            if finished is not None and finished[r]:
+                cand.append((float(c[r]), k, 0.0, eos))
+                continue
+            l = x[r].copy()
+            l[np.isnan(l)] = -np.inf
+            if mask is not None:
+                l[~mask[r]] = -np.inf
+            m = l.max()
+            if not np.isfinite(m):
+                continue
+            lse = m + math.log(np.exp(l - m).sum())
+            ids = np.nonzero(l > -np.inf)[0]
+            ids = ids[np.lexsort((ids, -l[ids]))][:n]
+            s = float(c[r]) + (l[ids] - lse)
+            tol = max(tol, EPS * (4 * abs(lse) + 2 * np.abs(l[ids] - lse).max() + 2 * np.abs(s).max()) + SUM_EPS)
+            cand += [(float(v), k, float(l[i]), int(i)) for v, i in zip(s, ids)]
+        out.append(sorted(cand, key=lambda t: (-t[0], t[1], -t[2], t[3])))
+    return out, tol
+
+
+def check(res, want, tol, K, n, eos, finished):
+    s, t, p, f = (res[k].cpu().numpy() for k in ("scores", "tokens", "parents", "finished"))
+    for b, cand in enumerate(want):
+        have = min(n, len(cand))
+        exact = {(k, i): (v, l, rank) for rank, (v, k, l, i) in enumerate(cand)}
+        seen = {}
+        for j in range(have):
+            key = (int(p[b, j]), int(t[b, j]))
+            assert key in exact, (b, j, key)  # a candidate of its beam's first n
+            v, l, _ = exact[key]
+            assert abs(s[b, j] - v) <= tol, (b, j, s[b, j], v, tol)
+            assert abs(s[b, j] - cand[j][0]) <= tol, (b, j)  # the j-th best score
+            if j:  # scores descend, the lower beam first on equal ones
+                assert s[b, j] < s[b, j - 1] or (s[b, j] == s[b, j - 1] and p[b, j] >= p[b, j - 1]), (b, j)
+            seen.setdefault(key[0], []).append(key)
+            done = finished is not None and bool(finished[b * K + key[0]])
+            assert f[b, j] == (done or key[1] == eos)
+        for k, keys in seen.items():  # within a beam: the first ones, in the logits' order
+            order = [(kk, i) for _, kk, _, i in sorted((c for c in cand if c[1] == k), key=lambda c: (-c[2], c[3]))]
+            assert keys == order[:len(keys)], (b, k)
+        for j in range(have, n):
+            assert s[b, j] == -np.inf and t[b, j] == (0 if eos is None else eos) and p[b, j] == j % K and f[b, j] == 1
+
+
+def run(x, c, K, n, finished=None, eos=None, mask=None, bs=None, stream=None):
+    dev = "cuda"
+    B, V = x.shape[0] // K, x.shape[1]
+    words = None
+    if mask is not None:
+        pad = np.zeros((x.shape[0], (V + 31) // 32 * 32), bool)
+        pad[:, :V] = mask.cpu().numpy() if torch.is_tensor(mask) else mask
+        words = torch.from_numpy(np.packbits(pad, axis=1, bitorder="little").view(np.int32).copy()).to(dev)
+    bs = bs or BeamSearch(B, K, V, n)
+    fin = None if finished is None else torch.from_numpy(np.asarray(finished, np.uint8)).to(dev)
+    res = bs.select(x, torch.from_numpy(np.asarray(c, np.float32)).to(dev), finished=fin, eos_id=eos, mask_words=words,
+                    stream=stream)
+    torch.cuda.synchronize()
+    return res
+
+
+def agree(x, c, K, n, finished=None, eos=None, mask=None, **kw):
+    res = run(x, c, K, n, finished, eos, mask, **kw)
+    want, tol = definition(x.float().cpu().numpy(), np.asarray(c, np.float32), finished, eos, mask, K, n)
+    check(res, want, tol, K, n, eos, finished)
+    return res
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,K,V,n", [(1, 1, 1, 1), (1, 1, 2, 4), (2, 3, 17, 6), (1, 4, 5003, 8), (3, 2, 4096, 64),
+                                     (1, 32, 777, 64), (2, 5, 50257, 5), (7, 4, 16381, 8), (40, 8, 33000, 16)])
+def test_selection(hip, dtype, B, K, V, n):
+    g = torch.Generator(device="cuda").manual_seed(B * 1000 + V)
+    x = (torch.randn(B * K, V, generator=g, device="cuda") * 2.5).to(dtype)
+    c = -30.0 * np.random.default_rng(V).random(B * K)
+    fin = np.random.default_rng(K).random(B * K) < 0.25
+    agree(x, c, K, n)
+    agree(x, c, K, n, finished=fin, eos=V // 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", range(8))
+def test_rows_at_any_alignment(hip, dtype, offset):
+    g = torch.Generator(device="cuda").manual_seed(offset)
+    K, V, n = 3, 4099, 6
+    big = (torch.randn(K * 4, V + 13, generator=g, device="cuda") * 3).to(dtype)
+    x = big[:, offset:offset + V]
+    agree(x, [-1.0 * i for i in range(K * 4)], K, n)
+
+
+def test_masks(hip):
+    """A fifth of the tokens, a single one, none, and all but one part."""
+    rng = np.random.default_rng(3)
+    K, V, n = 4, 20011, 8
+    x = torch.from_numpy(rng.standard_normal((8, V)).astype(np.float32) * 3).cuda()
+    mask = rng.random((8, V)) < 0.2
+    mask[1] = False
+    mask[2] = False
+    mask[2, V - 1] = True
+    mask[3] = False
+    mask[3, :5] = True
+    mask[5] = False
+    mask[6] = False
+    mask[7] = False
+    mask[4] = False
+    agree(x, -rng.random(8) * 5, K, n, mask=mask, eos=7)  # the second request has no candidate at all
+
+
+def test_special_logits(hip):
+    rng = np.random.default_rng(4)
+    K, V, n = 6, 9001, 12
+    x = rng.standard_normal((2 * K, V)).astype(np.float32)
+    x[0, 10:20] = np.nan
+    x[0, 0] = np.nan
+    x[1] = np.nan                       # no candidate
+    x[2, 5] = np.inf                    # none either: every other probability is 0
+    x[3] = -np.inf
+    x[3, 77] = 1.0                      # one candidate of probability 1
+    x[4] = np.finfo(np.float32).min     # lowest value everywhere: V equal candidates
+    x[5, ::2] = -np.inf
+    x[6, :] = 0.0
+    x[6, 1::2] = -0.0                   # equal to 0: the lower token first
+    x[7, 100] = np.finfo(np.float32).max
+    c = np.array([-1, -2, -3, -4, -5, -6, -1, -2, -np.inf, np.nan, np.inf, -3], np.float32)
+    agree(torch.from_numpy(x).cuda(), c, K, n)
+
+
+@pytest.mark.parametrize("levels", [1, 2, 40])
+@pytest.mark.parametrize("V", [300, 20000, 70000])
+def test_many_equal_logits(hip, levels, V):
+    rng = np.random.default_rng(levels)
+    x = rng.integers(0, levels, (6, V)).astype(np.float32)
+    agree(torch.from_numpy(x).cuda(), [0.0] * 6, 3, 33)
+    agree(torch.from_numpy(x).cuda().bfloat16(), [0.0, -1e6, 0.0, 0.0, 0.0, 0.0], 3, 64)
+
+
+def test_equal_scores_of_beams(hip):
+    """Beams that agree in everything: the lower beam first, at every rank."""
+    rng = np.random.default_rng(6)
+    row = rng.standard_normal(3000).astype(np.float32)
+    res = agree(torch.from_numpy(np.stack([row] * 8)).cuda(), [-2.0] * 8, 8, 24)
+    assert res["parents"].cpu().tolist()[0] == list(range(8)) * 3
+    fin = [1] * 8
+    res = agree(torch.from_numpy(np.stack([row] * 8)).cuda(), [-2.0] * 8, 8, 8, finished=fin, eos=5)
+    assert res["parents"].cpu().tolist()[0] == list(range(8)) and res["tokens"].unique().tolist() == [5]
+
+
+def test_long_rows_and_workspace_reuse(hip):
+    """A vocabulary of many parts; one workspace for batches of other sizes."""
+    rng = np.random.default_rng(8)
+    V, K = 600001, 2
+    bs = BeamSearch(9, K, V, 8)
+    for B in (1, 9, 2):
+        x = torch.from_numpy(rng.standard_normal((B * K, V)).astype(np.float32)).cuda()
+        agree(x, -rng.random(B * K), K, 8, bs=bs)
+
+
+def test_same_bits_every_time_and_on_streams(hip):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(64, 30000, generator=g, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    first = run(x, np.linspace(-9, 0, 64), 8, 16)
+    for _ in range(3):
+        again = run(x, np.linspace(-9, 0, 64), 8, 16, stream=torch.cuda.Stream())
+        for k in first:
+            assert torch.equal(first[k], again[k]), k
+
+
+def test_selection_in_a_graph(hip):
+    g = torch.Generator(device="cuda").manual_seed(10)
+    K, V, n = 4, 12345, 8
+    bs = BeamSearch(2, K, V, n)
+    x = torch.randn(2 * K, V, generator=g, device="cuda")
+    c = torch.zeros(2 * K, device="cuda")
+    out = bs.outputs(2)
+    bs.select(x, c, out=out)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        bs.select(x, c, out=out)
+    for i in range(4):
+        x.copy_(torch.randn(2 * K, V, generator=g, device="cuda") * (i + 1))
+        c.copy_(-torch.rand(2 * K, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = {k: v.clone() for k, v in out.items()}
+        want = run(x, c.cpu().numpy(), K, n)
+        for k in got:
+            assert torch.equal(got[k], want[k]), (i, k)
+
+
+# ---- states ---------------------------------------------------------------
+
+def moved(src, dst, parents, row_dim, length_dim=None, lengths=None):
+    """The definition, a row at a time."""
+    B, K = parents.shape
+    s, d = src.movedim(row_dim, 0), dst.movedim(row_dim, 0).clone()
+    for b in range(B):
+        for j in range(K):
+            p = int(parents[b, j])
+            p = p if 0 <= p < K else j
+            a, t = s[b * K + p], d[b * K + j]
+            if lengths is None:
+                t.copy_(a)
+            else:
+                at = length_dim - 1
+                n = max(0, min(int(lengths[b]), a.shape[at]))
+                t.narrow(at, 0, n).copy_(a.narrow(at, 0, n))
+    return d.movedim(0, row_dim)
+
+
+LAYOUTS = [((6, 5), 0, None), ((2, 6, 3, 7, 16), 1, 3), ((6, 9, 8), 0, 1), ((3, 2, 6, 5, 2, 24), 2, 4), ((6,), 0, None),
+           ((4, 6, 3), 1, None), ((6, 2, 11, 3), 0, 2), ((2, 6, 1, 40, 1, 128), 1, 3)]
+
+
+@pytest.mark.parametrize("shape,row_dim,length_dim", LAYOUTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.uint8, torch.int32])
+@pytest.mark.parametrize("place", ["other", "in place"])
+def test_reorder(hip, shape, row_dim, length_dim, dtype, place):
+    rng = np.random.default_rng(len(shape))
+    src = torch.from_numpy(rng.integers(0, 250, shape)).to(dtype).cuda()
+    for parents in ([[0, 1, 2], [2, 0, 0]], [[2, 2, 2], [1, 2, 0]], [[0, 1, 2], [0, 1, 2]], [[-1, 3, 1], [2, 1, 99]]):
+        par = torch.tensor(parents, dtype=torch.int32, device="cuda")
+        lens = None
+        if length_dim is not None:
+            lens = torch.tensor([rng.integers(0, shape[length_dim] + 1), shape[length_dim] + 5], dtype=torch.int32,
+                                device="cuda")
+        dst = src.clone() if place == "in place" else torch.full_like(src, 7)
+        want = moved(src, dst, par.cpu(), row_dim, length_dim, None if lens is None else lens.cpu())
+        if place == "in place":
+            got = reorder_states(dst, par, row_dim=row_dim, length_dim=length_dim, lengths=lens)
+            assert got is dst
+        else:
+            got = reorder_states(src, par, dst=dst, row_dim=row_dim, length_dim=length_dim, lengths=lens)
+        torch.cuda.synchronize()
+        assert torch.equal(got.cpu(), want.cpu())
+
+
+@pytest.mark.parametrize("beams", [1, 2, 4, 5, 8, 9, 16, 17, 32])
+def test_reorder_beams(hip, beams):
+    g = torch.Generator(device="cuda").manual_seed(beams)
+    src = torch.randn(3, 4 * beams, 2, 33, 8, generator=g, device="cuda").bfloat16()
+    par = torch.randint(0, beams, (4, beams), generator=g, device="cuda").int()
+    lens = torch.tensor([33, 0, 1, 20], dtype=torch.int32, device="cuda")
+    want = moved(src, src, par.cpu(), 1, 3, lens.cpu())
+    torch.cuda.synchronize()
+    got = reorder_states(src, par, row_dim=1, length_dim=3, lengths=lens, stream=torch.cuda.Stream())
+    torch.cuda.synchronize()
+    assert torch.equal(got.cpu(), want.cpu())
+
+
+def test_reorder_strided_views(hip):
+    """A slice of a larger cache, rows not next to each other."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache = torch.randn(2, 8, 3, 50, 16, generator=g, device="cuda")
+    view = cache[:, :6, 1:, :, :]
+    par = torch.tensor([[1, 0, 2], [2, 2, 0]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([50, 13], dtype=torch.int32, device="cuda")
+    want = cache.clone()
+    want[:, :6, 1:] = moved(view, view, par.cpu(), 1, 3, lens.cpu())
+    reorder_states(view, par, row_dim=1, length_dim=3, lengths=lens)
+    torch.cuda.synchronize()
+    assert torch.equal(cache, want)
+
+
+def test_reorder_past_32_bits(hip):
+    """Rows whose offsets pass 4 GiB."""
+    rows, per = 6, 1 << 30
+    state = torch.zeros(rows, per, dtype=torch.uint8, device="cuda")
+    for r in range(rows):
+        state[r, -1000:] = r + 1
+        state[r, :1000] = 100 + r
+    par = torch.tensor([[5, 5, 1, 0, 4, 2]], dtype=torch.int32, device="cuda")
+    reorder_states(state, par)
+    torch.cuda.synchronize()
+    assert state[:, -1].tolist() == [6, 6, 2, 1, 5, 3] and state[:, 999].tolist() == [105, 105, 101, 100, 104, 102]
+    assert state[:, 5000].tolist() == [0] * 6
+
+
+def test_refusals(hip):
+    bs = BeamSearch(2, 3, 100, 6)
+    x, c = torch.zeros(6, 100, device="cuda"), torch.zeros(6, device="cuda")
+    for bad in (lambda: bs.select(x[:5], c), lambda: bs.select(x[:, :99], c), lambda: bs.select(x.double(), c),
+                lambda: bs.select(x, c[:5]), lambda: bs.select(x, c.double()), lambda: bs.select(x, c.cpu()),
+                lambda: bs.select(x, c, finished=torch.zeros(6, dtype=torch.uint8, device="cuda")),
+                lambda: bs.select(x, c, eos_id=100), lambda: bs.select(torch.zeros(9, 100, device="cuda"), c),
+                lambda: bs.select(x, c, mask_words=torch.zeros(6, 3, dtype=torch.int32, device="cuda")),
+                lambda: bs.select(torch.zeros(6, 200, device="cuda")[:, ::2], c)):
+        with pytest.raises(ValueError):
+            bad()
+    for args in ((2, 33, 100, 6), (2, 3, 100, 65), (40000, 3, 100, 6), (2, 3, (1 << 23) + 1, 6)):
+        with pytest.raises(_lib.HiRocmError):
+            BeamSearch(*args)
+    par = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    s = torch.zeros(6, 4, 8, device="cuda")
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for bad in (lambda: reorder_states(s, par.long()), lambda: reorder_states(s[:5], par),
+                lambda: reorder_states(s, par, dst=s.double()), lambda: reorder_states(s, par, length_dim=1),
+                lambda: reorder_states(s, par, length_dim=0, lengths=lens),
+                lambda: reorder_states(s.transpose(1, 2), par, length_dim=1, lengths=lens),
+                lambda: reorder_states(s, par.cpu()), lambda: reorder_states(s.cpu(), par.cpu()),
+                lambda: reorder_states(s[:, :0], par)):
+        with pytest.raises(ValueError):
+            bad()
+    flat = torch.zeros(100, device="cuda")
+    with pytest.raises(_lib.HiRocmError):  # rows that share bytes
+        reorder_states(flat.as_strided((6, 8), (4, 1)), par)
+    with pytest.raises(_lib.HiRocmError):  # dst overlaps src
+        reorder_states(flat[:48].view(6, 8), par, dst=flat[8:56].view(6, 8))
