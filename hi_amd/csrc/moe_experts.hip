@@ -91,7 +91,7 @@ struct GroupedArgs {
   void* out;               // [places][out_stride]
   int64_t out_stride;
   int x_rows, top_k, places, experts, cols, k, swiglu, out_bf16;
-  int out_vec;  // four columns of out can be stored at once
+  int out_vec;  // rows of out start on 16 bytes
 };
 
 // The groups are cut into tiles of BM places, and the work is (tile, block of
@@ -148,7 +148,17 @@ __device__ __forceinline__ bool moe_work(const GroupedArgs& a, int blocks, MoeWo
   return false;
 }
 
-__device__ __forceinline__ float moe_silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u.  exp(-g) as 2^t (1 + ln 2 * what t = -g log2 e lost to its
+// rounding): within a few units of the last place, in a third of expf's and the
+// division's instructions (the product kernels repeat this for every register).
+__device__ __forceinline__ float moe_silu_mul(float g, float u) {
+  constexpr float kLog2e = 1.44269502e+00f, kLog2eLo = 1.92596299e-08f, kLn2 = 6.93147182e-01f;
+  const float t = -g * kLog2e;
+  const float lost = fmaf(-g, kLog2eLo, fmaf(-g, kLog2e, -t));
+  const float p = __builtin_amdgcn_exp2f(t);
+  const float e = fabsf(g) < 128.f ? fmaf(p, lost * kLn2, p) : p;  // (beyond: p is 0 or inf, or NaN)
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
 
 // The row of x behind place i.
 __device__ __forceinline__ const __bf16* moe_row(const GroupedArgs& a, int i) {
@@ -293,19 +303,155 @@ __global__ void __launch_bounds__(64 * kFewWaves) moe_few_kernel(GroupedArgs a) 
   }
 }
 
-// Many places an expert (prefill): BM places times BN weight rows a workgroup,
-// k in steps of 64 through two LDS buffers.  A wave multiplies (BM / WM) x (BN
-// / WN).  A step's operands are loaded into registers while the step before it
-// multiplies, then written to the other buffer; rows of 128 bytes with the
-// 16-byte chunk c of row j at c ^ (j & 7), so that 16 rows' reads of one chunk
-// meet all banks.
-template <int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) moe_many_kernel(GroupedArgs a) {
-  constexpr int T = 64 * WM * WN, XL = BM * 8 / T, WL = BN * 8 / T, MT = BM / WM / 16, NT = BN / WN / 16;
-  constexpr int STEP = (BM + BN) * 128;
-  static_assert(BM * 8 % T == 0 && BN * 8 % T == 0 && NT % 2 == 0, "tile split");
-  extern __shared__ __align__(16) unsigned char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r = lane & 15, g = lane >> 4;
+// Many places an expert (prefill): BM places times BN weight rows a workgroup
+// of eight waves, two a SIMD, a wave (BM / WM) x (BN / WN) of them.
+//
+// k goes in steps of BK through NB LDS buffers that loads fill directly (the
+// step NB - 1 ahead).  A step has two phases: read the step's operands from
+// LDS and start the loads of a later step; multiply.  Waves 4 to 7 run one
+// phase behind waves 0 to 3 (a barrier more before the first step), so on
+// every SIMD one wave reads while the other multiplies.  Why no buffer is
+// written while it is read: a wave's reads are done (lgkmcnt 0) before the
+// barrier that ends its phase, the other waves read the same step at most one
+// phase later, and the buffer of step s - 1 is filled again from step s's read
+// phase on.  Why a step is there when it is read: each wave waits for its own
+// loads of step s + 1 (all but the NB - 2 newest steps') before the barrier
+// that ends its reading of step s.
+//
+// A row of a step is BK * 2 bytes; its 16-byte chunk c lies at c ^ (row & 7)
+// (BK = 64) or c ^ (row / 2 & 3) (BK = 32), so that 16 rows' reads of a chunk
+// meet all banks.  A load writes 64 lanes x 16 contiguous bytes; the lanes
+// choose their global addresses so that the chunks land there.  Chunks past k
+// come from a zero.
+__device__ const uint4 moe_zero = {0u, 0u, 0u, 0u};
+
+typedef __attribute__((address_space(3))) void moe_lds;
+typedef const __attribute__((address_space(1))) void moe_global;
+
+// The barrier alone, with nothing moved across it (__syncthreads would also
+// wait for the loads in flight).
+__device__ __forceinline__ void moe_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+// vmcnt <= N, lgkmcnt 0
+template <int N>
+__device__ __forceinline__ void moe_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 7 << 4);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+template <int L>
+struct MoeSources {
+  const __bf16* p[L];
+};
+
+// The loads of a step's L rounds into `to` (this wave's part of the first).
+// A pointer of its own for what the step reads from LDS and one for what the
+// loads write: the compiler then knows that the reads need not wait for them.
+template <int L, int T>
+__device__ __forceinline__ void moe_fill(const MoeSources<L>& src, bool in, int k, char* to) {
+  #pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const void* from = in ? (const void*)(src.p[i] + k) : (const void*)&moe_zero;
+    __builtin_amdgcn_global_load_lds((moe_global*)from, (moe_lds*)(to + i * T * 16), 16, 0, 0);
+  }
+}
+
+template <int MT, int NT, int KH, int BK>
+__device__ __forceinline__ void moe_read(const char* __restrict__ xb, const char* __restrict__ wb, int r, int g,
+                                         moe_bf16x8 (&xf)[KH][MT], moe_bf16x8 (&wf)[KH][NT]) {
+  #pragma unroll
+  for (int h = 0; h < KH; ++h) {
+    const int at = BK == 64 ? ((g + 4 * h) ^ (r & 7)) * 16 : (g ^ ((r >> 1) & 3)) * 16;
+    #pragma unroll
+    for (int t = 0; t < NT; ++t) wf[h][t] = *reinterpret_cast<const moe_bf16x8*>(wb + t * (32 * BK) + at);
+    #pragma unroll
+    for (int m = 0; m < MT; ++m) xf[h][m] = *reinterpret_cast<const moe_bf16x8*>(xb + m * (32 * BK) + at);
+  }
+}
+
+// A wave's results, MT x 16 places (from p0) of NT x 16 columns (from c0, with
+// swiglu half as many), by way of its own LDS: 64 places at a time in rows of
+// 64 columns, written out 16 bytes a lane, a row's bytes next to each other.
+// Stored from the lanes that hold them, each store would touch 16 rows, and
+// the unrolled code would be ten times as long.
+constexpr int kMoeOutBytes = 16384;
+
+template <int MT, int NT>
+__device__ __forceinline__ void moe_tile_out(const GroupedArgs& a, moe_f32x4 (&acc)[MT][NT], char* mem, int p0, int i1,
+                                             int c0, int cols_out, int lane) {
+  static_assert(NT == 4, "64 columns a wave");
+  const int r = lane & 15, g = lane >> 4;
+  if (a.swiglu) {
+    #pragma unroll
+    for (int m = 0; m < MT; ++m)
+      #pragma unroll
+      for (int t = 0; t < NT / 2; ++t)
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) acc[m][t][q] = moe_silu_mul(acc[m][t][q], acc[m][t + NT / 2][q]);
+  }
+  const int wide = a.swiglu ? 32 : 64;  // columns of a row
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  #pragma unroll
+  for (int half = 0; half < (MT + 3) / 4; ++half) {
+    if (p0 + half * 64 >= i1) return;
+    // row j of 64 values: the 16-byte chunk c at c ^ (j & 7)
+    #pragma unroll
+    for (int m = half * 4; m < half * 4 + 4 && m < MT; ++m) {
+      const int j = (m - half * 4) * 16 + r;
+      #pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (a.out_bf16)
+          *reinterpret_cast<bf16x4*>(mem + j * 128 + ((t * 2 + (g >> 1)) ^ (j & 7)) * 16 + (g & 1) * 8) =
+              __builtin_convertvector(acc[m][t], bf16x4);
+        else
+          *reinterpret_cast<moe_f32x4*>(mem + j * 256 + ((t * 4 + g) ^ (j & 7)) * 16) = acc[m][t];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int es = a.out_bf16 ? 2 : 4, n = 16 / es;    // bytes of a value, values of a chunk
+    const int lanes = wide / n, rows = 64 / lanes;      // lanes of a row, rows at a time
+    const int c = lane % lanes, col = c0 + c * n;
+    const int left = min(i1 - p0 - half * 64, 64);
+    #pragma unroll 1
+    for (int j = lane / lanes; j < left; j += rows) {
+      const uint4 v = *reinterpret_cast<const uint4*>(mem + j * (64 * es) + (c ^ (j & 7)) * 16);
+      char* to = (char*)a.out + ((int64_t)(p0 + half * 64 + j) * a.out_stride + col) * es;
+      if (col + n <= cols_out && a.out_vec) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        #pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (q >= n || col + q >= cols_out) break;
+          if (a.out_bf16) ((uint16_t*)to)[q] = (uint16_t)(w[q >> 1] >> (q & 1) * 16);
+          else ((uint32_t*)to)[q] = w[q & 3];
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int BK, int NB>
+__global__ void __launch_bounds__(512) moe_many_kernel(GroupedArgs a) {
+  constexpr int T = 512, CH = BK / 8;                    // 16-byte chunks of a row
+  constexpr int XL = BM * CH / T, WL = BN * CH / T;      // loads a thread
+  constexpr int MT = BM / WM / 16, NT = BN / WN / 16, KH = BK / 32;
+  constexpr int ROW = BK * 2, STEP = (BM + BN) * ROW;
+  static_assert(WM * WN == 8 && XL >= 1 && WL >= 1 && BM * CH % T == 0 && BN * CH % T == 0 && NT % 2 == 0, "tile split");
+  extern __shared__ __align__(16) char moe_smem[];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wid % WM, wn = wid / WM;
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols;
   const int per = a.swiglu ? BN / 2 : BN;
@@ -320,28 +466,23 @@ __global__ void __launch_bounds__(64 * WM * WN) moe_many_kernel(GroupedArgs a) {
     const int in = j % WR;
     return min(c0 + j / WR * (WR / 2) + in % (WR / 2), cols_out - 1) + (in >= WR / 2 ? cols_out : 0);
   };
-  const int chunk = (tid & 7) ^ ((tid >> 3) & 7);  // (T / 8 rows a round: a multiple of 8)
-  const __bf16 *xp[XL], *wp[WL];
+  // this thread's chunk of the rows it loads (the same in every round: a round
+  // is a multiple of 8 rows)
+  const int jr = tid / CH;
+  const int chunk = (tid % CH) ^ (BK == 64 ? jr & 7 : jr >> 1 & 3);
+  MoeSources<XL> xs;
+  MoeSources<WL> ws;
   #pragma unroll
-  for (int i = 0; i < XL; ++i) xp[i] = moe_row(a, min(wk.i0 + (i * T + tid) / 8, wk.i1 - 1)) + 8 * chunk;
+  for (int i = 0; i < XL; ++i) xs.p[i] = moe_row(a, min(wk.i0 + i * (T / CH) + jr, wk.i1 - 1)) + 8 * chunk;
   #pragma unroll
   for (int i = 0; i < WL; ++i)
-    wp[i] = a.w + ((int64_t)wk.expert * a.cols + column((i * T + tid) / 8)) * a.k + 8 * chunk;
-  moe_bf16x8 xs[XL], ws[WL];
-  auto load = [&](int k) {
+    ws.p[i] = a.w + ((int64_t)wk.expert * a.cols + column(i * (T / CH) + jr)) * a.k + 8 * chunk;
+  auto fill = [&](int step) {
+    const int k = step * BK;
     const bool in = k + 8 * chunk < a.k;
-    const moe_bf16x8 zero = {};
-    #pragma unroll
-    for (int i = 0; i < XL; ++i) xs[i] = in ? moe_ld(xp[i] + k) : zero;
-    #pragma unroll
-    for (int i = 0; i < WL; ++i) ws[i] = in ? moe_ld(wp[i] + k) : zero;
-  };
-  auto stage = [&](int buf) {
-    unsigned char* b = lds + buf * STEP;
-    #pragma unroll
-    for (int i = 0; i < XL; ++i) *reinterpret_cast<moe_bf16x8*>(b + (i * T + tid) * 16) = xs[i];
-    #pragma unroll
-    for (int i = 0; i < WL; ++i) *reinterpret_cast<moe_bf16x8*>(b + BM * 128 + (i * T + tid) * 16) = ws[i];
+    char* to = moe_smem + step % NB * STEP + wid * 1024;
+    moe_fill<XL, T>(xs, in, k, to);
+    moe_fill<WL, T>(ws, in, k, to + BM * ROW);
   };
   moe_f32x4 acc[MT][NT];
   #pragma unroll
@@ -349,56 +490,39 @@ __global__ void __launch_bounds__(64 * WM * WN) moe_many_kernel(GroupedArgs a) {
     #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = moe_f32x4{0.f, 0.f, 0.f, 0.f};
   const bool busy = wk.i0 + wm * (BM / WM) < wk.i1;  // this wave has places
-  const int steps = (a.k + 63) / 64;
-  load(0);
-  stage(0);
-  __syncthreads();
+  const int steps = (a.k + BK - 1) / BK;
+  #pragma unroll
+  for (int s = 0; s < NB - 1; ++s) fill(s);
+  moe_wait<(XL + WL) * (NB - 2)>();
+  moe_barrier();
+  if (wid >= 4) moe_barrier();
   for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) load((s + 1) * 64);
+    moe_bf16x8 xf[KH][MT], wf[KH][NT];
+    const char* b = moe_smem + s % NB * STEP;
+    if (busy)
+      moe_read<MT, NT, KH, BK>(b + (wm * (BM / WM) + r) * ROW, b + BM * ROW + (wn * WR + r) * ROW, r, g, xf, wf);
+    fill(s + NB - 1);
+    moe_wait<(XL + WL) * (NB - 2)>();
+    moe_barrier();
     if (busy) {
-      const unsigned char* b = lds + (s & 1) * STEP;
-      const unsigned char* xb = b + (wm * (BM / WM) + r) * 128;
-      const unsigned char* wb = b + BM * 128 + (wn * WR + r) * 128;
+      __builtin_amdgcn_s_setprio(1);
       #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = ((g + 4 * h) ^ (r & 7)) * 16;
-        moe_bf16x8 wf[NT], xf[MT];
-        #pragma unroll
-        for (int t = 0; t < NT; ++t) wf[t] = *reinterpret_cast<const moe_bf16x8*>(wb + t * 2048 + at);
-        #pragma unroll
-        for (int m = 0; m < MT; ++m) xf[m] = *reinterpret_cast<const moe_bf16x8*>(xb + m * 2048 + at);
+      for (int h = 0; h < KH; ++h)
         #pragma unroll
         for (int m = 0; m < MT; ++m)
           #pragma unroll
           for (int t = 0; t < NT; ++t)
-            acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[t], xf[m], acc[m][t], 0, 0, 0);
-      }
+            acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[h][t], xf[h][m], acc[m][t], 0, 0, 0);
+      __builtin_amdgcn_s_setprio(0);
     }
-    if (s + 1 < steps) stage((s + 1) & 1);
-    __syncthreads();
+    moe_barrier();
   }
+  if (wid < 4) moe_barrier();
+  moe_wait<0>();  // no load may still write LDS when it is used again, or the workgroup ends
+  moe_barrier();
   if (!busy) return;
-  #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int p = wk.i0 + wm * (BM / WM) + 16 * m + r;
-    if (p >= wk.i1) continue;
-    if (a.swiglu) {
-      #pragma unroll
-      for (int t = 0; t < NT / 2; ++t) {
-        moe_f32x4 y;
-        #pragma unroll
-        for (int q = 0; q < 4; ++q) y[q] = moe_silu_mul(acc[m][t][q], acc[m][t + NT / 2][q]);
-        const int c = c0 + wn * (WR / 2) + t * 16 + 4 * g;
-        if (c < cols_out) moe_store(a, p, c, cols_out, y);
-      }
-    } else {
-      #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int c = c0 + wn * WR + t * 16 + 4 * g;
-        if (c < cols_out) moe_store(a, p, c, cols_out, acc[m][t]);
-      }
-    }
-  }
+  moe_tile_out<MT, NT>(a, acc, moe_smem + wid * kMoeOutBytes, wk.i0 + wm * (BM / WM), wk.i1,
+                       c0 + wn * (a.swiglu ? WR / 2 : WR), cols_out, lane);
 }
 
 // The largest grid that any split of the places over the experts needs (every
@@ -415,13 +539,13 @@ hipError_t launch_few(const GroupedArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int BK, int NB>
 hipError_t launch_many(const GroupedArgs& a, hipStream_t st) {
-  constexpr size_t bytes = 2 * (BM + BN) * 128;
-  auto* kernel = moe_many_kernel<BM, BN, WM, WN>;
+  constexpr size_t bytes = (size_t)NB * (BM + BN) * BK * 2;
+  auto* kernel = moe_many_kernel<BM, BN, WM, WN, BK, NB>;
   const hipError_t e = ensure_lds((const void*)kernel, bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)moe_grid(a, BM, BN)), dim3(64 * WM * WN), bytes, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)moe_grid(a, BM, BN)), dim3(512), bytes, st, a);
   return hipGetLastError();
 }
 
@@ -430,8 +554,8 @@ hipError_t launch_grouped(const GroupedArgs& a, hipStream_t st) {
   if (avg <= 8) return launch_few<1>(a, st);
   if (avg <= 20) return launch_few<2>(a, st);
   if (avg <= 40) return launch_few<4>(a, st);
-  if (avg <= 256) return launch_many<128, 256, 2, 4>(a, st);
-  return launch_many<256, 256, 2, 4>(a, st);
+  if (avg <= 256) return launch_many<128, 256, 2, 4, 64, 3>(a, st);
+  return launch_many<256, 256, 2, 4, 32, 4>(a, st);
 }
 
 // ---- combination ----------------------------------------------------------
@@ -525,7 +649,7 @@ int hi_rocm_moe_grouped_product(const void* x, int x_rows, int64_t x_stride, con
   a.k = k;
   a.swiglu = swiglu != 0;
   a.out_bf16 = out_dtype == HI_ROCM_DTYPE_BF16;
-  a.out_vec = (uintptr_t)out % (4 * moe_size(out_dtype)) == 0 && out_stride % 4 == 0;
+  a.out_vec = (uintptr_t)out % 16 == 0 && out_stride * moe_size(out_dtype) % 16 == 0;
   if (moe_grid(a, 16, 32) > INT32_MAX)
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_moe_grouped_product: too many places and columns");
   const hipError_t e = launch_grouped(a, (hipStream_t)stream);
