@@ -14,8 +14,8 @@
 // beam.
 //
 // Two kernels read each logit once:
-//  * beam_part_kernel: a part of a row in registers: its maximum, its sum of
-//    exponentials, and its first n_out candidates by (logit, token);
+//  * beam_part_kernel: a part of a row streams through registers: its maximum,
+//    its sum of exponentials, and its first n_out candidates by (logit, token);
 //  * beam_finish_kernel: a request: its beams' lse from the parts, and the
 //    first n_out of the parts' candidates.
 #include <hip/hip_runtime.h>
@@ -34,10 +34,14 @@ namespace {
 constexpr int kBeamMax = HI_ROCM_BEAM_MAX;
 constexpr int kBeamMaxOut = HI_ROCM_BEAM_MAX_OUT;
 constexpr int kPartThreads = 256;
-constexpr int kPartSlots = 256;      // candidates a part can hold before it ranks them
-constexpr int kFinishThreads = 1024;
+constexpr int kTileElems = 4096;     // elements of a part of a short step
+constexpr int kTileSlots = 256;      // candidates that such a part can hold before it ranks them
+constexpr int kPartSlots = 512;      // candidates that a wave of a streamed part can hold
+constexpr int kFinishThreads = 512;
+constexpr int kFinishHeld = 4;       // candidates a thread keeps in registers
 constexpr int kFinishSlots = 512;
 constexpr int kBeamMaxRows = 65536;
+
 
 struct BeamPart {
   float m;       // largest logit of the part (-inf: no candidate)
@@ -53,6 +57,7 @@ struct BeamArgs {
   const uint8_t* finished;    // [rows] or null
   const uint32_t* mask;       // [rows][mask_words] or null
   int V, K, n_out, n_parts, mask_words;
+  int tiles;                  // of a part
   uint32_t eos;
   BeamPart* parts;            // [rows][n_parts]
   uint64_t* cand;             // [rows][n_parts][n_out], descending
@@ -72,17 +77,41 @@ __device__ __forceinline__ uint32_t beam_okey(float x) {
 __device__ __forceinline__ float beam_okey_inv(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
 }
+constexpr float kBeamLowest = -3.402823466e38f;
 constexpr uint32_t kBeamNegInf = 0x007fffffu;  // beam_okey(-inf): keys above it are candidates
 
+// Wave reductions by DPP moves (lane 63 ends with the result).
+template <typename F>
+__device__ __forceinline__ uint32_t beam_wave_fold(uint32_t v, F f) {
+  v = f(v, dpp32<kDppShr1>(v, v));
+  v = f(v, dpp32<kDppShr1 + 1>(v, v));
+  v = f(v, dpp32<kDppShr1 + 3>(v, v));
+  v = f(v, dpp32<kDppShr1 + 7>(v, v));
+  v = f(v, dpp32<kDppBcast15, 0xa>(v, v));
+  v = f(v, dpp32<kDppBcast31, 0xc>(v, v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t beam_wave_umax(uint32_t v) {
+  return beam_wave_fold(v, [](uint32_t x, uint32_t y) { return max(x, y); });
+}
+__device__ __forceinline__ uint32_t beam_wave_umin(uint32_t v) {
+  return beam_wave_fold(v, [](uint32_t x, uint32_t y) { return min(x, y); });
+}
 __device__ __forceinline__ float beam_wave_max(float v) {
-  #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
+  return __uint_as_float(beam_wave_fold(__float_as_uint(v), [](uint32_t x, uint32_t y) {
+    return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+  }));
 }
 __device__ __forceinline__ float beam_wave_sum(float v) {
-  #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  auto add = [&](uint32_t w) { v += __uint_as_float(w); };
+  auto b = [&]() { return __float_as_uint(v); };
+  add(dpp32<kDppShr1, 0xf, true>(0u, b()));
+  add(dpp32<kDppShr1 + 1, 0xf, true>(0u, b()));
+  add(dpp32<kDppShr1 + 3, 0xf, true>(0u, b()));
+  add(dpp32<kDppShr1 + 7, 0xf, true>(0u, b()));
+  add(dpp32<kDppBcast15, 0xa>(0u, b()));
+  add(dpp32<kDppBcast31, 0xc>(0u, b()));
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)b(), 63));
 }
 
 // Whether a row takes part: a beam whose score is not finite has no
@@ -91,36 +120,51 @@ __device__ __forceinline__ bool beam_reads(const BeamArgs& a, int row) {
   return beam_finite(a.scores[row]) && !(a.finished && a.finished[row]);
 }
 
-// The n-th largest key of G a lane over the wave (0 when fewer are above 0),
-// bit by bit.
+// A key that at least n <= 64 of G keys a lane reach, and not many more: from
+// the bits that the largest key and the smallest lane's largest (64 keys reach
+// it) share downwards, until at most n + n / 2 + 1 reach it.
 template <int G>
 __device__ __forceinline__ uint32_t beam_wave_nth(const uint32_t (&key)[G], int n) {
-  uint32_t t = 0u;
+  uint32_t top = key[0];
+  #pragma unroll
+  for (int g = 1; g < G; ++g) top = max(top, key[g]);
+  const uint32_t lo = beam_wave_umin(top), hi = beam_wave_umax(top);
+  if (lo == hi) return lo;
+  const int first = 31 - __builtin_clz(lo ^ hi);
+  uint32_t t = hi & ~((2u << first) - 1u);
   #pragma unroll 1
-  for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1) {
-    const uint32_t c = t | bit;
+  for (int bit = first; bit >= 0; --bit) {
+    const uint32_t c = t | (1u << bit);
     int cnt = 0;
     #pragma unroll
     for (int g = 0; g < G; ++g) cnt += __popcll(__ballot(key[g] >= c));
-    if (cnt >= n) t = c;
+    if (cnt >= n) {
+      t = c;
+      if (cnt <= n + n / 2 + 1) break;
+    }
   }
   return t;
 }
 
-// A bound with at least n keys of the workgroup (W waves, G keys a lane) at
-// or above it: the smallest of the waves' ceil(n / W)-th keys, or the largest
-// of their n-th.
+// A bound that at least n keys of the workgroup (W waves, G keys a lane)
+// reach, if it holds n above `floor`: the smallest of the waves' ceil(n /
+// W)-th keys, or, where a wave has not as many, the largest of their n-th.
 template <int G, int W>
-__device__ __forceinline__ uint32_t beam_bound(const uint32_t (&key)[G], int n, uint32_t* red) {
-  const uint32_t share = beam_wave_nth<G>(key, (n + W - 1) / W);
-  const uint32_t full = beam_wave_nth<G>(key, n);
+__device__ __forceinline__ uint32_t beam_bound(const uint32_t (&key)[G], int n, uint32_t floor, uint32_t* red) {
   const int wid = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) { red[wid] = share; red[W + wid] = full; }
+  const uint32_t share = beam_wave_nth<G>(key, (n + W - 1) / W);
+  if ((threadIdx.x & 63) == 0) red[wid] = share;
   __syncthreads();
-  uint32_t lo = red[0], hi = red[W];
+  uint32_t b = red[0];
   #pragma unroll
-  for (int w = 1; w < W; ++w) { lo = min(lo, red[w]); hi = max(hi, red[W + w]); }
-  return max(lo, hi);
+  for (int w = 1; w < W; ++w) b = min(b, red[w]);
+  if (b > floor || W == 1) return b;
+  const uint32_t full = beam_wave_nth<G>(key, n);
+  if ((threadIdx.x & 63) == 0) red[W + wid] = full;
+  __syncthreads();
+  #pragma unroll
+  for (int w = 0; w < W; ++w) b = max(b, red[W + w]);
+  return b;
 }
 
 // 16 bytes of a row as floats.
@@ -140,21 +184,23 @@ struct BeamLoad<HI_ROCM_DTYPE_BF16> {
   }
 };
 
-// One part: kPartThreads * PER elements of a row, counted from the 16-byte
-// boundary at or before the row's start (rows start anywhere; the elements
-// before the start and after the end are no candidates).
-template <int DT, int PER>
-__global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
+// One part of a short step: kTileElems elements of a row, counted from the
+// 16-byte boundary at or before the row's start (rows start anywhere; the
+// elements before the start and after the end are no candidates).  All of it
+// is in registers at once, and little code runs, which is most of such a
+// launch's time: 4 rows of 151,936 f32 take 6.3 us, 8.2 with the streaming
+// kernel below.
+template <int DT>
+__global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
+  constexpr int PER = kTileElems / kPartThreads;
   constexpr int N = BeamLoad<DT>::N, L = PER / N, W = kPartThreads / 64, ES = 16 / N;
-  constexpr int G = 4;  // groups a thread for the bound
-  static_assert(PER % G == 0, "groups");
-  __shared__ uint64_t slots[kPartSlots];
+  constexpr int G = PER / 8;  // groups a thread
+  __shared__ uint64_t slots[kTileSlots];
   __shared__ uint64_t red64[W];
   __shared__ uint32_t red[2 * W];
-  __shared__ float redf[W];
+  __shared__ float redf[W], reds[W];
   __shared__ uint32_t counter;
   const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  if (!beam_reads(a, row)) return;
   const char* p0 = (const char*)a.logits + (int64_t)row * a.row_stride * ES;
   const int head = (int)((uintptr_t)p0 & 15) / ES;
   const int64_t base = (int64_t)part * (kPartThreads * PER);  // elements from the aligned start
@@ -164,11 +210,14 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   const int bytes = left < 0 ? 0 : (int)(left < kSpan ? left : kSpan);
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(p0 - head * ES + base * ES), 0, (bytes + 3) & ~3, kBufferConfig);
+  if (tid == 0) counter = 0u;
   float x[PER];
   {
     i32x4_t v[L];
     #pragma unroll
     for (int j = 0; j < L; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, (j * kPartThreads + tid) * 16, 0, 0);
+    // (the loads go out before it is known that the row takes part)
+    if (!beam_reads(a, row)) return;
     #pragma unroll
     for (int j = 0; j < L; ++j) {
       #pragma unroll
@@ -178,63 +227,80 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   const float ninf = -__builtin_inff();
   // token of x[j * N + q]: t0 + j * kPartThreads * N + q
   const int t0 = (int)base + tid * N - head;
-  const uint32_t* mrow = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
-  #pragma unroll
-  for (int j = 0; j < L; ++j) {
-    const int t = t0 + j * (kPartThreads * N);
-    uint64_t bits = ~0ull;
-    if (mrow) {
-      const int tc = t < 0 ? 0 : t, w = tc >> 5;
-      const uint64_t lo = w < a.mask_words ? mrow[w] : 0u, hi = w + 1 < a.mask_words ? mrow[w + 1] : 0u;
-      bits = ((hi << 32) | lo) >> (tc & 31);
-      if (t < 0) bits <<= -t;
+  // Inside the row and without a mask nothing is left out but NaN, which no
+  // maximum or comparison below takes, and which shows in the sum.
+  const bool inside = base >= head && base - head + kPartThreads * PER <= a.V && a.mask == nullptr;
+  if (!inside) {
+    const uint32_t* mrow = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
+    uint32_t lo[L], hi[L];
+    #pragma unroll
+    for (int j = 0; j < L; ++j) {
+      lo[j] = hi[j] = ~0u;
+      if (mrow) {
+        const int w = min(max(t0 + j * (kPartThreads * N), 0) >> 5, a.mask_words - 1);
+        lo[j] = mrow[w];
+        if (head != 0) hi[j] = mrow[min(w + 1, a.mask_words - 1)];  // (N tokens from a multiple of N share a word)
+      }
     }
     #pragma unroll
-    for (int q = 0; q < N; ++q) {
-      const float f = x[j * N + q];
-      const bool ok = t + q >= 0 && t + q < a.V && f == f && ((bits >> q) & 1ull);
-      x[j * N + q] = ok ? f : ninf;
+    for (int j = 0; j < L; ++j) {
+      const int t = t0 + j * (kPartThreads * N);
+      uint32_t bits = (uint32_t)(((uint64_t)hi[j] << 32 | lo[j]) >> (max(t, 0) & 31));
+      if (t < 0) bits <<= -t;
+      #pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const bool ok = t + q >= 0 && t + q < a.V && ((bits >> q) & 1u);
+        x[j * N + q] = ok ? x[j * N + q] : ninf;
+      }
     }
   }
   float gm[G];
   #pragma unroll
   for (int g = 0; g < G; ++g) {
-    gm[g] = x[g * (PER / G)];
+    gm[g] = fmaxf(x[8 * g], ninf);
     #pragma unroll
-    for (int i = 1; i < PER / G; ++i) gm[g] = fmaxf(gm[g], x[g * (PER / G) + i]);
+    for (int i = 1; i < 8; ++i) gm[g] = fmaxf(gm[g], x[8 * g + i]);
   }
-  float m = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
-  m = beam_wave_max(m);
-  if (lane == 0) redf[wid] = m;
-  if (tid == 0) counter = 0u;
-  __syncthreads();
+  float m = gm[0];
   #pragma unroll
-  for (int w = 0; w < W; ++w) m = fmaxf(m, redf[w]);
+  for (int g = 1; g < G; ++g) m = fmaxf(m, gm[g]);
+  m = beam_wave_max(m);
+  // each wave's sum by its own maximum, so that one exchange serves both
+  float s = 0.f;
+  if (beam_finite(m)) {
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) s += __expf(x[i] - m);
+    if (__ballot(!(s == s)) != 0ull) {  // a NaN logit
+      s = 0.f;
+      #pragma unroll
+      for (int i = 0; i < PER; ++i) s += x[i] == x[i] ? __expf(x[i] - m) : 0.f;
+    }
+    s = beam_wave_sum(s);
+  }
+  if (lane == 0) { redf[wid] = m; reds[wid] = s; }
+  // the part's candidates: all logits at or above a bound that n_out of them reach
+  uint32_t key[G];
+  #pragma unroll
+  for (int g = 0; g < G; ++g) key[g] = beam_okey(gm[g]);
+  const uint32_t bound = max(beam_bound<G, W>(key, a.n_out, kBeamNegInf, red), kBeamNegInf + 1u);
+  m = redf[0];
+  #pragma unroll
+  for (int w = 1; w < W; ++w) m = fmaxf(m, redf[w]);
   const int64_t slot = (int64_t)row * a.n_parts + part;
   if (!beam_finite(m)) {  // nothing allowed, or a +inf logit: the finish sees which
     if (tid == 0) a.parts[slot] = BeamPart{m, 0.f, 0u, 0u};
     return;
   }
-  float s = 0.f;
+  const float at_least = beam_okey_inv(bound);
   #pragma unroll
-  for (int i = 0; i < PER; ++i) s += __expf(x[i] - m);
-  s = beam_wave_sum(s);
-  // the part's candidates: all logits at or above a bound that n_out of them reach
-  uint32_t key[G];
-  #pragma unroll
-  for (int g = 0; g < G; ++g) key[g] = beam_okey(gm[g]);
-  const uint32_t bound = max(beam_bound<G, W>(key, a.n_out, red), kBeamNegInf + 1u);
-  __syncthreads();
-  if (lane == 0) redf[wid] = s;
-  #pragma unroll
-  for (int j = 0; j < L; ++j) {
+  for (int g = 0; g < G; ++g) {
+    if (gm[g] < at_least) continue;
     #pragma unroll
-    for (int q = 0; q < N; ++q) {
-      const uint32_t k = beam_okey(x[j * N + q]);
-      if (k >= bound) {
+    for (int i = 8 * g; i < 8 * g + 8; ++i) {
+      if (x[i] >= at_least) {
         const uint32_t o = atomicAdd(&counter, 1u);
-        if (o < (uint32_t)kPartSlots)
-          slots[o] = ((uint64_t)k << 32) | (0xffffffffu - (uint32_t)(t0 + j * (kPartThreads * N) + q));
+        const int t = t0 + i / N * (kPartThreads * N) + i % N;
+        if (o < (uint32_t)kTileSlots) slots[o] = ((uint64_t)beam_okey(x[i]) << 32) | (0xffffffffu - (uint32_t)t);
       }
     }
   }
@@ -243,12 +309,12 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   uint64_t* out = a.cand + slot * a.n_out;
   const int keep = min(n, a.n_out);
   if (tid == 0) {
-    s = redf[0];
+    s = 0.f;
     #pragma unroll
-    for (int w = 1; w < W; ++w) s += redf[w];
+    for (int w = 0; w < W; ++w) s += reds[w] * __expf(redf[w] - m);
     a.parts[slot] = BeamPart{m, s, (uint32_t)keep, 0u};
   }
-  if (n <= kPartSlots) {
+  if (n <= kTileSlots) {
     // rank by counting
     if (tid < n) {
       const uint64_t mine = slots[tid];
@@ -268,7 +334,7 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
       for (int q = 0; q < N; ++q) {
         const uint64_t k = ((uint64_t)beam_okey(x[j * N + q]) << 32) |
                            (0xffffffffu - (uint32_t)(t0 + j * (kPartThreads * N) + q));
-        if (k < prev && k > best) best = k;
+        if (x[j * N + q] >= at_least && k < prev && k > best) best = k;
       }
     }
     #pragma unroll
@@ -286,6 +352,318 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
     prev = best;
     if (tid == 0) out[r] = best;
   }
+}
+
+// A candidate as the part kernel lists it, and as the key it is ranked by.
+struct __align__(8) BeamRaw {
+  float logit;
+  uint32_t token;
+};
+__device__ __forceinline__ uint64_t beam_key(const BeamRaw& c) {
+  return ((uint64_t)beam_okey(c.logit) << 32) | (0xffffffffu - c.token);
+}
+__device__ __forceinline__ BeamRaw beam_raw(uint64_t key) {
+  return BeamRaw{beam_okey_inv((uint32_t)(key >> 32)), 0xffffffffu - (uint32_t)key};
+}
+// Set bits of a ballot below this lane's.
+__device__ __forceinline__ int beam_below(uint64_t b) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
+}
+// The largest of three numbers.  (fmaxf would first quiet each operand, an
+// instruction a logit; a signalling NaN's group is found by its sum.)
+__device__ __forceinline__ float beam_max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+
+// The largest n of a wave's count in (n, kPartSlots] candidates, moved to the
+// list's start; returns the upper half of the n-th's key, found bit by bit from the highest bit
+// in which the keys differ.  (Not inlined: the part kernel's loop has several
+// places for it.)
+__device__ __noinline__ uint32_t beam_prune(BeamRaw* list, int count, int n) {
+  constexpr int P = kPartSlots / 64;
+  const int lane = threadIdx.x & 63;
+  uint64_t k[P];
+  uint32_t hi = 0u, lo = 0xffffffffu;  // of the keys' upper halves
+  #pragma unroll
+  for (int j = 0; j < P; ++j) {
+    k[j] = 0ull;
+    if (lane + 64 * j < count) {
+      k[j] = beam_key(list[lane + 64 * j]);
+      hi = max(hi, (uint32_t)(k[j] >> 32));
+      lo = min(lo, (uint32_t)(k[j] >> 32));
+    }
+  }
+  hi = beam_wave_umax(hi);
+  lo = beam_wave_umin(lo);
+  int bit = hi == lo ? 31 : 63 - __builtin_clz(hi ^ lo);
+  uint64_t t = (uint64_t)hi << 32 & ~((2ull << bit) - 1ull);
+  #pragma unroll 1
+  for (; bit >= 0; --bit) {
+    const uint64_t c = t | (1ull << bit);
+    int cnt = 0;
+    #pragma unroll
+    for (int j = 0; j < P; ++j) cnt += __popcll(__ballot(k[j] >= c));
+    if (cnt >= n) t = c;
+    if (cnt == n) break;
+  }
+  int at = 0;
+  uint32_t low = 0xffffffffu;
+  #pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const uint64_t keep = __ballot(k[j] >= t);
+    if (k[j] >= t) {
+      list[at + beam_below(keep)] = beam_raw(k[j]);
+      low = min(low, (uint32_t)(k[j] >> 32));
+    }
+    at += __popcll(keep);
+  }
+  return beam_wave_umin(low);
+}
+
+// One part of a row: tiles [part * a.tiles, ...) of 64 lanes x 64 bytes,
+// counted from the 16-byte boundary at or before the row's start (rows start
+// anywhere; what lies before the start and after the end is no candidate).
+// Each wave takes every fourth tile, with the next one's loads in flight, and
+// needs no other wave until the end:
+//  * a lane keeps its running maximum and sum, rescaled once a tile;
+//  * the wave keeps its candidates in LDS: those at or above a bound that n_out
+//    of the four first tiles' groups reach (the only exchange before the end),
+//    or above the n_out-th kept after a full list was cut back to n_out, so
+//    that most tiles end at one comparison.
+// A tile a workgroup instead, with a bound and an exchange each, had twice the
+// instructions a logit and no loads in flight while it computed (64 x 8 rows of
+// 151,936 bf16: 52 us).
+template <int DT, bool MASK>
+__global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
+  constexpr int N = BeamLoad<DT>::N, L = 4, PER = L * N, W = kPartThreads / 64, ES = 16 / N;
+  constexpr int G = PER / 4, GN = 4;  // groups of 4 elements
+  __shared__ BeamRaw lists[W][kPartSlots];
+  __shared__ float redm[W], reds[W];
+  __shared__ int redn[W];
+  __shared__ uint32_t red[2 * W];
+  const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const char* p0 = (const char*)a.logits + (int64_t)row * a.row_stride * ES;
+  const int head = (int)((uintptr_t)p0 & 15) / ES;
+  // range-checked loads: bytes from this part's start to the row's or its end
+  const int64_t base = (int64_t)part * a.tiles * (64 * PER);  // elements from the aligned start
+  const int64_t left = ((int64_t)a.V + head - base) * ES;     // (the last part may lie after the row: nothing)
+  const int64_t span = (int64_t)a.tiles * (64 * 16 * L);
+  const int bytes = left < 0 ? 0 : (int)(left < span ? left : span);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(p0 - head * ES + base * ES), 0, (bytes + 3) & ~3, kBufferConfig);
+  const uint32_t* mrow = MASK ? a.mask + (int64_t)row * a.mask_words : nullptr;
+  i32x4_t next[L];
+  uint32_t word[L], word2[L];  // the mask words of the first token of each load and the next one
+  auto load = [&](int tile) {
+    #pragma unroll
+    for (int j = 0; j < L; ++j)
+      next[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, tile * (64 * 16 * L) + (j * 64 + lane) * 16, 0, 0);
+    if (MASK) {
+      const int64_t t = base + (int64_t)tile * (64 * PER) - head + lane * N;
+      #pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const int w = (int)min(max(t + j * (64 * N), (int64_t)0) >> 5, (int64_t)a.mask_words - 1);
+        word[j] = mrow[w];
+        word2[j] = head != 0 ? mrow[min(w + 1, a.mask_words - 1)] : 0u;  // (N tokens from a multiple of N share a word)
+      }
+    }
+  };
+  // (the first loads go out before it is known that the row takes part)
+  load(wid);
+  if (!beam_reads(a, row)) return;
+  const float ninf = -__builtin_inff();
+  BeamRaw* list = lists[wid];
+  int count = 0;
+  float m = ninf, s = 0.f;     // this lane's
+  float bound = 0.f;           // candidates are at or above it; once `full`, above it in the next tile
+  bool full = false, shared = false;
+  auto shared_bound = [&]() {
+    const uint32_t key[1] = {beam_okey(m)};
+    volatile uint32_t* v = red;
+    const uint32_t own = beam_wave_nth<1>(key, (a.n_out + W - 1) / W);
+    if (lane == 0) v[wid] = own;
+    uint32_t b = own;
+    #pragma unroll
+    for (int w = 0; w < W; ++w) b = min(b, v[w]);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
+  };
+  for (int tile = wid; tile < a.tiles; tile += W) {
+    float x[PER];
+    #pragma unroll
+    for (int j = 0; j < L; ++j) {
+      #pragma unroll
+      for (int q = 0; q < N; ++q) x[j * N + q] = BeamLoad<DT>::get(next[j], q);
+    }
+    uint32_t lo[L], hi[L];
+    if (MASK) {
+      #pragma unroll
+      for (int j = 0; j < L; ++j) { lo[j] = word[j]; hi[j] = word2[j]; }
+    }
+    if (tile + W < a.tiles) load(tile + W);
+    // token of x[j * N + q]: t0 + j * 64 * N + q
+    const int64_t e0 = base + (int64_t)tile * (64 * PER) - head;
+    if (e0 >= a.V && tile >= W) break;
+    const int t0 = (int)e0 + lane * N;
+    // Inside the row and without a mask nothing is left out but NaN, which no
+    // maximum or comparison below takes, and which shows in the sum.
+    if (e0 < 0 || e0 + 64 * PER > a.V || MASK) {
+      #pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const int t = t0 + j * (64 * N);
+        uint32_t bits = ~0u;
+        if (MASK) {
+          bits = (uint32_t)(((uint64_t)hi[j] << 32 | lo[j]) >> (max(t, 0) & 31));
+          if (t < 0) bits <<= -t;
+        }
+        #pragma unroll
+        for (int q = 0; q < N; ++q) {
+          const bool ok = t + q >= 0 && t + q < a.V && ((bits >> q) & 1u);
+          x[j * N + q] = ok ? x[j * N + q] : ninf;
+        }
+      }
+    }
+    // the groups' maxima, and the sum about the running maximum (of a lane
+    // without a finite logit: about the lowest value, which leaves its terms 0)
+    float gm[G], tm, mn, at, add;
+    auto sum = [&]() {
+      #pragma unroll
+      for (int g = 0; g < G; ++g)
+        gm[g] = beam_max3(beam_max3(x[GN * g], x[GN * g + 1], x[GN * g + 2]), x[GN * g + 3], ninf);
+      tm = gm[0];
+      #pragma unroll
+      for (int g = 1; g + 1 < G; g += 2) tm = beam_max3(tm, gm[g], gm[g + 1]);
+      tm = beam_max3(tm, gm[G - 1], ninf);
+      mn = beam_max3(m, tm, ninf);
+      at = beam_max3(mn, kBeamLowest, ninf);
+      add = 0.f;
+      #pragma unroll
+      for (int i = 0; i < PER; ++i) add += __expf(x[i] - at);
+    };
+    sum();
+    if (__ballot(!(add == add)) != 0ull) {  // a NaN logit counts as masked (+inf: the sum does not matter)
+      #pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = x[i] == x[i] ? x[i] : ninf;
+      sum();
+    }
+    s = s * __expf(beam_max3(m, kBeamLowest, ninf) - at) + add;
+    m = mn;
+    // candidates
+    if (tile < W) {  // every wave's first
+      uint32_t key[G / 2];  // groups of 8
+      #pragma unroll
+      for (int g = 0; g < G / 2; ++g) key[g] = beam_okey(beam_max3(gm[2 * g], gm[2 * g + 1], ninf));
+      const uint32_t k = beam_bound<G / 2, W>(key, a.n_out, kBeamNegInf, red);
+      shared = k > kBeamNegInf;
+      bound = beam_okey_inv(max(k, kBeamNegInf + 1u));
+    }
+    // n_out kept, by this wave or in all first tiles: equal logits of later
+    // tiles have higher tokens
+    if (tile / W == 1 && shared) full = true;
+    // The bound rises with what the waves have seen, after 2, 4, 8, ... tiles:
+    // each keeps the value that its share of n_out lanes reach, and all values
+    // at or above the least of these include n_out.  (One read early only
+    // bounds less.  The others may be tiles ahead, so an equal logit may still
+    // have a lower token.)
+    if (tile >= W && (tile / W & (tile / W - 1)) == 0) {
+      const float b = beam_okey_inv(shared_bound());
+      if (b > bound) { bound = b; full = false; }
+    }
+    if (__ballot(full ? tm > bound : tm >= bound) == 0ull) continue;
+    #pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (__ballot(gm[g] >= bound) == 0ull) continue;
+      #pragma unroll
+      for (int i = GN * g; i < GN * g + GN; ++i) {
+        const bool pass = full ? x[i] > bound : x[i] >= bound;
+        const uint64_t b = __ballot(pass);
+        if (b == 0ull) continue;
+        if (pass) list[count + beam_below(b)] = BeamRaw{x[i], (uint32_t)(t0 + i / N * (64 * N) + i % N)};
+        count = __builtin_amdgcn_readfirstlane(count + __popcll(b));
+      }
+      if (count > kPartSlots - 64 * GN) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const float low = beam_okey_inv((uint32_t)__builtin_amdgcn_readfirstlane((int)beam_prune(list, count, a.n_out)));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        count = a.n_out;
+        // a later logit of this tile may equal it with a lower token
+        if (low > bound) { bound = low; full = false; }
+      }
+    }
+    if (count >= a.n_out) full = true;
+
+  }
+  if (a.tiles > W) shared_bound();  // (else it has not moved since the first)
+  {
+    const float wm = beam_wave_max(m), at = fmaxf(wm, kBeamLowest);
+    s = beam_wave_sum(s * __expf(fmaxf(m, kBeamLowest) - at));
+    if (lane == 0) { redm[wid] = wm; reds[wid] = s; }
+  }
+  __syncthreads();
+  m = redm[0];
+  uint32_t last = red[0];  // n_out of the part's logits reach it
+  #pragma unroll
+  for (int w = 1; w < W; ++w) {
+    m = fmaxf(m, redm[w]);
+    last = min(last, red[w]);
+  }
+  const int64_t slot = (int64_t)row * a.n_parts + part;
+  if (!beam_finite(m)) {  // nothing allowed, or a +inf logit: the finish sees which
+    if (tid == 0) a.parts[slot] = BeamPart{m, 0.f, 0u, 0u};
+    return;
+  }
+  if (tid == 0) {
+    s = 0.f;
+    #pragma unroll
+    for (int w = 0; w < W; ++w) s += reds[w] * __expf(fmaxf(redm[w], kBeamLowest) - m);
+  }
+  // the wave's candidates that reach it, at most 64 of them, as keys
+  if (count > 0 && a.tiles > W) {
+    int kept = 0;
+    for (int j = 0; j < count; j += 64) {
+      BeamRaw c{0.f, 0u};
+      bool keep = false;
+      if (j + lane < count) {
+        c = list[j + lane];
+        keep = beam_okey(c.logit) >= last;
+      }
+      const uint64_t b = __ballot(keep);
+      if (keep) list[kept + beam_below(b)] = c;
+      kept = __builtin_amdgcn_readfirstlane(kept + __popcll(b));
+    }
+    count = kept;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (count > a.n_out) {
+    beam_prune(list, count, a.n_out);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    count = a.n_out;
+  }
+  uint64_t mine = 0ull;
+  if (lane < count) {
+    mine = beam_key(list[lane]);
+    reinterpret_cast<uint64_t*>(list)[lane] = mine;
+  }
+  if (lane == 0) redn[wid] = count;
+  __syncthreads();
+  if (tid == 0) {
+    int n = 0;
+    #pragma unroll
+    for (int w = 0; w < W; ++w) n += redn[w];
+    a.parts[slot] = BeamPart{m, s, (uint32_t)min(n, a.n_out), 0u};
+  }
+  // the waves' lists, ranked by counting
+  int rank = 0;
+  #pragma unroll 1
+  for (int w = 0; w < W; ++w) {
+    const int n = redn[w];
+    const uint64_t* other = reinterpret_cast<const uint64_t*>(lists[w]);
+    #pragma unroll 4
+    for (int i = 0; i < n; ++i) rank += other[i] > mine;
+  }
+  if (lane < count && rank < a.n_out) a.cand[slot * a.n_out + rank] = mine;
 }
 
 // A candidate of a request: (score, beam) and (logit, token), both descending
@@ -309,65 +687,93 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
   const int row0 = b * a.K;
   const float ninf = -__builtin_inff();
   if (tid == 0) counter = 0u;
+  // item i: place i % n_out of part (i / n_out) % n_parts of beam i / (n_out * n_parts);
+  // a finished beam has one, in its first place.  Each wave takes items of all
+  // beams, parts and places alike, so that its share of the best ones is even.
+  // The first kFinishHeld a thread are loaded ahead of the beams' sums (places
+  // that hold no candidate are loaded too, and dropped by their part's count).
+  const int first = lane * W + ((wid + lane) & (W - 1));
+  const int per_beam = a.n_parts * a.n_out, total = a.K * per_beam;
+  uint64_t held[kFinishHeld];
+  uint32_t count[kFinishHeld];
+  #pragma unroll
+  for (int h = 0; h < kFinishHeld; ++h) {
+    const int i = first + h * kFinishThreads;
+    held[h] = 0ull;
+    count[h] = 0u;
+    if (i < total) {
+      held[h] = a.cand[(int64_t)row0 * per_beam + i];
+      count[h] = a.parts[(int64_t)row0 * a.n_parts + i / a.n_out].n;
+    }
+  }
   for (int k = wid; k < a.K; k += W) {
     const int row = row0 + k;
     const float c = a.scores[row];
+    const bool fin = a.finished && a.finished[row];
+    const BeamPart* pp = a.parts + (int64_t)row * a.n_parts;
+    float m = ninf, s = 0.f;
+    for (int i = lane; i < a.n_parts; i += 64) {
+      const BeamPart p = pp[i];
+      // (a first pair needs no scaling: m is -inf)
+      const float hi = fmaxf(m, p.m);
+      s = beam_finite(hi) ? s * __expf(m - hi) + p.sum * __expf(p.m - hi) : 0.f;
+      m = hi;
+    }
+    const float top = beam_wave_max(m);
     uint32_t st = 0u;
     float l = 0.f;
     if (beam_finite(c)) {
-      if (a.finished && a.finished[row]) {
+      if (fin) {
         st = 2u;
-      } else {
-        const BeamPart* pp = a.parts + (int64_t)row * a.n_parts;
-        float m = ninf;
-        for (int i = lane; i < a.n_parts; i += 64) m = fmaxf(m, pp[i].m);
-        m = beam_wave_max(m);
-        if (beam_finite(m)) {
-          float s = 0.f;
-          for (int i = lane; i < a.n_parts; i += 64) s += pp[i].sum * __expf(pp[i].m - m);
-          s = beam_wave_sum(s);
-          l = m + logf(s);
-          st = 1u;
-        }
+      } else if (beam_finite(top)) {
+        l = top + logf(beam_wave_sum(s * __expf(m - top)));
+        st = 1u;
       }
     }
     if (lane == 0) { lse[k] = l; state[k] = st; }
   }
   __syncthreads();
-  // item i: place i % n_out of part (i / n_out) % n_parts of beam i / (n_out * n_parts);
-  // a finished beam has one, in its first place
-  const int per_beam = a.n_parts * a.n_out, total = a.K * per_beam;
-  auto item = [&](int i) -> BeamCand {
+  auto rated = [&](int i, uint64_t lo, uint32_t n) -> BeamCand {
     const int k = i / per_beam, r = i - k * per_beam;
     const uint32_t st = state[k];
     BeamCand x{0ull, 0ull};
     if (st == 0u) return x;
-    const int row = row0 + k;
-    float score;
+    float score = a.scores[row0 + k];
     if (st == 2u) {
       if (r != 0) return x;
-      score = a.scores[row];
-      x.lo = 0xffffffffu - a.eos;
+      lo = 0xffffffffu - a.eos;
     } else {
-      const int64_t slot = (int64_t)row * a.n_parts + r / a.n_out;
-      if ((uint32_t)(r % a.n_out) >= a.parts[slot].n) return x;
-      x.lo = a.cand[slot * a.n_out + r % a.n_out];
-      score = a.scores[row] + (beam_okey_inv((uint32_t)(x.lo >> 32)) - lse[k]);
+      if ((uint32_t)(r % a.n_out) >= n) return x;
+      score += beam_okey_inv((uint32_t)(lo >> 32)) - lse[k];
       if (!beam_finite(score)) return x;
     }
+    x.lo = lo;
     x.hi = ((uint64_t)beam_okey(score) << 32) | (0xffffffffu - (uint32_t)k);
     return x;
   };
+  auto item = [&](int i) -> BeamCand {
+    return rated(i, a.cand[(int64_t)row0 * per_beam + i], a.parts[(int64_t)row0 * a.n_parts + i / a.n_out].n);
+  };
   uint32_t best[1] = {0u};
-  for (int i = tid; i < total; i += kFinishThreads) best[0] = max(best[0], (uint32_t)(item(i).hi >> 32));
-  const uint32_t bound = max(beam_bound<1, W>(best, a.n_out, red), 1u);
-  for (int i = tid; i < total; i += kFinishThreads) {
-    const BeamCand x = item(i);
+  BeamCand mine[kFinishHeld];
+  #pragma unroll
+  for (int h = 0; h < kFinishHeld; ++h) {
+    const int i = first + h * kFinishThreads;
+    mine[h] = i < total ? rated(i, held[h], count[h]) : BeamCand{0ull, 0ull};
+    best[0] = max(best[0], (uint32_t)(mine[h].hi >> 32));
+  }
+  for (int i = first + kFinishHeld * kFinishThreads; i < total; i += kFinishThreads)
+    best[0] = max(best[0], (uint32_t)(item(i).hi >> 32));
+  const uint32_t bound = max(beam_bound<1, W>(best, a.n_out, 0u, red), 1u);
+  auto offer = [&](const BeamCand& x) {
     if ((uint32_t)(x.hi >> 32) >= bound) {
       const uint32_t o = atomicAdd(&counter, 1u);
       if (o < (uint32_t)kFinishSlots) slots[o] = x;
     }
-  }
+  };
+  #pragma unroll
+  for (int h = 0; h < kFinishHeld; ++h) offer(mine[h]);
+  for (int i = first + kFinishHeld * kFinishThreads; i < total; i += kFinishThreads) offer(item(i));
   __syncthreads();
   const int n = (int)counter;
   const int64_t o0 = (int64_t)b * a.n_out;
@@ -387,11 +793,11 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
     a.out_finished[o0 + r] = 1;
   }
   if (n <= kFinishSlots) {
-    if (tid < n) {
-      const BeamCand mine = slots[tid];
+    for (int j = tid; j < n; j += kFinishThreads) {
+      const BeamCand x = slots[j];
       int rank = 0;
-      for (int i = 0; i < n; ++i) rank += beam_before(slots[i], mine) ? 1 : 0;
-      if (rank < a.n_out) put(rank, mine);
+      for (int i = 0; i < n; ++i) rank += beam_before(slots[i], x) ? 1 : 0;
+      if (rank < a.n_out) put(rank, x);
     }
     return;
   }
@@ -424,14 +830,25 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
   }
 }
 
-// Elements of a part: large parts once their workgroups fill the chip.
-int beam_part_elems(int64_t rows, int V) {
-  const int64_t large = rows * ((V + 7 + kPartThreads * 64 - 1) / (kPartThreads * 64));
-  return kPartThreads * (large >= 512 ? 64 : 16);
-}
-int beam_parts(int64_t rows, int V) {
-  const int e = beam_part_elems(rows, V);
-  return (V + 7 + e - 1) / e;  // (up to 7 elements before the row's start)
+// How a row is cut: into parts of kTileElems while all rows' parts are few, or
+// into parts of `tiles` streamed tiles (a multiple of four: one a wave) that
+// leave about four workgroups a CU.  Whole steps, us, cut to parts and streamed:
+// 4 rows of 151,936 11.1 and 13.7 (f32), 11.0 and 17.9 (bf16); 128 rows 24.4 and
+// 26.1, 23.6 and 27.9; 256 rows (9,728 parts) 35.5 and 36.4, 34.2 and 34.2; 512
+// rows of bf16, a fifth of them finished, 53 and 47.
+constexpr int kBeamFewParts = 8192;
+struct BeamCut {
+  int tiles;  // 0: parts of kTileElems
+  int parts;
+};
+BeamCut beam_cut(int64_t rows, int V, int dtype) {
+  const int64_t len = (int64_t)V + 7;  // (up to 7 elements before the row's start)
+  const int64_t few = (len + kTileElems - 1) / kTileElems;
+  if (rows * few <= kBeamFewParts) return BeamCut{0, (int)few};
+  const int64_t tile = 64 * (dtype == HI_ROCM_DTYPE_F32 ? 16 : 32), steps = (len + 4 * tile - 1) / (4 * tile);
+  const int64_t want = std::max<int64_t>(1, std::min(steps, (1024 + rows - 1) / rows));
+  const int64_t tiles = 4 * ((steps + want - 1) / want);
+  return BeamCut{(int)tiles, (int)((len + tiles * tile - 1) / (tiles * tile))};
 }
 
 struct BeamLayout {
@@ -446,13 +863,16 @@ BeamLayout beam_layout(int64_t slots, int n_out) {
 }
 
 template <int DT>
-void launch_part(const BeamArgs& a, int rows, int elems, hipStream_t st) {
-  const dim3 grid((unsigned)a.n_parts, (unsigned)rows);
-  if (elems == kPartThreads * 64) hipLaunchKernelGGL((beam_part_kernel<DT, 64>), grid, dim3(kPartThreads), 0, st, a);
-  else hipLaunchKernelGGL((beam_part_kernel<DT, 16>), grid, dim3(kPartThreads), 0, st, a);
+void launch_parts(const BeamArgs& a, int rows, hipStream_t st) {
+  const dim3 grid((unsigned)a.n_parts, (unsigned)rows), threads(kPartThreads);
+  if (a.tiles == 0) hipLaunchKernelGGL(beam_tile_kernel<DT>, grid, threads, 0, st, a);
+  else if (a.mask) hipLaunchKernelGGL((beam_part_kernel<DT, true>), grid, threads, 0, st, a);
+  else hipLaunchKernelGGL((beam_part_kernel<DT, false>), grid, threads, 0, st, a);
 }
 
 // ---- states ---------------------------------------------------------------
+
+typedef uint32_t reorder_u32x4 __attribute__((ext_vector_type(4)));
 
 struct ReorderArgs {
   const char* src;
@@ -462,53 +882,72 @@ struct ReorderArgs {
   int K;
   int64_t outer, mid, positions, pos_bytes;
   int64_t outer_stride, row_stride, mid_stride;
-  int64_t cols;  // units of a row's piece: ceil(positions * pos_bytes / unit)
+  int64_t blocks;  // workgroups of a piece
 };
 
-// One thread owns one unit (16, 4 or 1 bytes) of all K rows of a request: it
+// One thread owns U units (16, 4 or 1 bytes) of all K rows of a request: it
 // reads what the rows need before it writes any of them, so dst may be src.
-template <typename T, int KM>
+// A workgroup stays in one piece (outer and mid index) of one request, so that
+// nothing but the column is divided per thread.
+template <typename T, int KM, int U>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(ReorderArgs a) {
   const int b = blockIdx.y;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.outer * a.mid * a.cols) return;
-  const int64_t piece = i / a.cols, col = i - piece * a.cols;
   int64_t len = a.positions;
   if (a.lengths) {
     const int64_t l = a.lengths[b];
     len = l < 0 ? 0 : (l < len ? l : len);
   }
-  if (col * (int64_t)sizeof(T) >= len * a.pos_bytes) return;
+  const int64_t units = (len * a.pos_bytes + (int64_t)sizeof(T) - 1) / (int64_t)sizeof(T);
+  const int64_t piece = blockIdx.x / (uint32_t)a.blocks, col0 = (int64_t)(blockIdx.x % (uint32_t)a.blocks) * (256 * U);
+  if (col0 >= units) return;
   const int64_t o = piece / a.mid, m = piece - o * a.mid;
-  const int64_t at = o * a.outer_stride + m * a.mid_stride + (int64_t)b * a.K * a.row_stride + col * (int64_t)sizeof(T);
+  const int64_t at = o * a.outer_stride + m * a.mid_stride + (int64_t)b * a.K * a.row_stride;
+  const T* src = reinterpret_cast<const T*>(a.src + at) + col0 + threadIdx.x;
+  T* dst = reinterpret_cast<T*>(a.dst + at) + col0 + threadIdx.x;
+  const int64_t row = a.row_stride / (int64_t)sizeof(T);
   const bool same = a.src == a.dst;
-  T v[KM];
-  int from[KM];
+  bool in[U];
+  #pragma unroll
+  for (int u = 0; u < U; ++u) in[u] = col0 + u * 256 + (int)threadIdx.x < units;
+  T v[KM][U];
+  bool moves[KM];
   #pragma unroll
   for (int j = 0; j < KM; ++j) {
-    from[j] = -1;
+    moves[j] = false;
     if (j < a.K) {
       const int p = a.parents[b * a.K + j];
       const int q = p < 0 || p >= a.K ? j : p;  // (a parent outside the request: the row stays)
-      if (!same || q != j) {
-        from[j] = q;
-        v[j] = *reinterpret_cast<const T*>(a.src + at + q * a.row_stride);
+      moves[j] = !same || q != j;
+      if (moves[j]) {
+        #pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (in[u]) v[j][u] = src[q * row + u * 256];
       }
     }
   }
   #pragma unroll
   for (int j = 0; j < KM; ++j)
-    if (from[j] >= 0) *reinterpret_cast<T*>(a.dst + at + j * a.row_stride) = v[j];
+    if (moves[j]) {
+      #pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (in[u]) dst[j * row + u * 256] = v[j][u];
+    }
+}
+
+template <typename T, int KM, int U>
+void launch_reorder_rows(ReorderArgs a, int batch, hipStream_t st) {
+  const int64_t units = (a.positions * a.pos_bytes + (int64_t)sizeof(T) - 1) / (int64_t)sizeof(T);
+  a.blocks = (units + 256 * U - 1) / (256 * U);
+  const dim3 grid((unsigned)(a.outer * a.mid * a.blocks), (unsigned)batch);
+  hipLaunchKernelGGL((beam_reorder_kernel<T, KM, U>), grid, dim3(256), 0, st, a);
 }
 
 template <typename T>
-void launch_reorder(ReorderArgs a, int batch, hipStream_t st) {
-  a.cols = (a.positions * a.pos_bytes + (int64_t)sizeof(T) - 1) / (int64_t)sizeof(T);
-  const dim3 grid((unsigned)((a.outer * a.mid * a.cols + 255) / 256), (unsigned)batch);
-  if (a.K <= 4) hipLaunchKernelGGL((beam_reorder_kernel<T, 4>), grid, dim3(256), 0, st, a);
-  else if (a.K <= 8) hipLaunchKernelGGL((beam_reorder_kernel<T, 8>), grid, dim3(256), 0, st, a);
-  else if (a.K <= 16) hipLaunchKernelGGL((beam_reorder_kernel<T, 16>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((beam_reorder_kernel<T, 32>), grid, dim3(256), 0, st, a);
+void launch_reorder(const ReorderArgs& a, int batch, hipStream_t st) {
+  if (a.K <= 4) launch_reorder_rows<T, 4, 4>(a, batch, st);
+  else if (a.K <= 8) launch_reorder_rows<T, 8, 2>(a, batch, st);
+  else if (a.K <= 16) launch_reorder_rows<T, 16, 1>(a, batch, st);
+  else launch_reorder_rows<T, 32, 1>(a, batch, st);
 }
 
 }  // namespace
@@ -526,7 +965,8 @@ int hi_rocm_beam_workspace_bytes(int max_batch, int beams, int vocab, int n_out,
                     "hi_rocm_beam_workspace_bytes: more than 32 beams, 64 outputs, 65536 rows or 2^23 tokens");
   int64_t slots = 0;
   for (int b = 1; b <= max_batch; ++b)
-    slots = std::max(slots, (int64_t)b * beams * beam_parts((int64_t)b * beams, vocab));
+    for (int dtype : {HI_ROCM_DTYPE_F32, HI_ROCM_DTYPE_BF16})
+      slots = std::max(slots, (int64_t)b * beams * beam_cut((int64_t)b * beams, vocab, dtype).parts);
   *out_bytes = beam_layout(slots, n_out).total;
   return HI_ROCM_OK;
 }
@@ -551,7 +991,9 @@ int hi_rocm_beam_select(const void* logits, int dtype, int batch, int beams, int
   const int rows = batch * beams;
   BeamArgs a;
   memset(&a, 0, sizeof(a));
-  a.n_parts = beam_parts(rows, vocab);
+  const BeamCut cut = beam_cut(rows, vocab, dtype);
+  a.tiles = cut.tiles;
+  a.n_parts = cut.parts;
   const BeamLayout L = beam_layout((int64_t)rows * a.n_parts, n_out);
   if (workspace == nullptr || workspace_bytes < L.total || (uintptr_t)workspace % 16 != 0)
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_beam_select: workspace missing, too small or not 16-byte aligned");
@@ -571,9 +1013,8 @@ int hi_rocm_beam_select(const void* logits, int dtype, int batch, int beams, int
   a.out_tokens = out_tokens;
   a.out_parents = out_parents;
   a.out_finished = out_finished;
-  const int elems = beam_part_elems(rows, vocab);
-  if (dtype == HI_ROCM_DTYPE_F32) launch_part<HI_ROCM_DTYPE_F32>(a, rows, elems, (hipStream_t)stream);
-  else launch_part<HI_ROCM_DTYPE_BF16>(a, rows, elems, (hipStream_t)stream);
+  if (dtype == HI_ROCM_DTYPE_F32) launch_parts<HI_ROCM_DTYPE_F32>(a, rows, (hipStream_t)stream);
+  else launch_parts<HI_ROCM_DTYPE_BF16>(a, rows, (hipStream_t)stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return api_hip_fail(e, "beam part launch");
   hipLaunchKernelGGL(beam_finish_kernel, dim3((unsigned)batch), dim3(kFinishThreads), 0, (hipStream_t)stream, a);
@@ -627,9 +1068,9 @@ int hi_rocm_beam_reorder(const void* src, void* dst, const int32_t* parents, int
   const uint64_t bits = s | t | (uint64_t)a.outer_stride | (uint64_t)a.row_stride | (uint64_t)a.mid_stride |
                         (uint64_t)pos_bytes;
   const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
-  if ((outer * mid * ((piece + unit - 1) / unit) + 255) / 256 > INT32_MAX)
-    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_beam_reorder: more than 2^39 units a request");
-  if (unit == 16) launch_reorder<int4>(a, batch, (hipStream_t)stream);
+  if (outer * mid > INT32_MAX || outer * mid * (((piece + unit - 1) / unit + 255) / 256) > INT32_MAX)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_beam_reorder: more than 2^31 pieces of 256 units a request");
+  if (unit == 16) launch_reorder<reorder_u32x4>(a, batch, (hipStream_t)stream);
   else if (unit == 4) launch_reorder<uint32_t>(a, batch, (hipStream_t)stream);
   else launch_reorder<uint8_t>(a, batch, (hipStream_t)stream);
   const hipError_t e = hipGetLastError();
