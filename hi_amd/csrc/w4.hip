@@ -22,10 +22,14 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "hi_rocm.h"
 #include "sampler_internal.h"
 
 namespace hi_rocm {
+hipError_t ensure_lds(const void* fn, size_t bytes);  // sampler_chunked.hip
+
 namespace {
 
 typedef __bf16 w4_bf16x8 __attribute__((ext_vector_type(8)));
@@ -33,7 +37,7 @@ typedef float w4_f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t w4_u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kW4Block = 128;   // inputs of a block
-constexpr int kW4Waves = 4;     // waves of a workgroup, splitting k
+constexpr int kW4Waves = 8;     // waves of a workgroup, splitting k
 
 struct W4Layout {
   int64_t n_tiles, k_blocks;
@@ -100,118 +104,234 @@ struct W4Args {
   int n_tiles, k_blocks;
 };
 
-// The eight weights of a word as 16 + q in bf16.
-__device__ __forceinline__ w4_bf16x8 w4_unpack(uint32_t w) {
-  w4_u32x4 v;
-  v[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
-  v[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-  v[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-  v[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+// The eight weights of a word as 16 + q in bf16: a shift and an and-or for two.
+// (`mask` and `sixteens` are 0x00780078 and 0x41804180, a scalar and a vector
+// register to the compiler: as literals neither would fit the and-or.)
+__device__ __forceinline__ w4_bf16x8 w4_unpack(uint32_t w, uint32_t mask, uint32_t sixteens) {
+  const w4_u32x4 v = {((w << 3) & mask) | sixteens, ((w >> 1) & mask) | sixteens, ((w >> 5) & mask) | sixteens,
+                      ((w >> 9) & mask) | sixteens};
   return __builtin_bit_cast(w4_bf16x8, v);
 }
 
-template <typename T>
-__device__ __forceinline__ float w4_float(T v) { return (float)v; }
+// The scales (or zeros) that a lane needs of a block: those of its output, as
+// one load.
+template <typename ST, int GPB>
+struct W4Scales {
+  typedef ST vec __attribute__((ext_vector_type(GPB)));
+  vec v;
+  __device__ __forceinline__ void load(const void* p, int64_t block, int r) {
+    v = *reinterpret_cast<const vec*>((const ST*)p + (block * 16 + r) * GPB);
+  }
+  __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
+};
+template <typename ST>
+struct W4Scales<ST, 1> {
+  ST v;
+  __device__ __forceinline__ void load(const void* p, int64_t block, int r) { v = ((const ST*)p)[block * 16 + r]; }
+  __device__ __forceinline__ float get(int) const { return (float)v; }
+};
 
-// MT tiles of 16 rows times one tile of 16 outputs; the workgroup's waves
-// split the blocks of k, and their sums are added in wave order.
+// A workgroup of eight waves takes groups of T tiles of 16 outputs, 16 MT rows
+// of x.  Its waves split k: in a pass each owns BPW blocks, whose part of x it
+// holds in registers while the weights of tile after tile stream past, R steps
+// (a step: a wave's BPW blocks of one tile) ahead, from group to group without
+// a pause.  So a weight is read once, nothing but weights is read in the loop
+// (x again in every pass, where k is longer than one), and the waves meet once
+// a group to add their sums, in wave order, through LDS.
+// MQ = 1: one row of x; of the four rows a lane's results hold only the first
+// is kept.
 // MFMA 16x16x32 bf16 (lane l = 16 g + r): A row r, elements 8 g .. 8 g + 7;
-// B column r, the same elements; D rows 4 g .. 4 g + 3 of column r.
-template <int MT, int G, typename ST>
+// B column r, the same elements; D rows 4 g .. 4 g + 3 of column r.  Rows past
+// the last repeat it and are dropped.
+template <int MT, int MQ, int T, int BPW, int R, int G, typename ST>
 __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
   constexpr int GPB = kW4Block / G, CH = G / 32;  // groups a block, MFMAs a group
-  __shared__ float part[kW4Waves - 1][MT * 4][64];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int nt = blockIdx.x, m0 = blockIdx.y * (16 * MT);
-  const int per = (a.k_blocks + kW4Waves - 1) / kW4Waves;
-  const int kb0 = wid * per, kb1 = min(kb0 + per, a.k_blocks);
+  static_assert(T == 1 || R == T, "a step's tile is its ring slot");
+  extern __shared__ __align__(16) float w4_part[];
+  typedef float sums __attribute__((ext_vector_type(MQ)));
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int groups = (a.n_tiles + T - 1) / T;
+  const int passes = (a.k_blocks + kW4Waves * BPW - 1) / (kW4Waves * BPW);
+  const int m0 = blockIdx.y * (16 * MT);
   const __bf16* xr[MT];
   #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int m = m0 + 16 * t + r;
-    xr[t] = a.x + (int64_t)(m < a.rows ? m : 0) * a.x_stride;
-  }
+  for (int m = 0; m < MT; ++m) xr[m] = a.x + (int64_t)min(m0 + 16 * m + r, a.rows - 1) * a.x_stride + 8 * g;
   w4_bf16x8 ones;
   #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
-  w4_f32x4 acc[MT];
-  #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
-  const ST* sp = (const ST*)a.scales;
-  const ST* zp = (const ST*)a.zeros;
-  for (int kb = kb0; kb < kb1; ++kb) {
-    const int64_t block = (int64_t)nt * a.k_blocks + kb;
-    const w4_u32x4 w = *reinterpret_cast<const w4_u32x4*>(a.q + block * 256 + lane * 4);
-    float s[GPB], z[GPB];
+
+  uint32_t mask = 0x00780078u, sixteens = 0x41804180u;
+  asm volatile("" : "+s"(mask), "+v"(sixteens));
+
+  w4_u32x4 wv[R][BPW];
+  W4Scales<ST, GPB> sv[R][BPW], zv[R][BPW];
+  // the step to load next: tile t of a group, in a pass
+  int lg = blockIdx.x, lp = 0, lt = 0;
+  auto load = [&](int slot) {
+    const int nt = min(lg * T + lt, a.n_tiles - 1);  // (past the last step: loads that nothing uses)
     #pragma unroll
-    for (int j = 0; j < GPB; ++j) {
-      s[j] = w4_float(sp[(block * 16 + r) * GPB + j]);
-      z[j] = 16.f + (zp ? w4_float(zp[(block * 16 + r) * GPB + j]) : 8.f);
+    for (int i = 0; i < BPW; ++i) {
+      const int64_t block = (int64_t)nt * a.k_blocks + min((lp * kW4Waves + wid) * BPW + i, a.k_blocks - 1);
+      wv[slot][i] = *reinterpret_cast<const w4_u32x4*>(a.q + block * 256 + lane * 4);
+      sv[slot][i].load(a.scales, block, r);
+      if (a.zeros) zv[slot][i].load(a.zeros, block, r);
     }
-    w4_bf16x8 b[4];
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = w4_unpack(w[i]);
-    #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      #pragma unroll
-      for (int j = 0; j < GPB; ++j) {
-        w4_f32x4 d = {0.f, 0.f, 0.f, 0.f}, e = {0.f, 0.f, 0.f, 0.f};
-        #pragma unroll
-        for (int i = j * CH; i < (j + 1) * CH; ++i) {
-          const int kk = kb * kW4Block + 32 * i + 8 * g;
-          w4_bf16x8 xa = {};
-          if (kk < a.k) xa = *reinterpret_cast<const w4_bf16x8*>(xr[t] + kk);
-          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, b[i], d, 0, 0, 0);
-          e = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa, ones, e, 0, 0, 0);
-        }
-        #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[t][q] = fmaf(s[j], fmaf(-z[j], e[q], d[q]), acc[t][q]);
+    if (++lt == T) {
+      lt = 0;
+      if (++lp == passes) {
+        lp = 0;
+        lg += gridDim.x;
       }
     }
-  }
-  if (wid > 0) {
+  };
+  w4_bf16x8 xf[BPW][4][MT];
+  auto load_x = [&](int pass) {
     #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int i = 0; i < BPW; ++i) {
       #pragma unroll
-      for (int q = 0; q < 4; ++q) part[wid - 1][t * 4 + q][lane] = acc[t][q];
-  }
-  __syncthreads();
-  if (wid > 0) return;
-  const int n = nt * 16 + r;
-  if (n >= a.n) return;
-  const float bias = a.bias ? a.bias[n] : 0.f;
+      for (int j = 0; j < 4; ++j) {
+        const int k = ((pass * kW4Waves + wid) * BPW + i) * kW4Block + 32 * j;
+        // (in steps of 32, k is inside or outside as a whole; every load is made)
+        const uint32_t in = k < a.k ? ~0u : 0u;
+        #pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const w4_u32x4 v = *reinterpret_cast<const w4_u32x4*>(xr[m] + min(k, a.k - 32));
+          xf[i][j][m] = __builtin_bit_cast(w4_bf16x8, v & in);
+        }
+      }
+    }
+  };
+  sums acc[T][MT];
+  auto clear = [&]() {
+    #pragma unroll
+    for (int t = 0; t < T; ++t)
+      #pragma unroll
+      for (int m = 0; m < MT; ++m)
+        #pragma unroll
+        for (int q = 0; q < MQ; ++q) acc[t][m][q] = 0.f;
+  };
+  auto multiply = [&](int slot, int t) {
+    #pragma unroll
+    for (int i = 0; i < BPW; ++i) {
+      // (Block after block: all blocks' products at once would not fit the
+      // registers, nor would the sums of x, which are the same for every tile.)
+      asm volatile("" : "+v"(ones), "+v"(wv[slot][i]));
+      #pragma unroll
+      for (int j = 0; j < GPB; ++j) {
+        const float s = sv[slot][i].get(j);
+        const float z = a.zeros ? 16.f + zv[slot][i].get(j) : 24.f;
+        w4_f32x4 d[MT], e[MT];
+        #pragma unroll
+        for (int m = 0; m < MT; ++m) d[m] = e[m] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int c = j * CH; c < (j + 1) * CH; ++c) {
+          const w4_bf16x8 b = w4_unpack(wv[slot][i][c], mask, sixteens);
+          #pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            d[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i][c][m], b, d[m], 0, 0, 0);
+            e[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i][c][m], ones, e[m], 0, 0, 0);
+          }
+        }
+        #pragma unroll
+        for (int m = 0; m < MT; ++m)
+          #pragma unroll
+          for (int q = 0; q < MQ; ++q) acc[t][m][q] = fmaf(s, fmaf(-z, e[m][q], d[m][q]), acc[t][m][q]);
+      }
+      #pragma unroll
+      for (int m = 0; m < MT; ++m)
+        #pragma unroll
+        for (int q = 0; q < MQ; ++q) {
+          float v = acc[t][m][q];
+          asm volatile("" : "+v"(v));
+          acc[t][m][q] = v;
+        }
+    }
+  };
+  auto finish = [&](int grp) {
+    sums* part = reinterpret_cast<sums*>(w4_part);
+    #pragma unroll
+    for (int t = 0; t < T; ++t)
+      #pragma unroll
+      for (int m = 0; m < MT; ++m) part[((wid * T + t) * MT + m) * 64 + lane] = acc[t][m];
+    __syncthreads();
+    for (int i = threadIdx.x; i < T * MT * 64; i += 64 * kW4Waves) {
+      const int l = i & 63, m = i / 64 % MT, t = i / 64 / MT;
+      const int n = (grp * T + t) * 16 + (l & 15), row = m0 + 16 * m + 4 * (l >> 4);
+      if (n >= a.n || row >= a.rows) continue;
+      sums y = part[i];
+      #pragma unroll
+      for (int w = 1; w < kW4Waves; ++w) y += part[w * T * MT * 64 + i];
+      const float bias = a.bias ? a.bias[n] : 0.f;
+      #pragma unroll
+      for (int q = 0; q < MQ; ++q) {
+        if (row + q >= a.rows) break;
+        const float v = a.bias ? y[q] + bias : y[q];
+        const int64_t at = (int64_t)(row + q) * a.out_stride + n;
+        if (a.out_bf16) ((__bf16*)a.out)[at] = (__bf16)v;
+        else ((float*)a.out)[at] = v;
+      }
+    }
+    __syncthreads();
+  };
+
   #pragma unroll
-  for (int t = 0; t < MT; ++t) {
+  for (int s = 0; s < R; ++s) load(s);
+  load_x(0);
+  clear();
+  int grp = blockIdx.x, pass = 0;
+  while (grp < groups) {
     #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int m = m0 + 16 * t + 4 * g + q;
-      if (m >= a.rows) continue;
-      float y = acc[t][q];
-      #pragma unroll
-      for (int w = 0; w < kW4Waves - 1; ++w) y += part[w][t * 4 + q][lane];
-      if (a.bias) y += bias;
-      if (a.out_bf16) ((__bf16*)a.out)[(int64_t)m * a.out_stride + n] = (__bf16)y;
-      else ((float*)a.out)[(int64_t)m * a.out_stride + n] = y;
+    for (int s = 0; s < R; ++s) {
+      const int t = T == 1 ? 0 : s;
+      if (grp < groups) {
+        if (passes > 1 && t == 0) load_x(pass);
+        multiply(s, t);
+        load(s);
+        if (t == T - 1 && ++pass == passes) {
+          finish(grp);
+          clear();
+          pass = 0;
+          grp += gridDim.x;
+        }
+      }
     }
   }
 }
 
-template <int MT, int G, typename ST>
-void launch_w4(const W4Args& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.n_tiles, (unsigned)((a.rows + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((w4_linear_kernel<MT, G, ST>), grid, dim3(64 * kW4Waves), 0, st, a);
+template <int MT, int MQ, int T, int BPW, int R, int G, typename ST>
+hipError_t launch_w4(const W4Args& a, hipStream_t st) {
+  const size_t bytes = (size_t)kW4Waves * T * MT * 64 * MQ * sizeof(float);
+  auto* kernel = w4_linear_kernel<MT, MQ, T, BPW, R, G, ST>;
+  const hipError_t e = ensure_lds((const void*)kernel, bytes);
+  if (e != hipSuccess) return e;
+  // one workgroup a CU stays and takes every 256th group
+  const int groups = (a.n_tiles + T - 1) / T;
+  const dim3 grid((unsigned)std::min(groups, 256), (unsigned)((a.rows + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * kW4Waves), bytes, st, a);
+  return hipGetLastError();
 }
 template <int G, typename ST>
-void launch_w4_rows(const W4Args& a, hipStream_t st) {
-  if (a.rows <= 16) launch_w4<1, G, ST>(a, st);
-  else if (a.rows <= 32) launch_w4<2, G, ST>(a, st);
-  else launch_w4<4, G, ST>(a, st);
+hipError_t launch_w4_rows(const W4Args& a, hipStream_t st) {
+  constexpr int R = G == 32 ? 2 : 3;
+  if (a.rows == 1) {
+    if (a.k_blocks <= 8) return launch_w4<1, 1, 1, 1, R, G, ST>(a, st);
+    if (a.k_blocks <= 16) return launch_w4<1, 1, 1, 2, R, G, ST>(a, st);
+    return launch_w4<1, 1, 1, 4, R, G, ST>(a, st);
+  }
+  if (a.rows <= 16) {
+    if (a.k_blocks <= 8) return launch_w4<1, 4, 1, 1, R, G, ST>(a, st);
+    if (a.k_blocks <= 16) return launch_w4<1, 4, 1, 2, R, G, ST>(a, st);
+    return launch_w4<1, 4, 1, 4, R, G, ST>(a, st);
+  }
+  if (a.rows <= 32) return launch_w4<2, 4, 4, 2, 4, G, ST>(a, st);
+  return launch_w4<4, 4, 4, 1, 4, G, ST>(a, st);
 }
 template <typename ST>
-void launch_w4_group(const W4Args& a, int group, hipStream_t st) {
-  if (group == 32) launch_w4_rows<32, ST>(a, st);
-  else if (group == 64) launch_w4_rows<64, ST>(a, st);
-  else launch_w4_rows<128, ST>(a, st);
+hipError_t launch_w4_group(const W4Args& a, int group, hipStream_t st) {
+  if (group == 32) return launch_w4_rows<32, ST>(a, st);
+  if (group == 64) return launch_w4_rows<64, ST>(a, st);
+  return launch_w4_rows<128, ST>(a, st);
 }
 
 // Sizes and types of a packed weight: HI_ROCM_OK, or a status with a message.
@@ -308,9 +428,8 @@ int hi_rocm_w4_linear(const void* x, int rows, int64_t x_stride, const void* pac
   a.out_bf16 = out_dtype == HI_ROCM_DTYPE_BF16;
   a.n_tiles = (int)L.n_tiles;
   a.k_blocks = (int)L.k_blocks;
-  if (scale_dtype == HI_ROCM_DTYPE_BF16) launch_w4_group<__bf16>(a, group, (hipStream_t)stream);
-  else launch_w4_group<float>(a, group, (hipStream_t)stream);
-  const hipError_t e = hipGetLastError();
+  const hipError_t e = scale_dtype == HI_ROCM_DTYPE_BF16 ? launch_w4_group<__bf16>(a, group, (hipStream_t)stream)
+                                                         : launch_w4_group<float>(a, group, (hipStream_t)stream);
   return e == hipSuccess ? HI_ROCM_OK : api_hip_fail(e, "w4 linear launch");
 }
 
