@@ -138,29 +138,35 @@ struct W4Scales<ST, 1> {
 // a pause.  So a weight is read once, nothing but weights is read in the loop
 // (x again in every pass, where k is longer than one), and the waves meet once
 // a group to add their sums, in wave order, through LDS.
+//
+// A group's e does not depend on the output: each wave makes it once a pass (a
+// product with ones) and keeps -24 e (-e with zeros) in LDS.  What goes into the
+// sum, s (d - (16 + z) e), follows one group behind, while the next group's
+// product runs.  (Products that start from -24 e would save an addition, but
+// weights of 0 would then not give 0.)
 // MQ = 1: one row of x; of the four rows a lane's results hold only the first
 // is kept.
 // MFMA 16x16x32 bf16 (lane l = 16 g + r): A row r, elements 8 g .. 8 g + 7;
 // B column r, the same elements; D rows 4 g .. 4 g + 3 of column r.  Rows past
 // the last repeat it and are dropped.
-template <int MT, int MQ, int T, int BPW, int R, int G, typename ST>
+template <int MT, int MQ, int T, int BPW, int R, int G, bool ZEROS, typename ST>
 __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
   constexpr int GPB = kW4Block / G, CH = G / 32;  // groups a block, MFMAs a group
+  constexpr int PART = kW4Waves * T * MT * 64;    // values of the waves' sums
+  constexpr bool TWO = MT == 1;                   // two buffers of them
   static_assert(T == 1 || R == T, "a step's tile is its ring slot");
-  extern __shared__ __align__(16) float w4_part[];
+  extern __shared__ __align__(16) float w4_lds[];
   typedef float sums __attribute__((ext_vector_type(MQ)));
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int groups = (a.n_tiles + T - 1) / T;
   const int passes = (a.k_blocks + kW4Waves * BPW - 1) / (kW4Waves * BPW);
   const int m0 = blockIdx.y * (16 * MT);
+  // this wave's e: [block][group][row tile][g] of four rows
+  w4_f32x4* ex = reinterpret_cast<w4_f32x4*>(w4_lds + (TWO ? 2 : 1) * PART * MQ) + wid * (BPW * GPB * MT * 4) + g;
   const __bf16* xr[MT];
   #pragma unroll
   for (int m = 0; m < MT; ++m) xr[m] = a.x + (int64_t)min(m0 + 16 * m + r, a.rows - 1) * a.x_stride + 8 * g;
-  w4_bf16x8 ones;
-  #pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
-
   uint32_t mask = 0x00780078u, sixteens = 0x41804180u;
   asm volatile("" : "+s"(mask), "+v"(sixteens));
 
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
       const int64_t block = (int64_t)nt * a.k_blocks + min((lp * kW4Waves + wid) * BPW + i, a.k_blocks - 1);
       wv[slot][i] = *reinterpret_cast<const w4_u32x4*>(a.q + block * 256 + lane * 4);
       sv[slot][i].load(a.scales, block, r);
-      if (a.zeros) zv[slot][i].load(a.zeros, block, r);
+      if (ZEROS) zv[slot][i].load(a.zeros, block, r);
     }
     if (++lt == T) {
       lt = 0;
@@ -201,6 +207,24 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
         }
       }
     }
+    w4_bf16x8 ones;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
+    #pragma unroll
+    for (int i = 0; i < BPW; ++i) {
+      #pragma unroll
+      for (int j = 0; j < GPB; ++j) {
+        #pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          w4_f32x4 e = {0.f, 0.f, 0.f, 0.f};
+          #pragma unroll
+          for (int c = j * CH; c < (j + 1) * CH; ++c)
+            e = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i][c][m], ones, e, 0, 0, 0);
+          if (r == 0) ex[((i * GPB + j) * MT + m) * 4] = ZEROS ? -e : -24.f * e;
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
   sums acc[T][MT];
   auto clear = [&]() {
@@ -212,44 +236,48 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
         for (int q = 0; q < MQ; ++q) acc[t][m][q] = 0.f;
   };
   auto multiply = [&](int slot, int t) {
-    #pragma unroll
-    for (int i = 0; i < BPW; ++i) {
-      // (Block after block: all blocks' products at once would not fit the
-      // registers, nor would the sums of x, which are the same for every tile.)
-      asm volatile("" : "+v"(ones), "+v"(wv[slot][i]));
-      #pragma unroll
-      for (int j = 0; j < GPB; ++j) {
-        const float s = sv[slot][i].get(j);
-        const float z = a.zeros ? 16.f + zv[slot][i].get(j) : 24.f;
-        w4_f32x4 d[MT], e[MT];
-        #pragma unroll
-        for (int m = 0; m < MT; ++m) d[m] = e[m] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
-        #pragma unroll
-        for (int c = j * CH; c < (j + 1) * CH; ++c) {
-          const w4_bf16x8 b = w4_unpack(wv[slot][i][c], mask, sixteens);
-          #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            d[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i][c][m], b, d[m], 0, 0, 0);
-            e[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i][c][m], ones, e[m], 0, 0, 0);
-          }
-        }
-        #pragma unroll
-        for (int m = 0; m < MT; ++m)
-          #pragma unroll
-          for (int q = 0; q < MQ; ++q) acc[t][m][q] = fmaf(s, fmaf(-z, e[m][q], d[m][q]), acc[t][m][q]);
-      }
+    w4_f32x4 d[2][MT], e[2][MT];
+    float s[2], z[2];
+    auto add = [&](int p) {
       #pragma unroll
       for (int m = 0; m < MT; ++m)
         #pragma unroll
         for (int q = 0; q < MQ; ++q) {
-          float v = acc[t][m][q];
+          // (group after group: all at once would not fit the registers)
+          const float w = ZEROS ? fmaf(z[p], e[p][m][q], d[p][m][q]) : d[p][m][q] + e[p][m][q];
+          float v = fmaf(s[p], w, acc[t][m][q]);
           asm volatile("" : "+v"(v));
           acc[t][m][q] = v;
         }
+    };
+    #pragma unroll
+    for (int i = 0; i < BPW; ++i) {
+      asm volatile("" : "+v"(wv[slot][i]));
+      #pragma unroll
+      for (int j = 0; j < GPB; ++j) {
+        const int p = (i * GPB + j) & 1;
+        s[p] = sv[slot][i].get(j);
+        if (ZEROS) z[p] = 16.f + zv[slot][i].get(j);
+        #pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          e[p][m] = ex[((i * GPB + j) * MT + m) * 4];
+          d[p][m] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        #pragma unroll
+        for (int c = j * CH; c < (j + 1) * CH; ++c) {
+          const w4_bf16x8 b = w4_unpack(wv[slot][i][c], mask, sixteens);
+          #pragma unroll
+          for (int m = 0; m < MT; ++m)
+            d[p][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i][c][m], b, d[p][m], 0, 0, 0);
+        }
+        if (i + j > 0) add(p ^ 1);
+      }
     }
+    add((BPW * GPB - 1) & 1);
   };
+  int buffer = 0;
   auto finish = [&](int grp) {
-    sums* part = reinterpret_cast<sums*>(w4_part);
+    sums* part = reinterpret_cast<sums*>(w4_lds) + buffer * PART;
     #pragma unroll
     for (int t = 0; t < T; ++t)
       #pragma unroll
@@ -272,7 +300,9 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
         else ((float*)a.out)[at] = v;
       }
     }
-    __syncthreads();
+    // (with two buffers the next group's barrier keeps the one after it off this one)
+    if (TWO) buffer ^= 1;
+    else __syncthreads();
   };
 
   #pragma unroll
@@ -299,10 +329,11 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
   }
 }
 
-template <int MT, int MQ, int T, int BPW, int R, int G, typename ST>
+template <int MT, int MQ, int T, int BPW, int R, int G, bool ZEROS, typename ST>
 hipError_t launch_w4(const W4Args& a, hipStream_t st) {
-  const size_t bytes = (size_t)kW4Waves * T * MT * 64 * MQ * sizeof(float);
-  auto* kernel = w4_linear_kernel<MT, MQ, T, BPW, R, G, ST>;
+  const size_t bytes = (size_t)kW4Waves * sizeof(float) *
+                       ((MT == 1 ? 2 : 1) * T * MT * 64 * MQ + BPW * (kW4Block / G) * MT * 16);
+  auto* kernel = w4_linear_kernel<MT, MQ, T, BPW, R, G, ZEROS, ST>;
   const hipError_t e = ensure_lds((const void*)kernel, bytes);
   if (e != hipSuccess) return e;
   // one workgroup a CU stays and takes every 256th group
@@ -311,27 +342,33 @@ hipError_t launch_w4(const W4Args& a, hipStream_t st) {
   hipLaunchKernelGGL(kernel, grid, dim3(64 * kW4Waves), bytes, st, a);
   return hipGetLastError();
 }
-template <int G, typename ST>
+template <int MQ, int G, bool ZEROS, typename ST>
+hipError_t launch_w4_tile(const W4Args& a, hipStream_t st) {
+  if (a.n_tiles < 512) {  // less than two tiles a CU
+    if (a.k_blocks <= 8) return launch_w4<1, MQ, 1, 1, 3, G, ZEROS, ST>(a, st);
+    if (a.k_blocks <= 16) return launch_w4<1, MQ, 1, 2, 3, G, ZEROS, ST>(a, st);
+    return launch_w4<1, MQ, 1, 4, 2, G, ZEROS, ST>(a, st);
+  }
+  if (a.k_blocks <= 8) return launch_w4<1, MQ, 4, 1, 4, G, ZEROS, ST>(a, st);
+  if (a.k_blocks <= 16) return launch_w4<1, MQ, 4, 2, 4, G, ZEROS, ST>(a, st);
+  return launch_w4<1, MQ, 2, 4, 2, G, ZEROS, ST>(a, st);
+}
+template <int G, bool ZEROS, typename ST>
 hipError_t launch_w4_rows(const W4Args& a, hipStream_t st) {
-  constexpr int R = G == 32 ? 2 : 3;
-  if (a.rows == 1) {
-    if (a.k_blocks <= 8) return launch_w4<1, 1, 1, 1, R, G, ST>(a, st);
-    if (a.k_blocks <= 16) return launch_w4<1, 1, 1, 2, R, G, ST>(a, st);
-    return launch_w4<1, 1, 1, 4, R, G, ST>(a, st);
-  }
-  if (a.rows <= 16) {
-    if (a.k_blocks <= 8) return launch_w4<1, 4, 1, 1, R, G, ST>(a, st);
-    if (a.k_blocks <= 16) return launch_w4<1, 4, 1, 2, R, G, ST>(a, st);
-    return launch_w4<1, 4, 1, 4, R, G, ST>(a, st);
-  }
-  if (a.rows <= 32) return launch_w4<2, 4, 4, 2, 4, G, ST>(a, st);
-  return launch_w4<4, 4, 4, 1, 4, G, ST>(a, st);
+  if (a.rows == 1) return launch_w4_tile<1, G, ZEROS, ST>(a, st);
+  if (a.rows <= 16) return launch_w4_tile<4, G, ZEROS, ST>(a, st);
+  if (a.rows <= 32) return launch_w4<2, 4, 4, 2, 4, G, ZEROS, ST>(a, st);
+  return launch_w4<4, 4, 4, 1, 4, G, ZEROS, ST>(a, st);
+}
+template <int G, typename ST>
+hipError_t launch_w4_zeros(const W4Args& a, hipStream_t st) {
+  return a.zeros ? launch_w4_rows<G, true, ST>(a, st) : launch_w4_rows<G, false, ST>(a, st);
 }
 template <typename ST>
 hipError_t launch_w4_group(const W4Args& a, int group, hipStream_t st) {
-  if (group == 32) return launch_w4_rows<32, ST>(a, st);
-  if (group == 64) return launch_w4_rows<64, ST>(a, st);
-  return launch_w4_rows<128, ST>(a, st);
+  if (group == 32) return launch_w4_zeros<32, ST>(a, st);
+  if (group == 64) return launch_w4_zeros<64, ST>(a, st);
+  return launch_w4_zeros<128, ST>(a, st);
 }
 
 // Sizes and types of a packed weight: HI_ROCM_OK, or a status with a message.
