@@ -14,7 +14,19 @@ import torch
 
 from . import _lib
 from ._lib import check, load
-from .sampler import _stream_ptr
+
+
+_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+# The checks below run before every call, next to kernels of a few
+# microseconds: torch.cuda.current_stream() alone takes 2.7 us, comparing two
+# torch.device objects more than their indexes.
+
+def _stream(stream: Optional[torch.cuda.Stream]) -> int:
+    """The handle of ``stream``, or of the current device's current one."""
+    return _raw_stream(_current_device()) if stream is None else stream.cuda_stream
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -29,18 +41,22 @@ def _empty(shape, dtype, device, stream: Optional[torch.cuda.Stream]) -> torch.T
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _same_device(what: str, dev: torch.device, **tensors) -> None:
-    if dev.type != "cuda":
+def _on(what: str, dev: int, *tensors: Optional[torch.Tensor]) -> None:
+    """All tensors on CUDA device ``dev``."""
+    if dev < 0:
         raise ValueError(f"{what}: needs CUDA tensors")
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: {name} is on {t.device}, not on {dev}")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: a tensor on {t.device}, not on cuda:{dev}")
 
 
 def _vector(what: str, name: str, t: torch.Tensor, dtypes, numel: int) -> None:
-    if t.dtype not in dtypes or not t.is_contiguous() or t.numel() != numel:
+    if t.dtype not in dtypes or t.numel() != numel or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {' or '.join(str(d) for d in dtypes)} tensor of "
                          f"{numel} values")
+
+
+_F32, _I32, _FLAG = (torch.float32,), (torch.int32,), (torch.uint8, torch.bool)
 
 
 class BeamSearch:
@@ -53,6 +69,7 @@ class BeamSearch:
         self.n_out = beams if n_out is None else n_out
         nbytes = ctypes.c_size_t()
         check(load().hi_rocm_beam_workspace_bytes(max_batch, beams, vocab, self.n_out, ctypes.byref(nbytes)))
+        self._bytes = nbytes.value
         self.workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
 
     def outputs(self, batch: int, stream: Optional[torch.cuda.Stream] = None) -> dict:
@@ -72,53 +89,53 @@ class BeamSearch:
         ``scores`` f32 and ``finished`` uint8 or bool of batch * beams values;
         ``mask_words`` int32 [batch * beams][ceil(vocab / 32)]."""
         what = "beam select"
-        if logits.dim() != 2 or logits.shape[1] != self.vocab or logits.stride(1) != 1:
-            raise ValueError(f"{what}: logits must be [batch * beams][{self.vocab}], tokens contiguous")
-        if logits.dtype not in (torch.float32, torch.bfloat16):
+        K, V = self.beams, self.vocab
+        if logits.dim() != 2 or logits.size(1) != V or logits.stride(1) != 1:
+            raise ValueError(f"{what}: logits must be [batch * beams][{V}], tokens contiguous")
+        dtype = _CODES.get(logits.dtype)
+        if dtype is None:
             raise ValueError(f"{what}: logits must be float32 or bfloat16")
-        rows = logits.shape[0]
-        batch = rows // self.beams
-        if rows != batch * self.beams or not 0 < batch <= self.max_batch:
-            raise ValueError(f"{what}: {rows} rows for {self.beams} beams, at most {self.max_batch} requests")
-        _vector(what, "scores", scores, (torch.float32,), rows)
+        rows = logits.size(0)
+        batch = rows // K
+        if rows != batch * K or not 0 < batch <= self.max_batch:
+            raise ValueError(f"{what}: {rows} rows for {K} beams, at most {self.max_batch} requests")
+        _vector(what, "scores", scores, _F32, rows)
         if finished is not None:
-            _vector(what, "finished", finished, (torch.uint8, torch.bool), rows)
+            _vector(what, "finished", finished, _FLAG, rows)
             if eos_id is None:
                 raise ValueError(f"{what}: finished beams need an eos_id")
         if mask_words is not None:
-            _vector(what, "mask_words", mask_words, (torch.int32,), rows * ((self.vocab + 31) // 32))
-        if eos_id is not None and not 0 <= eos_id < self.vocab:
+            _vector(what, "mask_words", mask_words, _I32, rows * ((V + 31) // 32))
+        if eos_id is not None and not 0 <= eos_id < V:
             raise ValueError(f"{what}: eos_id outside the vocabulary")
         if out is None:
             out = self.outputs(batch, stream)
         n = batch * self.n_out
-        _vector(what, "out scores", out["scores"], (torch.float32,), n)
-        _vector(what, "out tokens", out["tokens"], (torch.int32,), n)
-        _vector(what, "out parents", out["parents"], (torch.int32,), n)
-        _vector(what, "out finished", out["finished"], (torch.uint8, torch.bool), n)
-        _same_device(what, self.workspace.device, logits=logits, scores=scores, finished=finished,
-                     mask_words=mask_words, **{f"out {k}": v for k, v in out.items()})
+        o_scores, o_tokens, o_parents, o_finished = out["scores"], out["tokens"], out["parents"], out["finished"]
+        _vector(what, "out scores", o_scores, _F32, n)
+        _vector(what, "out tokens", o_tokens, _I32, n)
+        _vector(what, "out parents", o_parents, _I32, n)
+        _vector(what, "out finished", o_finished, _FLAG, n)
+        ws = self.workspace
+        _on(what, ws.get_device(), logits, scores, finished, mask_words, o_scores, o_tokens, o_parents, o_finished)
         check(load().hi_rocm_beam_select(
-            logits.data_ptr(), _lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16, batch, self.beams,
-            self.vocab, max(logits.stride(0), self.vocab), scores.data_ptr(), _ptr(finished),
-            _lib.BEAM_NO_EOS if eos_id is None else eos_id, _ptr(mask_words), self.n_out, out["scores"].data_ptr(),
-            out["tokens"].data_ptr(), out["parents"].data_ptr(), out["finished"].data_ptr(),
-            self.workspace.data_ptr(), self.workspace.numel(), _stream_ptr(stream)))
+            logits.data_ptr(), dtype, batch, K, V, max(logits.stride(0), V), scores.data_ptr(), _ptr(finished),
+            _lib.BEAM_NO_EOS if eos_id is None else eos_id, _ptr(mask_words), self.n_out, o_scores.data_ptr(),
+            o_tokens.data_ptr(), o_parents.data_ptr(), o_finished.data_ptr(), ws.data_ptr(), self._bytes,
+            _stream(stream)))
         return out
 
 
-def _one_stride(t: torch.Tensor, dims) -> tuple:
-    """(count, stride in elements) of consecutive dims that step evenly."""
-    dims = [d for d in dims if t.shape[d] != 1]
-    if not dims:
-        return 1, 0
-    for a, b in zip(dims, dims[1:]):
-        if t.stride(a) != t.shape[b] * t.stride(b):
-            raise ValueError("reorder states: dimensions of the state do not step evenly")
-    n = 1
-    for d in dims:
-        n *= t.shape[d]
-    return n, t.stride(dims[-1])
+def _one_stride(shape, strides, a: int, b: int) -> tuple:
+    """(count, stride in elements) of dimensions [a, b), which step evenly."""
+    n, step = 1, 0
+    for d in range(b - 1, a - 1, -1):
+        if shape[d] != 1:
+            if n != 1 and strides[d] != n * step:
+                raise ValueError("reorder states: dimensions of the state do not step evenly")
+            step = step if n != 1 else strides[d]
+            n *= shape[d]
+    return n, step
 
 
 def reorder_states(src: torch.Tensor, parents: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: int = 0,
@@ -132,43 +149,43 @@ def reorder_states(src: torch.Tensor, parents: torch.Tensor, dst: Optional[torch
     what = "reorder states"
     if dst is None:
         dst = src
-    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_contiguous():
+    if parents.dim() != 2 or parents.dtype is not torch.int32 or not parents.is_contiguous():
         raise ValueError(f"{what}: parents must be a contiguous int32 [batch][beams] tensor")
     batch, beams = parents.shape
-    nd = src.dim()
-    if not 0 <= row_dim < nd or src.shape[row_dim] != batch * beams:
+    shape, strides = src.shape, src.stride()
+    nd = len(shape)
+    if not 0 <= row_dim < nd or shape[row_dim] != batch * beams:
         raise ValueError(f"{what}: dimension {row_dim} must have batch * beams = {batch * beams} rows")
     if src.numel() == 0:
         raise ValueError(f"{what}: an empty state")
-    if dst.shape != src.shape or dst.stride() != src.stride() or dst.dtype != src.dtype:
+    if dst is not src and (dst.shape != shape or dst.stride() != strides or dst.dtype is not src.dtype):
         raise ValueError(f"{what}: dst must have the shape, strides and type of src")
     if (lengths is None) != (length_dim is None):
         raise ValueError(f"{what}: lengths and length_dim go together")
     if lengths is not None:
         if not row_dim < length_dim < nd:
             raise ValueError(f"{what}: length_dim must follow row_dim")
-        _vector(what, "lengths", lengths, (torch.int32,), batch)
+        _vector(what, "lengths", lengths, _I32, batch)
     es = src.element_size()
-    # the trailing dimensions that are contiguous: positions of a length, or
-    # one position of everything
-    inner = 1
-    first = nd
-    stop = length_dim + 1 if length_dim is not None else row_dim + 1
-    while first > stop and (src.shape[first - 1] == 1 or src.stride(first - 1) == inner):
+    # the trailing dimensions that are contiguous: what lies behind a length,
+    # or one position of everything
+    inner, first = 1, nd
+    stop = row_dim + 1 if length_dim is None else length_dim + 1
+    while first > stop and (shape[first - 1] == 1 or strides[first - 1] == inner):
         first -= 1
-        inner *= src.shape[first]
-    if length_dim is not None:
-        if first != stop or (src.shape[length_dim] != 1 and src.stride(length_dim) != inner):
-            raise ValueError(f"{what}: what lies behind length_dim, and its positions, must be contiguous")
-        positions, mids = src.shape[length_dim], range(row_dim + 1, length_dim)
+        inner *= shape[first]
+    if length_dim is None:
+        positions, mid_end = 1, first
     else:
-        positions, mids = 1, range(row_dim + 1, first)
-    outer, outer_stride = _one_stride(src, range(row_dim))
-    mid, mid_stride = _one_stride(src, mids)
-    _same_device(what, src.device, parents=parents, dst=dst, lengths=lengths)
+        if first != stop or (shape[length_dim] != 1 and strides[length_dim] != inner):
+            raise ValueError(f"{what}: what lies behind length_dim, and its positions, must be contiguous")
+        positions, mid_end = shape[length_dim], length_dim
+    outer, outer_stride = _one_stride(shape, strides, 0, row_dim)
+    mid, mid_stride = _one_stride(shape, strides, row_dim + 1, mid_end)
+    _on(what, src.get_device(), parents, dst, lengths)
     check(load().hi_rocm_beam_reorder(
         src.data_ptr(), dst.data_ptr(), parents.data_ptr(), batch, beams, outer, outer_stride * es,
-        src.stride(row_dim) * es, mid, mid_stride * es, positions, inner * es, _ptr(lengths), _stream_ptr(stream)))
+        strides[row_dim] * es, mid, mid_stride * es, positions, inner * es, _ptr(lengths), _stream(stream)))
     return dst
 
 

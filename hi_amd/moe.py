@@ -8,12 +8,8 @@ from typing import Optional
 
 import torch
 
-from . import _lib
 from ._lib import check, load
-from .beam import _empty, _same_device
-from .sampler import _stream_ptr
-
-_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+from .beam import _CODES, _empty, _on, _stream
 
 
 class RowGroups:
@@ -43,9 +39,9 @@ def group_rows(ids: torch.Tensor, experts: int, out: Optional[RowGroups] = None,
         out = RowGroups(ids.shape[0], ids.shape[1], experts, device=ids.device)
     if (out.tokens, out.top_k, out.experts) != (ids.shape[0], ids.shape[1], experts):
         raise ValueError(f"{what}: out is for {out.tokens} tokens, top {out.top_k} of {out.experts} experts")
-    _same_device(what, ids.device, out=out.order)
+    _on(what, ids.get_device(), out.order)
     check(load().hi_rocm_moe_group(ids.data_ptr(), out.tokens, out.top_k, experts, out.order.data_ptr(),
-                                   out.slots.data_ptr(), out.offsets.data_ptr(), _stream_ptr(stream)))
+                                   out.slots.data_ptr(), out.offsets.data_ptr(), _stream(stream)))
     return out
 
 
@@ -72,11 +68,11 @@ def grouped_product(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, ga
         out = _empty((groups.places, wide), dtype, x.device, stream)
     if out.shape != (groups.places, wide) or out.dtype not in _CODES or out.stride(1) != 1:
         raise ValueError(f"{what}: out must be a float32 or bfloat16 [{groups.places}][{wide}] tensor")
-    _same_device(what, x.device, weight=weight, groups=groups.order, out=out)
+    _on(what, x.get_device(), weight, groups.order, out)
     check(load().hi_rocm_moe_grouped_product(
         x.data_ptr(), rows, x.stride(0) if rows > 1 else k, groups.order.data_ptr() if gather else 0, groups.top_k,
         groups.offsets.data_ptr(), groups.places, experts, weight.data_ptr(), cols, k, int(swiglu), out.data_ptr(),
-        _CODES[out.dtype], out.stride(0) if groups.places > 1 else wide, _stream_ptr(stream)))
+        _CODES[out.dtype], out.stride(0) if groups.places > 1 else wide, _stream(stream)))
     return out
 
 
@@ -92,11 +88,11 @@ def combine(y: torch.Tensor, groups: RowGroups, weights: torch.Tensor, out: Opti
         out = _empty((groups.tokens, y.shape[1]), dtype, y.device, stream)
     if out.shape != (groups.tokens, y.shape[1]) or out.dtype not in _CODES or out.stride(1) != 1:
         raise ValueError(f"{what}: out must be a float32 or bfloat16 [{groups.tokens}][{y.shape[1]}] tensor")
-    _same_device(what, y.device, groups=groups.order, weights=weights, out=out)
+    _on(what, y.get_device(), groups.order, weights, out)
     check(load().hi_rocm_moe_combine(
         y.data_ptr(), _CODES[y.dtype], y.stride(0) if groups.places > 1 else y.shape[1], groups.slots.data_ptr(),
         groups.offsets.data_ptr(), groups.experts, weights.data_ptr(), groups.tokens, groups.top_k, y.shape[1],
-        out.data_ptr(), _CODES[out.dtype], out.stride(0) if groups.tokens > 1 else y.shape[1], _stream_ptr(stream)))
+        out.data_ptr(), _CODES[out.dtype], out.stride(0) if groups.tokens > 1 else y.shape[1], _stream(stream)))
     return out
 
 
@@ -109,8 +105,12 @@ class MoeExperts:
 
     def __init__(self, w_up: torch.Tensor, w_down: torch.Tensor, max_tokens: int, top_k: int):
         if (w_up.dim() != 3 or w_down.dim() != 3 or w_up.shape[1] % 2 or
-                w_down.shape != (w_up.shape[0], w_up.shape[2], w_up.shape[1] // 2)):
-            raise ValueError("moe experts: w_up [experts][2 * inter][hidden], w_down [experts][hidden][inter]")
+                w_down.shape != (w_up.shape[0], w_up.shape[2], w_up.shape[1] // 2) or
+                w_up.dtype is not torch.bfloat16 or w_down.dtype is not torch.bfloat16 or
+                not w_up.is_contiguous() or not w_down.is_contiguous()):
+            raise ValueError("moe experts: w_up [experts][2 * inter][hidden] and w_down [experts][hidden][inter], "
+                             "contiguous bfloat16")
+        _on("moe experts", w_up.get_device(), w_down)
         self.w_up, self.w_down, self.max_tokens, self.top_k = w_up, w_down, max_tokens, top_k
         self.experts, self.hidden, self.inter = w_up.shape[0], w_up.shape[2], w_down.shape[2]
         dev = w_up.device
@@ -124,21 +124,38 @@ class MoeExperts:
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         """x bfloat16 [tokens][hidden], ids int32 and weights float32
         [tokens][top_k] from the router; returns [tokens][hidden] (bfloat16,
-        or out's type)."""
-        tokens = x.shape[0]
-        if ids.dim() != 2 or ids.shape != (tokens, self.top_k) or not 0 < tokens <= self.max_tokens:
-            raise ValueError(f"moe experts: ids must be [tokens][{self.top_k}], at most {self.max_tokens} tokens")
-        g = self._groups
-        if tokens != self.max_tokens:
-            g = RowGroups.__new__(RowGroups)
-            g.tokens, g.top_k, g.experts = tokens, self.top_k, self.experts
-            n = tokens * self.top_k
-            g.order, g.slots, g.offsets = self._groups.order[:n], self._groups.slots[:n], self._groups.offsets
-        h, y = self._h[:g.places], self._y[:g.places]
-        group_rows(ids, self.experts, out=g, stream=stream)
-        grouped_product(x, self.w_up, g, gather=True, swiglu=True, out=h, stream=stream)
-        grouped_product(h, self.w_down, g, gather=False, out=y, stream=stream)
-        return combine(y, g, weights, out=out, stream=stream)
+        or out's type).  The buffers serve one stream at a time."""
+        what = "moe experts"
+        k, E, H, I = self.top_k, self.experts, self.hidden, self.inter
+        if x.dim() != 2 or x.dtype is not torch.bfloat16 or x.size(1) != H or x.stride(1) != 1:
+            raise ValueError(f"{what}: x must be a bfloat16 [tokens][{H}] tensor, inputs contiguous")
+        tokens = x.size(0)
+        if not 0 < tokens <= self.max_tokens:
+            raise ValueError(f"{what}: {tokens} tokens, at most {self.max_tokens}")
+        if ids.shape != (tokens, k) or ids.dtype is not torch.int32 or not ids.is_contiguous():
+            raise ValueError(f"{what}: ids must be a contiguous int32 [{tokens}][{k}] tensor")
+        if weights.shape != (tokens, k) or weights.dtype is not torch.float32 or not weights.is_contiguous():
+            raise ValueError(f"{what}: weights must be a contiguous float32 [{tokens}][{k}] tensor")
+        if out is None:
+            out = _empty((tokens, H), torch.bfloat16, x.device, stream)
+        code = _CODES.get(out.dtype)
+        if code is None or out.shape != (tokens, H) or out.stride(1) != 1:
+            raise ValueError(f"{what}: out must be a float32 or bfloat16 [{tokens}][{H}] tensor")
+        g, h, y = self._groups, self._h, self._y
+        _on(what, h.get_device(), x, ids, weights, out)
+        places, st, lib = tokens * k, _stream(stream), load()
+        order, slots, offsets = g.order.data_ptr(), g.slots.data_ptr(), g.offsets.data_ptr()
+        check(lib.hi_rocm_moe_group(ids.data_ptr(), tokens, k, E, order, slots, offsets, st))
+        check(lib.hi_rocm_moe_grouped_product(
+            x.data_ptr(), tokens, x.stride(0) if tokens > 1 else H, order, k, offsets, places, E,
+            self.w_up.data_ptr(), 2 * I, H, 1, h.data_ptr(), _CODES[h.dtype], I, st))
+        check(lib.hi_rocm_moe_grouped_product(
+            h.data_ptr(), places, I, 0, 1, offsets, places, E, self.w_down.data_ptr(), H, I, 0, y.data_ptr(),
+            _CODES[y.dtype], H, st))
+        check(lib.hi_rocm_moe_combine(
+            y.data_ptr(), _CODES[y.dtype], H, slots, offsets, E, weights.data_ptr(), tokens, k, H, out.data_ptr(), code,
+            out.stride(0) if tokens > 1 else H, st))
+        return out
 
 
 __all__ = ["RowGroups", "group_rows", "grouped_product", "combine", "MoeExperts"]

@@ -8,12 +8,8 @@ from typing import Optional
 
 import torch
 
-from . import _lib
 from ._lib import check, load
-from .beam import _empty, _ptr, _same_device
-from .sampler import _stream_ptr
-
-_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+from .beam import _CODES, _empty, _on, _ptr, _stream
 
 
 def quantize_w4(weight: torch.Tensor, group: int = 32, symmetric: bool = True, scale_dtype=torch.bfloat16):
@@ -60,32 +56,37 @@ class W4Linear:
             raise ValueError(f"{what}: zeros must be like scales")
         if bias is not None and (bias.shape != (self.n,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
             raise ValueError(f"{what}: bias must be a contiguous float32 [n] tensor")
-        _same_device(what, q.device, scales=scales, zeros=zeros, bias=bias)
+        _on(what, q.get_device(), scales, zeros, bias)
         self.bias, self.scale_dtype, self.has_zeros = bias, _CODES[scales.dtype], int(zeros is not None)
         lib, nbytes = load(), ctypes.c_size_t()
         check(lib.hi_rocm_w4_packed_bytes(self.n, self.k, self.group, self.scale_dtype, self.has_zeros,
                                           ctypes.byref(nbytes)))
+        self._bytes = nbytes.value
         self.packed = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
         check(lib.hi_rocm_w4_pack(q.data_ptr(), scales.data_ptr(), _ptr(zeros), self.scale_dtype, self.n, self.k,
-                                  self.group, self.packed.data_ptr(), self.packed.numel(), _stream_ptr(stream)))
+                                  self.group, self.packed.data_ptr(), self.packed.numel(), _stream(stream)))
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, dtype=torch.float32,
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         """x bfloat16 [rows][k], rows starting on 16 bytes; returns out
         [rows][n] (a new tensor of ``dtype`` when not given)."""
         what = "w4 linear"
-        if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != self.k or x.stride(1) != 1 or x.shape[0] == 0:
-            raise ValueError(f"{what}: x must be a bfloat16 [rows][{self.k}] tensor, inputs contiguous")
+        n, k = self.n, self.k
+        if x.dim() != 2 or x.dtype is not torch.bfloat16 or x.size(1) != k or x.stride(1) != 1 or x.size(0) == 0:
+            raise ValueError(f"{what}: x must be a bfloat16 [rows][{k}] tensor, inputs contiguous")
+        rows = x.size(0)
         if out is None:
-            out = _empty((x.shape[0], self.n), dtype, x.device, stream)
-        if out.shape != (x.shape[0], self.n) or out.dtype not in _CODES or out.stride(1) != 1:
-            raise ValueError(f"{what}: out must be a float32 or bfloat16 [{x.shape[0]}][{self.n}] tensor")
-        _same_device(what, self.packed.device, x=x, out=out)
-        rows = x.shape[0]
+            out = _empty((rows, n), dtype, x.device, stream)
+        code = _CODES.get(out.dtype)
+        if code is None or out.dim() != 2 or out.size(0) != rows or out.size(1) != n or out.stride(1) != 1:
+            raise ValueError(f"{what}: out must be a float32 or bfloat16 [{rows}][{n}] tensor, outputs contiguous")
+        packed = self.packed
+        _on(what, packed.get_device(), x, out)
+        # (a single row's stride says nothing)
         check(load().hi_rocm_w4_linear(
-            x.data_ptr(), rows, x.stride(0) if rows > 1 else self.k + -self.k % 8, self.packed.data_ptr(),
-            self.packed.numel(), self.scale_dtype, self.has_zeros, self.n, self.k, self.group, _ptr(self.bias),
-            out.data_ptr(), _CODES[out.dtype], out.stride(0) if rows > 1 else self.n, _stream_ptr(stream)))
+            x.data_ptr(), rows, x.stride(0) if rows > 1 else k, packed.data_ptr(), self._bytes, self.scale_dtype,
+            self.has_zeros, n, k, self.group, _ptr(self.bias), out.data_ptr(), code,
+            out.stride(0) if rows > 1 else n, _stream(stream)))
         return out
 
 
