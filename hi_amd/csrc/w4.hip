@@ -145,7 +145,13 @@ struct W4Scales<ST, 1> {
 // product runs.  (Products that start from -24 e would save an addition, but
 // weights of 0 would then not give 0.)
 // MQ = 1: one row of x; of the four rows a lane's results hold only the first
-// is kept.
+// is kept (4096 x 65536: 26.4 us, with all four 28.2).
+//
+// What bounds it: the weights' bytes for a row (4096 x 151936 in groups of 32,
+// 350 MB with the scales: 62 us, 5.6 TB/s), the latency of the loads and of the
+// two barriers for small weights (1184 x 1000: 6.6 us), and for 17 to 64 rows
+// the instructions of the groups' ends, two a row and output of four (32 rows,
+// 4096 x 16384 with zeros in groups of 128, 35 MB: 16.7 us, 2.2 TB/s).
 // MFMA 16x16x32 bf16 (lane l = 16 g + r): A row r, elements 8 g .. 8 g + 7;
 // B column r, the same elements; D rows 4 g .. 4 g + 3 of column r.  Rows past
 // the last repeat it and are dropped.
@@ -342,23 +348,43 @@ hipError_t launch_w4(const W4Args& a, hipStream_t st) {
   hipLaunchKernelGGL(kernel, grid, dim3(64 * kW4Waves), bytes, st, a);
   return hipGetLastError();
 }
-template <int MQ, int G, bool ZEROS, typename ST>
-hipError_t launch_w4_tile(const W4Args& a, hipStream_t st) {
-  if (a.n_tiles < 512) {  // less than two tiles a CU
-    if (a.k_blocks <= 8) return launch_w4<1, MQ, 1, 1, 3, G, ZEROS, ST>(a, st);
-    if (a.k_blocks <= 16) return launch_w4<1, MQ, 1, 2, 3, G, ZEROS, ST>(a, st);
-    return launch_w4<1, MQ, 1, 4, 2, G, ZEROS, ST>(a, st);
-  }
-  if (a.k_blocks <= 8) return launch_w4<1, MQ, 4, 1, 4, G, ZEROS, ST>(a, st);
-  if (a.k_blocks <= 16) return launch_w4<1, MQ, 4, 2, 4, G, ZEROS, ST>(a, st);
-  return launch_w4<1, MQ, 2, 4, 2, G, ZEROS, ST>(a, st);
-}
+// T and BPW.  Up to 16 blocks of k one pass holds all of x with BPW = 1 or 2;
+// then T = 1 while that is at most two workgroups a CU, else T = 4.  Longer k
+// takes T = 1 (in passes of 8 blocks) while that is at most one workgroup a CU,
+// else T = 2 with BPW = 4, a pass of up to 32 blocks, and beyond those T = 4
+// where T = 2 would be more than one workgroup a CU.  Whole calls, us (bf16
+// scales, groups of 32, k x n):
+//   1 row, 1024 x 4096: T = 1 3.2, 4 4.1; 1024 x 16384: 4.5 and 4.2;
+//     2048 x 8192: 4.7 and 5.7; 2048 x 16384: 6.0 and 6.3; 2048 x 65536: 16.7 and 16.4
+//   16 rows, 4096 x 4096: T = 1 8.0, 2 9.0, 4 12.7; 4096 x 16384: 18.3, 13.1, 15.0;
+//     1 row, 8192 x 16384: 29.2, 21.4, 18.5; 8192 x 8192: 15.2, 13.5, 16.9
+// MT = 2 where MT = 1 would be more than one workgroup a CU: 32 rows, 4096 x
+// 65536: 45.0, with MT = 1 59.3; 64 rows, 2048 x 8192: 10.7 and 12.1; but 32 rows,
+// 4096 x 4096 (256 workgroups with MT = 1): 14.4 and 9.2.
+// (MT = 4 read x too often to gain: 64 rows, 4096 x 65536 110, with MT = 2 86.)
+// With f32 scales and zeros for groups of 32, MT = 2 and T = 2 do not fit the
+// registers: 32 rows, 4096 x 65536: 108, with T = 4 69.
 template <int G, bool ZEROS, typename ST>
 hipError_t launch_w4_rows(const W4Args& a, hipStream_t st) {
-  if (a.rows == 1) return launch_w4_tile<1, G, ZEROS, ST>(a, st);
-  if (a.rows <= 16) return launch_w4_tile<4, G, ZEROS, ST>(a, st);
-  if (a.rows <= 32) return launch_w4<2, 4, 4, 2, 4, G, ZEROS, ST>(a, st);
-  return launch_w4<4, 4, 4, 1, 4, G, ZEROS, ST>(a, st);
+  const int64_t row_tiles = (a.rows + 15) / 16;
+  auto wgs = [&](int t) { return (a.n_tiles + t - 1) / t * row_tiles; };
+  const bool shrt = a.k_blocks <= 16;
+  const int t = wgs(1) <= (shrt ? 512 : 256) ? 1 : shrt ? 4 : a.k_blocks <= 32 || wgs(2) <= 256 ? 2 : 4;
+  const bool one = a.k_blocks <= 8;
+  if (a.rows == 1) {
+    if (t == 1) return one || !shrt ? launch_w4<1, 1, 1, 1, 3, G, ZEROS, ST>(a, st) : launch_w4<1, 1, 1, 2, 3, G, ZEROS, ST>(a, st);
+    if (t == 2) return launch_w4<1, 1, 2, 4, 2, G, ZEROS, ST>(a, st);
+    return one ? launch_w4<1, 1, 4, 1, 4, G, ZEROS, ST>(a, st) : launch_w4<1, 1, 4, 2, 4, G, ZEROS, ST>(a, st);
+  }
+  if (t == 1)
+    return one || !shrt ? launch_w4<1, 4, 1, 1, 3, G, ZEROS, ST>(a, st) : launch_w4<1, 4, 1, 2, 3, G, ZEROS, ST>(a, st);
+  if (row_tiles == 1 || wgs(t) <= 256) {
+    if (t == 2) return launch_w4<1, 4, 2, 4, 2, G, ZEROS, ST>(a, st);
+    return one ? launch_w4<1, 4, 4, 1, 4, G, ZEROS, ST>(a, st) : launch_w4<1, 4, 4, 2, 4, G, ZEROS, ST>(a, st);
+  }
+  if constexpr (G > 32 || !ZEROS || sizeof(ST) == 2)
+    if (t == 2) return launch_w4<2, 4, 2, 4, 2, G, ZEROS, ST>(a, st);
+  return one ? launch_w4<2, 4, 4, 1, 4, G, ZEROS, ST>(a, st) : launch_w4<2, 4, 4, 2, 4, G, ZEROS, ST>(a, st);
 }
 template <int G, typename ST>
 hipError_t launch_w4_zeros(const W4Args& a, hipStream_t st) {
