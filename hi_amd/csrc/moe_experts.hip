@@ -38,10 +38,11 @@ constexpr int kMoeMaxPairs = 1 << 22;
 // [0, experts), which come last and belong to no group).  Every workgroup
 // counts the ids below its own, so none waits for another; its waves own
 // consecutive stretches of the pairs, lane l of a stretch 4 consecutive pairs
-// at a time, so places follow the pairs' order.  A stretch of up to 2,048 pairs
-// (32,768 in all) is read once, all loads at once, and kept in registers.
-// (32,768 pairs of 64 experts: 3.9 us; with a load a lane and pair and a second
-// pass over memory 12.)
+// at a time, so places follow the pairs' order.  A stretch of up to 256 L pairs
+// is read once, all loads at once, and kept in registers.  What bounds it is
+// the latency of the loads, two scans and a barrier: 64 pairs 2.8 us.  Four
+// waves with 4 loads each, or 16 with 8, us for 4,096, 8,192 and 32,768 pairs of
+// 64 experts: 3.6, 5.1, 14.1 and 6.2, 6.4, 8.1.
 template <int W, int L>
 __global__ void __launch_bounds__(64 * W) moe_group_kernel(const uint32_t* ids, int pairs, int experts, int32_t* order,
                                                            int32_t* slots, int32_t* offsets) {
@@ -600,13 +601,31 @@ hipError_t launch_many(const GroupedArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// By the places an expert has on average: up to 8 a wave's 16 places suffice,
+// up to 20 its 32; above, the 64 would only gain where the next kernel leaves
+// CUs idle.  us at 8, 16, 24 and 40 places each of
+//   64 experts, 2048 x 2048:  16 places 96, 120, 149, 214; 32: 96, 107, 113, 168;
+//     64: 101, 109, 116, 128; tiles of 128: 124, 124, 124, 126
+//   128 experts, 1024 x 1536: 77, 92, 117, 166; 76, 82, 90, 135; 90, 94, 99, 108;
+//     78, 77, 78, 82
+// Tiles of 128 or of 256 places by the rounds that their workgroups, one a CU,
+// make: up to two count whole, and a round of 256 as 7/4 of one of 128.  An
+// expert's last tile counts as half a tile.  us at 128, 192, 256 and 512 places:
+//   64 experts, 2048 x 2048:  tiles of 128 149, 177, 209, 341; of 256 150, 159, 223, 329
+//   128 experts, 1024 x 1536: 124, 149, 180, 307; 116, 133, 175, 275
+//   16 experts, 1024 x 2048:  21, 22, 36, 58; 25, 27, 30, 55
 hipError_t launch_grouped(const GroupedArgs& a, hipStream_t st) {
   const int avg = a.places / a.experts;
   if (avg <= 8) return launch_few<1>(a, st);
   if (avg <= 20) return launch_few<2>(a, st);
-  if (avg <= 40) return launch_few<4>(a, st);
-  if (avg <= 256) return launch_many<128, 256, 64, 3>(a, st);
-  return launch_many<256, 256, 32, 4>(a, st);
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? 128 : 256;
+  auto rounds = [&](int bm) {  // in workgroups
+    const int64_t halves = avg < bm ? 2 * (int64_t)a.experts : 2 * (int64_t)a.places / bm + a.experts;
+    const int64_t n = halves * ((cols_out + per - 1) / per) / 2;
+    return n <= 512 ? (n + 255) / 256 * 256 : n;
+  };
+  if (7 * rounds(256) < 4 * rounds(128)) return launch_many<256, 256, 32, 4>(a, st);
+  return launch_many<128, 256, 64, 3>(a, st);
 }
 
 // ---- combination ----------------------------------------------------------
@@ -707,7 +726,7 @@ int hi_rocm_moe_group(const uint32_t* ids, int tokens, int top_k, int experts, i
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_moe_group: more than 2048 experts or 2^22 pairs");
   const int pairs = tokens * top_k;
   const dim3 grid((unsigned)(experts + 1));
-  if (pairs <= 4096)
+  if (pairs <= 8192)
     hipLaunchKernelGGL((moe_group_kernel<4, 4>), grid, dim3(256), 0, (hipStream_t)stream, ids, pairs, experts, order, slots,
                        offsets);
   else
