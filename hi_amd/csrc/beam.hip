@@ -40,8 +40,7 @@ constexpr int kPartSlots = 512;      // candidates that a wave of a streamed par
 constexpr int kFinishThreads = 512;
 constexpr int kFinishHeld = 4;       // candidates a thread keeps in registers
 constexpr int kFinishSlots = 512;
-constexpr int kBeamMaxRows = 65536;
-
+constexpr int kBeamMaxRows = 65535;  // (a grid's second dimension)
 
 struct BeamPart {
   float m;       // largest logit of the part (-inf: no candidate)
@@ -962,7 +961,7 @@ int hi_rocm_beam_workspace_bytes(int max_batch, int beams, int vocab, int n_out,
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_beam_workspace_bytes: invalid arguments");
   if (beams > kBeamMax || n_out > kBeamMaxOut || vocab > kMaxVocab || (int64_t)max_batch * beams > kBeamMaxRows)
     return api_fail(HI_ROCM_ERR_UNSUPPORTED,
-                    "hi_rocm_beam_workspace_bytes: more than 32 beams, 64 outputs, 65536 rows or 2^23 tokens");
+                    "hi_rocm_beam_workspace_bytes: more than 32 beams, 64 outputs, 65535 rows or 2^23 tokens");
   int64_t slots = 0;
   for (int b = 1; b <= max_batch; ++b)
     for (int dtype : {HI_ROCM_DTYPE_F32, HI_ROCM_DTYPE_BF16})
@@ -985,7 +984,7 @@ int hi_rocm_beam_select(const void* logits, int dtype, int batch, int beams, int
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_beam_select: logits not aligned to their type");
   if (finished != nullptr && eos_id == HI_ROCM_BEAM_NO_EOS)
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_beam_select: finished beams need an eos id");
-  if (beams > kBeamMax || n_out > kBeamMaxOut || vocab > kMaxVocab || (int64_t)batch * beams > kBeamMaxRows - 1)
+  if (beams > kBeamMax || n_out > kBeamMaxOut || vocab > kMaxVocab || (int64_t)batch * beams > kBeamMaxRows)
     return api_fail(HI_ROCM_ERR_UNSUPPORTED,
                     "hi_rocm_beam_select: more than 32 beams, 64 outputs, 65535 rows or 2^23 tokens");
   const int rows = batch * beams;
@@ -1028,7 +1027,7 @@ int hi_rocm_beam_reorder(const void* src, void* dst, const int32_t* parents, int
   if (src == nullptr || dst == nullptr || parents == nullptr || batch <= 0 || beams <= 0 || outer <= 0 || mid <= 0 ||
       positions <= 0 || pos_bytes <= 0 || outer_stride < 0 || row_stride < 0 || mid_stride < 0)
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_beam_reorder: invalid arguments");
-  if (beams > kBeamMax || batch > kBeamMaxRows - 1)
+  if (beams > kBeamMax || batch > kBeamMaxRows)
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_beam_reorder: more than 32 beams or 65535 requests");
   constexpr int64_t kBig = (int64_t)1 << 46;
   if (positions > kBig / pos_bytes || outer > kBig || mid > kBig || outer_stride > kBig || row_stride > kBig ||
@@ -1068,8 +1067,10 @@ int hi_rocm_beam_reorder(const void* src, void* dst, const int32_t* parents, int
   const uint64_t bits = s | t | (uint64_t)a.outer_stride | (uint64_t)a.row_stride | (uint64_t)a.mid_stride |
                         (uint64_t)pos_bytes;
   const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
-  if (outer * mid > INT32_MAX || outer * mid * (((piece + unit - 1) / unit + 255) / 256) > INT32_MAX)
-    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_beam_reorder: more than 2^31 pieces of 256 units a request");
+  // (a launch holds less than 2^32 threads; outer * mid * blocks: each below 2^46)
+  const int64_t blocks = ((piece + unit - 1) / unit + 255) / 256, most = UINT32_MAX / 256;
+  if (outer > most || mid > most / outer || blocks > most / (outer * mid))
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_beam_reorder: more than 2^24 pieces of 256 units a row");
   if (unit == 16) launch_reorder<reorder_u32x4>(a, batch, (hipStream_t)stream);
   else if (unit == 4) launch_reorder<uint32_t>(a, batch, (hipStream_t)stream);
   else launch_reorder<uint8_t>(a, batch, (hipStream_t)stream);

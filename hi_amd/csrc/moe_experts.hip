@@ -585,9 +585,14 @@ int64_t moe_grid(const GroupedArgs& a, int bm, int bn) {
   return (tiles * ((cols_out + per - 1) / per) + kXcds - 1) / kXcds * kXcds;
 }
 
+// (a launch holds less than 2^32 threads)
+bool moe_grid_fits(int64_t grid, int threads) { return grid <= UINT32_MAX / threads; }
+
 template <int MT>
 hipError_t launch_few(const GroupedArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(moe_few_kernel<MT>, dim3((unsigned)moe_grid(a, 16 * MT, kFewCols)), dim3(64 * kFewWaves), 0, st, a);
+  const int64_t grid = moe_grid(a, 16 * MT, kFewCols);
+  if (!moe_grid_fits(grid, 64 * kFewWaves)) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(moe_few_kernel<MT>, dim3((unsigned)grid), dim3(64 * kFewWaves), 0, st, a);
   return hipGetLastError();
 }
 
@@ -595,9 +600,11 @@ template <int BM, int BN, int BK, int NB>
 hipError_t launch_many(const GroupedArgs& a, hipStream_t st) {
   constexpr size_t bytes = (size_t)NB * (BM + BN) * BK * 2;
   auto* kernel = moe_many_kernel<BM, BN, BK, NB>;
+  const int64_t grid = moe_grid(a, BM, BN);
+  if (!moe_grid_fits(grid, 512)) return hipErrorInvalidConfiguration;
   const hipError_t e = ensure_lds((const void*)kernel, bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)moe_grid(a, BM, BN)), dim3(512), bytes, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(512), bytes, st, a);
   return hipGetLastError();
 }
 
@@ -769,9 +776,9 @@ int hi_rocm_moe_grouped_product(const void* x, int x_rows, int64_t x_stride, con
   a.swiglu = swiglu != 0;
   a.out_bf16 = out_dtype == HI_ROCM_DTYPE_BF16;
   a.out_vec = (uintptr_t)out % 16 == 0 && out_stride * moe_size(out_dtype) % 16 == 0;
-  if (moe_grid(a, 16, 32) > INT32_MAX)
-    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_moe_grouped_product: too many places and columns");
   const hipError_t e = launch_grouped(a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_moe_grouped_product: too many places and columns for one launch");
   return e == hipSuccess ? HI_ROCM_OK : api_hip_fail(e, "moe grouped product launch");
 }
 

@@ -438,8 +438,8 @@ int hi_rocm_w4_pack(const void* q, const void* scales, const void* zeros, int sc
   const int64_t blocks = L.n_tiles * L.k_blocks, words = blocks * 256;
   const int gpb = kW4Block / group;
   const int64_t count = blocks * 16 * gpb;
-  if ((words + 255) / 256 > INT32_MAX)
-    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_w4_pack: more than 2^31 blocks");
+  if (words > UINT32_MAX - 255)  // a thread each
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_w4_pack: more than 2^35 weights");
   hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(w4_pack_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, st, (const uint8_t*)q, n, k,
                      L.k_blocks, words, (uint32_t*)packed);
@@ -467,7 +467,8 @@ int hi_rocm_w4_linear(const void* x, int rows, int64_t x_stride, const void* pac
   const int rc = w4_check(n, k, group, scale_dtype, "hi_rocm_w4_linear: invalid arguments",
                           "hi_rocm_w4_linear: needs groups of 32, 64 or 128, k a multiple of them, n and k up to 2^24");
   if (rc != HI_ROCM_OK) return rc;
-  if (rows > 1 << 20) return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_w4_linear: more than 2^20 rows");
+  if (rows > 16 * 65535)  // (a grid's second dimension)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_w4_linear: more than 16 * 65535 rows");
   if ((uintptr_t)x % 16 != 0 || x_stride % 8 != 0)
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_w4_linear: needs rows of x that start on 16 bytes");
   if ((uintptr_t)out % (out_dtype == HI_ROCM_DTYPE_F32 ? 4 : 2) != 0 || (uintptr_t)bias % 4 != 0)

@@ -17,11 +17,12 @@ class RowGroups:
     ``order`` (the pair in each place), ``slots`` (each pair's place) and
     ``offsets`` (expert e's places are offsets[e] .. offsets[e + 1])."""
 
-    def __init__(self, tokens: int, top_k: int, experts: int, device="cuda"):
+    def __init__(self, tokens: int, top_k: int, experts: int, device="cuda",
+                 stream: Optional[torch.cuda.Stream] = None):
         self.tokens, self.top_k, self.experts = tokens, top_k, experts
-        self.order = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
-        self.slots = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
-        self.offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
+        self.order = _empty((tokens * top_k,), torch.int32, device, stream)
+        self.slots = _empty((tokens * top_k,), torch.int32, device, stream)
+        self.offsets = _empty((experts + 1,), torch.int32, device, stream)
 
     @property
     def places(self) -> int:
@@ -36,7 +37,7 @@ def group_rows(ids: torch.Tensor, experts: int, out: Optional[RowGroups] = None,
     if ids.dim() != 2 or ids.dtype != torch.int32 or not ids.is_contiguous() or ids.numel() == 0:
         raise ValueError(f"{what}: ids must be a contiguous int32 [tokens][top_k] tensor")
     if out is None:
-        out = RowGroups(ids.shape[0], ids.shape[1], experts, device=ids.device)
+        out = RowGroups(ids.shape[0], ids.shape[1], experts, device=ids.device, stream=stream)
     if (out.tokens, out.top_k, out.experts) != (ids.shape[0], ids.shape[1], experts):
         raise ValueError(f"{what}: out is for {out.tokens} tokens, top {out.top_k} of {out.experts} experts")
     _on(what, ids.get_device(), out.order)

@@ -62,7 +62,7 @@ class W4Linear:
         check(lib.hi_rocm_w4_packed_bytes(self.n, self.k, self.group, self.scale_dtype, self.has_zeros,
                                           ctypes.byref(nbytes)))
         self._bytes = nbytes.value
-        self.packed = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
+        self.packed = _empty((nbytes.value,), torch.uint8, q.device, stream)
         check(lib.hi_rocm_w4_pack(q.data_ptr(), scales.data_ptr(), _ptr(zeros), self.scale_dtype, self.n, self.k,
                                   self.group, self.packed.data_ptr(), self.packed.numel(), _stream(stream)))
 

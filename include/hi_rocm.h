@@ -384,7 +384,7 @@ int hi_rocm_profile_end(double* pass_ms, double* finish_ms, int* calls);
 #define HI_ROCM_BEAM_NO_EOS 0xffffffffu
 
 /* Workspace bytes hi_rocm_beam_select needs for up to max_batch requests of
- * `beams` beams (at most 65536 rows in all). */
+ * `beams` beams (at most 65535 rows in all). */
 int hi_rocm_beam_workspace_bytes(int max_batch, int beams, int vocab, int n_out, size_t* out_bytes);
 
 /* One step of beam search: the first n_out candidates of each request over
@@ -443,9 +443,10 @@ int hi_rocm_w4_pack(const void* q, const void* scales, const void* zeros, int sc
 /* out[m][c] = sum_k x[m][k] * w[c][k] + bias[c] for the packed weight w: x
  * bf16[rows][x_stride] (rows start on 16 bytes), bias f32[n] or NULL, out f32
  * or bf16 [rows][out_stride].  scale_dtype, has_zeros, n, k and group as
- * packed.  Made for the rows of a decode step (1 to 64; more take the weights
- * again for every 64).  A row's result does not depend on the other rows'
- * values; a row of x that holds inf or NaN gives NaN.  With f32 out it writes
+ * packed.  Made for the rows of a decode step (1 to 64; the weights are taken
+ * once for every 16 or 32 of them).  A row's result does not depend on the
+ * other rows' values, only on their number (by which k is split); a row of x
+ * that holds inf or NaN gives NaN.  With f32 out it writes
  * the logits that hi_rocm_sample and hi_rocm_beam_select read.  No
  * allocation: graph-capturable. */
 int hi_rocm_w4_linear(const void* x, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
