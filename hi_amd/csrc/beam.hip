@@ -76,6 +76,8 @@ __device__ __forceinline__ uint32_t beam_okey(float x) {
 __device__ __forceinline__ float beam_okey_inv(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
 }
+constexpr float kBeamLog2e = 1.44269502e+00f;
+constexpr float kBeamFused = 1e30f;  // logits up to this size can be scaled by log2 e
 constexpr float kBeamLowest = -3.402823466e38f;
 constexpr uint32_t kBeamNegInf = 0x007fffffu;  // beam_okey(-inf): keys above it are candidates
 
@@ -525,9 +527,9 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
       }
     }
     // the groups' maxima, and the sum about the running maximum (of a lane
-    // without a finite logit: about the lowest value, which leaves its terms 0)
-    float gm[G], tm, mn, at, add;
-    auto sum = [&]() {
+    // without a logit: about a low value, which leaves its terms 0)
+    float gm[G], tm, mn, at, add = 0.f;
+    auto maxima = [&]() {
       #pragma unroll
       for (int g = 0; g < G; ++g)
         gm[g] = beam_max3(beam_max3(x[GN * g], x[GN * g + 1], x[GN * g + 2]), x[GN * g + 3], ninf);
@@ -536,16 +538,26 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
       for (int g = 1; g + 1 < G; g += 2) tm = beam_max3(tm, gm[g], gm[g + 1]);
       tm = beam_max3(tm, gm[G - 1], ninf);
       mn = beam_max3(m, tm, ninf);
+    };
+    maxima();
+    // e^(x - at) as 2^(x log2 e - at log2 e), one fused operation and the
+    // exponential: the second product's rounding is that of a number of at's
+    // size, as the rounding of lse will be.
+    at = beam_max3(mn, -kBeamFused, ninf);
+    const float shift = -at * kBeamLog2e;
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) add += __builtin_amdgcn_exp2f(fmaf(x[i], kBeamLog2e, shift));
+    // NaN logits (masked; +inf: the sum does not matter) and logits whose
+    // products overflow
+    const bool odd = !(add < __builtin_inff()) || mn > kBeamFused || (mn < -kBeamFused && mn > ninf);
+    if (__ballot(odd) != 0ull) {
+      #pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = x[i] == x[i] ? x[i] : ninf;
+      maxima();
       at = beam_max3(mn, kBeamLowest, ninf);
       add = 0.f;
       #pragma unroll
       for (int i = 0; i < PER; ++i) add += __expf(x[i] - at);
-    };
-    sum();
-    if (__ballot(!(add == add)) != 0ull) {  // a NaN logit counts as masked (+inf: the sum does not matter)
-      #pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = x[i] == x[i] ? x[i] : ninf;
-      sum();
     }
     s = s * __expf(beam_max3(m, kBeamLowest, ninf) - at) + add;
     m = mn;
