@@ -36,7 +36,7 @@ constexpr int kBeamMaxOut = HI_ROCM_BEAM_MAX_OUT;
 constexpr int kPartThreads = 256;
 constexpr int kTileElems = 4096;     // elements of a part of a short step
 constexpr int kTileSlots = 256;      // candidates that such a part can hold before it ranks them
-constexpr int kPartSlots = 512;      // candidates that a wave of a streamed part can hold
+constexpr int kPartSlots = 256;      // groups of four logits that a wave of a streamed part can hold
 constexpr int kFinishThreads = 512;
 constexpr int kFinishHeld = 4;       // candidates a thread keeps in registers
 constexpr int kFinishSlots = 512;
@@ -355,17 +355,12 @@ __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
   }
 }
 
-// A candidate as the part kernel lists it, and as the key it is ranked by.
-struct __align__(8) BeamRaw {
-  float logit;
-  uint32_t token;
+// Groups of four neighbouring logits, as a wave of a streamed part lists them.
+typedef float beam_f32x4 __attribute__((ext_vector_type(4)));
+struct BeamList {
+  beam_f32x4 x[kPartSlots];
+  uint32_t token[kPartSlots];  // of the first
 };
-__device__ __forceinline__ uint64_t beam_key(const BeamRaw& c) {
-  return ((uint64_t)beam_okey(c.logit) << 32) | (0xffffffffu - c.token);
-}
-__device__ __forceinline__ BeamRaw beam_raw(uint64_t key) {
-  return BeamRaw{beam_okey_inv((uint32_t)(key >> 32)), 0xffffffffu - (uint32_t)key};
-}
 // Set bits of a ballot below this lane's.
 __device__ __forceinline__ int beam_below(uint64_t b) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
@@ -378,49 +373,74 @@ __device__ __forceinline__ float beam_max3(float x, float y, float z) {
   return r;
 }
 
-// The largest n of a wave's count in (n, kPartSlots] candidates, moved to the
-// list's start; returns the upper half of the n-th's key, found bit by bit from the highest bit
-// in which the keys differ.  (Not inlined: the part kernel's loop has several
-// places for it.)
-__device__ __noinline__ uint32_t beam_prune(BeamRaw* list, int count, int n) {
-  constexpr int P = kPartSlots / 64;
-  const int lane = threadIdx.x & 63;
-  uint64_t k[P];
-  uint32_t hi = 0u, lo = 0xffffffffu;  // of the keys' upper halves
+// The keys of group i's logits (0: below `floor`, or not in the list).
+__device__ __forceinline__ void beam_keys(const BeamList* list, int i, int count, uint32_t floor, uint64_t (&k)[4]) {
+  const beam_f32x4 x = list->x[min(i, kPartSlots - 1)];
+  const uint32_t t = list->token[min(i, kPartSlots - 1)];
   #pragma unroll
-  for (int j = 0; j < P; ++j) {
-    k[j] = 0ull;
-    if (lane + 64 * j < count) {
-      k[j] = beam_key(list[lane + 64 * j]);
-      hi = max(hi, (uint32_t)(k[j] >> 32));
-      lo = min(lo, (uint32_t)(k[j] >> 32));
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t o = beam_okey(x[q]);
+    k[q] = i < count && o >= floor ? (uint64_t)o << 32 | (0xffffffffu - (t + q)) : 0ull;
+  }
+}
+
+// The keys (logit, token) of the first n of a list's logits whose ordered bits
+// reach `floor`, in any order; returns how many.  A threshold is found bit by
+// bit from the highest bit in which the keys differ.  ONE: at most 64 groups,
+// whose keys stay in registers; else every step takes them from the list again.
+template <bool ONE>
+__device__ __forceinline__ int beam_first(const BeamList* list, int count, int n, uint32_t floor, uint64_t* out) {
+  const int lane = threadIdx.x & 63;
+  uint64_t k[4];
+  uint32_t hi = 0u, lo = 0xffffffffu;  // of the keys' upper halves
+  int all = 0;
+  #pragma unroll 1
+  for (int i = 0; i < (ONE ? 1 : count); i += 64) {
+    beam_keys(list, i + lane, count, floor, k);
+    #pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t o = (uint32_t)(k[q] >> 32);
+      hi = max(hi, o);
+      lo = min(lo, o - 1u);  // (0: none)
+      all += __popcll(__ballot(o != 0u));
     }
   }
-  hi = beam_wave_umax(hi);
-  lo = beam_wave_umin(lo);
-  int bit = hi == lo ? 31 : 63 - __builtin_clz(hi ^ lo);
-  uint64_t t = (uint64_t)hi << 32 & ~((2ull << bit) - 1ull);
-  #pragma unroll 1
-  for (; bit >= 0; --bit) {
-    const uint64_t c = t | (1ull << bit);
-    int cnt = 0;
-    #pragma unroll
-    for (int j = 0; j < P; ++j) cnt += __popcll(__ballot(k[j] >= c));
-    if (cnt >= n) t = c;
-    if (cnt == n) break;
+  uint64_t t = 1ull;
+  if (all > n) {
+    hi = beam_wave_umax(hi);
+    lo = beam_wave_umin(lo) + 1u;
+    int bit = hi == lo ? 31 : 63 - __builtin_clz(hi ^ lo);
+    t = (uint64_t)hi << 32 & ~((2ull << bit) - 1ull);
+    #pragma unroll 1
+    for (; bit >= 0; --bit) {
+      const uint64_t c = t | (1ull << bit);
+      int cnt = 0;
+      #pragma unroll 1
+      for (int i = 0; i < (ONE ? 1 : count); i += 64) {
+        if (!ONE) beam_keys(list, i + lane, count, floor, k);
+        #pragma unroll
+        for (int q = 0; q < 4; ++q) cnt += __popcll(__ballot(k[q] >= c));
+      }
+      if (cnt >= n) t = c;
+      if (cnt == n) break;
+    }
   }
   int at = 0;
-  uint32_t low = 0xffffffffu;
-  #pragma unroll
-  for (int j = 0; j < P; ++j) {
-    const uint64_t keep = __ballot(k[j] >= t);
-    if (k[j] >= t) {
-      list[at + beam_below(keep)] = beam_raw(k[j]);
-      low = min(low, (uint32_t)(k[j] >> 32));
+  #pragma unroll 1
+  for (int i = 0; i < (ONE ? 1 : count); i += 64) {
+    if (!ONE) beam_keys(list, i + lane, count, floor, k);
+    #pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint64_t keep = __ballot(k[q] >= t);
+      if (k[q] >= t) out[at + beam_below(keep)] = k[q];
+      at += __popcll(keep);
     }
-    at += __popcll(keep);
   }
-  return beam_wave_umin(low);
+  return at;
+}
+// (Not inlined: the loop over a part has a place for it a group.)
+__device__ __noinline__ int beam_first_of_many(const BeamList* list, int count, int n, uint32_t floor, uint64_t* out) {
+  return beam_first<false>(list, count, n, floor, out);
 }
 
 // One part of a row: tiles [part * a.tiles, ...) of 64 lanes x 64 bytes,
@@ -429,9 +449,9 @@ __device__ __noinline__ uint32_t beam_prune(BeamRaw* list, int count, int n) {
 // Each wave takes every fourth tile, with the next one's loads in flight, and
 // needs no other wave until the end:
 //  * a lane keeps its running maximum and sum, rescaled once a tile;
-//  * the wave keeps its candidates in LDS: those at or above a bound that n_out
-//    of the four first tiles' groups reach (the only exchange before the end),
-//    or above the n_out-th kept after a full list was cut back to n_out, so
+//  * the wave keeps its candidates in LDS, as groups of four logits that hold
+//    one at or above a bound: one that n_out of the four first tiles' groups
+//    reach, or the n_out-th kept after a full list was cut back to n_out, so
 //    that most tiles end at one comparison.
 // A tile a workgroup instead, with a bound and an exchange each, had twice the
 // instructions a logit and no loads in flight while it computed (64 x 8 rows of
@@ -440,7 +460,8 @@ template <int DT, bool MASK>
 __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   constexpr int N = BeamLoad<DT>::N, L = 4, PER = L * N, W = kPartThreads / 64, ES = 16 / N;
   constexpr int G = PER / 4, GN = 4;  // groups of 4 elements
-  __shared__ BeamRaw lists[W][kPartSlots];
+  __shared__ BeamList lists[W];
+  __shared__ uint64_t keys[W][kBeamMaxOut];
   __shared__ float redm[W], reds[W];
   __shared__ int redn[W];
   __shared__ uint32_t red[2 * W];
@@ -476,8 +497,8 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   load(wid);
   if (!beam_reads(a, row)) return;
   const float ninf = -__builtin_inff();
-  BeamRaw* list = lists[wid];
-  int count = 0;
+  BeamList* list = &lists[wid];
+  int count = 0, since = 0;    // groups in it, and those listed since the bound rose
   float m = ninf, s = 0.f;     // this lane's
   float bound = 0.f;           // candidates are at or above it; once `full`, above it in the next tile
   bool full = false, shared = false;
@@ -580,31 +601,46 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
     // have a lower token.)
     if (tile >= W && (tile / W & (tile / W - 1)) == 0) {
       const float b = beam_okey_inv(shared_bound());
-      if (b > bound) { bound = b; full = false; }
+      if (b > bound) {
+        bound = b;
+        full = false;
+        since = 0;
+      }
     }
-    if (__ballot(full ? tm > bound : tm >= bound) == 0ull) continue;
+    const uint64_t any = __ballot(full ? tm > bound : tm >= bound);
+    if (any == 0ull) continue;
     #pragma unroll
     for (int g = 0; g < G; ++g) {
-      if (__ballot(gm[g] >= bound) == 0ull) continue;
-      #pragma unroll
-      for (int i = GN * g; i < GN * g + GN; ++i) {
-        const bool pass = full ? x[i] > bound : x[i] >= bound;
-        const uint64_t b = __ballot(pass);
-        if (b == 0ull) continue;
-        if (pass) list[count + beam_below(b)] = BeamRaw{x[i], (uint32_t)(t0 + i / N * (64 * N) + i % N)};
-        count = __builtin_amdgcn_readfirstlane(count + __popcll(b));
+      const bool pass = full ? gm[g] > bound : gm[g] >= bound;
+      const uint64_t b = __ballot(pass);
+      if (b == 0ull) continue;
+      if (pass) {
+        const int i = count + beam_below(b);
+        list->x[i] = beam_f32x4{x[GN * g], x[GN * g + 1], x[GN * g + 2], x[GN * g + 3]};
+        list->token[i] = (uint32_t)(t0 + GN * g / N * (64 * N) + GN * g % N);
       }
-      if (count > kPartSlots - 64 * GN) {
+      count = __builtin_amdgcn_readfirstlane(count + __popcll(b));
+      since = __builtin_amdgcn_readfirstlane(since + __popcll(b));
+      if (count > kPartSlots - 64) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const float low = beam_okey_inv((uint32_t)__builtin_amdgcn_readfirstlane((int)beam_prune(list, count, a.n_out)));
+        count = __builtin_amdgcn_readfirstlane(
+            beam_first_of_many(list, count, a.n_out, kBeamNegInf + 1u, keys[wid]));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        count = a.n_out;
+        uint32_t low = 0xffffffffu;
+        if (lane < count) {
+          const uint64_t k = keys[wid][lane];
+          low = (uint32_t)(k >> 32);
+          list->x[lane] = beam_f32x4{beam_okey_inv(low), ninf, ninf, ninf};
+          list->token[lane] = 0xffffffffu - (uint32_t)k;
+        }
+        const float least = beam_okey_inv(beam_wave_umin(low));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         // a later logit of this tile may equal it with a lower token
-        if (low > bound) { bound = low; full = false; }
+        if (least > bound) { bound = least; full = false; }
+        since = count;
       }
     }
-    if (count >= a.n_out) full = true;
-
+    if (since >= a.n_out) full = true;
   }
   if (a.tiles > W) shared_bound();  // (else it has not moved since the first)
   {
@@ -630,33 +666,15 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
     #pragma unroll
     for (int w = 0; w < W; ++w) s += reds[w] * __expf(fmaxf(redm[w], kBeamLowest) - m);
   }
-  // the wave's candidates that reach it, at most 64 of them, as keys
-  if (count > 0 && a.tiles > W) {
-    int kept = 0;
-    for (int j = 0; j < count; j += 64) {
-      BeamRaw c{0.f, 0u};
-      bool keep = false;
-      if (j + lane < count) {
-        c = list[j + lane];
-        keep = beam_okey(c.logit) >= last;
-      }
-      const uint64_t b = __ballot(keep);
-      if (keep) list[kept + beam_below(b)] = c;
-      kept = __builtin_amdgcn_readfirstlane(kept + __popcll(b));
-    }
-    count = kept;
-  }
+  // the wave's first n_out that reach it
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  if (count > a.n_out) {
-    beam_prune(list, count, a.n_out);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    count = a.n_out;
-  }
-  uint64_t mine = 0ull;
-  if (lane < count) {
-    mine = beam_key(list[lane]);
-    reinterpret_cast<uint64_t*>(list)[lane] = mine;
-  }
+  const uint32_t floor = a.tiles > W ? max(last, kBeamNegInf + 1u) : kBeamNegInf + 1u;
+  if (count > 64)
+    count = __builtin_amdgcn_readfirstlane(beam_first_of_many(list, count, a.n_out, floor, keys[wid]));
+  else if (count > 0)
+    count = __builtin_amdgcn_readfirstlane(beam_first<true>(list, count, a.n_out, floor, keys[wid]));
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const uint64_t mine = lane < count ? keys[wid][lane] : 0ull;
   if (lane == 0) redn[wid] = count;
   __syncthreads();
   if (tid == 0) {
@@ -670,9 +688,8 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   #pragma unroll 1
   for (int w = 0; w < W; ++w) {
     const int n = redn[w];
-    const uint64_t* other = reinterpret_cast<const uint64_t*>(lists[w]);
     #pragma unroll 4
-    for (int i = 0; i < n; ++i) rank += other[i] > mine;
+    for (int i = 0; i < n; ++i) rank += keys[w][i] > mine;
   }
   if (lane < count && rank < a.n_out) a.cand[slot * a.n_out + rank] = mine;
 }
