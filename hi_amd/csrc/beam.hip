@@ -35,7 +35,7 @@ constexpr int kBeamMax = HI_ROCM_BEAM_MAX;
 constexpr int kBeamMaxOut = HI_ROCM_BEAM_MAX_OUT;
 constexpr int kPartThreads = 256;
 constexpr int kTileElems = 4096;     // elements of a part of a short step
-constexpr int kTileSlots = 256;      // candidates that such a part can hold before it ranks them
+constexpr int kTileSlots = 512;      // candidates that such a part can hold before it ranks them
 constexpr int kPartSlots = 256;      // groups of four logits that a wave of a streamed part can hold
 constexpr int kFinishThreads = 512;
 constexpr int kFinishHeld = 4;       // candidates a thread keeps in registers
@@ -57,6 +57,7 @@ struct BeamArgs {
   const uint32_t* mask;       // [rows][mask_words] or null
   int V, K, n_out, n_parts, mask_words;
   int tiles;                  // of a part
+  int list_threads;           // log2 of the threads that take a part's list in the finish
   uint32_t eos;
   BeamPart* parts;            // [rows][n_parts]
   uint64_t* cand;             // [rows][n_parts][n_out], descending
@@ -115,6 +116,13 @@ __device__ __forceinline__ float beam_wave_sum(float v) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)b(), 63));
 }
 
+// The sum over a lane's eight neighbours 8 i .. 8 i + 7.
+__device__ __forceinline__ int beam_sum8(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);   // lanes 1, 0, 3, 2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);   // lanes 2, 3, 0, 1
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);  // mirrored within the eight
+}
+
 // Whether a row takes part: a beam whose score is not finite has no
 // candidates, a finished one has a single candidate that needs no logits.
 __device__ __forceinline__ bool beam_reads(const BeamArgs& a, int row) {
@@ -149,7 +157,8 @@ __device__ __forceinline__ uint32_t beam_wave_nth(const uint32_t (&key)[G], int 
 
 // A bound that at least n keys of the workgroup (W waves, G keys a lane)
 // reach, if it holds n above `floor`: the smallest of the waves' ceil(n /
-// W)-th keys, or, where a wave has not as many, the largest of their n-th.
+// W)-th keys, or, where a wave has not as many (a row's last part), the m-th
+// largest of their ceil(n / m)-th, m = W / 2, W / 4, ..., 1.
 template <int G, int W>
 __device__ __forceinline__ uint32_t beam_bound(const uint32_t (&key)[G], int n, uint32_t floor, uint32_t* red) {
   const int wid = threadIdx.x >> 6;
@@ -159,12 +168,27 @@ __device__ __forceinline__ uint32_t beam_bound(const uint32_t (&key)[G], int n, 
   uint32_t b = red[0];
   #pragma unroll
   for (int w = 1; w < W; ++w) b = min(b, red[w]);
-  if (b > floor || W == 1) return b;
-  const uint32_t full = beam_wave_nth<G>(key, n);
-  if ((threadIdx.x & 63) == 0) red[W + wid] = full;
-  __syncthreads();
-  #pragma unroll
-  for (int w = 0; w < W; ++w) b = max(b, red[W + w]);
+  int had = (n + W - 1) / W;
+  #pragma unroll 1
+  for (int m = W / 2; m >= 1 && b <= floor; m /= 2) {
+    uint32_t mine = red[threadIdx.x & (W - 1)];  // (lane w < W: wave w's)
+    // (waves without as many keys have no more)
+    if (__popcll(__ballot(mine > floor) & ((1ull << W) - 1ull)) < m) continue;
+    const int need = (n + m - 1) / m;
+    if (need != had) {
+      const uint32_t more = beam_wave_nth<G>(key, need);
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) red[wid] = more;
+      __syncthreads();
+      had = need;
+      mine = red[threadIdx.x & (W - 1)];
+    }
+    #pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)mine, w);
+      if (__popcll(__ballot(mine >= r) & ((1ull << W) - 1ull)) >= m) b = max(b, r);
+    }
+  }
   return b;
 }
 
@@ -198,7 +222,7 @@ __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
   constexpr int G = PER / 8;  // groups a thread
   __shared__ uint64_t slots[kTileSlots];
   __shared__ uint64_t red64[W];
-  __shared__ uint32_t red[2 * W];
+  __shared__ uint32_t red[W];
   __shared__ float redf[W], reds[W];
   __shared__ uint32_t counter;
   const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -306,7 +330,7 @@ __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
     }
   }
   __syncthreads();
-  const int n = (int)counter;
+  int n = (int)counter;
   uint64_t* out = a.cand + slot * a.n_out;
   const int keep = min(n, a.n_out);
   if (tid == 0) {
@@ -316,12 +340,29 @@ __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
     a.parts[slot] = BeamPart{m, s, (uint32_t)keep, 0u};
   }
   if (n <= kTileSlots) {
-    // rank by counting
-    if (tid < n) {
-      const uint64_t mine = slots[tid];
+    // far more than n_out (a row's last part): only those that reach a better bound
+    if (n > 2 * a.n_out + 64) {
+      static_assert(kTileSlots == 2 * kPartThreads, "two slots a thread");
+      const uint64_t own[2] = {tid < n ? slots[tid] : 0ull, tid + kPartThreads < n ? slots[tid + kPartThreads] : 0ull};
+      const uint32_t half[2] = {(uint32_t)(own[0] >> 32), (uint32_t)(own[1] >> 32)};
+      const uint32_t least = beam_bound<2, W>(half, a.n_out, 0u, red);
+      __syncthreads();
+      if (tid == 0) counter = 0u;
+      __syncthreads();
+      #pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (half[j] >= least) slots[atomicAdd(&counter, 1u)] = own[j];
+      __syncthreads();
+      n = (int)counter;
+    }
+    // ranks by counting, eight lanes a candidate
+    for (int j = tid >> 3; j < n; j += kPartThreads / 8) {
+      const uint64_t mine = slots[j];
       int rank = 0;
-      for (int i = 0; i < n; ++i) rank += slots[i] > mine;
-      if (rank < a.n_out) out[rank] = mine;
+      #pragma unroll 4
+      for (int i = tid & 7; i < n; i += 8) rank += slots[i] > mine;
+      rank = beam_sum8(rank);
+      if ((tid & 7) == 0 && rank < a.n_out) out[rank] = mine;
     }
     return;
   }
@@ -464,7 +505,7 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   __shared__ uint64_t keys[W][kBeamMaxOut];
   __shared__ float redm[W], reds[W];
   __shared__ int redn[W];
-  __shared__ uint32_t red[2 * W];
+  __shared__ uint32_t red[W];
   const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const char* p0 = (const char*)a.logits + (int64_t)row * a.row_stride * ES;
@@ -707,33 +748,36 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
   constexpr int W = kFinishThreads / 64;
   __shared__ BeamCand slots[kFinishSlots];
   __shared__ BeamCand redc[W];
-  __shared__ float lse[kBeamMax];
+  __shared__ float lse[kBeamMax], base[kBeamMax];  // base: the beams' scores
   __shared__ uint32_t state[kBeamMax];  // 0: no candidates, 1: its parts' candidates, 2: finished
-  __shared__ uint32_t red[2 * W];
+  __shared__ uint32_t red[W];
   __shared__ uint32_t counter;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int row0 = b * a.K;
   const float ninf = -__builtin_inff();
   if (tid == 0) counter = 0u;
-  // item i: place i % n_out of part (i / n_out) % n_parts of beam i / (n_out * n_parts);
-  // a finished beam has one, in its first place.  Each wave takes items of all
-  // beams, parts and places alike, so that its share of the best ones is even.
-  // The first kFinishHeld a thread are loaded ahead of the beams' sums (places
-  // that hold no candidate are loaded too, and dropped by their part's count).
-  const int first = lane * W + ((wid + lane) & (W - 1));
-  const int per_beam = a.n_parts * a.n_out, total = a.K * per_beam;
+  // A list: what a part kept of a beam, in order (a finished beam has one
+  // candidate, the first of its first list).  Q threads take a list, thread
+  // `sub` every Q-th place from its own, and the lists beyond 512 / Q in further
+  // rounds.  Lists go round the waves, so that beams and places are spread
+  // evenly over them.  The first kFinishHeld a thread are loaded ahead of the
+  // beams' sums (places that hold no candidate too: dropped by their count).
+  // First a bound from the threads' first candidates, then all that reach it:
+  // the work follows n_out and the lists, not their product (32 f32 rows of
+  // 151,936 as one request's beams, 64 candidates: the whole step 28 us, with
+  // every place of every list rated 107).
+  const int lists = a.K * a.n_parts;
+  const int qs = a.list_threads, Q = 1 << qs, turn = lane * W + wid;
+  auto sub_of = [&](int list) { return (turn + list + (list >> 3)) & (Q - 1); };
+  auto cand = [&](int list, int place) { return a.cand[((int64_t)row0 * a.n_parts + list) * a.n_out + place]; };
+  auto kept = [&](int list) { return (int)a.parts[(int64_t)row0 * a.n_parts + list].n; };
+  const int list0 = turn >> qs, sub0 = sub_of(list0);
   uint64_t held[kFinishHeld];
-  uint32_t count[kFinishHeld];
+  int kept0 = 0;
+  if (list0 < lists) kept0 = kept(list0);
   #pragma unroll
-  for (int h = 0; h < kFinishHeld; ++h) {
-    const int i = first + h * kFinishThreads;
-    held[h] = 0ull;
-    count[h] = 0u;
-    if (i < total) {
-      held[h] = a.cand[(int64_t)row0 * per_beam + i];
-      count[h] = a.parts[(int64_t)row0 * a.n_parts + i / a.n_out].n;
-    }
-  }
+  for (int j = 0; j < kFinishHeld; ++j)
+    held[j] = list0 < lists && sub0 + j * Q < a.n_out ? cand(list0, sub0 + j * Q) : 0ull;
   for (int k = wid; k < a.K; k += W) {
     const int row = row0 + k;
     const float c = a.scores[row];
@@ -758,20 +802,20 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
         st = 1u;
       }
     }
-    if (lane == 0) { lse[k] = l; state[k] = st; }
+    if (lane == 0) { lse[k] = l; base[k] = c; state[k] = st; }
   }
   __syncthreads();
-  auto rated = [&](int i, uint64_t lo, uint32_t n) -> BeamCand {
-    const int k = i / per_beam, r = i - k * per_beam;
+  auto rated = [&](int list, int place, uint64_t lo, int n) -> BeamCand {
+    const int k = list / a.n_parts;
     const uint32_t st = state[k];
     BeamCand x{0ull, 0ull};
     if (st == 0u) return x;
-    float score = a.scores[row0 + k];
+    float score = base[k];
     if (st == 2u) {
-      if (r != 0) return x;
+      if (place != 0 || list != k * a.n_parts) return x;
       lo = 0xffffffffu - a.eos;
     } else {
-      if ((uint32_t)(r % a.n_out) >= n) return x;
+      if (place >= n) return x;
       score += beam_okey_inv((uint32_t)(lo >> 32)) - lse[k];
       if (!beam_finite(score)) return x;
     }
@@ -779,30 +823,51 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
     x.hi = ((uint64_t)beam_okey(score) << 32) | (0xffffffffu - (uint32_t)k);
     return x;
   };
-  auto item = [&](int i) -> BeamCand {
-    return rated(i, a.cand[(int64_t)row0 * per_beam + i], a.parts[(int64_t)row0 * a.n_parts + i / a.n_out].n);
-  };
+  auto score_of = [](const BeamCand& x) { return (uint32_t)(x.hi >> 32); };
+  // a bound that n_out of the threads' first candidates reach
   uint32_t best[1] = {0u};
   BeamCand mine[kFinishHeld];
   #pragma unroll
-  for (int h = 0; h < kFinishHeld; ++h) {
-    const int i = first + h * kFinishThreads;
-    mine[h] = i < total ? rated(i, held[h], count[h]) : BeamCand{0ull, 0ull};
-    best[0] = max(best[0], (uint32_t)(mine[h].hi >> 32));
+  for (int j = 0; j < kFinishHeld; ++j) {
+    mine[j] = BeamCand{0ull, 0ull};
+    if (list0 < lists && sub0 + j * Q < a.n_out) mine[j] = rated(list0, sub0 + j * Q, held[j], kept0);
   }
-  for (int i = first + kFinishHeld * kFinishThreads; i < total; i += kFinishThreads)
-    best[0] = max(best[0], (uint32_t)(item(i).hi >> 32));
-  const uint32_t bound = max(beam_bound<1, W>(best, a.n_out, 0u, red), 1u);
+  best[0] = score_of(mine[0]);
+  for (int list = list0 + (kFinishThreads >> qs); list < lists; list += kFinishThreads >> qs)
+    best[0] = max(best[0], score_of(rated(list, sub_of(list), cand(list, sub_of(list)), kept(list))));
+  uint32_t bound = max(beam_bound<1, W>(best, a.n_out, 0u, red), 1u);
   auto offer = [&](const BeamCand& x) {
-    if ((uint32_t)(x.hi >> 32) >= bound) {
-      const uint32_t o = atomicAdd(&counter, 1u);
-      if (o < (uint32_t)kFinishSlots) slots[o] = x;
-    }
+    if (score_of(x) < bound) return false;
+    const uint32_t o = atomicAdd(&counter, 1u);
+    if (o < (uint32_t)kFinishSlots) slots[o] = x;
+    return true;
   };
-  #pragma unroll
-  for (int h = 0; h < kFinishHeld; ++h) offer(mine[h]);
-  for (int i = first + kFinishHeld * kFinishThreads; i < total; i += kFinishThreads) offer(item(i));
-  __syncthreads();
+  for (;;) {
+    // all that reach it: a list's scores descend
+    bool more = true;
+    #pragma unroll
+    for (int j = 0; j < kFinishHeld; ++j)
+      if (more) more = offer(mine[j]);
+    int place = more ? sub0 + kFinishHeld * Q : a.n_out;
+    for (int list = list0; list < lists;) {
+      if (place < a.n_out && offer(rated(list, place, cand(list, place), kept(list)))) {
+        place += Q;
+      } else {
+        list += kFinishThreads >> qs;
+        place = sub_of(list);
+      }
+    }
+    __syncthreads();
+    if (counter <= (uint32_t)kFinishSlots) break;
+    // too many: again, with a bound that n_out of those that were kept reach
+    const uint32_t key[1] = {score_of(slots[tid])};
+    const uint32_t higher = beam_bound<1, W>(key, a.n_out, 0u, red);
+    if (higher <= bound) break;
+    bound = higher;
+    __syncthreads();
+    if (tid == 0) counter = 0u;
+    __syncthreads();
+  }
   const int n = (int)counter;
   const int64_t o0 = (int64_t)b * a.n_out;
   auto put = [&](int r, const BeamCand& x) {
@@ -821,20 +886,25 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
     a.out_finished[o0 + r] = 1;
   }
   if (n <= kFinishSlots) {
-    for (int j = tid; j < n; j += kFinishThreads) {
+    // ranks by counting, eight lanes a candidate
+    for (int j = tid >> 3; j < n; j += kFinishThreads / 8) {
       const BeamCand x = slots[j];
       int rank = 0;
-      for (int i = 0; i < n; ++i) rank += beam_before(slots[i], x) ? 1 : 0;
-      if (rank < a.n_out) put(rank, x);
+      #pragma unroll 4
+      for (int i = tid & 7; i < n; i += 8) rank += beam_before(slots[i], x) ? 1 : 0;
+      rank = beam_sum8(rank);
+      if ((tid & 7) == 0 && rank < a.n_out) put(rank, x);
     }
     return;
   }
   // many equal scores: one candidate after another
+  const int total = lists * a.n_out;
   BeamCand prev{~0ull, ~0ull};
   for (int r = 0; r < keep; ++r) {
     BeamCand top{0ull, 0ull};
     for (int i = tid; i < total; i += kFinishThreads) {
-      const BeamCand x = item(i);
+      const int list = i / a.n_out, place = i - list * a.n_out;
+      const BeamCand x = rated(list, place, cand(list, place), kept(list));
       if (beam_before(prev, x) && beam_before(x, top)) top = x;
     }
     #pragma unroll
@@ -860,19 +930,25 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
 
 // How a row is cut: into parts of kTileElems while all rows' parts are few, or
 // into parts of `tiles` streamed tiles (a multiple of four: one a wave) that
-// leave about four workgroups a CU.  Whole steps, us, cut to parts and streamed:
-// 4 rows of 151,936 11.1 and 13.7 (f32), 11.0 and 17.9 (bf16); 128 rows 24.4 and
-// 26.1, 23.6 and 27.9; 256 rows (9,728 parts) 35.5 and 36.4, 34.2 and 34.2; 512
-// rows of bf16, a fifth of them finished, 53 and 47.
-constexpr int kBeamFewParts = 8192;
+// leave about four workgroups a CU.  Whole steps of 8 candidates, us, cut to
+// parts and streamed:
+//   4 rows of 151,936 (152 parts): f32 11.2 and 12.6, bf16 11.3 and 15.5
+//   384 rows of 50,257 (4,992): 23.2 and 26.2, 23.0 and 27.3
+//   512 rows of 50,257 (6,656): 28.3 and 28.7, 27.1 and 27.1
+//   1,024 rows of 32,000 (8,192): 36.0 and 28.7, 35.2 and 27.5
+// A mask costs the streaming kernel more (its words come with every tile):
+//   1,024 rows of 50,257 (13,312): 60.2 and 58.5, 54.3 and 59.0
+//   512 rows of 151,936 (19,456): 82.6 and 74.2, 69.7 and 76.1
+//   768 rows of 128,256 (24,576): 101.1 and 104.1, 88.8 and 76.9
+constexpr int kBeamFewParts = 6144, kBeamFewMasked = 3 * kBeamFewParts;
 struct BeamCut {
   int tiles;  // 0: parts of kTileElems
   int parts;
 };
-BeamCut beam_cut(int64_t rows, int V, int dtype) {
+BeamCut beam_cut(int64_t rows, int V, int dtype, bool masked) {
   const int64_t len = (int64_t)V + 7;  // (up to 7 elements before the row's start)
   const int64_t few = (len + kTileElems - 1) / kTileElems;
-  if (rows * few <= kBeamFewParts) return BeamCut{0, (int)few};
+  if (rows * few <= (masked ? kBeamFewMasked : kBeamFewParts)) return BeamCut{0, (int)few};
   const int64_t tile = 64 * (dtype == HI_ROCM_DTYPE_F32 ? 16 : 32), steps = (len + 4 * tile - 1) / (4 * tile);
   const int64_t want = std::max<int64_t>(1, std::min(steps, (1024 + rows - 1) / rows));
   const int64_t tiles = 4 * ((steps + want - 1) / want);
@@ -994,7 +1070,8 @@ int hi_rocm_beam_workspace_bytes(int max_batch, int beams, int vocab, int n_out,
   int64_t slots = 0;
   for (int b = 1; b <= max_batch; ++b)
     for (int dtype : {HI_ROCM_DTYPE_F32, HI_ROCM_DTYPE_BF16})
-      slots = std::max(slots, (int64_t)b * beams * beam_cut((int64_t)b * beams, vocab, dtype).parts);
+      for (bool masked : {false, true})
+        slots = std::max(slots, (int64_t)b * beams * beam_cut((int64_t)b * beams, vocab, dtype, masked).parts);
   *out_bytes = beam_layout(slots, n_out).total;
   return HI_ROCM_OK;
 }
@@ -1019,9 +1096,10 @@ int hi_rocm_beam_select(const void* logits, int dtype, int batch, int beams, int
   const int rows = batch * beams;
   BeamArgs a;
   memset(&a, 0, sizeof(a));
-  const BeamCut cut = beam_cut(rows, vocab, dtype);
+  const BeamCut cut = beam_cut(rows, vocab, dtype, mask_words != nullptr);
   a.tiles = cut.tiles;
   a.n_parts = cut.parts;
+  while ((2 << a.list_threads) * beams * a.n_parts <= kFinishThreads && (1 << a.list_threads) < n_out) ++a.list_threads;
   const BeamLayout L = beam_layout((int64_t)rows * a.n_parts, n_out);
   if (workspace == nullptr || workspace_bytes < L.total || (uintptr_t)workspace % 16 != 0)
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_beam_select: workspace missing, too small or not 16-byte aligned");

@@ -340,3 +340,85 @@ def test_refusals(hip):
         reorder_states(flat.as_strided((6, 8), (4, 1)), par)
     with pytest.raises(_lib.HiRocmError):  # dst overlaps src
         reorder_states(flat[:48].view(6, 8), par, dst=flat[8:56].view(6, 8))
+
+
+def definition_on_gpu(x, c, mask, K, n):
+    """`definition` without finished beams, rows all at once."""
+    x = x.double().masked_fill(x.isnan(), -torch.inf)
+    if mask is not None:
+        x = x.masked_fill(~mask, -torch.inf)
+    m = x.amax(1, keepdim=True)
+    lse = m + (x - m).exp().sum(1, keepdim=True).log()
+    top, ids = torch.sort(x, dim=1, descending=True, stable=True)
+    top, ids = top[:, :n], ids[:, :n]
+    score = torch.as_tensor(c, dtype=torch.float32).double().cuda()[:, None] + (top - lse)
+    ok = torch.isfinite(score)
+    big = lambda t: t[ok.expand_as(t)].abs().max().item()
+    tol = EPS * (4 * big(lse.expand_as(score)) + 2 * big(top - lse) + 2 * big(score)) + SUM_EPS
+    out = []
+    for s, l, i, k in zip(*(t.view(-1, K, n).cpu().tolist() for t in (score, top, ids, ok))):
+        cand = [(s[b][j], b, l[b][j], i[b][j]) for b in range(K) for j in range(n) if k[b][j]]
+        out.append(sorted(cand, key=lambda t: (-t[0], t[1], -t[2], t[3])))
+    return out, tol
+
+
+def _streamed(kind, rows, V, dtype):
+    """Rows for the kernel that streams a row through four waves."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(rows, V, generator=g, device="cuda").mul_(2.5)
+    if kind == "few values":  # ties all over, also among the best
+        x = (x * 2).round() / 2
+    if kind == "odd":
+        up = torch.arange(V, device="cuda", dtype=torch.float32)
+        x[0] = up * 1e-3  # every tile holds better ones than those before it
+        x[1] = -up * 1e-3
+        x[2] = 1.0
+        x[3, : V - 3] = -torch.inf
+        x[4, ::3] = torch.nan
+        x[8] = torch.where(up % 1000 == 999, 8.0, 0.0)
+        x[9, V - 200:] = 50.0
+    if kind == "extreme":  # (scores of these sizes leave only the order within a beam to check)
+        x[5, :] = -3.0e38
+        x[5, V // 2] = -2.9e38
+        x[6, 7] = 3.0e38
+        x[7] = (torch.arange(V, device="cuda") % 5) - 1e4
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind,K,V,n", [("plain", 8, 40000, 16), ("few values", 4, 40003, 8), ("few values", 8, 40000, 64),
+                                        ("odd", 2, 40000, 16), ("odd", 2, 33333, 64), ("extreme", 2, 33333, 16), ("plain", 32, 25001, 64)])
+def test_streamed_rows(hip, dtype, kind, K, V, n):
+    rows = 1024
+    x = _streamed(kind, rows, V, dtype)
+    c = -np.random.default_rng(n).random(rows).astype(np.float32)
+    res = run(x, c, K, n)
+    want, tol = definition_on_gpu(x, c, None, K, n)
+    check(res, want, tol, K, n, None, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("share", [0.3, 0.001])
+def test_streamed_masks(hip, dtype, share):
+    rows, K, V, n = 2048, 4, 40000, 16
+    x = _streamed("few values", rows, V, dtype)
+    mask = torch.rand(rows, V, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < share
+    mask[5] = False
+    c = -np.random.default_rng(3).random(rows).astype(np.float32)
+    res = run(x, c, K, n, mask=mask)
+    want, tol = definition_on_gpu(x, c, mask, K, n)
+    check(res, want, tol, K, n, None, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,K,V,n", [(1, 32, 9000, 64), (2, 16, 8192 + 384, 64), (1, 32, 50257, 64), (3, 1, 4096 + 1105, 64),
+                                     (2, 7, 37000, 56), (1, 32, 151936, 64), (5, 3, 8192 + 3, 40)])
+def test_many_candidates(hip, dtype, B, K, V, n):
+    """Parts that end early, and as many candidates as a request may keep."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(B * K, V, generator=g, device="cuda").mul_(2.5).to(dtype)
+    for spread in (0.5, 40.0):
+        c = (-np.random.default_rng(K).random(B * K) * spread).astype(np.float32)
+        res = run(x, c, K, n)
+        want, tol = definition_on_gpu(x, c, None, K, n)
+        check(res, want, tol, K, n, None, None)
