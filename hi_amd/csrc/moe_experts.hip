@@ -403,7 +403,7 @@ __device__ __forceinline__ void moe_fill(const MoeSources<L>& src, bool in, int 
   }
 }
 
-template <int MT, int NT, int KH, int BK>
+template <int MT, int NT, int KH, int BK, int WM>
 __device__ __forceinline__ void moe_read(const char* __restrict__ xb, const char* __restrict__ wb, int r, int g,
                                          moe_bf16x8 (&xf)[KH][MT], moe_bf16x8 (&wf)[KH][NT]) {
   #pragma unroll
@@ -413,18 +413,18 @@ __device__ __forceinline__ void moe_read(const char* __restrict__ xb, const char
     for (int t = 0; t < NT; ++t) wf[h][t] = *reinterpret_cast<const moe_bf16x8*>(wb + t * (32 * BK) + at);
     #pragma unroll
     for (int m = 0; m < MT; ++m)
-      xf[h][m] = *reinterpret_cast<const moe_bf16x8*>(xb + m * (64 * BK) + at);
+      xf[h][m] = *reinterpret_cast<const moe_bf16x8*>(xb + m * (WM * 32 * BK) + at);
   }
 }
 
-// A wave's results, MT x 16 places (every other 16 from p0) of NT x 16 columns
+// A wave's results, MT x 16 places (every WM-th 16 from p0) of NT x 16 columns
 // (from c0, with swiglu half as many), by way of its own LDS: 64 places at a
 // time in rows of 64 columns, written out 16 bytes a lane, a row's bytes next to each other.
 // Stored from the lanes that hold them, each store would touch 16 rows, and
 // the unrolled code would be ten times as long.
 constexpr int kMoeOutBytes = 16384;
 
-template <int MT, int NT>
+template <int MT, int NT, int WM>
 __device__ __forceinline__ void moe_tile_out(const GroupedArgs& a, moe_f32x4 (&acc)[MT][NT], char* mem, int p0, int i1,
                                              int c0, int cols_out, int lane) {
   static_assert(NT == 4, "64 columns a wave");
@@ -441,7 +441,7 @@ __device__ __forceinline__ void moe_tile_out(const GroupedArgs& a, moe_f32x4 (&a
   typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
   #pragma unroll
   for (int half = 0; half < (MT + 3) / 4; ++half) {
-    if (p0 + half * 128 >= i1) return;
+    if (p0 + half * (WM * 64) >= i1) return;
     // row j of 64 values: the 16-byte chunk c at c ^ (j & 7)
     #pragma unroll
     for (int m = half * 4; m < half * 4 + 4 && m < MT; ++m) {
@@ -463,7 +463,7 @@ __device__ __forceinline__ void moe_tile_out(const GroupedArgs& a, moe_f32x4 (&a
     const int c = lane % lanes, col = c0 + c * n;
     #pragma unroll 1
     for (int j = lane / lanes; j < (MT < 4 ? MT * 16 : 64); j += rows) {
-      const int p = p0 + half * 128 + (j >> 4) * 32 + (j & 15);
+      const int p = p0 + half * (WM * 64) + (j >> 4) * (WM * 16) + (j & 15);
       if (p >= i1) break;
       const uint4 v = *reinterpret_cast<const uint4*>(mem + j * (64 * es) + (c ^ (j & 7)) * 16);
       char* to = (char*)a.out + ((int64_t)p * a.out_stride + col) * es;
@@ -483,13 +483,13 @@ __device__ __forceinline__ void moe_tile_out(const GroupedArgs& a, moe_f32x4 (&a
   }
 }
 
-template <int BM, int BN, int MT, int BK, int NB>
+template <int BM, int BN, int MT, int BK, int NB>  // MT: of BM / 16 / WM, what the tile has places for
 __device__ __forceinline__ void moe_many_tile(const GroupedArgs& a, const MoeWork& wk, char* moe_smem) {
   constexpr int T = 512, CH = BK / 8;                    // 16-byte chunks of a row
   constexpr int XL = BM * CH / T, WL = BN * CH / T;      // loads a thread
-  constexpr int WM = 2, WN = 4, NT = BN / WN / 16, KH = BK / 32;
+  constexpr int WN = BN / 64, WM = 8 / WN, NT = 4, KH = BK / 32;
   constexpr int ROW = BK * 2, STEP = (BM + BN) * ROW;
-  static_assert(MT * 32 <= BM && XL >= 1 && WL >= 1 && BM * CH % T == 0 && BN * CH % T == 0 && NT % 2 == 0, "tile split");
+  static_assert(MT * WM * 16 <= BM && XL >= 1 && WL >= 1 && BM * CH % T == 0 && BN * CH % T == 0, "tile split");
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wid % WM, wn = wid / WM;
@@ -536,7 +536,7 @@ __device__ __forceinline__ void moe_many_tile(const GroupedArgs& a, const MoeWor
   for (int s = 0; s < steps; ++s) {
     moe_bf16x8 xf[KH][MT], wf[KH][NT];
     const char* b = moe_smem + s % NB * STEP;
-    moe_read<MT, NT, KH, BK>(b + (wm * 16 + r) * ROW, b + BM * ROW + (wn * WR + r) * ROW, r, g, xf, wf);
+    moe_read<MT, NT, KH, BK, WM>(b + (wm * 16 + r) * ROW, b + BM * ROW + (wn * WR + r) * ROW, r, g, xf, wf);
     fill(s + NB - 1);
     moe_wait<(XL + WL) * (NB - 2)>();
     moe_barrier();
@@ -554,25 +554,25 @@ __device__ __forceinline__ void moe_many_tile(const GroupedArgs& a, const MoeWor
   if (wid < 4) moe_barrier();
   moe_wait<0>();  // no load may still write LDS when it is used again, or the workgroup ends
   moe_barrier();
-  moe_tile_out<MT, NT>(a, acc, moe_smem + wid * kMoeOutBytes, wk.i0 + wm * 16, wk.i1,
+  moe_tile_out<MT, NT, WM>(a, acc, moe_smem + wid * kMoeOutBytes, wk.i0 + wm * 16, wk.i1,
                        c0 + wn * (a.swiglu ? WR / 2 : WR), cols_out, lane);
 }
 
-// Two waves share the places, every other 16 of them, so a tile of fewer
-// places than BM is multiplied as one of a quarter, a half or three quarters.
-// (32,768 places of 64 experts, 2048 x 2048: 311 us against 322 with every tile
-// multiplied whole.)
+// WM waves share the places, every WM-th 16 of them, so a tile of fewer places
+// than BM is multiplied as one of a quarter, a half or three quarters (with four
+// waves, a half).  (32,768 places of 64 experts, 2048 x 2048: 311 us against 322
+// with every tile multiplied whole.)
 template <int BM, int BN, int BK, int NB>
 __global__ void __launch_bounds__(512) moe_many_kernel(GroupedArgs a) {
   extern __shared__ __align__(16) char moe_smem[];
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? BN / 2 : BN;
   MoeWork wk;
   if (!moe_work<BM>(a, (cols_out + per - 1) / per, wk)) return;
-  constexpr int MT = BM / 32;
+  constexpr int WM = 8 / (BN / 64), MT = BM / 16 / WM;
   switch ((wk.i1 - wk.i0 + BM / 4 - 1) / (BM / 4)) {
-    case 1: return moe_many_tile<BM, BN, MT / 4, BK, NB>(a, wk, moe_smem);
+    case 1: return moe_many_tile<BM, BN, (MT + 3) / 4, BK, NB>(a, wk, moe_smem);
     case 2: return moe_many_tile<BM, BN, MT / 2, BK, NB>(a, wk, moe_smem);
-    case 3: return moe_many_tile<BM, BN, MT * 3 / 4, BK, NB>(a, wk, moe_smem);
+    case 3: return moe_many_tile<BM, BN, (MT * 3 + 3) / 4, BK, NB>(a, wk, moe_smem);
     default: return moe_many_tile<BM, BN, MT, BK, NB>(a, wk, moe_smem);
   }
 }
@@ -615,6 +615,10 @@ hipError_t launch_many(const GroupedArgs& a, hipStream_t st) {
 //     64: 101, 109, 116, 128; tiles of 128: 124, 124, 124, 126
 //   128 experts, 1024 x 1536: 77, 92, 117, 166; 76, 82, 90, 135; 90, 94, 99, 108;
 //     78, 77, 78, 82
+// Where tiles of 128 x 256 would leave half the CUs idle, tiles of 128 x 128: us
+// with 256 and 128 columns: 1,358 places of 8 experts, 1880 x 992: 30.5 and
+// 23.6; 600 of 16, 2048 x 1024: 27.7 and 22.6; 800 of 16, 1024 x 512: 15.8 and
+// 12.9.
 // Tiles of 128 or of 256 places by the rounds that their workgroups, one a CU,
 // make: up to two count whole, and a round of 256 as 7/4 of one of 128.  An
 // expert's last tile counts as half a tile.  us at 128, 192, 256 and 512 places:
@@ -626,11 +630,12 @@ hipError_t launch_grouped(const GroupedArgs& a, hipStream_t st) {
   if (avg <= 8) return launch_few<1>(a, st);
   if (avg <= 20) return launch_few<2>(a, st);
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? 128 : 256;
-  auto rounds = [&](int bm) {  // in workgroups
+  auto wgs = [&](int bm) {
     const int64_t halves = avg < bm ? 2 * (int64_t)a.experts : 2 * (int64_t)a.places / bm + a.experts;
-    const int64_t n = halves * ((cols_out + per - 1) / per) / 2;
-    return n <= 512 ? (n + 255) / 256 * 256 : n;
+    return halves * ((cols_out + per - 1) / per) / 2;
   };
+  auto rounds = [&](int bm) { return wgs(bm) <= 512 ? (wgs(bm) + 255) / 256 * 256 : wgs(bm); };
+  if (wgs(128) <= 128) return launch_many<128, 128, 64, 4>(a, st);
   if (7 * rounds(256) < 4 * rounds(128)) return launch_many<256, 256, 32, 4>(a, st);
   return launch_many<128, 256, 64, 3>(a, st);
 }

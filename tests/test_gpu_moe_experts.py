@@ -256,3 +256,28 @@ def test_refusals(hip):
     wide = torch.zeros(4, 64, device="cuda").bfloat16()
     with pytest.raises(_lib.HiRocmError):  # rows that do not start on 16 bytes
         grouped_product(wide[:, 4:36], w, groups)
+
+
+@pytest.mark.parametrize("kind", ["spread", "one", "strays"])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("tokens,top_k,experts,cols,k", [(1200, 1, 40, 1030, 72), (2000, 2, 24, 1536, 136),
+                                                         (4800, 1, 16, 2048, 104), (2500, 4, 12, 1800, 64)])
+def test_products_of_many_workgroups(hip, tokens, top_k, experts, cols, k, swiglu, kind):
+    """Tiles of 128 and of 256 places with more workgroups than half the card's
+    CUs, into rows that can and that cannot be written 16 bytes at a time."""
+    ids = routes(tokens, top_k, experts, tokens + k, kind)
+    g = gen(cols)
+    x = torch.randn(tokens, k, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(experts, cols, k, generator=g, device="cuda") * k ** -0.5).bfloat16()
+    groups = group_rows(ids, experts)
+    order, _, offsets = definition(ids, experts)
+    y, tol = product(x, w, order, offsets, top_k, True, swiglu)
+    end = int(offsets[-1])
+    wide = cols // 2 if swiglu else cols
+    for dtype in (torch.float32, torch.bfloat16):
+        for pad in (0, 3):
+            out = torch.full((tokens * top_k, wide + pad), 77.0, dtype=dtype, device="cuda")
+            grouped_product(x, w, groups, swiglu=swiglu, out=out[:, :wide])
+            torch.cuda.synchronize()
+            agree(out[:, :wide], y, tol, end)
+            assert (out[:, wide:] == 77.0).all() and (out[end:] == 77.0).all()
