@@ -13,9 +13,10 @@
 // knowing lse, and no rounding of a score decides between two tokens of a
 // beam.
 //
-// Two kernels read each logit once:
-//  * beam_part_kernel: a part of a row streams through registers: its maximum,
-//    its sum of exponentials, and its first n_out candidates by (logit, token);
+// Two kernels, the first reads each logit once:
+//  * a part of a row: its maximum, its sum of exponentials, and its first n_out
+//    candidates by (logit, token); beam_tile_kernel while the parts are few,
+//    beam_part_kernel for many rows;
 //  * beam_finish_kernel: a request: its beams' lse from the parts, and the
 //    first n_out of the parts' candidates.
 #include <hip/hip_runtime.h>
@@ -494,9 +495,11 @@ __device__ __noinline__ int beam_first_of_many(const BeamList* list, int count, 
 //    one at or above a bound: one that n_out of the four first tiles' groups
 //    reach, or the n_out-th kept after a full list was cut back to n_out, so
 //    that most tiles end at one comparison.
-// A tile a workgroup instead, with a bound and an exchange each, had twice the
-// instructions a logit and no loads in flight while it computed (64 x 8 rows of
-// 151,936 bf16: 52 us).
+// Parts of kTileElems by the kernel above instead have more instructions a logit
+// and no loads in flight while they compute (64 x 8 rows of 151,936 bf16, a
+// fifth of them finished, the whole step: 57 us, with this kernel 41).  What
+// bounds it: bytes behind 64 MB (6.3 TB/s from 65,536 to 262,144 logits a row),
+// and about 16 us of launches, first and last tiles, and the finish.
 template <int DT, bool MASK>
 __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   constexpr int N = BeamLoad<DT>::N, L = 4, PER = L * N, W = kPartThreads / 64, ES = 16 / N;
@@ -989,10 +992,11 @@ struct ReorderArgs {
   int64_t blocks;  // workgroups of a piece
 };
 
-// One thread owns U units (16, 4 or 1 bytes) of all K rows of a request: it
+// One thread owns U units (16, 4, 2 or 1 bytes) of all K rows of a request: it
 // reads what the rows need before it writes any of them, so dst may be src.
 // A workgroup stays in one piece (outer and mid index) of one request, so that
-// nothing but the column is divided per thread.
+// nothing but the column is divided per thread.  Bound by the bytes read and
+// written: 1.3 GB of 8 requests' 8 beams 270 us, 4.9 TB/s, what a copy reaches.
 template <typename T, int KM, int U>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(ReorderArgs a) {
   const int b = blockIdx.y;
@@ -1046,6 +1050,9 @@ void launch_reorder_rows(ReorderArgs a, int batch, hipStream_t st) {
   hipLaunchKernelGGL((beam_reorder_kernel<T, KM, U>), grid, dim3(256), 0, st, a);
 }
 
+// Up to 16 units a thread.  us with the fitting kernel and the next larger one:
+// K = 4 (537 MB) 143 and 146, K = 8 (1,074 MB) 331 and 356, K = 16 (2,147 MB)
+// 776 and 837.
 template <typename T>
 void launch_reorder(const ReorderArgs& a, int batch, hipStream_t st) {
   if (a.K <= 4) launch_reorder_rows<T, 4, 4>(a, batch, st);
@@ -1173,13 +1180,17 @@ int hi_rocm_beam_reorder(const void* src, void* dst, const int32_t* parents, int
   a.mid_stride = mid > 1 ? mid_stride : 0;
   const uint64_t bits = s | t | (uint64_t)a.outer_stride | (uint64_t)a.row_stride | (uint64_t)a.mid_stride |
                         (uint64_t)pos_bytes;
-  const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+  // the widest unit in which all rows start and end: 537 MB in 4 rows a request
+  // 126 us; from an address on 4 bytes 136, on 2 bytes 169 (by bytes three times
+  // the first)
+  const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
   // (a launch holds less than 2^32 threads; outer * mid * blocks: each below 2^46)
   const int64_t blocks = ((piece + unit - 1) / unit + 255) / 256, most = UINT32_MAX / 256;
   if (outer > most || mid > most / outer || blocks > most / (outer * mid))
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_beam_reorder: more than 2^24 pieces of 256 units a row");
   if (unit == 16) launch_reorder<reorder_u32x4>(a, batch, (hipStream_t)stream);
   else if (unit == 4) launch_reorder<uint32_t>(a, batch, (hipStream_t)stream);
+  else if (unit == 2) launch_reorder<uint16_t>(a, batch, (hipStream_t)stream);
   else launch_reorder<uint8_t>(a, batch, (hipStream_t)stream);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? HI_ROCM_OK : api_hip_fail(e, "beam reorder launch");
