@@ -116,6 +116,9 @@ class BeamSearch:
         _vector(what, "out tokens", o_tokens, _I32, n)
         _vector(what, "out parents", o_parents, _I32, n)
         _vector(what, "out finished", o_finished, _FLAG, n)
+        if self.n_out != K and (o_scores.data_ptr() == scores.data_ptr() or
+                                (finished is not None and o_finished.data_ptr() == finished.data_ptr())):
+            raise ValueError(f"{what}: outputs over inputs need n_out = beams")
         ws = self.workspace
         _on(what, ws.get_device(), logits, scores, finished, mask_words, o_scores, o_tokens, o_parents, o_finished)
         check(load().hi_rocm_beam_select(

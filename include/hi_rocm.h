@@ -406,7 +406,9 @@ int hi_rocm_beam_workspace_bytes(int max_batch, int beams, int vocab, int n_out,
  *   out_scores f32[batch][n_out], out_tokens u32, out_parents i32 (the beam
  *   within its request), out_finished u8 (the parent was finished, or the
  *   token is eos_id).  Places without a candidate: score -inf, token eos_id
- *   (0 without one), parent j % beams, finished.
+ *   (0 without one), parent j % beams, finished.  With n_out = beams the
+ *   scores and finished flags may be written over the ones read; else no
+ *   output may overlap an input.
  * The workspace needs no initial value; one stream at a time.  No allocation
  * and no host synchronisation: graph-capturable. */
 int hi_rocm_beam_select(const void* logits, int dtype, int batch, int beams, int vocab, int64_t row_stride,

@@ -342,6 +342,33 @@ def test_refusals(hip):
         reorder_states(flat[:48].view(6, 8), par, dst=flat[8:56].view(6, 8))
 
 
+def test_scores_in_place(hip):
+    """With n_out = beams a step's scores and flags may replace the last one's."""
+    B, K, V = 9, 4, 5000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    bs = BeamSearch(B, K, V)
+    x = torch.randn(B * K, V, generator=g, device="cuda").mul_(2.5)
+    c = -torch.rand(B * K, generator=g, device="cuda")
+    f = (torch.rand(B * K, generator=g, device="cuda") < 0.4).to(torch.uint8)
+    want = bs.select(x, c.clone(), finished=f.clone(), eos_id=3)
+    out = bs.outputs(B)
+    out["scores"].copy_(c.view(B, K))
+    out["finished"].copy_(f.view(B, K))
+    got = bs.select(x, out["scores"], finished=out["finished"], eos_id=3, out=out)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    two = BeamSearch(B, K, V, 2 * K)
+    with pytest.raises(ValueError):
+        o = two.outputs(B)
+        o["scores"] = c.view(-1)[:1].expand(1)  # (not even the right size)
+        two.select(x, c, out=o)
+    o = two.outputs(B)
+    both = torch.empty(B * 2 * K, device="cuda")
+    both[:B * K] = c
+    o["scores"] = both
+    with pytest.raises(ValueError, match="outputs over inputs"):
+        two.select(x, both[:B * K], out=o)
+
+
 def definition_on_gpu(x, c, mask, K, n):
     """`definition` without finished beams, rows all at once."""
     x = x.double().masked_fill(x.isnan(), -torch.inf)
