@@ -83,6 +83,14 @@ constexpr float kBeamFused = 1e30f;  // logits up to this size can be scaled by 
 constexpr float kBeamLowest = -3.402823466e38f;
 constexpr uint32_t kBeamNegInf = 0x007fffffu;  // beam_okey(-inf): keys above it are candidates
 
+// The largest of three numbers.  (fmaxf would first quiet each operand, an
+// instruction a logit; a signalling NaN's group is found by its sum.)
+__device__ __forceinline__ float beam_max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+
 // Wave reductions by DPP moves (lane 63 ends with the result).
 template <typename F>
 __device__ __forceinline__ uint32_t beam_wave_fold(uint32_t v, F f) {
@@ -102,7 +110,7 @@ __device__ __forceinline__ uint32_t beam_wave_umin(uint32_t v) {
 }
 __device__ __forceinline__ float beam_wave_max(float v) {
   return __uint_as_float(beam_wave_fold(__float_as_uint(v), [](uint32_t x, uint32_t y) {
-    return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+    return __float_as_uint(beam_max3(__uint_as_float(x), __uint_as_float(y), __uint_as_float(y)));
   }));
 }
 __device__ __forceinline__ float beam_wave_sum(float v) {
@@ -124,11 +132,35 @@ __device__ __forceinline__ int beam_sum8(int v) {
   return v + __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);  // mirrored within the eight
 }
 
+// N elements that are tokens t .. t + N - 1, where they are outside the row or
+// masked: -inf.  lo and hi: the mask word of max(t, 0) and the next one (~0: none).
+template <int N>
+__device__ __forceinline__ void beam_leave_out(float* x, int t, int V, uint32_t lo, uint32_t hi) {
+  uint32_t bits = (uint32_t)(((uint64_t)hi << 32 | lo) >> (max(t, 0) & 31));
+  if (t < 0) bits <<= -t;
+  bits &= (1u << min(max(V - t, 0), N)) - 1u;
+  #pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)bits, q, 1);
+    x[q] = __uint_as_float((__float_as_uint(x[q]) & keep) | (0xff800000u & ~keep));
+  }
+}
+
 // Whether a row takes part: a beam whose score is not finite has no
 // candidates, a finished one has a single candidate that needs no logits.
-__device__ __forceinline__ bool beam_reads(const BeamArgs& a, int row) {
-  return beam_finite(a.scores[row]) && !(a.finished && a.finished[row]);
-}
+struct BeamFlag {  // (its loads go out where it is made; without flags it reads a byte of the score)
+  float score;
+  bool flags;
+  uint8_t done;
+  __device__ __forceinline__ BeamFlag(const BeamArgs& a, int row)
+      : score(a.scores[row]), flags(a.finished != nullptr),
+        done(*(flags ? a.finished + row : reinterpret_cast<const uint8_t*>(a.scores + row))) {}
+  __device__ __forceinline__ bool reads() const {
+    uint32_t d = done;
+    asm volatile("" : "+v"(d));  // (looked at here, not where it was loaded)
+    return beam_finite(score) && !(flags && d != 0u);
+  }
+};
 
 // A key that at least n <= 64 of G keys a lane reach, and not many more: from
 // the bits that the largest key and the smallest lane's largest (64 keys reach
@@ -214,8 +246,8 @@ struct BeamLoad<HI_ROCM_DTYPE_BF16> {
 // 16-byte boundary at or before the row's start (rows start anywhere; the
 // elements before the start and after the end are no candidates).  All of it
 // is in registers at once, and little code runs, which is most of such a
-// launch's time: 4 rows of 151,936 f32 take 6.3 us, 8.2 with the streaming
-// kernel below.
+// launch's time: 4 rows of 151,936 f32 take 6.0 us, 8.2 with the streaming
+// kernel below; 120 masked rows of 50,257 (1,560 parts) 10 us.
 template <int DT>
 __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
   constexpr int PER = kTileElems / kPartThreads;
@@ -237,66 +269,57 @@ __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(p0 - head * ES + base * ES), 0, (bytes + 3) & ~3, kBufferConfig);
   if (tid == 0) counter = 0u;
-  float x[PER];
-  {
-    i32x4_t v[L];
-    #pragma unroll
-    for (int j = 0; j < L; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, (j * kPartThreads + tid) * 16, 0, 0);
-    // (the loads go out before it is known that the row takes part)
-    if (!beam_reads(a, row)) return;
-    #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      #pragma unroll
-      for (int q = 0; q < N; ++q) x[j * N + q] = BeamLoad<DT>::get(v[j], q);
-    }
-  }
   const float ninf = -__builtin_inff();
   // token of x[j * N + q]: t0 + j * kPartThreads * N + q
   const int t0 = (int)base + tid * N - head;
   // Inside the row and without a mask nothing is left out but NaN, which no
   // maximum or comparison below takes, and which shows in the sum.
   const bool inside = base >= head && base - head + kPartThreads * PER <= a.V && a.mask == nullptr;
+  const uint32_t* mrow = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
+  // all loads go out before it is known that the row takes part
+  const BeamFlag flag(a, row);
+  i32x4_t v[L];
+  #pragma unroll
+  for (int j = 0; j < L; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, (j * kPartThreads + tid) * 16, 0, 0);
+  uint32_t lo[L], hi[L];
+  #pragma unroll
+  for (int j = 0; j < L; ++j) lo[j] = hi[j] = ~0u;
+  if (mrow) {
+    #pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const int w = min(max(t0 + j * (kPartThreads * N), 0) >> 5, a.mask_words - 1);
+      lo[j] = mrow[w];
+      hi[j] = mrow[min(w + 1, a.mask_words - 1)];  // (unused where N tokens from a multiple of N share a word)
+    }
+  }
+  if (!flag.reads()) return;
+  float x[PER];
+  #pragma unroll
+  for (int j = 0; j < L; ++j) {
+    #pragma unroll
+    for (int q = 0; q < N; ++q) x[j * N + q] = BeamLoad<DT>::get(v[j], q);
+  }
   if (!inside) {
-    const uint32_t* mrow = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
-    uint32_t lo[L], hi[L];
     #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      lo[j] = hi[j] = ~0u;
-      if (mrow) {
-        const int w = min(max(t0 + j * (kPartThreads * N), 0) >> 5, a.mask_words - 1);
-        lo[j] = mrow[w];
-        if (head != 0) hi[j] = mrow[min(w + 1, a.mask_words - 1)];  // (N tokens from a multiple of N share a word)
-      }
-    }
-    #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      const int t = t0 + j * (kPartThreads * N);
-      uint32_t bits = (uint32_t)(((uint64_t)hi[j] << 32 | lo[j]) >> (max(t, 0) & 31));
-      if (t < 0) bits <<= -t;
-      #pragma unroll
-      for (int q = 0; q < N; ++q) {
-        const bool ok = t + q >= 0 && t + q < a.V && ((bits >> q) & 1u);
-        x[j * N + q] = ok ? x[j * N + q] : ninf;
-      }
-    }
+    for (int j = 0; j < L; ++j) beam_leave_out<N>(x + j * N, t0 + j * (kPartThreads * N), a.V, lo[j], hi[j]);
   }
   float gm[G];
   #pragma unroll
   for (int g = 0; g < G; ++g) {
-    gm[g] = fmaxf(x[8 * g], ninf);
+    gm[g] = ninf;
     #pragma unroll
-    for (int i = 1; i < 8; ++i) gm[g] = fmaxf(gm[g], x[8 * g + i]);
+    for (int i = 0; i < 8; i += 2) gm[g] = beam_max3(gm[g], x[8 * g + i], x[8 * g + i + 1]);
   }
-  float m = gm[0];
-  #pragma unroll
-  for (int g = 1; g < G; ++g) m = fmaxf(m, gm[g]);
-  m = beam_wave_max(m);
+  static_assert(G == 2, "two groups a thread");
+  float m = beam_wave_max(beam_max3(gm[0], gm[1], ninf));
   // each wave's sum by its own maximum, so that one exchange serves both
   float s = 0.f;
   if (beam_finite(m)) {
+    // e^(x - m) as 2^(x log2 e - m log2 e), as in the streaming kernel below
+    const float shift = -m * kBeamLog2e;
     #pragma unroll
-    for (int i = 0; i < PER; ++i) s += __expf(x[i] - m);
-    if (__ballot(!(s == s)) != 0ull) {  // a NaN logit
+    for (int i = 0; i < PER; ++i) s += __builtin_amdgcn_exp2f(fmaf(x[i], kBeamLog2e, shift));
+    if (fabsf(m) > kBeamFused || __ballot(!(s == s)) != 0ull) {  // products that overflow, or a NaN logit
       s = 0.f;
       #pragma unroll
       for (int i = 0; i < PER; ++i) s += x[i] == x[i] ? __expf(x[i] - m) : 0.f;
@@ -407,14 +430,6 @@ struct BeamList {
 __device__ __forceinline__ int beam_below(uint64_t b) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
 }
-// The largest of three numbers.  (fmaxf would first quiet each operand, an
-// instruction a logit; a signalling NaN's group is found by its sum.)
-__device__ __forceinline__ float beam_max3(float x, float y, float z) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-  return r;
-}
-
 // The keys of group i's logits (0: below `floor`, or not in the list).
 __device__ __forceinline__ void beam_keys(const BeamList* list, int i, int count, uint32_t floor, uint64_t (&k)[4]) {
   const beam_f32x4 x = list->x[min(i, kPartSlots - 1)];
@@ -533,13 +548,14 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
       for (int j = 0; j < L; ++j) {
         const int w = (int)min(max(t + j * (64 * N), (int64_t)0) >> 5, (int64_t)a.mask_words - 1);
         word[j] = mrow[w];
-        word2[j] = head != 0 ? mrow[min(w + 1, a.mask_words - 1)] : 0u;  // (N tokens from a multiple of N share a word)
+        word2[j] = head != 0 ? mrow[min(w + 1, a.mask_words - 1)] : ~0u;  // (N tokens from a multiple of N share a word)
       }
     }
   };
   // (the first loads go out before it is known that the row takes part)
+  const BeamFlag flag(a, row);
   load(wid);
-  if (!beam_reads(a, row)) return;
+  if (!flag.reads()) return;
   const float ninf = -__builtin_inff();
   BeamList* list = &lists[wid];
   int count = 0, since = 0;    // groups in it, and those listed since the bound rose
@@ -577,19 +593,8 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
     // maximum or comparison below takes, and which shows in the sum.
     if (e0 < 0 || e0 + 64 * PER > a.V || MASK) {
       #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        const int t = t0 + j * (64 * N);
-        uint32_t bits = ~0u;
-        if (MASK) {
-          bits = (uint32_t)(((uint64_t)hi[j] << 32 | lo[j]) >> (max(t, 0) & 31));
-          if (t < 0) bits <<= -t;
-        }
-        #pragma unroll
-        for (int q = 0; q < N; ++q) {
-          const bool ok = t + q >= 0 && t + q < a.V && ((bits >> q) & 1u);
-          x[j * N + q] = ok ? x[j * N + q] : ninf;
-        }
-      }
+      for (int j = 0; j < L; ++j)
+        beam_leave_out<N>(x + j * N, t0 + j * (64 * N), a.V, MASK ? lo[j] : ~0u, MASK ? hi[j] : ~0u);
     }
     // the groups' maxima, and the sum about the running maximum (of a lane
     // without a logit: about a low value, which leaves its terms 0)
