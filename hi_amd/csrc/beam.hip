@@ -524,6 +524,9 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   __shared__ float redm[W], reds[W];
   __shared__ int redn[W];
   __shared__ uint32_t red[W];
+  // what a wave's share of n_out lanes reach (0: nothing yet); not `red`, which a
+  // slower wave may still read when a faster one is a tile ahead
+  __shared__ uint32_t reach[W];
   const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const char* p0 = (const char*)a.logits + (int64_t)row * a.row_stride * ES;
@@ -564,7 +567,7 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   bool full = false, shared = false;
   auto shared_bound = [&]() {
     const uint32_t key[1] = {beam_okey(m)};
-    volatile uint32_t* v = red;
+    volatile uint32_t* v = reach;
     const uint32_t own = beam_wave_nth<1>(key, (a.n_out + W - 1) / W);
     if (lane == 0) v[wid] = own;
     uint32_t b = own;
@@ -636,6 +639,7 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
       uint32_t key[G / 2];  // groups of 8
       #pragma unroll
       for (int g = 0; g < G / 2; ++g) key[g] = beam_okey(beam_max3(gm[2 * g], gm[2 * g + 1], ninf));
+      if (lane == 0) reach[wid] = 0u;
       const uint32_t k = beam_bound<G / 2, W>(key, a.n_out, kBeamNegInf, red);
       shared = k > kBeamNegInf;
       bound = beam_okey_inv(max(k, kBeamNegInf + 1u));
@@ -691,7 +695,7 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
     }
     if (since >= a.n_out) full = true;
   }
-  if (a.tiles > W) shared_bound();  // (else it has not moved since the first)
+  if (a.tiles > W) shared_bound();
   {
     const float wm = beam_wave_max(m), at = fmaxf(wm, kBeamLowest);
     s = beam_wave_sum(s * __expf(fmaxf(m, kBeamLowest) - at));
@@ -699,11 +703,11 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
   }
   __syncthreads();
   m = redm[0];
-  uint32_t last = red[0];  // n_out of the part's logits reach it
+  uint32_t last = reach[0];  // n_out of the part's logits reach it
   #pragma unroll
   for (int w = 1; w < W; ++w) {
     m = fmaxf(m, redm[w]);
-    last = min(last, red[w]);
+    last = min(last, reach[w]);
   }
   const int64_t slot = (int64_t)row * a.n_parts + part;
   if (!beam_finite(m)) {  // nothing allowed, or a +inf logit: the finish sees which
