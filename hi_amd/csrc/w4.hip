@@ -149,9 +149,10 @@ struct W4Scales<ST, 1> {
 //
 // What bounds it: the weights' bytes for a row (4096 x 151936 in groups of 32,
 // 350 MB with the scales: 62 us, 5.6 TB/s), the latency of the loads and of the
-// two barriers for small weights (1184 x 1000: 6.6 us), and for 17 to 64 rows
-// the instructions of the groups' ends, two a row and output of four (32 rows,
-// 4096 x 16384 with zeros in groups of 128, 35 MB: 16.7 us, 2.2 TB/s).
+// two barriers for small weights (1184 x 1000: 6.6 us), and for more rows x,
+// which every CU reads from the L2s: 32 rows, 4096 x 16384 with zeros in groups
+// of 128, 35 MB of weights: 16.7 us, of which the 64 MB of x in all take 7 (16
+// rows: 3.5 of 12).
 // MFMA 16x16x32 bf16 (lane l = 16 g + r): A row r, elements 8 g .. 8 g + 7;
 // B column r, the same elements; D rows 4 g .. 4 g + 3 of column r.  Rows past
 // the last repeat it and are dropped.
