@@ -170,7 +170,9 @@ __device__ __forceinline__ uint32_t beam_wave_nth(const uint32_t (&key)[G], int 
   uint32_t top = key[0];
   #pragma unroll
   for (int g = 1; g < G; ++g) top = max(top, key[g]);
-  const uint32_t lo = beam_wave_umin(top), hi = beam_wave_umax(top);
+  const uint32_t hi = beam_wave_umax(top);
+  if (n == 1) return hi;
+  const uint32_t lo = beam_wave_umin(top);
   if (lo == hi) return lo;
   const int first = 31 - __builtin_clz(lo ^ hi);
   uint32_t t = hi & ~((2u << first) - 1u);
