@@ -155,11 +155,12 @@ struct BeamFlag {  // (its loads go out where it is made; without flags it reads
   __device__ __forceinline__ BeamFlag(const BeamArgs& a, int row)
       : score(a.scores[row]), flags(a.finished != nullptr),
         done(*(flags ? a.finished + row : reinterpret_cast<const uint8_t*>(a.scores + row))) {}
-  __device__ __forceinline__ bool reads() const {
+  __device__ __forceinline__ bool finished() const {
     uint32_t d = done;
     asm volatile("" : "+v"(d));  // (looked at here, not where it was loaded)
-    return beam_finite(score) && !(flags && d != 0u);
+    return flags && d != 0u;
   }
+  __device__ __forceinline__ bool reads() const { return beam_finite(score) && !finished(); }
 };
 
 // A key that at least n <= 64 of G keys a lane reach, and not many more: from
@@ -794,8 +795,8 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
     held[j] = list0 < lists && sub0 + j * Q < a.n_out ? cand(list0, sub0 + j * Q) : 0ull;
   for (int k = wid; k < a.K; k += W) {
     const int row = row0 + k;
-    const float c = a.scores[row];
-    const bool fin = a.finished && a.finished[row];
+    const BeamFlag flag(a, row);
+    const float c = flag.score;
     const BeamPart* pp = a.parts + (int64_t)row * a.n_parts;
     float m = ninf, s = 0.f;
     for (int i = lane; i < a.n_parts; i += 64) {
@@ -809,7 +810,7 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(BeamArgs a)
     uint32_t st = 0u;
     float l = 0.f;
     if (beam_finite(c)) {
-      if (fin) {
+      if (flag.finished()) {
         st = 2u;
       } else if (beam_finite(top)) {
         l = top + logf(beam_wave_sum(s * __expf(m - top)));
