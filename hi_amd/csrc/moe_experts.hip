@@ -371,9 +371,13 @@ __global__ void __launch_bounds__(64 * kFewWaves) moe_few_kernel(GroupedArgs a) 
 // workgroups, whose results all CUs write at about the same time.  With 64
 // experts 311 to 340: their weights come from memory once (537 MB) instead of
 // from the L2s, and tiles are not full.  (Tried: five buffers instead of four;
-// 64 of k in two buffers; 128 x 64 a wave with four waves; two workgroups a CU;
-// workgroups that stay and load the next tile under this one's last steps:
-// within 2% or slower.)
+// 64 of k in two buffers; 128 x 128 a wave with four waves; two workgroups a CU;
+// workgroups that stay and load the next tile under this one's last steps;
+// bodies for every 32 places: within 2% or slower.  In the loop reading the
+// operands and filling the buffers take LDS as long as the products take the
+// matrix cores, 1,024 cycles a step.  Weights straight to registers would take a
+// third of that off, but beside loads to LDS the compiler waits for all of them:
+// 320 us.)
 __device__ const uint4 moe_zero = {0u, 0u, 0u, 0u};
 
 typedef __attribute__((address_space(3))) void moe_lds;
