@@ -190,12 +190,15 @@ __device__ __forceinline__ bool moe_work(const GroupedArgs& a, int blocks, MoeWo
 // silu(g) * u.  exp(-g) as 2^t (1 + ln 2 * what t = -g log2 e lost to its
 // rounding): within a few units of the last place, in a third of expf's and the
 // division's instructions (the product kernels repeat this for every register).
+// Where 2^t overflows (g from -88.73 down) there is nothing to correct, as inf
+// times what was lost would be NaN: the result is -0 there (|silu(g)| < 2^-121),
+// and may be from g = -87.34, where 1 / (1 + exp(-g)) is no normal number.
 __device__ __forceinline__ float moe_silu_mul(float g, float u) {
   constexpr float kLog2e = 1.44269502e+00f, kLog2eLo = 1.92596299e-08f, kLn2 = 6.93147182e-01f;
   const float t = -g * kLog2e;
   const float lost = fmaf(-g, kLog2eLo, fmaf(-g, kLog2e, -t));
   const float p = __builtin_amdgcn_exp2f(t);
-  const float e = fabsf(g) < 128.f ? fmaf(p, lost * kLn2, p) : p;  // (beyond: p is 0 or inf, or NaN)
+  const float e = fabsf(t) < 128.f ? fmaf(p, lost * kLn2, p) : p;  // (beyond: p is 0 or inf, or NaN)
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 

@@ -281,3 +281,37 @@ def test_products_of_many_workgroups(hip, tokens, top_k, experts, cols, k, swigl
             torch.cuda.synchronize()
             agree(out[:, :wide], y, tol, end)
             assert (out[:, wide:] == 77.0).all() and (out[end:] == 77.0).all()
+
+
+@pytest.mark.parametrize("tokens,experts,inter", [(40, 5, 40), (60, 5, 40), (200, 5, 40), (2400, 40, 520), (4000, 4, 3820)])
+def test_gates_of_any_size(hip, tokens, experts, inter):
+    """silu(gate) up over gates from -400 to 400, every 0.1 from -130 to 130, by
+    each product kernel: 8 and 12 places an expert, 40, 60 with more workgroups
+    than half the card's CUs, and 1,000.
+
+    Gates are multiples of 2^-8 below 512, given as the sum of two bf16 weights,
+    and ups small whole numbers, so both sums are exact.  What is left: the
+    exponential (2 eps), its correction (1), 1 + e (1), the reciprocal (2), two
+    products (2) and the correction's own terms (2); a reciprocal below the
+    smallest normal number may be taken as 0, which is off by |g u| 2^-126."""
+    ids = (torch.arange(tokens, device="cuda", dtype=torch.int32) % experts).view(-1, 1)
+    groups = group_rows(ids, experts)
+    g = torch.cat((torch.linspace(-130.0, 130.0, 2601), torch.tensor([-400.0, -150.0, -88.7228, 88.7229, 150.0, 400.0])))
+    g = (g.double() * 256).round().cuda() / 256
+    x = torch.zeros(tokens, 64, device="cuda").bfloat16()
+    x[:, :2] = 1.0
+    x[:, 2] = torch.arange(1, tokens + 1, device="cuda") % 7 - 3.0
+    w = torch.zeros(experts, 2 * inter, 64, device="cuda").bfloat16()
+    w[:, inter:, 2] = 1.0
+    places = groups.order.long()
+    for first in range(0, g.numel(), experts * inter):
+        gate = g[(first + torch.arange(experts * inter, device="cuda")) % g.numel()].view(experts, inter)
+        w[:, :inter, 0] = gate.float().bfloat16()
+        w[:, :inter, 1] = (gate - w[:, :inter, 0].double()).float().bfloat16()
+        got = grouped_product(x, w, groups, swiglu=True, dtype=torch.float32).double()
+        up = x[places, 2].double()[:, None]
+        gate = gate[ids.view(-1).long()[places]]
+        want = gate / (1.0 + torch.exp(-gate)) * up
+        tol = 10 * EPS * want.abs() + (gate * up).abs() * 2.0 ** -126
+        bad = ~((got - want).abs() <= tol)
+        assert not bad.any(), (first, gate[bad][:5].tolist(), got[bad][:5].tolist(), want[bad][:5].tolist())
