@@ -85,7 +85,8 @@ class BeamSearch:
                out: Optional[dict] = None, stream: Optional[torch.cuda.Stream] = None) -> dict:
         """The first ``n_out`` candidates of each request: ``scores``,
         ``tokens``, ``parents`` (beam within the request) and ``finished``,
-        [batch][n_out] each.  ``logits`` [batch * beams][vocab] f32 or bf16;
+        [batch][n_out] each.  ``logits`` [batch * beams][vocab] f32 or bf16, rows at
+        least vocab apart (no expanded row);
         ``scores`` f32 and ``finished`` uint8 or bool of batch * beams values;
         ``mask_words`` int32 [batch * beams][ceil(vocab / 32)]."""
         what = "beam select"
@@ -99,6 +100,9 @@ class BeamSearch:
         batch = rows // K
         if rows != batch * K or not 0 < batch <= self.max_batch:
             raise ValueError(f"{what}: {rows} rows for {K} beams, at most {self.max_batch} requests")
+        stride = logits.stride(0) if rows > 1 else V  # (a single row's says nothing)
+        if stride < V:
+            raise ValueError(f"{what}: rows of logits overlap")
         _vector(what, "scores", scores, _F32, rows)
         if finished is not None:
             _vector(what, "finished", finished, _FLAG, rows)
@@ -122,7 +126,7 @@ class BeamSearch:
         ws = self.workspace
         _on(what, ws.get_device(), logits, scores, finished, mask_words, o_scores, o_tokens, o_parents, o_finished)
         check(load().hi_rocm_beam_select(
-            logits.data_ptr(), dtype, batch, K, V, max(logits.stride(0), V), scores.data_ptr(), _ptr(finished),
+            logits.data_ptr(), dtype, batch, K, V, stride, scores.data_ptr(), _ptr(finished),
             _lib.BEAM_NO_EOS if eos_id is None else eos_id, _ptr(mask_words), self.n_out, o_scores.data_ptr(),
             o_tokens.data_ptr(), o_parents.data_ptr(), o_finished.data_ptr(), ws.data_ptr(), self._bytes,
             _stream(stream)))
