@@ -84,7 +84,9 @@ constexpr float kBeamLowest = -3.402823466e38f;
 constexpr uint32_t kBeamNegInf = 0x007fffffu;  // beam_okey(-inf): keys above it are candidates
 
 // The largest of three numbers.  (fmaxf would first quiet each operand, an
-// instruction a logit; a signalling NaN's group is found by its sum.)
+// instruction a logit.)  A quiet NaN is passed over, but a signalling one takes
+// the place of all before it: whoever may have met a NaN, which shows in the sum
+// of the exponentials, takes NaN out and the maxima again.
 __device__ __forceinline__ float beam_max3(float x, float y, float z) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
@@ -275,8 +277,8 @@ __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
   const float ninf = -__builtin_inff();
   // token of x[j * N + q]: t0 + j * kPartThreads * N + q
   const int t0 = (int)base + tid * N - head;
-  // Inside the row and without a mask nothing is left out but NaN, which no
-  // maximum or comparison below takes, and which shows in the sum.
+  // Inside the row and without a mask nothing is left out but NaN, which shows
+  // in the sum.
   const bool inside = base >= head && base - head + kPartThreads * PER <= a.V && a.mask == nullptr;
   const uint32_t* mrow = a.mask ? a.mask + (int64_t)row * a.mask_words : nullptr;
   // all loads go out before it is known that the row takes part
@@ -306,29 +308,41 @@ __global__ void __launch_bounds__(kPartThreads) beam_tile_kernel(BeamArgs a) {
     #pragma unroll
     for (int j = 0; j < L; ++j) beam_leave_out<N>(x + j * N, t0 + j * (kPartThreads * N), a.V, lo[j], hi[j]);
   }
-  float gm[G];
-  #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    gm[g] = ninf;
+  float gm[G], m;
+  auto maxima = [&]() {
     #pragma unroll
-    for (int i = 0; i < 8; i += 2) gm[g] = beam_max3(gm[g], x[8 * g + i], x[8 * g + i + 1]);
-  }
-  static_assert(G == 2, "two groups a thread");
-  float m = beam_wave_max(beam_max3(gm[0], gm[1], ninf));
+    for (int g = 0; g < G; ++g) {
+      gm[g] = ninf;
+      #pragma unroll
+      for (int i = 0; i < 8; i += 2) gm[g] = beam_max3(gm[g], x[8 * g + i], x[8 * g + i + 1]);
+    }
+    static_assert(G == 2, "two groups a thread");
+    m = beam_wave_max(beam_max3(gm[0], gm[1], ninf));
+  };
+  maxima();
   // each wave's sum by its own maximum, so that one exchange serves both
   float s = 0.f;
-  if (beam_finite(m)) {
+  bool odd = !beam_finite(m) || fabsf(m) > kBeamFused;  // (products that overflow)
+  if (!odd) {
     // e^(x - m) as 2^(x log2 e - m log2 e), as in the streaming kernel below
     const float shift = -m * kBeamLog2e;
     #pragma unroll
     for (int i = 0; i < PER; ++i) s += __builtin_amdgcn_exp2f(fmaf(x[i], kBeamLog2e, shift));
-    if (fabsf(m) > kBeamFused || __ballot(!(s == s)) != 0ull) {  // products that overflow, or a NaN logit
-      s = 0.f;
-      #pragma unroll
-      for (int i = 0; i < PER; ++i) s += x[i] == x[i] ? __expf(x[i] - m) : 0.f;
-    }
-    s = beam_wave_sum(s);
+    odd = __ballot(!(s == s)) != 0ull;  // a NaN logit
   }
+  if (odd) {
+    // (a signalling NaN may have replaced the maxima found before it, the wave's
+    // among them)
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = x[i] == x[i] ? x[i] : ninf;
+    maxima();
+    s = 0.f;
+    if (beam_finite(m)) {
+      #pragma unroll
+      for (int i = 0; i < PER; ++i) s += __expf(x[i] - m);
+    }
+  }
+  s = beam_wave_sum(s);
   if (lane == 0) { redf[wid] = m; reds[wid] = s; }
   // the part's candidates: all logits at or above a bound that n_out of them reach
   uint32_t key[G];
@@ -595,8 +609,8 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
     const int64_t e0 = base + (int64_t)tile * (64 * PER) - head;
     if (e0 >= a.V && tile >= W) break;
     const int t0 = (int)e0 + lane * N;
-    // Inside the row and without a mask nothing is left out but NaN, which no
-    // maximum or comparison below takes, and which shows in the sum.
+    // Inside the row and without a mask nothing is left out but NaN, which shows
+    // in the sum.
     if (e0 < 0 || e0 + 64 * PER > a.V || MASK) {
       #pragma unroll
       for (int j = 0; j < L; ++j)

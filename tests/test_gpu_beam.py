@@ -449,3 +449,36 @@ def test_many_candidates(hip, dtype, B, K, V, n):
         res = run(x, c, K, n)
         want, tol = definition_on_gpu(x, c, None, K, n)
         check(res, want, tol, K, n, None, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [2048, 4999, 40000])
+@pytest.mark.parametrize("n", [1, 8, 64])
+def test_signalling_nan(hip, dtype, V, n):
+    """NaN logits of either kind count as masked, wherever they lie beside a
+    row's largest logits: at each of eight neighbours of the largest one, in
+    every other place, in all of a part but one place."""
+    rng = np.random.default_rng(V + n)
+    x = torch.from_numpy(rng.standard_normal((56 + 8, V)).astype(np.float32) * 2.5).cuda().to(dtype)
+    nan = torch.zeros(x.shape, dtype=torch.bool, device="cuda")
+    for r in range(56):
+        best, other = r // 7, r % 7
+        other += other >= best
+        at = int(rng.integers(0, V // 8)) * 8
+        x[r, at + best] = 20.0
+        nan[r, at + other] = True
+    for r in range(56, 64):
+        nan[r, r % 2::2] = True                    # every other place
+        if r >= 60:
+            nan[r] = True                          # all, but one place of each 1,000
+            nan[r, r % 8::1000] = False
+    bits, word = (torch.int32, 0x7f800001) if dtype is torch.float32 else (torch.int16, 0x7f81)
+    x.view(bits)[nan] = word
+    c = -rng.random(64).astype(np.float32)
+    with np.errstate(invalid="ignore"):  # (numpy's cast of a signalling NaN)
+        agree(x, c, 1, n)
+    if V == 40000:  # rows enough for the kernel that streams them
+        many = x.repeat(16, 1)
+        res = run(many, np.tile(c, 16), 1, n)
+        want, tol = definition_on_gpu(many, np.tile(c, 16), None, 1, n)
+        check(res, want, tol, 1, n, None, None)
