@@ -707,7 +707,8 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(BeamArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         // a later logit of this tile may equal it with a lower token
         if (least > bound) { bound = least; full = false; }
-        since = count;
+        // (after a rise by what other waves have seen, some kept are below it)
+        since = __popcll(__ballot(lane < count && low >= beam_okey(bound)));
       }
     }
     if (since >= a.n_out) full = true;

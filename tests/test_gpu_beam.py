@@ -482,3 +482,26 @@ def test_signalling_nan(hip, dtype, V, n):
         res = run(many, np.tile(c, 16), 1, n)
         want, tol = definition_on_gpu(many, np.tile(c, 16), None, 1, n)
         check(res, want, tol, 1, n, None, None)
+
+
+def test_equal_logits_of_waves_apart(hip):
+    """The lower token among equal logits, where one wave of a part is far
+    behind the others.  The first wave's tiles (1,024 logits, every fourth) rise
+    in steps that fill its list; the others have little to list, and 16 lanes of
+    each reach 2 at their eighth tile, before the first wave gets to its fifth:
+    there 16 lanes reach 2, in its sixth 48 more.  Those 64 come before the
+    others' 48."""
+    rows, V, n, tile = 1024, 40000, 64, 1024
+    row = torch.full((V,), 0.5)
+    at = lambda step, wave: (step * 4 + wave) * tile
+    for wave in range(4):
+        row[at(0, wave):at(0, wave) + tile] = 1.0
+    row[at(1, 0):at(1, 0) + tile] = 1.25
+    row[at(2, 0):at(2, 0) + tile] = 1.5
+    row[at(3, 0):at(3, 0) + tile * 3 // 4] = 1.75
+    first = [at(4, 0) + 4 * lane for lane in range(16)] + [at(5, 0) + 4 * lane for lane in range(48)]
+    later = [at(7, wave) + 4 * lane for wave in (1, 2, 3) for lane in range(16)]
+    row[first + later] = 2.0
+    x = row.cuda().repeat(rows, 1)
+    res = run(x, np.zeros(rows, np.float32), 1, n)
+    assert (res["tokens"].cpu() == torch.tensor(first, dtype=torch.int32)).all()
