@@ -39,7 +39,8 @@ class W4Linear:
     """y = x w^T + bias for the 4-bit weight w = (q - zero) * scale, laid out
     once.  ``q`` uint8 [n][k / 2] (input 2 j in byte j's low nibble),
     ``scales`` and ``zeros`` (None: 8) [n][k / group] float32 or bfloat16,
-    group 32, 64 or 128; ``bias`` float32 [n] or None."""
+    group 32, 64 or 128; ``bias`` float32 [n] or None.  They are packed on
+    ``stream``, which must come after what made them, and need not be kept."""
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
                  bias: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
@@ -65,6 +66,10 @@ class W4Linear:
         self.packed = _empty((nbytes.value,), torch.uint8, q.device, stream)
         check(lib.hi_rocm_w4_pack(q.data_ptr(), scales.data_ptr(), _ptr(zeros), self.scale_dtype, self.n, self.k,
                                   self.group, self.packed.data_ptr(), self.packed.numel(), _stream(stream)))
+        if stream is not None:  # (they may be freed before the packing has run)
+            for t in (q, scales, zeros):
+                if t is not None:
+                    t.record_stream(stream)
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, dtype=torch.float32,
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:

@@ -181,3 +181,25 @@ def test_refusals(hip):
     wide = torch.zeros(2, 256, device="cuda").bfloat16()
     with pytest.raises(_lib.HiRocmError):  # rows that do not start on 16 bytes
         lin(wide[:, 1:129])
+
+
+def test_packing_on_another_stream(hip):
+    """The quantised weight may be freed as soon as the call returns: its memory
+    serves no new tensor before the packing, on a busy stream, has read it."""
+    n, k = 4096, 1024
+    q, s, z = weights(n, k, 32, torch.float32, True, seed=6)
+    x = torch.randn(2, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6)).bfloat16()
+    want = W4Linear(q, s, z)(x)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        torch.cuda._sleep(200_000_000)
+    lin = W4Linear(q, s, z, stream=st)
+    busy = not st.query()
+    old = {t.data_ptr() for t in (q, s, z)}
+    shapes = [(t.shape, t.dtype) for t in (q, s, z)]
+    del q, s, z
+    new = [torch.full(shape, 3, dtype=dtype, device="cuda") for shape, dtype in shapes]
+    assert busy and not old & {t.data_ptr() for t in new}
+    torch.cuda.synchronize()
+    assert torch.equal(lin(x), want)
