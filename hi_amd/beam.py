@@ -24,9 +24,13 @@ _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cud
 # microseconds: torch.cuda.current_stream() alone takes 2.7 us, comparing two
 # torch.device objects more than their indexes.
 
-def _stream(stream: Optional[torch.cuda.Stream]) -> int:
-    """The handle of ``stream``, or of the current device's current one."""
-    return _raw_stream(_current_device()) if stream is None else stream.cuda_stream
+def _stream(what: str, dev: int, stream: Optional[torch.cuda.Stream]) -> int:
+    """The handle of ``stream``, or of the current device's current one, which
+    must be on CUDA device ``dev`` as the tensors are."""
+    at = _current_device() if stream is None else stream.device_index
+    if at != dev:
+        raise ValueError(f"{what}: tensors on cuda:{dev}, the stream on cuda:{at}")
+    return _raw_stream(dev) if stream is None else stream.cuda_stream
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -129,7 +133,7 @@ class BeamSearch:
             logits.data_ptr(), dtype, batch, K, V, stride, scores.data_ptr(), _ptr(finished),
             _lib.BEAM_NO_EOS if eos_id is None else eos_id, _ptr(mask_words), self.n_out, o_scores.data_ptr(),
             o_tokens.data_ptr(), o_parents.data_ptr(), o_finished.data_ptr(), ws.data_ptr(), self._bytes,
-            _stream(stream)))
+            _stream(what, ws.get_device(), stream)))
         return out
 
 
@@ -192,7 +196,8 @@ def reorder_states(src: torch.Tensor, parents: torch.Tensor, dst: Optional[torch
     _on(what, src.get_device(), parents, dst, lengths)
     check(load().hi_rocm_beam_reorder(
         src.data_ptr(), dst.data_ptr(), parents.data_ptr(), batch, beams, outer, outer_stride * es,
-        strides[row_dim] * es, mid, mid_stride * es, positions, inner * es, _ptr(lengths), _stream(stream)))
+        strides[row_dim] * es, mid, mid_stride * es, positions, inner * es, _ptr(lengths),
+        _stream(what, src.get_device(), stream)))
     return dst
 
 

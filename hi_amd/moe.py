@@ -42,7 +42,8 @@ def group_rows(ids: torch.Tensor, experts: int, out: Optional[RowGroups] = None,
         raise ValueError(f"{what}: out is for {out.tokens} tokens, top {out.top_k} of {out.experts} experts")
     _on(what, ids.get_device(), out.order)
     check(load().hi_rocm_moe_group(ids.data_ptr(), out.tokens, out.top_k, experts, out.order.data_ptr(),
-                                   out.slots.data_ptr(), out.offsets.data_ptr(), _stream(stream)))
+                                   out.slots.data_ptr(), out.offsets.data_ptr(),
+                                   _stream(what, ids.get_device(), stream)))
     return out
 
 
@@ -73,7 +74,7 @@ def grouped_product(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, ga
     check(load().hi_rocm_moe_grouped_product(
         x.data_ptr(), rows, x.stride(0) if rows > 1 else k, groups.order.data_ptr() if gather else 0, groups.top_k,
         groups.offsets.data_ptr(), groups.places, experts, weight.data_ptr(), cols, k, int(swiglu), out.data_ptr(),
-        _CODES[out.dtype], out.stride(0) if groups.places > 1 else wide, _stream(stream)))
+        _CODES[out.dtype], out.stride(0) if groups.places > 1 else wide, _stream(what, x.get_device(), stream)))
     return out
 
 
@@ -93,7 +94,8 @@ def combine(y: torch.Tensor, groups: RowGroups, weights: torch.Tensor, out: Opti
     check(load().hi_rocm_moe_combine(
         y.data_ptr(), _CODES[y.dtype], y.stride(0) if groups.places > 1 else y.shape[1], groups.slots.data_ptr(),
         groups.offsets.data_ptr(), groups.experts, weights.data_ptr(), groups.tokens, groups.top_k, y.shape[1],
-        out.data_ptr(), _CODES[out.dtype], out.stride(0) if groups.tokens > 1 else y.shape[1], _stream(stream)))
+        out.data_ptr(), _CODES[out.dtype], out.stride(0) if groups.tokens > 1 else y.shape[1],
+        _stream(what, y.get_device(), stream)))
     return out
 
 
@@ -144,7 +146,7 @@ class MoeExperts:
             raise ValueError(f"{what}: out must be a float32 or bfloat16 [{tokens}][{H}] tensor")
         g, h, y = self._groups, self._h, self._y
         _on(what, h.get_device(), x, ids, weights, out)
-        places, st, lib = tokens * k, _stream(stream), load()
+        places, st, lib = tokens * k, _stream(what, h.get_device(), stream), load()
         order, slots, offsets = g.order.data_ptr(), g.slots.data_ptr(), g.offsets.data_ptr()
         check(lib.hi_rocm_moe_group(ids.data_ptr(), tokens, k, E, order, slots, offsets, st))
         check(lib.hi_rocm_moe_grouped_product(

@@ -65,7 +65,8 @@ class W4Linear:
         self._bytes = nbytes.value
         self.packed = _empty((nbytes.value,), torch.uint8, q.device, stream)
         check(lib.hi_rocm_w4_pack(q.data_ptr(), scales.data_ptr(), _ptr(zeros), self.scale_dtype, self.n, self.k,
-                                  self.group, self.packed.data_ptr(), self.packed.numel(), _stream(stream)))
+                                  self.group, self.packed.data_ptr(), self.packed.numel(),
+                                  _stream(what, q.get_device(), stream)))
         if stream is not None:  # (they may be freed before the packing has run)
             for t in (q, scales, zeros):
                 if t is not None:
@@ -91,7 +92,7 @@ class W4Linear:
         check(load().hi_rocm_w4_linear(
             x.data_ptr(), rows, x.stride(0) if rows > 1 else k, packed.data_ptr(), self._bytes, self.scale_dtype,
             self.has_zeros, n, k, self.group, _ptr(self.bias), out.data_ptr(), code,
-            out.stride(0) if rows > 1 else n, _stream(stream)))
+            out.stride(0) if rows > 1 else n, _stream(what, packed.get_device(), stream)))
         return out
 
 
