@@ -505,3 +505,32 @@ def test_equal_logits_of_waves_apart(hip):
     x = row.cuda().repeat(rows, 1)
     res = run(x, np.zeros(rows, np.float32), 1, n)
     assert (res["tokens"].cpu() == torch.tensor(first, dtype=torch.int32)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("requests,V", [(2, 9001), (170, 40000)])
+def test_scores_beside_special_rows(hip, dtype, requests, V):
+    """Beams with NaN, infinite, equal and single logits among ordinary ones,
+    and none whose size would widen the scores' bound: by both kernels."""
+    K, n = 6, 12
+    rng = np.random.default_rng(V)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(requests * K, V, generator=g, device="cuda").mul_(2.5).to(dtype)
+    x[0, 10:20] = torch.nan
+    x[0, 0] = torch.nan
+    x[1] = torch.nan                  # no candidate
+    x[2, 5] = torch.inf               # none either
+    x[3] = -torch.inf
+    x[3, 77] = 1.0                    # one candidate of probability 1
+    x[4, ::2] = -torch.inf
+    x[6] = 0.0
+    x[6, 1::2] = -0.0                 # equal to 0: the lower token first
+    x[7, V - 1] = 30.0                # probability 1 but for rounding
+    x[8, : V - 3] = -torch.inf
+    c = -rng.random(requests * K).astype(np.float32) * 8
+    c[9], c[10], c[11] = -np.inf, np.nan, np.inf
+    for beams in (K, 1):  # (as requests of their own every row's scores are seen)
+        res = run(x, c, beams, n)
+        want, tol = definition_on_gpu(x, c, None, beams, n)
+        assert tol < 3e-5
+        check(res, want, tol, beams, n, None, None)
