@@ -315,3 +315,46 @@ def test_gates_of_any_size(hip, tokens, experts, inter):
         tol = 10 * EPS * want.abs() + (gate * up).abs() * 2.0 ** -126
         bad = ~((got - want).abs() <= tol)
         assert not bad.any(), (first, gate[bad][:5].tolist(), got[bad][:5].tolist(), want[bad][:5].tolist())
+
+
+@pytest.mark.parametrize("kind", ["spread", "one"])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("tokens,top_k,experts,cols,k", [(16, 4, 16, 100, 704), (3, 2, 6, 70, 2056), (75, 4, 20, 136, 520),
+                                                         (64, 2, 8, 130, 1032), (150, 2, 6, 200, 1000),
+                                                         (1200, 1, 40, 1030, 520), (2000, 2, 24, 1536, 520)])
+def test_products_over_many_steps(hip, tokens, top_k, experts, cols, k, swiglu, kind):
+    """Each product kernel with k of many more steps than it has buffers: 4, 1,
+    15 and 16 places an expert, 50, 30 and 166 with more workgroups."""
+    ids = routes(tokens, top_k, experts, tokens + k, kind)
+    g = gen(cols)
+    x = torch.randn(tokens, k, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(experts, cols, k, generator=g, device="cuda") * k ** -0.5).bfloat16()
+    groups = group_rows(ids, experts)
+    order, _, offsets = definition(ids, experts)
+    y, tol = product(x, w, order, offsets, top_k, True, swiglu)
+    for dtype in (torch.float32, torch.bfloat16):
+        agree(grouped_product(x, w, groups, swiglu=swiglu, dtype=dtype), y, tol, tokens * top_k)
+
+
+@pytest.mark.parametrize("tokens,k,E,H,I", [(70, 4, 20, 520, 264), (300, 4, 10, 1032, 136), (1000, 4, 24, 1536, 768)])
+def test_larger_layers(hip, tokens, k, E, H, I):
+    """As test_layer, by the kernels for more places an expert."""
+    g = gen(tokens)
+    up = (torch.randn(E, 2 * I, H, generator=g, device="cuda") * H ** -0.5).bfloat16()
+    down = (torch.randn(E, H, I, generator=g, device="cuda") * I ** -0.5).bfloat16()
+    x = torch.randn(tokens, H, generator=g, device="cuda").bfloat16()
+    ids = routes(tokens, k, E, tokens, "strays")
+    wts = torch.softmax(torch.randn(tokens, k, generator=g, device="cuda"), 1)
+    order, slots, offsets = definition(ids, E)
+    h, dh = product(x, up, order, offsets, k, True, True)
+    dh = dh + half_unit(h.abs() + dh)
+    y, dy = product(h, down, order, offsets, k, False, False)
+    carried, _ = product(dh, down.abs(), order, offsets, k, False, False)
+    back = torch.from_numpy(slots)
+    w = wts.double().cpu()[:, :, None]
+    want = (y[back].view(tokens, k, H) * w).sum(1)
+    tol = ((dy + carried)[back].view(tokens, k, H) * w).sum(1) * 1.001
+    out = torch.empty(tokens, H, device="cuda")
+    layer = MoeExperts(up, down, max_tokens=tokens + 5, top_k=k)
+    agree(layer(x, ids, wts, out=out), want, tol, tokens)
+    agree(layer(x, ids, wts), want, tol, tokens)

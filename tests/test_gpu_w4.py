@@ -203,3 +203,28 @@ def test_packing_on_another_stream(hip):
     assert busy and not old & {t.data_ptr() for t in new}
     torch.cuda.synchronize()
     assert torch.equal(lin(x), want)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("sdtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows,n,blocks", [
+    # one row: one tile of outputs a workgroup, two, four; k in one pass and in several
+    (1, 4000, 20), (1, 8100, 12), (1, 4300, 20), (1, 4300, 37), (1, 8300, 5), (1, 8300, 13), (1, 8300, 35),
+    # up to 16 rows, the same
+    (5, 4000, 20), (5, 8100, 12), (8, 4300, 20), (16, 8300, 5), (9, 8300, 13), (9, 8300, 35),
+    # more, 16 rows a workgroup and 32
+    (40, 2000, 5), (40, 4300, 13), (24, 8300, 5), (40, 8300, 13), (20, 4300, 20), (20, 8300, 35)])
+def test_every_split(hip, group, sdtype, zeros, rows, n, blocks):
+    """Each way to share outputs, rows and k among workgroups and waves; the
+    last block of 128 inputs holds one group."""
+    k = (blocks - 1) * 128 + group
+    q, s, z = weights(n, k, group, sdtype, zeros, seed=n + blocks)
+    x = torch.randn(rows, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(rows)).bfloat16()
+    bias = torch.randn(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n)) if rows % 2 else None
+    lin = W4Linear(q, s, z, bias=bias)
+    got, half = lin(x), lin(x, dtype=torch.bfloat16)
+    at = torch.cat((torch.arange(0, n, 29), torch.arange(n - 20, n))).cuda().unique()
+    y, tol = exact(x, q[at], s[at], z[at] if zeros else None, group, None if bias is None else bias[at])
+    agree(got[:, at], y, tol)
+    agree(half[:, at], y, tol)
