@@ -183,7 +183,7 @@ def test_refusals(hip):
         lin(wide[:, 1:129])
 
 
-def test_packing_on_another_stream(hip):
+def test_packing_on_another_stream(hip, new_stream):
     """The quantised weight may be freed as soon as the call returns: its memory
     serves no new tensor before the packing, on a busy stream, has read it."""
     n, k = 4096, 1024
@@ -191,7 +191,7 @@ def test_packing_on_another_stream(hip):
     x = torch.randn(2, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6)).bfloat16()
     want = W4Linear(q, s, z)(x)
     torch.cuda.synchronize()
-    st = torch.cuda.Stream()
+    st = new_stream()
     with torch.cuda.stream(st):
         torch.cuda._sleep(200_000_000)
     lin = W4Linear(q, s, z, stream=st)

@@ -31,7 +31,7 @@ def test_strides_of_logits_that_pass():
 
 
 @pytest.mark.gpu
-def test_tensors_and_stream_on_one_device(hip, monkeypatch):
+def test_tensors_and_stream_on_one_device(hip, new_stream, monkeypatch):
     """A call whose tensors are not on its stream's device (the current one, or
     the given stream's) is refused."""
     ids = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
@@ -52,9 +52,10 @@ def test_tensors_and_stream_on_one_device(hip, monkeypatch):
     class Elsewhere:
         device_index, cuda_stream = 1, 0
 
+    other = new_stream()
     for call in calls:
         call()
-        call(stream=torch.cuda.Stream())
+        call(stream=other)
         with pytest.raises(ValueError, match="the stream on cuda:1"):
             call(stream=Elsewhere())
     torch.cuda.synchronize()
