@@ -368,12 +368,13 @@ __global__ void __launch_bounds__(64 * kFewWaves) moe_few_kernel(GroupedArgs a) 
 // choose their global addresses so that the chunks land there.  Chunks past k
 // come from a zero.
 //
-// What bounds it: 32,768 places of 8 experts, 2048 x 2048: 241 us, 1,140
-// TFLOP/s, of which the products of tiles in flight take 200 us (a large dense
-// product of the same size 192) and the rest is beginnings and ends of
-// workgroups, whose results all CUs write at about the same time.  With 64
-// experts 311 to 340: their weights come from memory once (537 MB) instead of
-// from the L2s, and tiles are not full.  (Tried: five buffers instead of four;
+// What bounds it: 32,768 places of 8 experts, 2048 x 2048: 229 to 241 us from
+// card to card, 1,140 to 1,200 TFLOP/s, of which the products of tiles in flight
+// take 200 us (a large dense product of the same size 192) and the rest is
+// beginnings and ends of workgroups, whose results all CUs write at about the
+// same time.  With 64 experts of a router's sizes 311 to 340: tiles are not full,
+// and the short ones end up in any round (experts of equal size: 254), and the
+// weights come from memory once (537 MB) instead of from the L2s.  (Tried: five buffers instead of four;
 // 64 of k in two buffers; 128 x 128 a wave with four waves; two workgroups a CU;
 // workgroups that stay and load the next tile under this one's last steps;
 // bodies for every 32 places: within 2% or slower.  In the loop reading the
@@ -649,6 +650,9 @@ hipError_t launch_many(const GroupedArgs& a, hipStream_t st) {
 //   64 experts, 2048 x 2048:  tiles of 128 149, 177, 209, 341; of 256 150, 159, 223, 329
 //   128 experts, 1024 x 1536: 124, 149, 180, 307; 116, 133, 175, 275
 //   16 experts, 1024 x 2048:  21, 22, 36, 58; 25, 27, 30, 55
+// The rule takes the slower side of some rows above: 128 experts of 128 and of 256
+// places (124 for 116, 180 for 175), 16 of 512 (58 for 55), and 64 of 24 places
+// (124 for 113, the bound of 20).
 hipError_t launch_grouped(const GroupedArgs& a, hipStream_t st) {
   const int avg = a.places / a.experts;
   if (avg <= 8) return launch_few<1>(a, st);

@@ -363,8 +363,15 @@ hipError_t launch_w4(const W4Args& a, hipStream_t st) {
 // 65536: 45.0, with MT = 1 59.3; 64 rows, 2048 x 8192: 10.7 and 12.1; but 32 rows,
 // 4096 x 4096 (256 workgroups with MT = 1): 14.4 and 9.2.
 // (MT = 4 read x too often to gain: 64 rows, 4096 x 65536 110, with MT = 2 86.)
-// With f32 scales and zeros for groups of 32, MT = 2 and T = 2 do not fit the
-// registers: 32 rows, 4096 x 65536: 108, with T = 4 69.
+// With f32 scales and zeros for groups of 32, MT = 2 and T = 2 are far from
+// fitting the registers: 32 rows, 4096 x 65536: 108, with T = 4 69.  Three other
+// types spill 8 to 11 registers there and still win or lose little (32 rows, 4096
+// x 65536 with T = 2 and 4, then 4096 x 16384): groups of 32 with bf16 scales and
+// zeros 59 and 69, 23.6 and 22.2; with f32 scales 52 and 65, 21.8 and 21.7; of 64
+// with f32 scales and zeros 48 and 62, 20.3 and 20.6.
+// Beyond 64 rows the weights are unpacked again for every 32 of them: 4096 x
+// 14336, 128, 512 and 2,048 rows: 55, 210 and 825 (a bf16 library product of
+// unpacked weights 25, 55 and 164).
 template <int G, bool ZEROS, typename ST>
 hipError_t launch_w4_rows(const W4Args& a, hipStream_t st) {
   const int64_t row_tiles = (a.rows + 15) / 16;

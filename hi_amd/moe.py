@@ -103,6 +103,9 @@ class MoeExperts:
     """The expert layer: y[t] = sum_s w[t][s] down_e (silu(gate_e x[t]) * (up_e
     x[t])), e = ids[t][s].  ``w_up`` bfloat16 [experts][2 * inter][hidden]
     (gate rows, then up rows), ``w_down`` bfloat16 [experts][hidden][inter].
+    The activations between the two products are rounded to bfloat16, as in a
+    bfloat16 model (a relative error of 0.0023 of a bfloat16 result, 0.0017
+    with them in f32); all sums are f32.
     Buffers for up to ``max_tokens`` tokens are allocated once; calls allocate
     nothing when ``out`` is given."""
 
@@ -117,8 +120,9 @@ class MoeExperts:
         self.w_up, self.w_down, self.max_tokens, self.top_k = w_up, w_down, max_tokens, top_k
         self.experts, self.hidden, self.inter = w_up.shape[0], w_up.shape[2], w_down.shape[2]
         dev = w_up.device
-        # The activations between the products are what the second product
-        # reads, bf16; its results stay f32 until they are summed.
+        # The activations between the products are what the second product's
+        # matrix instructions take, bf16; its results stay f32 until they are
+        # summed.
         self._h = torch.empty(max_tokens * top_k, self.inter, dtype=torch.bfloat16, device=dev)
         self._y = torch.empty(max_tokens * top_k, self.hidden, dtype=torch.float32, device=dev)
         self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev)

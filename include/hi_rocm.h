@@ -389,8 +389,8 @@ int hi_rocm_beam_workspace_bytes(int max_batch, int beams, int vocab, int n_out,
 
 /* One step of beam search: the first n_out candidates of each request over
  * its beams and the vocabulary.
- *   logits     [batch * beams][row_stride] of `dtype` (f32 or bf16), rows at
- *              any alignment of their type
+ *   logits     [batch * beams][row_stride >= vocab] of `dtype` (f32 or bf16),
+ *              rows at any alignment of their type
  *   scores     f32[batch * beams] cumulative log-probabilities; a beam whose
  *              score is not finite has no candidates (-inf: unused, as all
  *              beams but one of a request's first step)
@@ -448,9 +448,9 @@ int hi_rocm_w4_pack(const void* q, const void* scales, const void* zeros, int sc
  * packed.  Made for the rows of a decode step (1 to 64; the weights are taken
  * once for every 16 or 32 of them).  A row's result does not depend on the
  * other rows' values, only on their number (by which k is split); a row of x
- * that holds inf or NaN gives NaN.  With f32 out it writes
- * the logits that hi_rocm_sample and hi_rocm_beam_select read.  No
- * allocation: graph-capturable. */
+ * that holds inf or NaN gives NaN, and so may one whose |x| sum to 2^123 over a
+ * group (the sums of up to 31 x are f32).  With f32 out it writes the logits that
+ * hi_rocm_sample and hi_rocm_beam_select read.  No allocation: graph-capturable. */
 int hi_rocm_w4_linear(const void* x, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
                       int scale_dtype, int has_zeros, int n, int k, int group, const float* bias, void* out,
                       int out_dtype, int64_t out_stride, void* stream);
@@ -472,7 +472,8 @@ int hi_rocm_moe_group(const uint32_t* ids, int tokens, int top_k, int experts, i
  * groups' order); out f32 or bf16 [places][out_stride].  With swiglu the
  * columns are gate and up halves and out[i][c] = silu(gate c) * (up c), cols /
  * 2 wide.  k a multiple of 8, rows on 16 bytes.  Places behind
- * offsets[experts] are not written.  Sums in f32, one rounding to out's type.
+ * offsets[experts] are not written.  Sums in f32, one rounding to out's type:
+ * what a second product reads (bf16) is rounded to 8 bits between the two.
  * No allocation: graph-capturable. */
 int hi_rocm_moe_grouped_product(const void* x, int x_rows, int64_t x_stride, const int32_t* order, int top_k,
                                 const int32_t* offsets, int places, int experts, const void* weight, int cols, int k,
