@@ -30,9 +30,10 @@ ROW_PARAMS_DTYPE = np.dtype(
 assert ROW_PARAMS_DTYPE.itemsize == 40
 
 OK, ERR_ARGS, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_MX4 = 0, 1, 2
 FLAG_REP_ONCE = 1
 MAX_LOGPROBS = 1024
+MX4_FEW_ROWS, SPEC_NO_TOKEN = 16, 0xFFFFFFFF
 BEAM_MAX, BEAM_MAX_OUT, BEAM_NO_EOS = 32, 64, 0xFFFFFFFF
 
 # Every function include/*.h declares, with its ctypes signature.
@@ -86,6 +87,18 @@ SIGNATURES = {
     "hi_rocm_moe_group": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "hi_rocm_moe_grouped_product": (_i, [_vp, _i, _i64, _vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _vp, _i, _i64, _vp]),
     "hi_rocm_moe_combine": (_i, [_vp, _i, _i64, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _i, _i64, _vp]),
+    "hi_rocm_spec_sampled_workspace_bytes": (_i, [_i, _i, ctypes.POINTER(_sz)]),
+    "hi_rocm_spec_verify_sampled": (_i, [_vp, _i, _i, _i, _i, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                         _sz, _vp]),
+    "hi_rocm_mx4_quantize": (_i, [_vp, _i, _i64, _i, _i64, _vp, _vp, _vp]),
+    "hi_rocm_mx4_dequantize": (_i, [_vp, _vp, _i64, _i, _vp, _i, _i64, _vp]),
+    "hi_rocm_mx4_rows_bytes": (_i, [_i64, _i, ctypes.POINTER(_sz)]),
+    "hi_rocm_mx4_rows": (_i, [_vp, _i, _i64, _i, _i64, _vp, _sz, _vp]),
+    "hi_rocm_mx4_packed_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
+    "hi_rocm_mx4_pack": (_i, [_vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "hi_rocm_mx4_linear": (_i, [_vp, _i, _i, _i64, _vp, _sz, _i, _i, _vp, _vp, _i, _i64, _vp, _sz, _vp]),
+    "hi_rocm_mx4_grouped_product": (_i, [_vp, _i, _i, _i64, _vp, _i, _vp, _i, _i, _vp, _sz, _i, _i, _i, _vp, _i, _i64,
+                                         _sz, _vp, _sz, _vp]),
     "hi_rocm_last_error": (ctypes.c_char_p, []),
     "hi_rocm_version": (ctypes.c_char_p, []),
     # include/hi_rocm_host.h

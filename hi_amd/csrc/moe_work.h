@@ -1,0 +1,96 @@
+// How products grouped by expert split their work over workgroups, and the
+// gate's function: shared by the bf16 and the 4-bit expert products.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "wave_ops.h"
+
+namespace hi_rocm {
+
+// The groups are cut into tiles of BM places, and the work is (tile, block of
+// columns).  A workgroup finds its own from the offsets (64 experts a wave
+// scan), so one launch of the largest possible grid serves any raggedness.
+// Workgroups go round the 8 XCDs by their number; each XCD takes a contiguous
+// stretch of the work, in which an expert's tiles of one block of columns
+// follow each other, so that its L2 sees a block of weights once and an
+// expert's rows while they are in use.
+constexpr int kXcds = 8;
+
+struct MoeWork {
+  int expert, i0, i1, block;  // places [i0, i1), column block
+};
+
+template <int BM, typename Args>
+__device__ __forceinline__ bool moe_work(const Args& a, int blocks, MoeWork& wk) {
+  const int lane = threadIdx.x & 63;
+  auto count = [&](int e, int& s) {
+    s = 0;
+    if (e >= a.experts) return 0;
+    s = min(max(a.offsets[e], 0), a.places);
+    return max(min(a.offsets[e + 1], a.places) - s, 0);
+  };
+  int tiles = 0;
+  for (int e0 = 0; e0 < a.experts; e0 += 64) {
+    int s;
+    tiles += (count(e0 + lane, s) + BM - 1) / BM;
+  }
+  tiles = (int)wave_incl_scan_u32((uint32_t)tiles);
+  tiles = __builtin_amdgcn_readlane(tiles, 63);
+  const int64_t total = (int64_t)tiles * blocks, per = (total + kXcds - 1) / kXcds;
+  const int64_t slot = blockIdx.x / kXcds, w = blockIdx.x % kXcds * per + slot;
+  if (slot >= per || w >= total) return false;
+  int before = 0;  // tiles of the experts before e0
+  for (int e0 = 0; e0 < a.experts; e0 += 64) {
+    int s;
+    const int n = count(e0 + lane, s), mine = (n + BM - 1) / BM;
+    const int incl = before + (int)wave_incl_scan_u32((uint32_t)mine);
+    const uint64_t hit = __ballot((int64_t)incl * blocks > w && (int64_t)(incl - mine) * blocks <= w);
+    if (hit != 0ull) {
+      const int l = __builtin_ctzll(hit);
+      const int first = __builtin_amdgcn_readlane(incl - mine, l), nt = __builtin_amdgcn_readlane(mine, l);
+      const int start = __builtin_amdgcn_readlane(s, l), places = __builtin_amdgcn_readlane(n, l);
+      const int local = (int)(w - (int64_t)first * blocks);
+      // tiles of one size, a multiple of 16 places
+      const int size = ((places + nt - 1) / nt + 15) & ~15;
+      wk.expert = e0 + l;
+      wk.block = local / nt;
+      wk.i0 = start + min(local % nt * size, places);
+      wk.i1 = min(wk.i0 + size, start + places);
+      return wk.i0 < wk.i1;
+    }
+    before = __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+// silu(g) * u.  exp(-g) as 2^t (1 + ln 2 * what t = -g log2 e lost to its
+// rounding): within a few units of the last place, in a third of expf's and the
+// division's instructions (the product kernels repeat this for every register).
+// Where 2^t overflows (g from -88.73 down) there is nothing to correct, as inf
+// times what was lost would be NaN: the result is -0 there (|silu(g)| < 2^-121),
+// and may be from g = -87.34, where 1 / (1 + exp(-g)) is no normal number.
+__device__ __forceinline__ float moe_silu_mul(float g, float u) {
+  constexpr float kLog2e = 1.44269502e+00f, kLog2eLo = 1.92596299e-08f, kLn2 = 6.93147182e-01f;
+  const float t = -g * kLog2e;
+  const float lost = fmaf(-g, kLog2eLo, fmaf(-g, kLog2e, -t));
+  const float p = __builtin_amdgcn_exp2f(t);
+  const float e = fabsf(t) < 128.f ? fmaf(p, lost * kLn2, p) : p;  // (beyond: p is 0 or inf, or NaN)
+  return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+
+// The largest grid that any split of the places over the experts needs (every
+// expert ends in at most one short tile).
+template <typename Args>
+int64_t moe_grid(const Args& a, int bm, int bn) {
+  const int64_t tiles = a.places / bm + std::min(a.experts, a.places);
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? bn / 2 : bn;
+  return (tiles * ((cols_out + per - 1) / per) + kXcds - 1) / kXcds * kXcds;
+}
+
+// (a launch holds less than 2^32 threads)
+inline bool moe_grid_fits(int64_t grid, int threads) { return grid <= UINT32_MAX / threads; }
+
+}  // namespace hi_rocm

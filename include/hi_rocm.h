@@ -35,6 +35,8 @@ extern "C" {
 
 #define HI_ROCM_DTYPE_F32 0
 #define HI_ROCM_DTYPE_BF16 1
+/* Microscaled 4-bit "rows" (hi_rocm_mx4_rows), in the calls that name it. */
+#define HI_ROCM_DTYPE_MX4 2
 
 /* Repetition penalty once per distinct history token instead of once per
  * occurrence. */
@@ -176,6 +178,45 @@ int hi_rocm_sample_lm_head_ext(const void* hidden, const void* weight, const flo
 int hi_rocm_spec_verify_greedy(const void* logits, int batch, int max_draft, int vocab, const void* draft_tokens,
                                const void* draft_len, void* out_greedy, void* out_tokens, void* out_count,
                                void* stream);
+
+/* What a place behind the emitted tokens holds. */
+#define HI_ROCM_SPEC_NO_TOKEN 0xffffffffu
+
+/* Workspace bytes hi_rocm_spec_verify_sampled needs for up to max_batch
+ * requests (at most 65535). */
+int hi_rocm_spec_sampled_workspace_bytes(int max_batch, int vocab, size_t* out_bytes);
+
+/* Verification of sampled drafts by the rejection rule, with the target's
+ * probabilities and given random numbers: the emitted tokens follow the target's
+ * distribution.
+ *   target_probs  f32 or bf16 (dtype) [batch][max_draft + 1][vocab]: row i of a
+ *                 request is the distribution after its first i drafts, as it is
+ *                 sampled from (temperature and cut-offs applied); rows at any
+ *                 alignment of their type, strides in values, values contiguous
+ *   draft_probs   the same of the draft model, [batch][max_draft][vocab], or NULL
+ *                 where drafts were not sampled (their probability is 1)
+ *   draft_tokens  u32[batch][max_draft], draft_len i32[batch] (NULL: all max_draft;
+ *                 clamped to 0 .. max_draft)
+ *   uniforms      f32[batch][max_draft + 1] in [0, 1): number i decides draft i,
+ *                 the last draws the token after the accepted drafts
+ * Draft i, token t, is accepted if u_i q_i(t) < p_i(t), and the drafts before it
+ * are (never where p is 0 or NaN, or t is no token of the vocabulary).  Then, with
+ * n drafts accepted, the least token j with r_0 + .. + r_j > u (r_0 + .. +
+ * r_vocab-1): r = max(p_n - q_n, 0) after a rejection, else p_n; negative and NaN r
+ * count as 0.  Where nothing is left of p_n - q_n, r = p_n; where p_n holds nothing
+ * above 0, token 0.  Products and sums are f64, so a token depends on no order of
+ * f32 sums; probabilities should be finite.  They need not sum to 1, but p and q
+ * are compared as they are.
+ * Writes out_tokens u32[batch][max_draft + 1] (the accepted drafts, the drawn
+ * token, then HI_ROCM_SPEC_NO_TOKEN) and out_count i32[batch] (n + 1); no output
+ * may overlap an input.  The workspace is zeroed once before its first use, every
+ * call leaves it ready for the next; one stream at a time.  No allocation and no host
+ * synchronisation: graph-capturable. */
+int hi_rocm_spec_verify_sampled(const void* target_probs, int dtype, int batch, int max_draft, int vocab,
+                                int64_t target_batch_stride, int64_t target_row_stride, const void* draft_probs,
+                                int64_t draft_batch_stride, int64_t draft_row_stride, const uint32_t* draft_tokens,
+                                const int32_t* draft_len, const float* uniforms, uint32_t* out_tokens,
+                                int32_t* out_count, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- decode-step upkeep on the device (the reference keeps these on the
  *      host: generated tokens in a Vec, crates/hi-cuda/src/lib.rs:4342, and
@@ -485,6 +526,67 @@ int hi_rocm_moe_grouped_product(const void* x, int x_rows, int64_t x_stride, con
 int hi_rocm_moe_combine(const void* y, int y_dtype, int64_t y_stride, const int32_t* slots, const int32_t* offsets,
                         int experts, const float* weights, int tokens, int top_k, int cols, void* out, int out_dtype,
                         int64_t out_stride, void* stream);
+
+/* ---- microscaled 4-bit floating point (MXFP4): rounding and products ---- */
+
+/* A block of 32 values along k: E2M1 codes (bit 3 the sign, then 0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6) times 2^(s - 127) for the block's byte s, 255 NaN.  Codes u8
+ * [rows][k / 2], value 2 j in the low, 2 j + 1 in the high nibble of byte j; scales
+ * u8[rows][k / 32].  k is a multiple of 32. */
+#define HI_ROCM_MX4_MAX_K (1 << 24)
+#define HI_ROCM_MX4_MAX_ROWS (1 << 22)
+/* Up to so many rows of x, the products round bf16 rows as they read them. */
+#define HI_ROCM_MX4_FEW_ROWS 16
+
+/* Rounds x (f32 or bf16 [rows][x_stride], rows on 16 bytes): s = floor(log2 a) + 125
+ * for a block's largest magnitude a, at least 0 (and 0 for a = 0); values times
+ * 2^(127 - s) to the nearest code, ties to the even one, beyond 6 to 6, signs
+ * kept.  A block with an infinity or NaN gets s = 255 and codes 0.  Codes on 16
+ * bytes.  No output may overlap an input, here and below. */
+int hi_rocm_mx4_quantize(const void* x, int dtype, int64_t rows, int k, int64_t x_stride, uint8_t* codes,
+                         uint8_t* scales, void* stream);
+
+/* The values again, f32 or bf16 [rows][out_stride], rows on 16 bytes.  Exact, but
+ * for values beyond the type's largest (infinity). */
+int hi_rocm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k, void* out, int out_dtype,
+                           int64_t out_stride, void* stream);
+
+/* "Rows": the same rounding, codes and scales in the order that the products read
+ * as x (HI_ROCM_DTYPE_MX4), for an x that several products take.  16-byte aligned. */
+int hi_rocm_mx4_rows_bytes(int64_t rows, int k, size_t* out_bytes);
+int hi_rocm_mx4_rows(const void* x, int dtype, int64_t rows, int k, int64_t x_stride, void* out, size_t out_bytes,
+                     void* stream);
+
+/* Lays weights [experts][n][k] out for the products, once (experts 1 for a linear
+ * layer): codes on 16 bytes and scales as above into packed, on 16 bytes. */
+int hi_rocm_mx4_packed_bytes(int experts, int n, int k, size_t* out_bytes);
+int hi_rocm_mx4_pack(const uint8_t* codes, const uint8_t* scales, int experts, int n, int k, void* packed,
+                     size_t packed_bytes, void* stream);
+
+/* out[m][c] = sum_k Q(x[m])[k] * w[c][k] + bias[c], Q the rounding above: x bf16
+ * [rows][x_stride] (rows on 16 bytes) or rows (x_dtype HI_ROCM_DTYPE_MX4, x_stride
+ * not used); bias f32[n] or NULL; out f32 or bf16 [rows][out_stride].  Sums are f32,
+ * products exact.  A row's result does not depend on the other rows' values; a row
+ * that holds an infinity or NaN gives NaN; where the magnitudes of a sum's terms pass
+ * f32's largest, it may be an infinity or NaN.  With more than HI_ROCM_MX4_FEW_ROWS bf16
+ * rows the workspace holds them rounded (hi_rocm_mx4_rows_bytes of them, 16-byte
+ * aligned, no initial value, one stream at a time); else it may be NULL.  At most
+ * 2^22 rows.  No allocation: graph-capturable. */
+int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
+                       int n, int k, const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* hi_rocm_moe_grouped_product with such weights: x, x_rows and workspace as above,
+ * order, top_k, offsets, places and swiglu as there (with swiglu halves of a
+ * multiple of 32 columns).  out f32 or bf16 [places][out_stride], or with swiglu
+ * rows (out_dtype HI_ROCM_DTYPE_MX4, out_bytes as hi_rocm_mx4_rows_bytes of places
+ * and cols / 2, out_stride not used): what the second product reads, rounded from
+ * the f32 activations without a step between.  out_bytes counts for rows only. */
+int hi_rocm_mx4_grouped_product(const void* x, int x_dtype, int x_rows, int64_t x_stride, const int32_t* order,
+                                int top_k, const int32_t* offsets, int places, int experts, const void* packed,
+                                size_t packed_bytes, int cols, int k, int swiglu, void* out, int out_dtype,
+                                int64_t out_stride, size_t out_bytes, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 /* Thread-local message for the last non-zero status. */
 const char* hi_rocm_last_error(void);
