@@ -310,30 +310,6 @@ __global__ void __launch_bounds__(64 * kFewWaves) moe_few_kernel(GroupedArgs a) 
 // operands and filling the buffers take LDS as long as the products take the
 // matrix cores, 1,024 cycles a step.  Weights straight to registers take a third
 // of that off, but two waves then load the same weights: 323 us.)
-__device__ const uint4 moe_zero = {0u, 0u, 0u, 0u};
-
-typedef __attribute__((address_space(3))) void moe_lds;
-typedef const __attribute__((address_space(1))) void moe_global;
-
-// The barrier alone, with nothing moved across it (__syncthreads would also
-// wait for the loads in flight).
-__device__ __forceinline__ void moe_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
-}
-// vmcnt <= N, lgkmcnt 0
-template <int N>
-__device__ __forceinline__ void moe_wait() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 7 << 4);
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
-}
-
 template <int L>
 struct MoeSources {
   const __bf16* p[L];

@@ -81,6 +81,33 @@ __device__ __forceinline__ float moe_silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
+// ---- what the product kernels' loops through LDS are made of ----
+
+// (a chunk past the end of k)
+static __device__ const uint4 moe_zero = {0u, 0u, 0u, 0u};
+
+typedef __attribute__((address_space(3))) void moe_lds;
+typedef const __attribute__((address_space(1))) void moe_global;
+
+// The barrier alone, with nothing moved across it (__syncthreads would also
+// wait for the loads in flight).
+__device__ __forceinline__ void moe_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+// vmcnt <= N, lgkmcnt 0
+template <int N>
+__device__ __forceinline__ void moe_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 7 << 4);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
 // The largest grid that any split of the places over the experts needs (every
 // expert ends in at most one short tile).
 template <typename Args>

@@ -10,9 +10,9 @@
 //
 // Two layouts follow that.  "Rows" (what a product reads as x): codes
 // [rows][k / 2], then scales [rows][quads][16] with block 4 (4 q + j) + g of k
-// in byte 4 g + j of quad q, a lane's four steps in one word.  "Packed"
-// (weights): codes [tile of 16 rows][step][lane][16 bytes], then scales
-// [tile][quad][lane][4 bytes], padded with zero codes and scales of one.
+// in byte 4 g + j of quad q, a lane's four steps in one word; scales behind k are
+// one.  "Packed" (weights): codes [tile of 16 rows][step][lane][16 bytes], then
+// scales [tile][quad][row][16], padded with zero codes and scales of one.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

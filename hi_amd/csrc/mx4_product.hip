@@ -19,6 +19,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "hi_rocm.h"
 #include "moe_work.h"
@@ -92,6 +93,14 @@ __device__ __forceinline__ void mx4_store(const Mx4Args& a, int p, int c, int co
   }
 }
 
+// The scale of block b of place p; the last one's also sets those behind k.
+__device__ __forceinline__ void mx4_store_scale(const Mx4Args& a, int p, int b, uint32_t s) {
+  uint8_t* to = a.out_scales + (int64_t)p * a.out_scale_stride;
+  to[mx4_scale_at(b)] = (uint8_t)s;
+  if (b + 1 == a.cols / 2 / kMx4Block)
+    for (int i = b + 1; i & 15; ++i) to[mx4_scale_at(i)] = 127;
+}
+
 // A block of 32 columns (from c, a multiple of 32) of place p as codes: lane 16
 // g + r has columns 4 g .. + 3 of both halves.  All lanes of a place together.
 __device__ __forceinline__ void mx4_store_codes(const Mx4Args& a, int p, bool in, int c, int g, const mx4_f32x4& lo,
@@ -107,7 +116,7 @@ __device__ __forceinline__ void mx4_store_codes(const Mx4Args& a, int p, bool in
   uint8_t* to = (uint8_t*)a.out + (int64_t)p * a.out_stride + c / 2 + 2 * g;
   *reinterpret_cast<uint16_t*>(to) = (uint16_t)codes;
   *reinterpret_cast<uint16_t*>(to + 8) = (uint16_t)(codes >> 16);
-  if (g == 0) a.out_scales[(int64_t)p * a.out_scale_stride + mx4_scale_at(c / kMx4Block)] = (uint8_t)s;
+  if (g == 0) mx4_store_scale(a, p, c / kMx4Block, s);
 }
 
 // Few places (decode): the weights are what is read.  The workgroup's waves
@@ -133,7 +142,7 @@ __global__ void __launch_bounds__(64 * W) mx4_few_kernel(Mx4Args a) {
     if (a.swiglu) tile = c0 / 16 + t % (NT / 2) + (t >= NT / 2 ? cols_out / 16 : 0);
     const int64_t at = (int64_t)wk.expert * a.tiles + min(tile, a.tiles - 1);
     wp[t] = a.w + at * a.steps * 1024 + lane * 16;
-    sp[t] = a.w_scales + at * a.quads * 256 + lane * 4;
+    sp[t] = a.w_scales + at * a.quads * 256 + r * 16 + g * 4;
   }
   const uint8_t* xp[MT];
   const uint8_t* xs[MT];
@@ -246,6 +255,310 @@ __global__ void __launch_bounds__(64 * W) mx4_few_kernel(Mx4Args a) {
   }
 }
 
+// Many places (prompts, many requests): BM places times BN weight rows a
+// workgroup of eight waves, two a SIMD, a wave every WM-th 32 of the places by 64
+// of the weight rows, with MFMA 32x32x64 (lane 32 h + r: row r, block h of the
+// half step; D rows 8 i + 4 h .. + 3 of column r in registers 4 i .. + 3).
+//
+// k goes in steps of 128 through four LDS buffers that loads fill directly, three
+// steps ahead, and the scales of four steps (16 bytes a row) through two buffers, a
+// quad ahead.  A step has two phases: read the step's operands from LDS and
+// start a later step's loads; multiply.  Waves 4 to 7 run one phase behind waves
+// 0 to 3 (a barrier more before the first step), so on every SIMD one wave reads
+// while the other multiplies.  Why no buffer is written while it is read: a
+// wave's reads are done (lgkmcnt 0) before the barrier that ends its phase, the
+// other waves read the same step at most one phase later, and the buffer of step
+// s - 1 is filled again from step s's read phase on; a quad's scales are read at
+// its first step and their buffer filled again from the next quad's first step
+// on.  Why a step is there when it is read: each wave waits for its own loads of
+// step s + 1 before the barrier that ends its reading of step s, the next quad's
+// scales, started before the loads of a quad's first step, among those of its
+// third.
+//
+// A row of a step is 64 bytes; its 16-byte chunk c lies at c ^ (row / 2 & 3), so
+// that the reads of a chunk of eight rows meet all banks.  A load writes 64 lanes
+// x 16 contiguous bytes; the lanes choose their global addresses so that the
+// chunks land there.  Chunks of x past k hold what follows in memory (the next
+// row, or the scales): any code is finite, and meets weights of 0 and scales of 1.
+typedef float mx4_f32x16 __attribute__((ext_vector_type(16)));
+
+template <int J>
+__device__ __forceinline__ mx4_f32x16 mx4_mfma32(const mx4_i32x4& a, const mx4_i32x4& b, const mx4_f32x16& c, int sa,
+                                                 int sb) {
+  const mx4_i32x8 wa = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
+  const mx4_i32x8 wb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, J, sa, J, sb);
+}
+
+constexpr int kMx4Buffers = 4;
+
+template <int BM, int BN>
+struct Mx4Tile {
+  static constexpr int T = 512, STEP = (BM + BN) * 64, SCALES = (BM + BN) * 16;
+  static constexpr int XL = BM * 4 / T, WL = BN * 4 / T;  // loads a thread and step
+  static constexpr int WN = BN / 64, WM = 8 / WN, MT = BM / 32 / WM;
+  static constexpr int OUT = MT == 1 ? 8192 : 16384;  // a wave's results, 32 or 64 places of 64 columns
+  static constexpr size_t BYTES = std::max<size_t>(kMx4Buffers * STEP + 2 * SCALES, 8 * OUT);
+  static_assert(XL >= 1 && WL >= 1 && MT >= 1 && BM + BN <= T, "tile split");
+};
+
+// A wave's results by way of its own LDS, 64 places at a time in rows of 64
+// columns, written out 16 bytes a lane, a row's bytes next to each other.
+template <int MT, int WM>
+__device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
+                                             int c0, int cols_out, int lane) {
+  const int r = lane & 31, h = lane >> 5;
+  if (a.swiglu) {
+    #pragma unroll
+    for (int m = 0; m < MT; ++m)
+      #pragma unroll
+      for (int i = 0; i < 16; ++i) acc[m][0][i] = moe_silu_mul(acc[m][0][i], acc[m][1][i]);
+    if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
+      // the wave's 32 columns are a block; a place's other half is lane ^ 32's
+      #pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint32_t most = 0u;
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(acc[m][0][i]) & 0x7fffffffu);
+        most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+        const uint32_t s = mx4_scale_of(most >> 23);
+        uint32_t mine[2], theirs[2];
+        #pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float v[8];
+          #pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = acc[m][0][q * 8 + i];
+          mine[q] = mx4_codes(v, s);  // columns 16 q + 4 h .. + 3, then 8 on
+          theirs[q] = (uint32_t)__shfl_xor((int)mine[q], 32, 64);
+        }
+        const int p = p0 + m * (WM * 32) + r;
+        if (p < i1 && c0 < cols_out) {
+          const uint32_t lo = h ? theirs[1] : mine[0], hi = h ? mine[1] : theirs[0];
+          uint2 w;
+          w.x = (lo & 0xffffu) | hi << 16;
+          w.y = lo >> 16 | (hi & 0xffff0000u);
+          *reinterpret_cast<uint2*>((uint8_t*)a.out + (int64_t)p * a.out_stride + c0 / 2 + 8 * h) = w;
+          if (h == 0) mx4_store_scale(a, p, c0 / kMx4Block, s);
+        }
+      }
+      return;
+    }
+  }
+  const bool bf16 = a.out_dtype == HI_ROCM_DTYPE_BF16;
+  const int wide = a.swiglu ? 32 : 64;  // columns of a row
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  #pragma unroll
+  for (int half = 0; half < (MT + 1) / 2; ++half) {
+    if (p0 + half * (WM * 64) >= i1) return;
+    // row j of 64 values: the 16-byte chunk c at c ^ (j & 7)
+    #pragma unroll
+    for (int m = half * 2; m < half * 2 + 2 && m < MT; ++m) {
+      const int j = (m - half * 2) * 32 + r;
+      #pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const mx4_f32x4 y = {acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
+          if (bf16)
+            *reinterpret_cast<bf16x4*>(mem + j * 128 + ((t * 4 + i) ^ (j & 7)) * 16 + h * 8) =
+                __builtin_convertvector(y, bf16x4);
+          else
+            *reinterpret_cast<mx4_f32x4*>(mem + j * 256 + ((t * 8 + i * 2 + h) ^ (j & 7)) * 16) = y;
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int es = bf16 ? 2 : 4, n = 16 / es;       // bytes of a value, values of a chunk
+    const int lanes = wide / n, rows = 64 / lanes;  // lanes of a row, rows at a time
+    const int c = lane % lanes, col = c0 + c * n;
+    #pragma unroll 1
+    for (int j = lane / lanes; j < (MT < 2 ? 32 : 64); j += rows) {
+      const int p = p0 + half * (WM * 64) + (j >> 5) * (WM * 32) + (j & 31);
+      if (p >= i1) break;
+      const uint4 v = *reinterpret_cast<const uint4*>(mem + j * (64 * es) + (c ^ (j & 7)) * 16);
+      char* to = (char*)a.out + ((int64_t)p * a.out_stride + col) * es;
+      if (col + n <= cols_out && a.out_vec) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        #pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (q >= n || col + q >= cols_out) break;
+          if (bf16) ((uint16_t*)to)[q] = (uint16_t)(w[q >> 1] >> (q & 1) * 16);
+          else ((uint32_t*)to)[q] = w[q & 3];
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int BM, int BN, int MT>  // MT: what the tile has places for
+__device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& wk, char* smem) {
+  typedef Mx4Tile<BM, BN> Tile;
+  constexpr int T = Tile::T, STEP = Tile::STEP, SCALES = Tile::SCALES, XL = Tile::XL, WL = Tile::WL;
+  constexpr int WM = Tile::WM, NB = kMx4Buffers, L = XL + WL;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wid % WM, wn = wid / WM;
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols;
+  const int c0 = wk.block * (a.swiglu ? BN / 2 : BN);
+  // the weight row behind row j of the tile: with swiglu each wave's 64 are half
+  // gate, half up
+  auto column = [&](int j) {
+    if (!a.swiglu) return c0 + j;
+    const int c = c0 + j / 64 * 32 + j % 32;
+    return c < cols_out ? c + (j & 32 ? cols_out : 0) : a.cols;
+  };
+  // (rows past the weight's last tile: that tile's)
+  auto weight_row = [&](int j) { return min(column(j), a.tiles * 16 - 16 + (j & 15)); };
+  const int jr = tid / 4;                       // this thread's row in each round of loads
+  const int chunk = (tid & 3) ^ (jr >> 1 & 3);  // and the chunk that lands there
+  const uint8_t* xp[XL];
+  const uint8_t* wp[WL];
+  const int64_t base = (int64_t)wk.expert * a.tiles;
+  #pragma unroll
+  for (int i = 0; i < XL; ++i)
+    xp[i] = a.x + (int64_t)mx4_row(a, min(wk.i0 + i * (T / 4) + jr, wk.i1 - 1)) * a.x_stride + 16 * chunk;
+  #pragma unroll
+  for (int i = 0; i < WL; ++i) {
+    const int row = weight_row(i * (T / 4) + jr);
+    wp[i] = a.w + (base + row / 16) * a.steps * 1024 + chunk * 256 + row % 16 * 16;
+  }
+  // the scales: a row a thread
+  const uint8_t* sp;
+  int sq;  // bytes from quad to quad
+  if (tid < BM) {
+    sp = a.x_scales + (int64_t)mx4_row(a, min(wk.i0 + tid, wk.i1 - 1)) * a.x_scale_stride;
+    sq = 16;
+  } else {
+    const int row = weight_row(min(tid - BM, BN - 1));
+    sp = a.w_scales + (base + row / 16) * a.quads * 256 + row % 16 * 16;
+    sq = 256;
+  }
+  char* const scales = smem + NB * STEP;
+  // (past the last step, the last one's again, for buffers that are not read)
+  auto fill = [&](int step, int buffer) {
+    char* to = smem + buffer * STEP + wid * 1024;
+    const int64_t at = min(step, a.steps - 1);
+    #pragma unroll
+    for (int i = 0; i < XL; ++i)
+      __builtin_amdgcn_global_load_lds((moe_global*)(xp[i] + at * 64), (moe_lds*)(to + i * T * 16), 16, 0, 0);
+    #pragma unroll
+    for (int i = 0; i < WL; ++i)
+      __builtin_amdgcn_global_load_lds((moe_global*)(wp[i] + at * 1024), (moe_lds*)(to + BM * 64 + i * T * 16), 16, 0, 0);
+  };
+  auto fill_scales = [&](int quad) {
+    // (waves past the tile's rows have nothing to load, and one load less to wait for)
+    if (wid * 64 < BM + BN)
+      __builtin_amdgcn_global_load_lds((moe_global*)(sp + (int64_t)min(quad, a.quads - 1) * sq),
+                                       (moe_lds*)(scales + (quad & 1) * SCALES + wid * 1024), 16, 0, 0);
+  };
+  mx4_f32x16 acc[MT][2];
+  #pragma unroll
+  for (int m = 0; m < MT; ++m)
+    #pragma unroll
+    for (int t = 0; t < 2; ++t)
+      #pragma unroll
+      for (int i = 0; i < 16; ++i) acc[m][t][i] = 0.f;
+  fill_scales(0);
+  #pragma unroll
+  for (int s = 0; s < NB - 1; ++s) fill(s, s);
+  moe_wait<L * (NB - 2)>();
+  moe_barrier();
+  if (wid >= 4) moe_barrier();
+  int xs[MT][2], ws[2][2];
+  const char* const xrow = smem + (wm * 32 + r) * 64;
+  const char* const wrow = smem + BM * 64 + (wn * 64 + r) * 64;
+  auto step = [&](auto j_, int quad) {
+    constexpr int J = decltype(j_)::value;
+    mx4_i32x4 xf[MT][2], wf[2][2];
+    if (J == 0) {
+      const char* sc = scales + (quad & 1) * SCALES;
+      #pragma unroll
+      for (int m = 0; m < MT; ++m)
+        #pragma unroll
+        for (int u = 0; u < 2; ++u)
+          xs[m][u] = *reinterpret_cast<const int*>(sc + (m * (WM * 32) + wm * 32 + r) * 16 + u * 8 + h * 4);
+      #pragma unroll
+      for (int t = 0; t < 2; ++t)
+        #pragma unroll
+        for (int u = 0; u < 2; ++u)
+          ws[t][u] = *reinterpret_cast<const int*>(sc + (BM + wn * 64 + t * 32 + r) * 16 + u * 8 + h * 4);
+    }
+    #pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = J * STEP + ((2 * u + h) ^ (r >> 1 & 3)) * 16;
+      #pragma unroll
+      for (int t = 0; t < 2; ++t) wf[t][u] = *reinterpret_cast<const mx4_i32x4*>(wrow + t * 2048 + at);
+      #pragma unroll
+      for (int m = 0; m < MT; ++m) xf[m][u] = *reinterpret_cast<const mx4_i32x4*>(xrow + m * (WM * 2048) + at);
+    }
+    if (J == 0) fill_scales(quad + 1);
+    fill(quad * 4 + J + NB - 1, (J + NB - 1) % NB);
+    // all but the two newest steps', and the scales' that came between
+    if (J < 2 && wid * 64 < BM + BN) moe_wait<L * (NB - 2) + 1>();
+    else moe_wait<L * (NB - 2)>();
+    moe_barrier();
+    __builtin_amdgcn_s_setprio(1);
+    #pragma unroll
+    for (int u = 0; u < 2; ++u)
+      #pragma unroll
+      for (int m = 0; m < MT; ++m)
+        #pragma unroll
+        for (int t = 0; t < 2; ++t) acc[m][t] = mx4_mfma32<J>(wf[t][u], xf[m][u], acc[m][t], ws[t][u], xs[m][u]);
+    __builtin_amdgcn_s_setprio(0);
+    moe_barrier();
+  };
+  for (int quad = 0; quad < a.quads; ++quad) {
+    step(std::integral_constant<int, 0>(), quad);
+    if (quad * 4 + 1 >= a.steps) break;
+    step(std::integral_constant<int, 1>(), quad);
+    if (quad * 4 + 2 >= a.steps) break;
+    step(std::integral_constant<int, 2>(), quad);
+    if (quad * 4 + 3 >= a.steps) break;
+    step(std::integral_constant<int, 3>(), quad);
+  }
+  if (wid < 4) moe_barrier();
+  moe_wait<0>();  // no load may still write LDS when it is used again, or the workgroup ends
+  moe_barrier();
+  if (a.bias != nullptr) {
+    #pragma unroll
+    for (int t = 0; t < 2; ++t)
+      #pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = c0 + wn * 64 + t * 32 + i / 4 * 8 + h * 4 + i % 4;
+        const float b = c < cols_out ? a.bias[c] : 0.f;
+        #pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m][t][i] += b;
+      }
+  }
+  mx4_tile_out<MT, WM>(a, acc, smem + wid * Tile::OUT, wk.i0 + wm * 32, wk.i1, c0 + wn * (a.swiglu ? 32 : 64), cols_out,
+                       lane);
+}
+
+// WM waves share the places, every WM-th 32 of them, so a tile of fewer places
+// than BM is multiplied as one of a quarter, a half or three quarters.
+template <int BM, int BN>
+__global__ void __launch_bounds__(512) mx4_many_kernel(Mx4Args a) {
+  extern __shared__ __align__(16) char mx4_smem[];
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? BN / 2 : BN;
+  MoeWork wk;
+  if (!mx4_work<BM>(a, (cols_out + per - 1) / per, wk)) return;
+  constexpr int MT = Mx4Tile<BM, BN>::MT, WM = Mx4Tile<BM, BN>::WM;
+  const int need = (wk.i1 - wk.i0 + WM * 32 - 1) / (WM * 32);
+  if constexpr (MT == 4) {
+    if (need == 1) return mx4_many_tile<BM, BN, 1>(a, wk, mx4_smem);
+    if (need == 2) return mx4_many_tile<BM, BN, 2>(a, wk, mx4_smem);
+    if (need == 3) return mx4_many_tile<BM, BN, 3>(a, wk, mx4_smem);
+  } else if constexpr (MT == 2) {
+    if (need == 1) return mx4_many_tile<BM, BN, 1>(a, wk, mx4_smem);
+  }
+  mx4_many_tile<BM, BN, MT>(a, wk, mx4_smem);
+}
+
 int64_t mx4_grid(const Mx4Args& a, int bm, int bn) {
   if (a.offsets != nullptr) return moe_grid(a, bm, bn);
   const int64_t nt = ((int64_t)a.places + bm - 1) / bm;
@@ -260,9 +573,27 @@ hipError_t launch_few(const Mx4Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int BM, int BN>
+hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
+  auto* kernel = mx4_many_kernel<BM, BN>;
+  const int64_t grid = mx4_grid(a, BM, BN);
+  if (!moe_grid_fits(grid, 512)) return hipErrorInvalidConfiguration;
+  const hipError_t e = ensure_lds((const void*)kernel, Mx4Tile<BM, BN>::BYTES);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(512), (unsigned)(Mx4Tile<BM, BN>::BYTES), st, a);
+  return hipGetLastError();
+}
+
 hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
   if (!codes) return launch_few<1, 4, 4, false>(a, st);
-  return launch_few<4, 4, 4, true>(a, st);
+  const int avg = a.places / a.experts;
+  if (avg <= 8) return launch_few<1, 4, 4, true>(a, st);
+  if (avg <= 64) return launch_few<4, 4, 4, true>(a, st);
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? 64 : 128;
+  const int64_t small = (int64_t)((a.places + 127) / 128) * ((cols_out + per - 1) / per);
+  if (small <= 512) return launch_many<128, 128>(a, st);
+  if (avg <= 256) return launch_many<128, 256>(a, st);
+  return launch_many<256, 256>(a, st);
 }
 
 bool mx4_float(int d) { return d == HI_ROCM_DTYPE_F32 || d == HI_ROCM_DTYPE_BF16; }

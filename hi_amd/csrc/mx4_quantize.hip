@@ -70,10 +70,11 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, int64_t x
     else c = mx4_codes(v[i][0], s);
     if (un.in) {
       *reinterpret_cast<uint32_t*>(codes + un.row * (k / 2) + un.at / 2) = c;
-      if ((lane & 3) == 0) {
-        const int b = un.at / kMx4Block;
-        scales[un.row * scale_stride + (ROWS ? mx4_scale_at(b) : b)] = (uint8_t)s;
-      }
+    }
+    // (scales behind k: the unit's row is one of x's, its values are not)
+    if ((lane & 3) == 0 && (un.in || (ROWS && u0 + i < units))) {
+      const int b = un.at / kMx4Block;
+      scales[un.row * scale_stride + (ROWS ? mx4_scale_at(b) : b)] = (uint8_t)(un.in ? s : 127u);
     }
   }
 }
@@ -134,13 +135,13 @@ __global__ void __launch_bounds__(256) mx4_pack_scales_kernel(const uint8_t* sca
                                                               int64_t quads, int64_t count, uint32_t* out) {
   const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (w >= count) return;
-  const int lane = (int)(w & 63);
+  const int r = (int)(w >> 2) & 15, g = (int)(w & 3);
   const int64_t block = w >> 6, quad = block % quads, tile = block / quads % tiles, e = block / quads / tiles;
-  const int64_t row = tile * 16 + (lane & 15);
+  const int64_t row = tile * 16 + r;
   uint32_t v = 0u;
   #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int64_t b = quad * 16 + j * 4 + (lane >> 4);
+    const int64_t b = quad * 16 + j * 4 + g;
     const uint32_t s = row < n && b < blocks ? scales[(e * n + row) * blocks + b] : 127u;
     v |= s << (8 * j);
   }
