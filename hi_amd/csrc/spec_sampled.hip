@@ -29,8 +29,14 @@ namespace {
 
 constexpr int kSampledWaves = 4;
 constexpr int kSampledThreads = 64 * kSampledWaves;
-constexpr int kSampledFew = 2;    // loads a lane has in flight of a row: few parts ..
-constexpr int kSampledMany = 8;   // .. or long ones
+constexpr size_t kSampledLine = 128;
+// Values a lane has in flight of a row: enough to stream, few enough that their
+// f64 sums do not take longer than the loads' latency.  us with 4, 8 .. 64 KB parts
+// of f32 (8, 16, 32, 64 values a lane): 1 request of 151,936 6.2, 6.0, 6.7, 8.5; 64
+// requests 17.4, 15.4, 16.4, 17.9; bf16 (16, 32, 64, 128 values) 6.5, 6.9, 8.8, 12.5
+// and 13.6, 13.1, 14.6, 19.2.
+constexpr int kSampledValues = 16;
+constexpr int kSampledSpan = kSampledThreads * kSampledValues;  // values of a part
 
 struct SampledArgs {
   const void* target;
@@ -42,7 +48,7 @@ struct SampledArgs {
   const float* uniforms;     // [batch][K + 1]
   uint32_t* out_tokens;      // [batch][K + 1]
   int32_t* out_count;        // [batch]
-  uint32_t* counters;        // [batch], 0 between calls
+  uint32_t* counters;        // [batch], a line each, 0 between calls
   double* sums;              // [batch][parts * kSampledWaves]
   int V, K, parts;
 };
@@ -98,10 +104,28 @@ __device__ __forceinline__ double sampled_at(const SampledRest<T>& s, int j) {
   return sampled_rest(sampled_value(s.p + j), q);
 }
 
-__device__ __forceinline__ double sampled_wave_sum(double v) {
-  #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Sums over the wave's lanes up to each, by moves within the registers (six
+// steps through LDS took 0.2 us more a sum).
+template <int CTRL, int ROW_MASK = 0xf, bool BC = false>
+__device__ __forceinline__ double sampled_up(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = dpp32<CTRL, ROW_MASK, BC>(0u, (uint32_t)b), hi = dpp32<CTRL, ROW_MASK, BC>(0u, (uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double sampled_wave_scan(double v) {
+  v += sampled_up<kDppShr1, 0xf, true>(v);
+  v += sampled_up<kDppShr1 + 1, 0xf, true>(v);
+  v += sampled_up<kDppShr1 + 3, 0xf, true>(v);
+  v += sampled_up<kDppShr1 + 7, 0xf, true>(v);
+  v += sampled_up<kDppBcast15, 0xa>(v);
+  v += sampled_up<kDppBcast31, 0xc>(v);
   return v;
+}
+constexpr int kSampledHeld = 2;
+
+// A wave's sum, as its workgroup wrote it (from wherever it ran).
+__device__ __forceinline__ double sampled_sum(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 struct SampledLds {
@@ -116,12 +140,7 @@ struct SampledLds {
 // in `before` the sum before it.  All threads get both.
 __device__ __forceinline__ int sampled_pick(SampledLds& L, double v, double base, double bound, double& before) {
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  double incl = v;
-  #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += up;
-  }
+  double incl = sampled_wave_scan(v);
   __syncthreads();
   if (lane == 63) L.wave[wid] = incl;
   __syncthreads();
@@ -177,9 +196,9 @@ __device__ __forceinline__ int sampled_alone(SampledLds& L, const SampledRest<T>
   constexpr int kTile = kSampledThreads * 8;
   double total = 0.0;
   for (int j = threadIdx.x; j < V; j += kSampledThreads) total += sampled_at(s, j);
-  total = sampled_wave_sum(total);
+  total = sampled_wave_scan(total);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) L.wave[threadIdx.x >> 6] = total;
+  if ((threadIdx.x & 63) == 63) L.wave[threadIdx.x >> 6] = total;
   __syncthreads();
   total = 0.0;
   for (int w = 0; w < kSampledWaves; ++w) total += L.wave[w];
@@ -190,9 +209,9 @@ __device__ __forceinline__ int sampled_alone(SampledLds& L, const SampledRest<T>
     const int j1 = min(j0 + kTile, V);
     double sum = 0.0;
     for (int j = j0 + (int)threadIdx.x; j < j1; j += kSampledThreads) sum += sampled_at(s, j);
-    sum = sampled_wave_sum(sum);
+    sum = sampled_wave_scan(sum);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) L.wave[threadIdx.x >> 6] = sum;
+    if ((threadIdx.x & 63) == 63) L.wave[threadIdx.x >> 6] = sum;
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < kSampledWaves; ++w) sum += L.wave[w];
@@ -207,43 +226,50 @@ __device__ __forceinline__ int sampled_alone(SampledLds& L, const SampledRest<T>
   return token;
 }
 
-template <typename T, int I>
+template <typename T>
 __global__ void __launch_bounds__(kSampledThreads) spec_sampled_kernel(SampledArgs a) {
   __shared__ SampledLds L;
-  constexpr int E = SampledRow<T>::E, kWave = 64 * E * I;  // values of a wave
+  constexpr int E = SampledRow<T>::E, I = kSampledValues / E, kWave = 64 * kSampledValues;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / (uint32_t)a.parts, part = blockIdx.x % (uint32_t)a.parts;
   const int V = a.V, K = a.K;
   const T* target = (const T*)a.target + (int64_t)b * a.target_batch;
   const T* draft = a.draft != nullptr ? (const T*)a.draft + (int64_t)b * a.draft_batch : nullptr;
-  const int k = a.lengths != nullptr ? min(max(a.lengths[b], 0), K) : K;
-  // the accepted drafts, by every wave for itself
-  int n = k;
-  for (int i0 = 0; i0 < k; i0 += 64) {
+  // The accepted drafts, by every wave for itself (no load waits for the number
+  // of drafts: those past it are looked at in vain).
+  int k = K;
+  if (a.lengths != nullptr) k = min(max(a.lengths[b], 0), K);
+  const float u = a.uniforms[(int64_t)b * (K + 1) + K];
+  int n = K;
+  uint32_t certain = (uint32_t)V;
+  for (int i0 = 0; i0 < K; i0 += 64) {
     const int i = i0 + lane;
     bool rejected = false;
-    if (i < k) {
-      const uint32_t t = a.tokens[(int64_t)b * K + i];
-      const float u = a.uniforms[(int64_t)b * (K + 1) + i];
+    uint32_t t = (uint32_t)V;
+    if (i < K) {
+      t = a.tokens[(int64_t)b * K + i];
+      const float ui = a.uniforms[(int64_t)b * (K + 1) + i];
       rejected = true;
       if (t < (uint32_t)V) {
         const float p = sampled_value(target + i * a.target_row + t);
         const float q = draft != nullptr ? sampled_value(draft + i * a.draft_row + t) : 1.f;
-        rejected = !((double)u * (double)q < (double)p);
+        rejected = !((double)ui * (double)q < (double)p);
       }
     }
     const uint64_t no = __ballot(rejected);
     if (no != 0ull) {
-      n = i0 + __builtin_ctzll(no);
+      const int l = __builtin_ctzll(no);
+      n = i0 + l;
+      certain = (uint32_t)__builtin_amdgcn_readlane((int)t, l);
       break;
     }
   }
-  n = __builtin_amdgcn_readfirstlane(n);
+  n = __builtin_amdgcn_readfirstlane(min(n, k));
   SampledRest<T> s;
   s.p = target + n * a.target_row;
   s.q = n < k && draft != nullptr ? draft + n * a.draft_row : nullptr;
-  s.certain = n < k && draft == nullptr ? a.tokens[(int64_t)b * K + n] : (uint32_t)V;
+  s.certain = n < k && draft == nullptr ? certain : (uint32_t)V;
   // this wave's part
   const int j0 = min((part * kSampledWaves + wid) * kWave, V), j1 = min(j0 + kWave, V);
   SampledRow<T> rp, rq;
@@ -266,34 +292,40 @@ __global__ void __launch_bounds__(kSampledThreads) spec_sampled_kernel(SampledAr
       sum += j < j1 ? r : 0.0;
     }
   }
-  sum = sampled_wave_sum(sum);
+  sum = sampled_wave_scan(sum);
   double* sums = a.sums + (int64_t)b * a.parts * kSampledWaves;
-  if (lane == 0)
+  if (lane == 63)
     __hip_atomic_store(sums + part * kSampledWaves + wid, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // the request's last workgroup goes on
+  // The request's last workgroup goes on.  All that it reads of the others are
+  // the sums, written and read past the caches that one XCD has to itself (atomics
+  // of the agent's scope), and each wave's has arrived (vmcnt 0) before its
+  // workgroup counts: no fence, whose write-back of an XCD's L2 costs more than
+  // the whole call.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
-    __threadfence();
-    L.last = atomicAdd(a.counters + b, 1u) == (uint32_t)(a.parts - 1);
-    if (L.last) {
-      __threadfence();
-      a.counters[b] = 0u;
-    }
+    uint32_t* counter = a.counters + b * (kSampledLine / 4);
+    L.last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+             (uint32_t)(a.parts - 1);
+    if (L.last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!L.last) return;
+  // Each thread's waves, up to kSampledHeld of them in registers.
   const int pieces = a.parts * kSampledWaves, per = (pieces + kSampledThreads - 1) / kSampledThreads;
   const int c0 = min(tid * per, pieces), c1 = min(c0 + per, pieces);
-  double mine = 0.0;
-  for (int c = c0; c < c1; ++c) mine += __hip_atomic_load(sums + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  double total = sampled_wave_sum(mine);
-  if (lane == 0) L.wave[wid] = total;
+  double held[kSampledHeld], mine = 0.0;
+  #pragma unroll
+  for (int i = 0; i < kSampledHeld; ++i) held[i] = c0 + i < c1 ? sampled_sum(sums + c0 + i) : 0.0;
+  #pragma unroll
+  for (int i = 0; i < kSampledHeld; ++i) mine += held[i];
+  for (int c = c0 + kSampledHeld; c < c1; ++c) mine += sampled_sum(sums + c);
+  double total = sampled_wave_scan(mine);
+  if (lane == 63) L.wave[wid] = total;
   __syncthreads();
   total = 0.0;
   #pragma unroll
   for (int w = 0; w < kSampledWaves; ++w) total += L.wave[w];
-  const float u = a.uniforms[(int64_t)b * (K + 1) + K];
   int token = -1;
   if (total > 0.0) {
     const double bound = (double)u * total;
@@ -301,22 +333,52 @@ __global__ void __launch_bounds__(kSampledThreads) spec_sampled_kernel(SampledAr
     const int at = sampled_pick(L, mine, 0.0, bound, before);
     // (at is a thread: some share is above 0)
     if (tid == at) {
-      int c = c0, found = c0;
-      for (; c < c1; ++c) {
-        const double v = __hip_atomic_load(sums + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (!(v > 0.0)) continue;
+      int found = c0;
+      bool over = false;
+      auto look = [&](int c, double v) {
+        if (over || !(v > 0.0)) return;
         found = c;
         L.base = before;
-        if (before + v > bound) break;
+        over = before + v > bound;
         before += v;
-      }
+      };
+      #pragma unroll
+      for (int i = 0; i < kSampledHeld; ++i) look(c0 + i, held[i]);
+      for (int c = c0 + kSampledHeld; c < c1 && !over; ++c) look(c, sampled_sum(sums + c));
       L.at = found;
     }
     __syncthreads();
-    const int c = L.at;
+    const int c = __builtin_amdgcn_readfirstlane(L.at);
     const double base = L.base;
+    // that wave's values again, a load a thread
+    static_assert(kSampledThreads * E >= kWave, "one load covers a wave's part");
+    const int w0 = min(c * kWave, V), w1 = min(w0 + kWave, V);
+    rp.open(s.p + w0, w1 - w0);
+    rq.open(s.q != nullptr ? s.q + w0 : s.p + w0, s.q != nullptr ? w1 - w0 : 0);
+    const i32x4_t p4 = rp.load(tid * E), q4 = rq.load(tid * E);  // (behind the part: out of range, zero)
+    double r[E], share = 0.0;
+    #pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = w0 + tid * E + e;
+      const float q = (uint32_t)j == s.certain ? 1.f : SampledRow<T>::get(q4, e);
+      const double v = sampled_rest(SampledRow<T>::get(p4, e), q);
+      r[e] = j < w1 ? v : 0.0;
+      share += r[e];
+    }
+    const int in = sampled_pick(L, share, base, bound, before);
+    if (tid == in) {
+      bool over = false;
+      #pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (over || !(r[e] > 0.0)) continue;
+        token = w0 + tid * E + e;
+        before += r[e];
+        over = before > bound;
+      }
+      L.at = token;
+    }
     __syncthreads();
-    token = sampled_token(L, s, min(c * kWave, V), min((c + 1) * kWave, V), base, bound);
+    token = L.at;
   } else {
     s.q = nullptr;
     s.certain = (uint32_t)V;
@@ -332,29 +394,25 @@ __global__ void __launch_bounds__(kSampledThreads) spec_sampled_kernel(SampledAr
   if (tid == 0) a.out_count[b] = n + 1;
 }
 
-int sampled_parts(int vocab, int size, int loads) {
-  const int64_t span = (int64_t)kSampledThreads * (16 / size) * loads;
-  return (int)((vocab + span - 1) / span);
-}
+int sampled_parts(int vocab) { return (int)(((int64_t)vocab + kSampledSpan - 1) / kSampledSpan); }
 
-// The counters, which are 0 between calls, have a place that no batch or
-// vocabulary moves; behind them the sums, enough for either type.
+// The first half of a workspace holds the counters, which are 0 between calls, a
+// cache line each: counts on one line take some 5 ns after each other, wherever
+// they come from (64 requests of 151,936 f32: 15 us, with counters side by side 27).
+// The second holds the sums.  So the counters' place depends on the workspace's
+// size alone, not on a call's batch and vocabulary.
 constexpr int kSampledMaxBatch = 65535;
-constexpr size_t kSampledSums = 65536 * 4;
-size_t sampled_bytes(int64_t batch, int vocab) {
-  return kSampledSums + (size_t)batch * sampled_parts(vocab, 4, kSampledFew) * kSampledWaves * 8;
+size_t sampled_half(int64_t batch, int vocab) {
+  const size_t sums = (size_t)batch * sampled_parts(vocab) * kSampledWaves * 8;
+  return (std::max((size_t)batch * kSampledLine, sums) + kSampledLine - 1) / kSampledLine * kSampledLine;
 }
 
 template <typename T>
 hipError_t launch_sampled(SampledArgs& a, int batch, hipStream_t st) {
-  // Parts short enough that every CU has some: 32 KB where there are enough.
-  const bool many = (int64_t)batch * sampled_parts(a.V, sizeof(T), kSampledMany) >= 512;
-  a.parts = sampled_parts(a.V, sizeof(T), many ? kSampledMany : kSampledFew);
+  a.parts = sampled_parts(a.V);
   const int64_t groups = (int64_t)batch * a.parts;
   if (groups > UINT32_MAX / kSampledThreads) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)groups);
-  if (many) hipLaunchKernelGGL((spec_sampled_kernel<T, kSampledMany>), grid, dim3(kSampledThreads), 0, st, a);
-  else hipLaunchKernelGGL((spec_sampled_kernel<T, kSampledFew>), grid, dim3(kSampledThreads), 0, st, a);
+  hipLaunchKernelGGL((spec_sampled_kernel<T>), dim3((unsigned)groups), dim3(kSampledThreads), 0, st, a);
   return hipGetLastError();
 }
 
@@ -370,7 +428,7 @@ int hi_rocm_spec_sampled_workspace_bytes(int max_batch, int vocab, size_t* out_b
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_spec_sampled_workspace_bytes: invalid arguments");
   if (max_batch > kSampledMaxBatch || vocab > kMaxVocab)
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_spec_sampled_workspace_bytes: more than 65535 requests or 2^23 tokens");
-  *out_bytes = sampled_bytes(max_batch, vocab);
+  *out_bytes = 2 * sampled_half(max_batch, vocab);
   return HI_ROCM_OK;
 }
 
@@ -391,7 +449,7 @@ int hi_rocm_spec_verify_sampled(const void* target_probs, int dtype, int batch, 
   if (batch > kSampledMaxBatch || vocab > kMaxVocab || max_draft > 65535)
     return api_fail(HI_ROCM_ERR_UNSUPPORTED,
                     "hi_rocm_spec_verify_sampled: more than 65535 requests or drafts, or 2^23 tokens");
-  if ((uintptr_t)workspace % 16 != 0 || workspace_bytes < sampled_bytes(batch, vocab))
+  if ((uintptr_t)workspace % 16 != 0 || workspace_bytes < 2 * sampled_half(batch, vocab))
     return api_fail(HI_ROCM_ERR_ARGS,
                     "hi_rocm_spec_verify_sampled: workspace not on 16 bytes, or too small "
                     "(hi_rocm_spec_sampled_workspace_bytes)");
@@ -408,7 +466,7 @@ int hi_rocm_spec_verify_sampled(const void* target_probs, int dtype, int batch, 
   a.out_tokens = out_tokens;
   a.out_count = out_count;
   a.counters = (uint32_t*)workspace;
-  a.sums = (double*)((char*)workspace + kSampledSums);
+  a.sums = (double*)((char*)workspace + workspace_bytes / (2 * kSampledLine) * kSampledLine);
   a.V = vocab;
   a.K = max_draft;
   const hipError_t e = dtype == HI_ROCM_DTYPE_F32 ? launch_sampled<float>(a, batch, (hipStream_t)stream)

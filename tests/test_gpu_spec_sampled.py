@@ -128,7 +128,7 @@ def test_workspace_serves_any_batch(hip):
     for i, B in enumerate((64, 1, 33, 2, 64, 5)):
         dtype = (torch.float32, torch.bfloat16)[i % 2]
         check(*make(B, 3, 40000, dtype, i % 3 != 0, seed=i), plan=plan)
-    assert int(plan.workspace[:65536 * 4].view(torch.int32).abs().sum()) == 0
+    assert not plan.workspace[:plan.workspace.numel() // 2].any()  # the counters' half
 
 
 def test_frequencies(hip):
