@@ -33,7 +33,7 @@ OK, ERR_ARGS, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 DTYPE_F32, DTYPE_BF16, DTYPE_MX4 = 0, 1, 2
 FLAG_REP_ONCE = 1
 MAX_LOGPROBS = 1024
-MX4_FEW_ROWS, SPEC_NO_TOKEN = 16, 0xFFFFFFFF
+SPEC_NO_TOKEN = 0xFFFFFFFF
 BEAM_MAX, BEAM_MAX_OUT, BEAM_NO_EOS = 32, 64, 0xFFFFFFFF
 
 # Every function include/*.h declares, with its ctypes signature.
@@ -96,6 +96,7 @@ SIGNATURES = {
     "hi_rocm_mx4_rows": (_i, [_vp, _i, _i64, _i, _i64, _vp, _sz, _vp]),
     "hi_rocm_mx4_packed_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
     "hi_rocm_mx4_pack": (_i, [_vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "hi_rocm_mx4_workspace_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
     "hi_rocm_mx4_linear": (_i, [_vp, _i, _i, _i64, _vp, _sz, _i, _i, _vp, _vp, _i, _i64, _vp, _sz, _vp]),
     "hi_rocm_mx4_grouped_product": (_i, [_vp, _i, _i, _i64, _vp, _i, _vp, _i, _i, _vp, _sz, _i, _i, _i, _vp, _i, _i64,
                                          _sz, _vp, _sz, _vp]),

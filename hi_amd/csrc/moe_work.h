@@ -32,8 +32,15 @@ __device__ __forceinline__ bool moe_work(const Args& a, int blocks, MoeWork& wk)
     s = min(max(a.offsets[e], 0), a.places);
     return max(min(a.offsets[e + 1], a.places) - s, 0);
   };
+  // the first 256 experts' counts, asked for together and kept
+  constexpr int kKept = 4;
+  int start_of[kKept], count_of[kKept];
+  #pragma unroll
+  for (int c = 0; c < kKept; ++c) count_of[c] = c * 64 < a.experts ? count(c * 64 + lane, start_of[c]) : 0;
   int tiles = 0;
-  for (int e0 = 0; e0 < a.experts; e0 += 64) {
+  #pragma unroll
+  for (int c = 0; c < kKept; ++c) tiles += (count_of[c] + BM - 1) / BM;
+  for (int e0 = 64 * kKept; e0 < a.experts; e0 += 64) {
     int s;
     tiles += (count(e0 + lane, s) + BM - 1) / BM;
   }
@@ -44,8 +51,17 @@ __device__ __forceinline__ bool moe_work(const Args& a, int blocks, MoeWork& wk)
   if (slot >= per || w >= total) return false;
   int before = 0;  // tiles of the experts before e0
   for (int e0 = 0; e0 < a.experts; e0 += 64) {
-    int s;
-    const int n = count(e0 + lane, s), mine = (n + BM - 1) / BM;
+    int s, n = 0;
+    if (e0 < 64 * kKept) {
+      #pragma unroll
+      for (int c = 0; c < kKept; ++c) {
+        s = e0 == c * 64 ? start_of[c] : s;
+        n = e0 == c * 64 ? count_of[c] : n;
+      }
+    } else {
+      n = count(e0 + lane, s);
+    }
+    const int mine = (n + BM - 1) / BM;
     const int incl = before + (int)wave_incl_scan_u32((uint32_t)mine);
     const uint64_t hit = __ballot((int64_t)incl * blocks > w && (int64_t)(incl - mine) * blocks <= w);
     if (hit != 0ull) {
@@ -104,6 +120,15 @@ __device__ __forceinline__ void moe_wait() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 7 << 4);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// lgkmcnt 0
+__device__ __forceinline__ void moe_wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("" ::: "memory");
 }

@@ -53,6 +53,7 @@ struct Mx4Args {
 };
 
 // This workgroup's tile of BM places and block of columns.
+constexpr int kMx4Rows = 4;
 template <int BM>
 __device__ __forceinline__ bool mx4_work(const Mx4Args& a, int blocks, MoeWork& wk) {
   if (a.offsets != nullptr) return moe_work<BM>(a, blocks, wk);
@@ -60,9 +61,15 @@ __device__ __forceinline__ bool mx4_work(const Mx4Args& a, int blocks, MoeWork& 
   const int64_t total = (int64_t)nt * blocks, per = (total + kXcds - 1) / kXcds;
   const int64_t slot = blockIdx.x / kXcds, w = blockIdx.x % kXcds * per + slot;
   if (slot >= per || w >= total) return false;
+  // One expert: up to kMx4Rows tiles of places by all blocks, then the next tiles.
+  // What an XCD's CUs run at a time is then some tiles by some blocks, and its L2
+  // serves each of them more than once.
+  const int64_t group = w / ((int64_t)kMx4Rows * blocks);
+  const int first = (int)group * kMx4Rows, rows = min(nt - first, kMx4Rows);
+  const int local = (int)(w - group * kMx4Rows * blocks);
   wk.expert = 0;
-  wk.block = (int)(w / nt);
-  wk.i0 = (int)(w % nt) * BM;
+  wk.block = local / rows;
+  wk.i0 = (first + local % rows) * BM;
   wk.i1 = min(wk.i0 + BM, a.places);
   return true;
 }
@@ -119,21 +126,40 @@ __device__ __forceinline__ void mx4_store_codes(const Mx4Args& a, int p, bool in
   if (g == 0) mx4_store_scale(a, p, c / kMx4Block, s);
 }
 
-// Few places (decode): the weights are what is read.  The workgroup's waves
-// split k; each streams 16 NT columns' blocks straight into registers, two steps
-// ahead, and multiplies them with up to 16 MT places.  The waves' sums are added
-// in wave order.
-template <int MT, int NT, int W, bool CODES>
-__global__ void __launch_bounds__(64 * W) mx4_few_kernel(Mx4Args a) {
-  __shared__ mx4_f32x4 part[W - 1][MT * NT][64];
-  constexpr int COLS = 16 * NT;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wid = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+// Few places (decode): the weights are what is read.  The workgroup's waves take
+// the steps of k in turn; each streams 16 NT columns' blocks straight into
+// registers, D steps ahead, and multiplies them with up to 16 MT places.  Rounded
+// rows of x come the same way; bf16 ones are rounded into LDS first, while the
+// first weights are on their way (loads return in order: asked for in the loop, x
+// would hold up every weight asked for before it).  The waves' sums are added in
+// wave order.
+constexpr int kFewWaves = 4;
+
+// bytes from row to row of x in LDS: 16 rows' reads of a block meet all banks
+__host__ __device__ __forceinline__ int few_code_stride(int steps) { return steps * 64 + 16; }
+__host__ __device__ __forceinline__ int few_scale_stride(int quads) { return quads * 16 + 4; }
+
+template <int MT, int NT, int D, bool CODES>
+__global__ void __launch_bounds__(64 * kFewWaves) mx4_few_kernel(Mx4Args a) {
+  extern __shared__ __align__(16) char few_smem[];
+  constexpr int W = kFewWaves, COLS = 16 * NT;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols;
   const int per = a.swiglu ? COLS / 2 : COLS;
   MoeWork wk;
   if (!mx4_work<16 * MT>(a, (cols_out + per - 1) / per, wk)) return;
-  const int c0 = wk.block * per;
+  const int c0 = wk.block * per, n_places = wk.i1 - wk.i0;
+  // bf16 rows: this thread's blocks of them, asked for before the weights
+  const int blocks = a.k / kMx4Block, todo = CODES ? 0 : n_places * blocks;
+  uint4 raw[4];
+  auto raw_load = [&](int b) {
+    const int j = b / blocks;
+    const uint4* p = reinterpret_cast<const uint4*>(a.x + mx4_row(a, wk.i0 + j) * a.x_stride) + (b - j * blocks) * 4;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = p[i];
+  };
+  if (!CODES && tid < todo) raw_load(tid);
   const uint8_t* wp[NT];
   const uint8_t* sp[NT];
   #pragma unroll
@@ -146,112 +172,143 @@ __global__ void __launch_bounds__(64 * W) mx4_few_kernel(Mx4Args a) {
   }
   const uint8_t* xp[MT];
   const uint8_t* xs[MT];
-  #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int64_t row = mx4_row(a, min(wk.i0 + 16 * m + r, wk.i1 - 1));
-    xp[m] = a.x + row * a.x_stride + g * (CODES ? 16 : 64);
-    xs[m] = CODES ? a.x_scales + row * a.x_scale_stride + 4 * g : nullptr;
+  if constexpr (CODES) {
+    #pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int64_t row = mx4_row(a, min(wk.i0 + 16 * m + r, wk.i1 - 1));
+      xp[m] = a.x + row * a.x_stride + 16 * g;
+      xs[m] = a.x_scales + row * a.x_scale_stride + 4 * g;
+    }
   }
   mx4_f32x4 acc[MT][NT];
   #pragma unroll
   for (int m = 0; m < MT; ++m)
     #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = mx4_f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int XL = CODES ? 1 : 4;
-  mx4_i32x4 wv[2][NT];
-  int ws[2][NT];
-  uint4 xv[2][MT][XL];
-  uint32_t xsc[2][MT];
+  mx4_i32x4 wv[D][NT], xv[D][MT];
+  int ws[D][NT], xsc[D][MT];
   auto load = [&](int slot, int step) {
-    const bool in = step * kMx4Step + g * kMx4Block < a.k;
     #pragma unroll
     for (int t = 0; t < NT; ++t) {
       wv[slot][t] = *reinterpret_cast<const mx4_i32x4*>(wp[t] + (int64_t)step * 1024);
-      ws[slot][t] = sp[t][(step >> 2) * 256 + (step & 3)];
+      ws[slot][t] = *reinterpret_cast<const int*>(sp[t] + (step >> 2) * 256);
     }
-    #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    if constexpr (CODES) {
+      // (past k: the row's neighbours or scales, any code being finite, meet weights
+      // of 0 and scales of 1)
       #pragma unroll
-      for (int i = 0; i < XL; ++i)
-        xv[slot][m][i] = in ? reinterpret_cast<const uint4*>(xp[m] + (int64_t)step * (CODES ? 64 : 256))[i]
-                            : uint4{0u, 0u, 0u, 0u};
-      xsc[slot][m] = CODES ? (in ? xs[m][(step >> 2) * 16 + (step & 3)] : 127u) : 0u;
+      for (int m = 0; m < MT; ++m) {
+        xv[slot][m] = *reinterpret_cast<const mx4_i32x4*>(xp[m] + (int64_t)step * 64);
+        xsc[slot][m] = *reinterpret_cast<const int*>(xs[m] + (step >> 2) * 16);
+      }
     }
   };
-  auto multiply = [&](int slot) {
+  #pragma unroll
+  for (int d = 0; d < D; ++d) load(d, min(wid + d * W, a.steps - 1));
+  const int xc_stride = few_code_stride(a.steps), xs_stride = few_scale_stride(a.quads);
+  char* const x_scales = few_smem + n_places * xc_stride;
+  if constexpr (!CODES) {
+    // (blocks behind k in its last step: zeros)
+    const int tail = a.steps * 4 - blocks;
+    for (int i = tid; i < n_places * tail; i += 64 * W) {
+      const int j = i / tail, b = blocks + i - j * tail;
+      *reinterpret_cast<uint4*>(few_smem + j * xc_stride + b * 16) = uint4{0u, 0u, 0u, 0u};
+      x_scales[j * xs_stride + mx4_scale_at(b)] = 127;
+    }
+    for (int b = tid; b < todo; b += 64 * W) {
+      const uint32_t s = mx4_scale_of(mx4_field(mx4_max_pair(mx4_max_pair(mx4_max_of(raw[0]), mx4_max_of(raw[1])),
+                                                             mx4_max_pair(mx4_max_of(raw[2]), mx4_max_of(raw[3])))));
+      const uint4 c = {mx4_codes(raw[0], s), mx4_codes(raw[1], s), mx4_codes(raw[2], s), mx4_codes(raw[3], s)};
+      const int j = b / blocks, kb = b - j * blocks;
+      if (b + 64 * W < todo) raw_load(b + 64 * W);
+      *reinterpret_cast<uint4*>(few_smem + j * xc_stride + kb * 16) = c;
+      x_scales[j * xs_stride + mx4_scale_at(kb)] = (char)s;
+    }
+    moe_wait_lds();  // (the weights stay on their way)
+    moe_barrier();
+  }
+  const int rr = min(r, n_places - 1);  // (MT = 1 here)
+  const char* const xrow = few_smem + rr * xc_stride + g * 16;
+  const char* const srow = x_scales + rr * xs_stride + g * 4;
+  const int shift = (wid & 3) * 8;  // every step of this wave's is the same of its quad
+  auto multiply = [&](int slot, int step) {
     #pragma unroll
     for (int m = 0; m < MT; ++m) {
       mx4_i32x4 xc;
-      uint32_t s;
+      int s;
       if constexpr (CODES) {
-        xc = __builtin_bit_cast(mx4_i32x4, xv[slot][m][0]);
+        xc = xv[slot][m];
         s = xsc[slot][m];
       } else {
-        s = mx4_scale_of(mx4_field(mx4_max_pair(mx4_max_pair(mx4_max_of(xv[slot][m][0]), mx4_max_of(xv[slot][m][1])),
-                                                mx4_max_pair(mx4_max_of(xv[slot][m][2]), mx4_max_of(xv[slot][m][3])))));
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) xc[i] = (int)mx4_codes(xv[slot][m][i], s);
+        xc = *reinterpret_cast<const mx4_i32x4*>(xrow + step * 64);
+        s = *reinterpret_cast<const int*>(srow + (step >> 2) * 16);
       }
+      s = (int)((uint32_t)s >> shift);
       #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[m][t] = mx4_mfma<0, 0>(wv[slot][t], xc, acc[m][t], ws[slot][t], (int)s);
+      for (int t = 0; t < NT; ++t)
+        acc[m][t] = mx4_mfma<0, 0>(wv[slot][t], xc, acc[m][t], (int)((uint32_t)ws[slot][t] >> shift), s);
     }
   };
-  const int share = (a.steps + W - 1) / W;
-  const int b0 = min(wid * share, a.steps), b1 = min(b0 + share, a.steps);
-  if (b0 < b1) load(0, b0);
-  if (b0 + 1 < b1) load(1, b0 + 1);
-  for (int b = b0; b < b1; b += 2) {
-    multiply(0);
-    if (b + 2 < b1) load(0, b + 2);
-    if (b + 1 < b1) {
-      multiply(1);
-      if (b + 3 < b1) load(1, b + 3);
+  // (no condition stands between a load and its use: the compiler would have to
+  // wait for all that may be on its way.  Past the last step a slot loads that again.)
+  int s = wid;
+  for (; s + D * W < a.steps; s += D * W) {
+    #pragma unroll
+    for (int d = 0; d < D; ++d) {
+      multiply(d, s + d * W);
+      load(d, min(s + (d + D) * W, a.steps - 1));
     }
   }
-  if (wid > 0) {
-    #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      #pragma unroll
-      for (int t = 0; t < NT; ++t) part[wid - 1][m * NT + t][lane] = acc[m][t];
-  }
-  __syncthreads();
-  if (wid > 0) return;
   #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int d = 0; d < D; ++d)
+    if (s + d * W < a.steps) multiply(d, s + d * W);
+  mx4_f32x4* const part = reinterpret_cast<mx4_f32x4*>(few_smem);
+  if constexpr (!CODES) moe_barrier();  // (x's place; its reads are behind their products)
+  #pragma unroll
+  for (int m = 0; m < MT; ++m)
     #pragma unroll
-    for (int t = 0; t < NT; ++t)
-      #pragma unroll
-      for (int w = 0; w < W - 1; ++w) acc[m][t] += part[w][m * NT + t][lane];
-    const int p = wk.i0 + 16 * m + r;
-    const bool in = p < wk.i1;
-    if (a.swiglu) {
-      if constexpr (NT >= 2) {
+    for (int t = 0; t < NT; ++t) part[((m * NT + t) * W + wid) * 64 + lane] = acc[m][t];
+  __syncthreads();
+  auto total = [&](int m, int t) {
+    mx4_f32x4 y = part[((m * NT + t) * W) * 64 + lane];
+    #pragma unroll
+    for (int w = 1; w < W; ++w) y += part[((m * NT + t) * W + w) * 64 + lane];
+    return y;
+  };
+  if (a.swiglu) {
+    if constexpr (NT >= 2) {
+      for (int m = wid; m < MT; m += W) {
+        const int p = wk.i0 + 16 * m + r;
+        const bool in = p < wk.i1;
+        mx4_f32x4 y[NT / 2];
         #pragma unroll
-        for (int t = 0; t < NT / 2; ++t)
+        for (int t = 0; t < NT / 2; ++t) {
+          const mx4_f32x4 gate = total(m, t), up = total(m, t + NT / 2);
           #pragma unroll
-          for (int q = 0; q < 4; ++q) acc[m][t][q] = moe_silu_mul(acc[m][t][q], acc[m][t + NT / 2][q]);
+          for (int q = 0; q < 4; ++q) y[t][q] = moe_silu_mul(gate[q], up[q]);
+        }
         if constexpr (NT == 4) {
           if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
-            mx4_store_codes(a, p, in, c0, g, acc[m][0], acc[m][1]);
+            mx4_store_codes(a, p, in, c0, g, y[0], y[1]);
             continue;
           }
         }
         #pragma unroll
         for (int t = 0; t < NT / 2; ++t)
-          if (in && c0 + t * 16 + 4 * g < cols_out) mx4_store(a, p, c0 + t * 16 + 4 * g, cols_out, acc[m][t]);
-      }
-    } else {
-      #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int c = c0 + t * 16 + 4 * g;
-        if (!in || c >= cols_out) continue;
-        if (a.bias != nullptr) {
-          #pragma unroll
-          for (int q = 0; q < 4; ++q) acc[m][t][q] += c + q < cols_out ? a.bias[c + q] : 0.f;
-        }
-        mx4_store(a, p, c, cols_out, acc[m][t]);
+          if (in && c0 + t * 16 + 4 * g < cols_out) mx4_store(a, p, c0 + t * 16 + 4 * g, cols_out, y[t]);
       }
     }
+    return;
+  }
+  for (int i = wid; i < MT * NT; i += W) {
+    const int m = i / NT, t = i % NT, p = wk.i0 + 16 * m + r, c = c0 + t * 16 + 4 * g;
+    if (p >= wk.i1 || c >= cols_out) continue;
+    mx4_f32x4 y = total(m, t);
+    if (a.bias != nullptr) {
+      #pragma unroll
+      for (int q = 0; q < 4; ++q) y[q] += c + q < cols_out ? a.bias[c + q] : 0.f;
+    }
+    mx4_store(a, p, c, cols_out, y);
   }
 }
 
@@ -275,8 +332,8 @@ __global__ void __launch_bounds__(64 * W) mx4_few_kernel(Mx4Args a) {
 // scales, started before the loads of a quad's first step, among those of its
 // third.
 //
-// A row of a step is 64 bytes; its 16-byte chunk c lies at c ^ (row / 2 & 3), so
-// that the reads of a chunk of eight rows meet all banks.  A load writes 64 lanes
+// A row of a step is 64 bytes; its 16-byte chunk c lies at c ^ (row / 4 & 3), so
+// that the reads of a chunk of 16 rows meet all banks.  A load writes 64 lanes
 // x 16 contiguous bytes; the lanes choose their global addresses so that the
 // chunks land there.  Chunks of x past k hold what follows in memory (the next
 // row, or the scales): any code is finite, and meets weights of 0 and scales of 1.
@@ -415,7 +472,7 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
   // (rows past the weight's last tile: that tile's)
   auto weight_row = [&](int j) { return min(column(j), a.tiles * 16 - 16 + (j & 15)); };
   const int jr = tid / 4;                       // this thread's row in each round of loads
-  const int chunk = (tid & 3) ^ (jr >> 1 & 3);  // and the chunk that lands there
+  const int chunk = (tid & 3) ^ (jr >> 2 & 3);  // and the chunk that lands there
   const uint8_t* xp[XL];
   const uint8_t* wp[WL];
   const int64_t base = (int64_t)wk.expert * a.tiles;
@@ -490,7 +547,7 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
     }
     #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int at = J * STEP + ((2 * u + h) ^ (r >> 1 & 3)) * 16;
+      const int at = J * STEP + ((2 * u + h) ^ (r >> 2 & 3)) * 16;
       #pragma unroll
       for (int t = 0; t < 2; ++t) wf[t][u] = *reinterpret_cast<const mx4_i32x4*>(wrow + t * 2048 + at);
       #pragma unroll
@@ -565,11 +622,17 @@ int64_t mx4_grid(const Mx4Args& a, int bm, int bn) {
   return (nt * (((int64_t)a.cols + bn - 1) / bn) + kXcds - 1) / kXcds * kXcds;
 }
 
-template <int MT, int NT, int W, bool CODES>
+template <int MT, int NT, int D, bool CODES>
 hipError_t launch_few(const Mx4Args& a, hipStream_t st) {
   const int64_t grid = mx4_grid(a, 16 * MT, 16 * NT);
-  if (!moe_grid_fits(grid, 64 * W)) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((mx4_few_kernel<MT, NT, W, CODES>), dim3((unsigned)grid), dim3(64 * W), 0, st, a);
+  if (!moe_grid_fits(grid, 64 * kFewWaves)) return hipErrorInvalidConfiguration;
+  int bytes = MT * NT * kFewWaves * 1024;  // the waves' sums, and before them x
+  if (!CODES)
+    bytes = std::max(bytes, std::min(a.places, 16 * MT) * (few_code_stride(a.steps) + few_scale_stride(a.quads)));
+  auto* kernel = mx4_few_kernel<MT, NT, D, CODES>;
+  const hipError_t e = ensure_lds((const void*)kernel, bytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * kFewWaves), (unsigned)bytes, st, a);
   return hipGetLastError();
 }
 
@@ -585,10 +648,12 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
 }
 
 hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
-  if (!codes) return launch_few<1, 4, 4, false>(a, st);
+  const bool longer = a.steps > 2 * kFewWaves;
+  if (!codes) return longer ? launch_few<1, 4, 4, false>(a, st) : launch_few<1, 4, 2, false>(a, st);
   const int avg = a.places / a.experts;
-  if (avg <= 8) return launch_few<1, 4, 4, true>(a, st);
-  if (avg <= 64) return launch_few<4, 4, 4, true>(a, st);
+  if (avg <= 16) return longer ? launch_few<1, 4, 4, true>(a, st) : launch_few<1, 4, 2, true>(a, st);
+  if (avg <= 32) return launch_few<2, 4, 2, true>(a, st);
+  if (avg <= 64) return launch_few<4, 4, 2, true>(a, st);
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? 64 : 128;
   const int64_t small = (int64_t)((a.places + 127) / 128) * ((cols_out + per - 1) / per);
   if (small <= 512) return launch_many<128, 128>(a, st);
@@ -599,13 +664,19 @@ hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
 bool mx4_float(int d) { return d == HI_ROCM_DTYPE_F32 || d == HI_ROCM_DTYPE_BF16; }
 int mx4_size(int d) { return d == HI_ROCM_DTYPE_F32 ? 4 : 2; }
 
+// Few bf16 rows are rounded by each workgroup in LDS, at most 16 of them and 65,536
+// values (36 KB); more, beforehand in a workspace.
+bool mx4_needs_rows(int64_t x_rows, int64_t places, int k) {
+  return x_rows > 16 || std::min<int64_t>(places, 16) * k > 65536;
+}
+
 // x as a product reads it: "rows" given, bf16 rows as they are when they are
 // few, or "rows" made of them in the workspace.
 int mx4_take_x(const char* name, Mx4Args& a, const void* x, int x_dtype, int64_t x_rows, int64_t x_stride, void* ws,
                size_t ws_bytes, hipStream_t st, bool& codes) {
   const Mx4Rows L = mx4_rows_layout(x_rows, a.k);
   a.x_rows = (int)x_rows;
-  codes = x_dtype == HI_ROCM_DTYPE_MX4 || x_rows > HI_ROCM_MX4_FEW_ROWS;
+  codes = x_dtype == HI_ROCM_DTYPE_MX4 || mx4_needs_rows(x_rows, a.places, a.k);
   if (!codes) {
     a.x = (const uint8_t*)x;
     a.x_stride = x_stride * 2;
@@ -631,7 +702,7 @@ int mx4_fail(int status, const char* name, const char* what) {
 
 // What both products check of x and the weight.
 int mx4_check(const char* name, const void* x, int x_dtype, int64_t x_rows, int64_t x_stride, const void* packed,
-              size_t packed_bytes, int experts, int n, int k, const void* ws, size_t ws_bytes) {
+              size_t packed_bytes, int places, int experts, int n, int k, const void* ws, size_t ws_bytes) {
   if (x == nullptr || packed == nullptr || x_rows <= 0 || n <= 0 || k <= 0 || experts <= 0 ||
       (x_dtype != HI_ROCM_DTYPE_BF16 && x_dtype != HI_ROCM_DTYPE_MX4) || (x_dtype == HI_ROCM_DTYPE_BF16 && x_stride < k))
     return mx4_fail(HI_ROCM_ERR_ARGS, name, "invalid arguments");
@@ -642,9 +713,9 @@ int mx4_check(const char* name, const void* x, int x_dtype, int64_t x_rows, int6
     return mx4_fail(HI_ROCM_ERR_ARGS, name, "packed not on 16 bytes, or too small (hi_rocm_mx4_packed_bytes)");
   if ((uintptr_t)x % 16 != 0 || (x_dtype == HI_ROCM_DTYPE_BF16 && x_stride % 8 != 0))
     return mx4_fail(HI_ROCM_ERR_UNSUPPORTED, name, "needs rows that start on 16 bytes");
-  if (x_dtype == HI_ROCM_DTYPE_BF16 && x_rows > HI_ROCM_MX4_FEW_ROWS &&
+  if (x_dtype == HI_ROCM_DTYPE_BF16 && mx4_needs_rows(x_rows, places, k) &&
       (ws == nullptr || (uintptr_t)ws % 16 != 0 || ws_bytes < mx4_rows_layout(x_rows, k).total))
-    return mx4_fail(HI_ROCM_ERR_ARGS, name, "workspace not on 16 bytes, or too small (hi_rocm_mx4_rows_bytes)");
+    return mx4_fail(HI_ROCM_ERR_ARGS, name, "workspace not on 16 bytes, or too small (hi_rocm_mx4_workspace_bytes)");
   return HI_ROCM_OK;
 }
 
@@ -667,11 +738,22 @@ using namespace hi_rocm;
 
 extern "C" {
 
+int hi_rocm_mx4_workspace_bytes(int x_rows, int places, int k, size_t* out_bytes) {
+  if (x_rows <= 0 || places <= 0 || k <= 0 || out_bytes == nullptr)
+    return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_mx4_workspace_bytes: invalid arguments");
+  if (k % kMx4Block != 0 || k > HI_ROCM_MX4_MAX_K || x_rows > HI_ROCM_MX4_MAX_ROWS || places > HI_ROCM_MX4_MAX_ROWS)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED,
+                    "hi_rocm_mx4_workspace_bytes: needs k a multiple of 32 up to 2^24, at most 2^22 rows and places");
+  *out_bytes = mx4_needs_rows(x_rows, places, k) ? mx4_rows_layout(x_rows, k).total : 0;
+  return HI_ROCM_OK;
+}
+
 int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
                        int n, int k, const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                        size_t workspace_bytes, void* stream) {
   const char* name = "hi_rocm_mx4_linear";
-  const int bad = mx4_check(name, x, x_dtype, rows, x_stride, packed, packed_bytes, 1, n, k, workspace, workspace_bytes);
+  const int bad = mx4_check(name, x, x_dtype, rows, x_stride, packed, packed_bytes, rows, 1, n, k, workspace,
+                            workspace_bytes);
   if (bad != HI_ROCM_OK) return bad;
   if (out == nullptr || !mx4_float(out_dtype) || out_stride < n || (uintptr_t)out % mx4_size(out_dtype) != 0 ||
       (uintptr_t)bias % 4 != 0)
@@ -702,7 +784,8 @@ int hi_rocm_mx4_grouped_product(const void* x, int x_dtype, int x_rows, int64_t 
                                 void* stream) {
   const char* name = "hi_rocm_mx4_grouped_product";
   const int bad =
-      mx4_check(name, x, x_dtype, x_rows, x_stride, packed, packed_bytes, experts, cols, k, workspace, workspace_bytes);
+      mx4_check(name, x, x_dtype, x_rows, x_stride, packed, packed_bytes, places, experts, cols, k, workspace,
+                workspace_bytes);
   if (bad != HI_ROCM_OK) return bad;
   const int wide = swiglu ? cols / 2 : cols;
   const bool to_rows = out_dtype == HI_ROCM_DTYPE_MX4;

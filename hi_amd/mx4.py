@@ -9,7 +9,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from ._lib import DTYPE_BF16, DTYPE_MX4, MX4_FEW_ROWS, check, load
+from ._lib import DTYPE_BF16, DTYPE_MX4, check, load
 from .beam import _CODES, _empty, _on, _ptr, _stream
 from .moe import RowGroups
 
@@ -140,6 +140,7 @@ class Mx4Linear:
         self.bias = bias
         self.packed = _pack(what, codes, scales, 1, stream)
         self._bytes = self.packed.numel()
+        self._work = {}  # rows: bytes of their workspace
 
     def __call__(self, x: Union[torch.Tensor, Mx4Rows], out: Optional[torch.Tensor] = None, dtype=torch.float32,
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
@@ -165,10 +166,12 @@ class Mx4Linear:
             raise ValueError(f"{what}: out must be a float32 or bfloat16 [{rows}][{n}] tensor, outputs contiguous")
         _on(what, dev, memory, out)
         lib, st = load(), _stream(what, dev, stream)
-        if code_x == DTYPE_BF16 and rows > MX4_FEW_ROWS:
-            # a call's own: calls on several streams, or captured ones, share nothing
-            work_bytes = _size(lib.hi_rocm_mx4_rows_bytes, rows, k)
-            work = _empty((work_bytes,), torch.uint8, packed.device, stream)
+        if code_x == DTYPE_BF16:
+            work_bytes = self._work.get(rows)
+            if work_bytes is None:
+                work_bytes = self._work[rows] = _size(lib.hi_rocm_mx4_workspace_bytes, rows, rows, k)
+            if work_bytes:  # a call's own: calls on several streams, or captured ones, share nothing
+                work = _empty((work_bytes,), torch.uint8, packed.device, stream)
         # (a single row's stride says nothing)
         check(lib.hi_rocm_mx4_linear(
             at, code_x, rows, stride, packed.data_ptr(), self._bytes, n, k, _ptr(self.bias), out.data_ptr(), code,

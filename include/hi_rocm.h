@@ -536,8 +536,6 @@ int hi_rocm_moe_combine(const void* y, int y_dtype, int64_t y_stride, const int3
  * u8[rows][k / 32].  k is a multiple of 32. */
 #define HI_ROCM_MX4_MAX_K (1 << 24)
 #define HI_ROCM_MX4_MAX_ROWS (1 << 22)
-/* Up to so many rows of x, the products round bf16 rows as they read them. */
-#define HI_ROCM_MX4_FEW_ROWS 16
 
 /* Rounds x (f32 or bf16 [rows][x_stride], rows on 16 bytes): s = floor(log2 a) + 125
  * for a block's largest magnitude a, at least 0 (and 0 for a = 0); values times
@@ -564,15 +562,19 @@ int hi_rocm_mx4_packed_bytes(int experts, int n, int k, size_t* out_bytes);
 int hi_rocm_mx4_pack(const uint8_t* codes, const uint8_t* scales, int experts, int n, int k, void* packed,
                      size_t packed_bytes, void* stream);
 
+/* Bytes of the workspace that the products below need for bf16 x: 0 where the rows
+ * are few enough to be rounded on the way, else those of hi_rocm_mx4_rows.  places:
+ * the rows of a linear layer, tokens * top_k of a grouped product. */
+int hi_rocm_mx4_workspace_bytes(int x_rows, int places, int k, size_t* out_bytes);
+
 /* out[m][c] = sum_k Q(x[m])[k] * w[c][k] + bias[c], Q the rounding above: x bf16
  * [rows][x_stride] (rows on 16 bytes) or rows (x_dtype HI_ROCM_DTYPE_MX4, x_stride
  * not used); bias f32[n] or NULL; out f32 or bf16 [rows][out_stride].  Sums are f32,
  * products exact.  A row's result does not depend on the other rows' values; a row
  * that holds an infinity or NaN gives NaN; where the magnitudes of a sum's terms pass
- * f32's largest, it may be an infinity or NaN.  With more than HI_ROCM_MX4_FEW_ROWS bf16
- * rows the workspace holds them rounded (hi_rocm_mx4_rows_bytes of them, 16-byte
- * aligned, no initial value, one stream at a time); else it may be NULL.  At most
- * 2^22 rows.  No allocation: graph-capturable. */
+ * f32's largest, it may be an infinity or NaN.  The workspace
+ * (hi_rocm_mx4_workspace_bytes; NULL where that is 0 or x is rows) is on 16 bytes, needs no
+ * initial value and serves one stream at a time.  At most 2^22 rows.  No allocation: graph-capturable. */
 int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
                        int n, int k, const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                        size_t workspace_bytes, void* stream);
