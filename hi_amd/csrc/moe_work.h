@@ -26,17 +26,17 @@ struct MoeWork {
 template <int BM, typename Args>
 __device__ __forceinline__ bool moe_work(const Args& a, int blocks, MoeWork& wk) {
   const int lane = threadIdx.x & 63;
+  // (past the last expert: none, without a branch that a load would wait behind)
   auto count = [&](int e, int& s) {
-    s = 0;
-    if (e >= a.experts) return 0;
-    s = min(max(a.offsets[e], 0), a.places);
-    return max(min(a.offsets[e + 1], a.places) - s, 0);
+    const int from = a.offsets[min(e, a.experts)], to = a.offsets[min(e + 1, a.experts)];
+    s = min(max(from, 0), a.places);
+    return max(min(to, a.places) - s, 0);
   };
   // the first 256 experts' counts, asked for together and kept
   constexpr int kKept = 4;
   int start_of[kKept], count_of[kKept];
   #pragma unroll
-  for (int c = 0; c < kKept; ++c) count_of[c] = c * 64 < a.experts ? count(c * 64 + lane, start_of[c]) : 0;
+  for (int c = 0; c < kKept; ++c) count_of[c] = count(c * 64 + lane, start_of[c]);
   int tiles = 0;
   #pragma unroll
   for (int c = 0; c < kKept; ++c) tiles += (count_of[c] + BM - 1) / BM;

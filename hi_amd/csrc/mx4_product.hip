@@ -127,28 +127,35 @@ __device__ __forceinline__ void mx4_store_codes(const Mx4Args& a, int p, bool in
 }
 
 // Few places (decode): the weights are what is read.  The workgroup's waves take
-// the steps of k in turn; each streams 16 NT columns' blocks straight into
-// registers, D steps ahead, and multiplies them with up to 16 MT places.  Rounded
-// rows of x come the same way; bf16 ones are rounded into LDS first, while the
-// first weights are on their way (loads return in order: asked for in the loop, x
-// would hold up every weight asked for before it).  The waves' sums are added in
-// wave order.
+// the steps of k in turn; each streams 64 columns' blocks straight into registers,
+// a step ahead, and multiplies them with up to 16 MT places.  Rounded rows of x come
+// the same way; bf16 ones are rounded into LDS first, while the first weights are on
+// their way (loads return in order: asked for in the loop, x would hold up every
+// weight asked for before it).  The waves' sums are added in wave order.
+// What hides the latency of a workgroup's beginning and end is the number of
+// workgroups a CU holds: with two or four steps ahead (120 and 156 registers) a
+// head of 151,936 x 4096 took 56 us, with one (six workgroups a CU) 55; 200 tokens'
+// experts 44 and 47, with one 40; with eight (spilling) 66 and 42.
 constexpr int kFewWaves = 4;
+constexpr int kFewCols = 64;
 
 // bytes from row to row of x in LDS: 16 rows' reads of a block meet all banks
 __host__ __device__ __forceinline__ int few_code_stride(int steps) { return steps * 64 + 16; }
 __host__ __device__ __forceinline__ int few_scale_stride(int quads) { return quads * 16 + 4; }
 
-template <int MT, int NT, int D, bool CODES>
-__global__ void __launch_bounds__(64 * kFewWaves) mx4_few_kernel(Mx4Args a) {
+template <int MT, bool CODES>
+__global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kernel(Mx4Args a) {
   extern __shared__ __align__(16) char few_smem[];
-  constexpr int W = kFewWaves, COLS = 16 * NT;
+  constexpr int W = kFewWaves, COLS = kFewCols, NT = COLS / 16;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols;
   const int per = a.swiglu ? COLS / 2 : COLS;
   MoeWork wk;
   if (!mx4_work<16 * MT>(a, (cols_out + per - 1) / per, wk)) return;
+  // (all lanes' alike, which divisions in vector registers hide from the compiler)
+  wk.expert = __builtin_amdgcn_readfirstlane(wk.expert);
+  wk.block = __builtin_amdgcn_readfirstlane(wk.block);
   const int c0 = wk.block * per, n_places = wk.i1 - wk.i0;
   // bf16 rows: this thread's blocks of them, asked for before the weights
   const int blocks = a.k / kMx4Block, todo = CODES ? 0 : n_places * blocks;
@@ -160,24 +167,24 @@ __global__ void __launch_bounds__(64 * kFewWaves) mx4_few_kernel(Mx4Args a) {
     for (int i = 0; i < 4; ++i) raw[i] = p[i];
   };
   if (!CODES && tid < todo) raw_load(tid);
-  const uint8_t* wp[NT];
-  const uint8_t* sp[NT];
+  // The weights by buffer loads, whose addresses are a lane's constant and scalars:
+  // two halves of the tiles (with swiglu gate columns, then up columns), each tile
+  // so many bytes behind its half's first.
+  constexpr int HN = NT / 2;
+  __amdgpu_buffer_rsrc_t wr[2], sr[2];
+  int w_tile[NT], s_tile[NT];
+  const int w_lane = lane * 16, s_lane = r * 16 + g * 4;
   #pragma unroll
-  for (int t = 0; t < NT; ++t) {  // with swiglu tiles of gate columns, then the same of up columns
-    int tile = c0 / 16 + t;
-    if (a.swiglu) tile = c0 / 16 + t % (NT / 2) + (t >= NT / 2 ? cols_out / 16 : 0);
-    const int64_t at = (int64_t)wk.expert * a.tiles + min(tile, a.tiles - 1);
-    wp[t] = a.w + at * a.steps * 1024 + lane * 16;
-    sp[t] = a.w_scales + at * a.quads * 256 + r * 16 + g * 4;
-  }
-  const uint8_t* xp[MT];
-  const uint8_t* xs[MT];
-  if constexpr (CODES) {
+  for (int u = 0; u < 2; ++u) {
+    const int tile = min(c0 / 16 + u * (a.swiglu ? cols_out / 16 : HN), a.tiles - 1);
+    const int64_t at = (int64_t)wk.expert * a.tiles + tile;
+    wr[u] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + at * a.steps * 1024), 0, -1, kBufferConfig);
+    sr[u] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w_scales + at * a.quads * 256), 0, -1, kBufferConfig);
     #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int64_t row = mx4_row(a, min(wk.i0 + 16 * m + r, wk.i1 - 1));
-      xp[m] = a.x + row * a.x_stride + 16 * g;
-      xs[m] = a.x_scales + row * a.x_scale_stride + 4 * g;
+    for (int i = 0; i < HN; ++i) {
+      const int behind = min(i, a.tiles - 1 - tile);
+      w_tile[u * HN + i] = behind * a.steps * 1024;
+      s_tile[u * HN + i] = behind * a.quads * 256;
     }
   }
   mx4_f32x4 acc[MT][NT];
@@ -185,26 +192,38 @@ __global__ void __launch_bounds__(64 * kFewWaves) mx4_few_kernel(Mx4Args a) {
   for (int m = 0; m < MT; ++m)
     #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = mx4_f32x4{0.f, 0.f, 0.f, 0.f};
-  mx4_i32x4 wv[D][NT], xv[D][MT];
-  int ws[D][NT], xsc[D][MT];
-  auto load = [&](int slot, int step) {
+  const uint8_t* xp[MT];
+  const uint8_t* xs[MT];
+  mx4_i32x4 wv[NT], xv[MT];
+  int ws[NT], xsc[MT];
+  auto load_w = [&](int step) {
     #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      wv[slot][t] = *reinterpret_cast<const mx4_i32x4*>(wp[t] + (int64_t)step * 1024);
-      ws[slot][t] = *reinterpret_cast<const int*>(sp[t] + (step >> 2) * 256);
+      wv[t] = __builtin_amdgcn_raw_buffer_load_b128(wr[t / HN], w_lane, w_tile[t] + step * 1024, 0);
+      ws[t] = __builtin_amdgcn_raw_buffer_load_b32(sr[t / HN], s_lane, s_tile[t] + (step >> 2) * 256, 0);
     }
+  };
+  auto load_x = [&](int step) {
     if constexpr (CODES) {
       // (past k: the row's neighbours or scales, any code being finite, meet weights
       // of 0 and scales of 1)
       #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        xv[slot][m] = *reinterpret_cast<const mx4_i32x4*>(xp[m] + (int64_t)step * 64);
-        xsc[slot][m] = *reinterpret_cast<const int*>(xs[m] + (step >> 2) * 16);
+        xv[m] = *reinterpret_cast<const mx4_i32x4*>(xp[m] + (int64_t)step * 64);
+        xsc[m] = *reinterpret_cast<const int*>(xs[m] + (step >> 2) * 16);
       }
     }
   };
-  #pragma unroll
-  for (int d = 0; d < D; ++d) load(d, min(wid + d * W, a.steps - 1));
+  load_w(min(wid, a.steps - 1));
+  if constexpr (CODES) {  // (behind the weights, which need no row's number)
+    #pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int64_t row = mx4_row(a, min(wk.i0 + 16 * m + r, wk.i1 - 1));
+      xp[m] = a.x + row * a.x_stride + 16 * g;
+      xs[m] = a.x_scales + row * a.x_scale_stride + 4 * g;
+    }
+    load_x(min(wid, a.steps - 1));
+  }
   const int xc_stride = few_code_stride(a.steps), xs_stride = few_scale_stride(a.quads);
   char* const x_scales = few_smem + n_places * xc_stride;
   if constexpr (!CODES) {
@@ -231,14 +250,14 @@ __global__ void __launch_bounds__(64 * kFewWaves) mx4_few_kernel(Mx4Args a) {
   const char* const xrow = few_smem + rr * xc_stride + g * 16;
   const char* const srow = x_scales + rr * xs_stride + g * 4;
   const int shift = (wid & 3) * 8;  // every step of this wave's is the same of its quad
-  auto multiply = [&](int slot, int step) {
+  auto multiply = [&](int step) {
     #pragma unroll
     for (int m = 0; m < MT; ++m) {
       mx4_i32x4 xc;
       int s;
       if constexpr (CODES) {
-        xc = xv[slot][m];
-        s = xsc[slot][m];
+        xc = xv[m];
+        s = xsc[m];
       } else {
         xc = *reinterpret_cast<const mx4_i32x4*>(xrow + step * 64);
         s = *reinterpret_cast<const int*>(srow + (step >> 2) * 16);
@@ -246,22 +265,16 @@ __global__ void __launch_bounds__(64 * kFewWaves) mx4_few_kernel(Mx4Args a) {
       s = (int)((uint32_t)s >> shift);
       #pragma unroll
       for (int t = 0; t < NT; ++t)
-        acc[m][t] = mx4_mfma<0, 0>(wv[slot][t], xc, acc[m][t], (int)((uint32_t)ws[slot][t] >> shift), s);
+        acc[m][t] = mx4_mfma<0, 0>(wv[t], xc, acc[m][t], (int)((uint32_t)ws[t] >> shift), s);
     }
   };
-  // (no condition stands between a load and its use: the compiler would have to
-  // wait for all that may be on its way.  Past the last step a slot loads that again.)
   int s = wid;
-  for (; s + D * W < a.steps; s += D * W) {
-    #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      multiply(d, s + d * W);
-      load(d, min(s + (d + D) * W, a.steps - 1));
-    }
+  for (; s + W < a.steps; s += W) {
+    multiply(s);
+    load_w(s + W);
+    load_x(s + W);
   }
-  #pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (s + d * W < a.steps) multiply(d, s + d * W);
+  if (s < a.steps) multiply(s);
   mx4_f32x4* const part = reinterpret_cast<mx4_f32x4*>(few_smem);
   if constexpr (!CODES) moe_barrier();  // (x's place; its reads are behind their products)
   #pragma unroll
@@ -276,26 +289,22 @@ __global__ void __launch_bounds__(64 * kFewWaves) mx4_few_kernel(Mx4Args a) {
     return y;
   };
   if (a.swiglu) {
-    if constexpr (NT >= 2) {
-      for (int m = wid; m < MT; m += W) {
-        const int p = wk.i0 + 16 * m + r;
-        const bool in = p < wk.i1;
-        mx4_f32x4 y[NT / 2];
+    // 32 columns at a time, two tiles of gate and two of up: a block of codes
+    for (int i = wid; i < MT * (NT / 4); i += W) {
+      const int m = i / (NT / 4), b = i % (NT / 4), c = c0 + b * 32, p = wk.i0 + 16 * m + r;
+      mx4_f32x4 y[2];
+      #pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const mx4_f32x4 gate = total(m, 2 * b + t), up = total(m, NT / 2 + 2 * b + t);
         #pragma unroll
-        for (int t = 0; t < NT / 2; ++t) {
-          const mx4_f32x4 gate = total(m, t), up = total(m, t + NT / 2);
-          #pragma unroll
-          for (int q = 0; q < 4; ++q) y[t][q] = moe_silu_mul(gate[q], up[q]);
-        }
-        if constexpr (NT == 4) {
-          if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
-            mx4_store_codes(a, p, in, c0, g, y[0], y[1]);
-            continue;
-          }
-        }
+        for (int q = 0; q < 4; ++q) y[t][q] = moe_silu_mul(gate[q], up[q]);
+      }
+      if (c >= cols_out) continue;
+      if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
+        mx4_store_codes(a, p, p < wk.i1, c, g, y[0], y[1]);
+      } else if (p < wk.i1) {
         #pragma unroll
-        for (int t = 0; t < NT / 2; ++t)
-          if (in && c0 + t * 16 + 4 * g < cols_out) mx4_store(a, p, c0 + t * 16 + 4 * g, cols_out, y[t]);
+        for (int t = 0; t < 2; ++t) mx4_store(a, p, c + t * 16 + 4 * g, cols_out, y[t]);
       }
     }
     return;
@@ -622,14 +631,14 @@ int64_t mx4_grid(const Mx4Args& a, int bm, int bn) {
   return (nt * (((int64_t)a.cols + bn - 1) / bn) + kXcds - 1) / kXcds * kXcds;
 }
 
-template <int MT, int NT, int D, bool CODES>
+template <int MT, bool CODES>
 hipError_t launch_few(const Mx4Args& a, hipStream_t st) {
-  const int64_t grid = mx4_grid(a, 16 * MT, 16 * NT);
+  const int64_t grid = mx4_grid(a, 16 * MT, kFewCols);
   if (!moe_grid_fits(grid, 64 * kFewWaves)) return hipErrorInvalidConfiguration;
-  int bytes = MT * NT * kFewWaves * 1024;  // the waves' sums, and before them x
+  int bytes = MT * (kFewCols / 16) * kFewWaves * 1024;  // the waves' sums, and before them x
   if (!CODES)
     bytes = std::max(bytes, std::min(a.places, 16 * MT) * (few_code_stride(a.steps) + few_scale_stride(a.quads)));
-  auto* kernel = mx4_few_kernel<MT, NT, D, CODES>;
+  auto* kernel = mx4_few_kernel<MT, CODES>;
   const hipError_t e = ensure_lds((const void*)kernel, bytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * kFewWaves), (unsigned)bytes, st, a);
@@ -648,12 +657,11 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
 }
 
 hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
-  const bool longer = a.steps > 2 * kFewWaves;
-  if (!codes) return longer ? launch_few<1, 4, 4, false>(a, st) : launch_few<1, 4, 2, false>(a, st);
+  if (!codes) return launch_few<1, false>(a, st);
   const int avg = a.places / a.experts;
-  if (avg <= 16) return longer ? launch_few<1, 4, 4, true>(a, st) : launch_few<1, 4, 2, true>(a, st);
-  if (avg <= 32) return launch_few<2, 4, 2, true>(a, st);
-  if (avg <= 64) return launch_few<4, 4, 2, true>(a, st);
+  if (avg <= 16) return launch_few<1, true>(a, st);
+  if (avg <= 32) return launch_few<2, true>(a, st);
+  if (avg <= 64) return launch_few<4, true>(a, st);
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? 64 : 128;
   const int64_t small = (int64_t)((a.places + 127) / 128) * ((cols_out + per - 1) / per);
   if (small <= 512) return launch_many<128, 128>(a, st);
