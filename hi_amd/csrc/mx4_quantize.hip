@@ -32,7 +32,8 @@ __device__ __forceinline__ Mx4Unit mx4_unit(int64_t u, int64_t units, int quads,
 // Bound by the bytes: 2 or 4 read and 0.53 written a value.
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, int64_t x_stride, int64_t units, int quads, int k,
-                                                           uint8_t* codes, uint8_t* scales, int64_t scale_stride) {
+                                                           uint8_t* codes, int64_t code_stride, uint8_t* scales,
+                                                           int64_t scale_stride) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int L = F32 ? 2 : 1;
   const int lane = threadIdx.x & 63;
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, int64_t x
     if constexpr (F32) c = mx4_codes(f, s);
     else c = mx4_codes(v[i][0], s);
     if (un.in) {
-      *reinterpret_cast<uint32_t*>(codes + un.row * (k / 2) + un.at / 2) = c;
+      *reinterpret_cast<uint32_t*>(codes + un.row * code_stride + un.at / 2) = c;
     }
     // (scales behind k: the unit's row is one of x's, its values are not)
     if ((lane & 3) == 0 && (un.in || (ROWS && u0 + i < units))) {
@@ -153,16 +154,16 @@ int mx4_size(int dtype) { return dtype == HI_ROCM_DTYPE_F32 ? 4 : 2; }
 
 template <bool ROWS>
 hipError_t launch_quantize(const void* x, int dtype, int64_t rows, int k, int64_t x_stride, uint8_t* codes,
-                           uint8_t* scales, int64_t scale_stride, hipStream_t st) {
+                           int64_t code_stride, uint8_t* scales, int64_t scale_stride, hipStream_t st) {
   const int quads = (k + kMx4Quad - 1) / kMx4Quad;
   const int64_t units = rows * quads;
   const dim3 grid((unsigned)((units + 4 * kMx4Units - 1) / (4 * kMx4Units)));
   if (dtype == HI_ROCM_DTYPE_F32)
     hipLaunchKernelGGL((mx4_quantize_kernel<float, ROWS>), grid, dim3(256), 0, st, (const float*)x, x_stride, units,
-                       quads, k, codes, scales, scale_stride);
+                       quads, k, codes, code_stride, scales, scale_stride);
   else
     hipLaunchKernelGGL((mx4_quantize_kernel<__bf16, ROWS>), grid, dim3(256), 0, st, (const __bf16*)x, x_stride, units,
-                       quads, k, codes, scales, scale_stride);
+                       quads, k, codes, code_stride, scales, scale_stride);
   return hipGetLastError();
 }
 
@@ -177,7 +178,8 @@ bool mx4_rows_fit(int64_t rows, int k) {
 // Rows for the products (mx4_product.hip), arguments checked there.
 hipError_t mx4_make_rows(const void* x, int dtype, int64_t rows, int k, int64_t x_stride, void* out, hipStream_t st) {
   const Mx4Rows L = mx4_rows_layout(rows, k);
-  return launch_quantize<true>(x, dtype, rows, k, x_stride, (uint8_t*)out, (uint8_t*)out + L.scales, L.scale_stride, st);
+  return launch_quantize<true>(x, dtype, rows, k, x_stride, (uint8_t*)out, L.code_stride, (uint8_t*)out + L.scales,
+                               L.scale_stride, st);
 }
 
 }  // namespace hi_rocm
@@ -195,7 +197,8 @@ int hi_rocm_mx4_quantize(const void* x, int dtype, int64_t rows, int k, int64_t 
                     "hi_rocm_mx4_quantize: needs k a multiple of 32, rows and codes that start on 16 bytes");
   if (k > HI_ROCM_MX4_MAX_K || !mx4_rows_fit(rows, k))
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_mx4_quantize: more than 2^24 inputs, or too many rows");
-  const hipError_t e = launch_quantize<false>(x, dtype, rows, k, x_stride, codes, scales, k / kMx4Block, (hipStream_t)stream);
+  const hipError_t e = launch_quantize<false>(x, dtype, rows, k, x_stride, codes, k / 2, scales, k / kMx4Block,
+                                              (hipStream_t)stream);
   return e == hipSuccess ? HI_ROCM_OK : api_hip_fail(e, "mx4 quantize launch");
 }
 

@@ -64,8 +64,9 @@ def product(x, packed, groups, cols, k, swiglu=False, gather=True, dtype=torch.f
 def values_of(rows):
     """The values (float64) and scale bytes of Mx4Rows."""
     k, n = rows.k, rows.rows
-    codes = rows.memory[:n * (k // 2)].view(n, k // 2)
-    begin, quads = -(-n * (k // 2) // 256) * 256, -(-k // 512)
+    stride, quads = (-(-k // 256) | 1) * 128, -(-k // 512)
+    codes = rows.memory[:n * stride].view(n, stride)[:, :k // 2]
+    begin = n * stride
     s = rows.memory[begin:begin + n * quads * 16].view(n, quads, 4, 4)  # [g][j]: block 4 j + g
     s = s.transpose(2, 3).reshape(n, quads * 16)[:, :k // 32].contiguous()
     return O.values(codes.contiguous(), s), s.cpu()
