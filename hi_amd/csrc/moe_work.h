@@ -133,6 +133,16 @@ __device__ __forceinline__ void moe_wait_lds() {
   asm volatile("" ::: "memory");
 }
 
+// vmcnt <= N alone: what was read from LDS may still be on its way.
+template <int N>
+__device__ __forceinline__ void moe_wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 7 << 4 | 15 << 8);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
 // The largest grid that any split of the places over the experts needs (every
 // expert ends in at most one short tile).
 template <typename Args>

@@ -39,7 +39,7 @@ inline Mx4Rows mx4_rows_layout(int64_t rows, int k) {
   L.code_stride = (((int64_t)k / 2 + 127) / 128 | 1) * 128;
   L.scale_stride = ((int64_t)k + kMx4Quad - 1) / kMx4Quad * 16;
   L.scales = (size_t)rows * L.code_stride;
-  L.total = L.scales + (size_t)rows * L.scale_stride;
+  L.total = L.scales + (size_t)rows * L.scale_stride + kMx4Quad / 2;  // (a last quad's codes may be read whole)
   return L;
 }
 

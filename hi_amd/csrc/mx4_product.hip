@@ -321,31 +321,24 @@ __global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kerne
   }
 }
 
-// Many places (prompts, many requests): BM places times BN weight rows a
-// workgroup of eight waves, two a SIMD, a wave every WM-th 32 of the places by 64
-// of the weight rows, with MFMA 32x32x64 (lane 32 h + r: row r, block h of the
-// half step; D rows 8 i + 4 h .. + 3 of column r in registers 4 i .. + 3).
+// Many places (prompts, many requests): 32 MT places by 256 weight rows a workgroup
+// of four waves, a wave all of the places by 64 of the rows, with MFMA 32x32x64
+// (lane 32 h + r: row r, block h of a half step; D rows 8 i + 4 h .. + 3 of column r
+// in registers 4 i .. + 3).
 //
-// k goes in steps of 128 through four LDS buffers that loads fill directly, three
-// steps ahead, and the scales of four steps (16 bytes a row) through two buffers, a
-// quad ahead.  A step has two phases: read the step's operands from LDS and
-// start a later step's loads; multiply.  Waves 4 to 7 run one phase behind waves
-// 0 to 3 (a barrier more before the first step), so on every SIMD one wave reads
-// while the other multiplies.  Why no buffer is written while it is read: a
-// wave's reads are done (lgkmcnt 0) before the barrier that ends its phase, the
-// other waves read the same step at most one phase later, and the buffer of step
-// s - 1 is filled again from step s's read phase on; a quad's scales are read at
-// its first step and their buffer filled again from the next quad's first step
-// on.  Why a step is there when it is read: each wave waits for its own loads of
-// step s + 1 before the barrier that ends its reading of step s, the next quad's
-// scales, started before the loads of a quad's first step, among those of its
-// third.
+// Weights go from memory straight to registers, where no other wave needs them,
+// kMx4Ahead steps ahead.  x goes through LDS a quad of steps at a time, filled by
+// direct loads a quad ahead, with its scales; so there is a barrier a quad, and two
+// workgroups a CU work through each other's beginnings, ends and waits.  Before the
+// barrier each wave waits for its own loads of the quad that is read behind it:
+// loads return in order, and at least 4 kMx4Ahead of weights were started later.
+// Behind it the other buffer is filled, whose reads all waves have waited for.
 //
-// A row of a step is 64 bytes; its 16-byte chunk c lies at c ^ (row / 4 & 3), so
-// that the reads of a chunk of 16 rows meet all banks.  A load writes 64 lanes
-// x 16 contiguous bytes; the lanes choose their global addresses so that the
-// chunks land there.  Chunks of x past k hold what follows in memory (the next
-// row, or the scales): any code is finite, and meets weights of 0 and scales of 1.
+// A row of a quad is 256 bytes; its 16-byte chunk c lies at c ^ (row & 15), so that
+// the reads of a chunk of 16 rows meet all banks.  A load writes 64 lanes x 16
+// contiguous bytes; the lanes choose their global addresses so that the chunks land
+// there.  Chunks of x past k hold what follows in memory (the next row, or the
+// scales): any code is finite, and meets weights of 0 and scales of 1.
 typedef float mx4_f32x16 __attribute__((ext_vector_type(16)));
 
 template <int J>
@@ -356,21 +349,22 @@ __device__ __forceinline__ mx4_f32x16 mx4_mfma32(const mx4_i32x4& a, const mx4_i
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, J, sa, J, sb);
 }
 
-constexpr int kMx4Buffers = 4;
+constexpr int kMx4ManyCols = 256;
+constexpr int kMx4OutBytes = 8192;  // a wave's, for 32 places of 64 columns
 
-template <int BM, int BN>
+template <int MT>
 struct Mx4Tile {
-  static constexpr int T = 512, STEP = (BM + BN) * 64, SCALES = (BM + BN) * 16;
-  static constexpr int XL = BM * 4 / T, WL = BN * 4 / T;  // loads a thread and step
-  static constexpr int WN = BN / 64, WM = 8 / WN, MT = BM / 32 / WM;
-  static constexpr int OUT = MT == 1 ? 8192 : 16384;  // a wave's results, 32 or 64 places of 64 columns
-  static constexpr size_t BYTES = std::max<size_t>(kMx4Buffers * STEP + 2 * SCALES, 8 * OUT);
-  static_assert(XL >= 1 && WL >= 1 && MT >= 1 && BM + BN <= T, "tile split");
+  static constexpr int BM = 32 * MT;
+  static constexpr int AHEAD = MT > 2 ? 2 : 4;  // steps; more do not fit 256 registers
+  static constexpr int CODES = BM * 256, BUFFER = CODES + 8192;  // bytes of a quad's codes, with 256 rows' scales twice
+  static constexpr int L = BM / 16 + 2;                             // loads a thread and quad
+  static constexpr int BYTES = std::max(2 * BUFFER, 4 * kMx4OutBytes);
 };
 
-// A wave's results by way of its own LDS, 64 places at a time in rows of 64
-// columns, written out 16 bytes a lane, a row's bytes next to each other.
-template <int MT, int WM>
+// A wave's results by way of its own LDS, 32 places at a time, written out 16
+// bytes a lane, a row's bytes next to each other.  With swiglu half 0 of acc is the
+// gate and half 1 up.
+template <int MT>
 __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
                                              int c0, int cols_out, int lane) {
   const int r = lane & 31, h = lane >> 5;
@@ -380,7 +374,7 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
       #pragma unroll
       for (int i = 0; i < 16; ++i) acc[m][0][i] = moe_silu_mul(acc[m][0][i], acc[m][1][i]);
     if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
-      // the wave's 32 columns are a block; a place's other half is lane ^ 32's
+      // the 32 columns are a block; a place's other half is lane ^ 32's
       #pragma unroll
       for (int m = 0; m < MT; ++m) {
         uint32_t most = 0u;
@@ -397,7 +391,7 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
           mine[q] = mx4_codes(v, s);  // columns 16 q + 4 h .. + 3, then 8 on
           theirs[q] = (uint32_t)__shfl_xor((int)mine[q], 32, 64);
         }
-        const int p = p0 + m * (WM * 32) + r;
+        const int p = p0 + m * 32 + r;
         if (p < i1 && c0 < cols_out) {
           const uint32_t lo = h ? theirs[1] : mine[0], hi = h ? mine[1] : theirs[0];
           uint2 w;
@@ -411,37 +405,33 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
     }
   }
   const bool bf16 = a.out_dtype == HI_ROCM_DTYPE_BF16;
-  const int wide = a.swiglu ? 32 : 64;  // columns of a row
+  const int wide = a.swiglu ? 32 : 64;            // columns of a row
+  const int es = bf16 ? 2 : 4, n = 16 / es;       // bytes of a value, values of a chunk
+  const int lanes = wide / n, rows = 64 / lanes;  // lanes of a row, rows at a time
+  const int c = lane % lanes, col = c0 + c * n;
   typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
   #pragma unroll
-  for (int half = 0; half < (MT + 1) / 2; ++half) {
-    if (p0 + half * (WM * 64) >= i1) return;
+  for (int m = 0; m < MT; ++m) {
+    if (p0 + m * 32 >= i1) return;
     // row j of 64 values: the 16-byte chunk c at c ^ (j & 7)
     #pragma unroll
-    for (int m = half * 2; m < half * 2 + 2 && m < MT; ++m) {
-      const int j = (m - half * 2) * 32 + r;
+    for (int t = 0; t < 2; ++t) {
       #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const mx4_f32x4 y = {acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
-          if (bf16)
-            *reinterpret_cast<bf16x4*>(mem + j * 128 + ((t * 4 + i) ^ (j & 7)) * 16 + h * 8) =
-                __builtin_convertvector(y, bf16x4);
-          else
-            *reinterpret_cast<mx4_f32x4*>(mem + j * 256 + ((t * 8 + i * 2 + h) ^ (j & 7)) * 16) = y;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const mx4_f32x4 y = {acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
+        if (bf16)
+          *reinterpret_cast<bf16x4*>(mem + r * 128 + ((t * 4 + i) ^ (r & 7)) * 16 + h * 8) =
+              __builtin_convertvector(y, bf16x4);
+        else
+          *reinterpret_cast<mx4_f32x4*>(mem + r * 256 + ((t * 8 + i * 2 + h) ^ (r & 7)) * 16) = y;
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int es = bf16 ? 2 : 4, n = 16 / es;       // bytes of a value, values of a chunk
-    const int lanes = wide / n, rows = 64 / lanes;  // lanes of a row, rows at a time
-    const int c = lane % lanes, col = c0 + c * n;
     #pragma unroll 1
-    for (int j = lane / lanes; j < (MT < 2 ? 32 : 64); j += rows) {
-      const int p = p0 + half * (WM * 64) + (j >> 5) * (WM * 32) + (j & 31);
+    for (int j = lane / lanes; j < 32; j += rows) {
+      const int p = p0 + m * 32 + j;
       if (p >= i1) break;
       const uint4 v = *reinterpret_cast<const uint4*>(mem + j * (64 * es) + (c ^ (j & 7)) * 16);
       char* to = (char*)a.out + ((int64_t)p * a.out_stride + col) * es;
@@ -461,66 +451,60 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
   }
 }
 
-template <int BM, int BN, int MT>  // MT: what the tile has places for
+template <int MT>
 __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& wk, char* smem) {
-  typedef Mx4Tile<BM, BN> Tile;
-  constexpr int T = Tile::T, STEP = Tile::STEP, SCALES = Tile::SCALES, XL = Tile::XL, WL = Tile::WL;
-  constexpr int WM = Tile::WM, NB = kMx4Buffers, L = XL + WL;
+  typedef Mx4Tile<MT> Tile;
+  constexpr int BM = Tile::BM, D = Tile::AHEAD, L = Tile::L;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wid % WM, wn = wid / WM;
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols;
-  const int c0 = wk.block * (a.swiglu ? BN / 2 : BN);
-  // the weight row behind row j of the tile: with swiglu each wave's 64 are half
-  // gate, half up
-  auto column = [&](int j) {
-    if (!a.swiglu) return c0 + j;
-    const int c = c0 + j / 64 * 32 + j % 32;
-    return c < cols_out ? c + (j & 32 ? cols_out : 0) : a.cols;
-  };
-  // (rows past the weight's last tile: that tile's)
-  auto weight_row = [&](int j) { return min(column(j), a.tiles * 16 - 16 + (j & 15)); };
-  const int jr = tid / 4;                       // this thread's row in each round of loads
-  const int chunk = (tid & 3) ^ (jr >> 2 & 3);  // and the chunk that lands there
-  const uint8_t* xp[XL];
-  const uint8_t* wp[WL];
-  const int64_t base = (int64_t)wk.expert * a.tiles;
+  const int expert = __builtin_amdgcn_readfirstlane(wk.expert), block = __builtin_amdgcn_readfirstlane(wk.block);
+  // this wave's first column: with swiglu 32 of gate and the same of up
+  const int c0 = block * (a.swiglu ? kMx4ManyCols / 2 : kMx4ManyCols) + wid * (a.swiglu ? 32 : 64);
+  // Its weights: two halves of 32 rows (two tiles; past the last one, that again).
+  __amdgpu_buffer_rsrc_t wr[2];
+  int w_lane[2];
   #pragma unroll
-  for (int i = 0; i < XL; ++i)
-    xp[i] = a.x + (int64_t)mx4_row(a, min(wk.i0 + i * (T / 4) + jr, wk.i1 - 1)) * a.x_stride + 16 * chunk;
+  for (int t = 0; t < 2; ++t) {
+    const int tile = min(c0 / 16 + t * (a.swiglu ? cols_out / 16 : 2), a.tiles - 1);
+    const int64_t at = (int64_t)expert * a.tiles + tile;
+    wr[t] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + at * a.steps * 1024), 0, -1, kBufferConfig);
+    w_lane[t] = min(r >> 4, a.tiles - 1 - tile) * a.steps * 1024 + h * 256 + (r & 15) * 16;
+  }
+  // the scales of the weight row behind lane's place in the wave
+  const int half = lane >> 5, tile_s = min(c0 / 16 + half * (a.swiglu ? cols_out / 16 : 2), a.tiles - 1);
+  const uint8_t* const wsp =
+      a.w_scales +
+      ((int64_t)expert * a.tiles + min(tile_s + (lane >> 4 & 1), a.tiles - 1)) * a.quads * 256 + (lane & 15) * 16;
+  // x: a round of loads takes 16 rows, this thread's chunk of one
+  const int jr = tid / 16, chunk = (tid & 15) ^ jr;
+  const uint8_t* xp[L - 2];
   #pragma unroll
-  for (int i = 0; i < WL; ++i) {
-    const int row = weight_row(i * (T / 4) + jr);
-    wp[i] = a.w + (base + row / 16) * a.steps * 1024 + chunk * 256 + row % 16 * 16;
-  }
-  // the scales: a row a thread
-  const uint8_t* sp;
-  int sq;  // bytes from quad to quad
-  if (tid < BM) {
-    sp = a.x_scales + (int64_t)mx4_row(a, min(wk.i0 + tid, wk.i1 - 1)) * a.x_scale_stride;
-    sq = 16;
-  } else {
-    const int row = weight_row(min(tid - BM, BN - 1));
-    sp = a.w_scales + (base + row / 16) * a.quads * 256 + row % 16 * 16;
-    sq = 256;
-  }
-  char* const scales = smem + NB * STEP;
-  // (past the last step, the last one's again, for buffers that are not read)
-  auto fill = [&](int step, int buffer) {
-    char* to = smem + buffer * STEP + wid * 1024;
-    const int64_t at = min(step, a.steps - 1);
+  for (int i = 0; i < L - 2; ++i)
+    xp[i] = a.x + (int64_t)mx4_row(a, min(wk.i0 + i * 16 + jr, wk.i1 - 1)) * a.x_stride + 16 * chunk;
+  const uint8_t* const sp =
+      a.x_scales + (int64_t)mx4_row(a, min(wk.i0 + min(tid, BM - 1), wk.i1 - 1)) * a.x_scale_stride;
+  auto fill = [&](int quad) {  // (past the last quad, that again, for a buffer that is not read)
+    char* to = smem + (quad & 1) * Tile::BUFFER;
+    const int at = min(quad, a.quads - 1);
     #pragma unroll
-    for (int i = 0; i < XL; ++i)
-      __builtin_amdgcn_global_load_lds((moe_global*)(xp[i] + at * 64), (moe_lds*)(to + i * T * 16), 16, 0, 0);
-    #pragma unroll
-    for (int i = 0; i < WL; ++i)
-      __builtin_amdgcn_global_load_lds((moe_global*)(wp[i] + at * 1024), (moe_lds*)(to + BM * 64 + i * T * 16), 16, 0, 0);
+    for (int i = 0; i < L - 2; ++i)
+      __builtin_amdgcn_global_load_lds((moe_global*)(xp[i] + (int64_t)at * 256), (moe_lds*)(to + i * 4096 + wid * 1024), 16,
+                                       0, 0);
+    // (every thread one row's scales, past the tile's the last one's: no branch, behind
+    // which the compiler would not know how many loads are on their way)
+    __builtin_amdgcn_global_load_lds((moe_global*)(sp + (int64_t)at * 16), (moe_lds*)(to + Tile::CODES + wid * 1024), 16, 0,
+                                     0);
+    __builtin_amdgcn_global_load_lds((moe_global*)(wsp + (int64_t)at * 256),
+                                     (moe_lds*)(to + Tile::CODES + 4096 + wid * 1024), 16, 0, 0);
   };
-  auto fill_scales = [&](int quad) {
-    // (waves past the tile's rows have nothing to load, and one load less to wait for)
-    if (wid * 64 < BM + BN)
-      __builtin_amdgcn_global_load_lds((moe_global*)(sp + (int64_t)min(quad, a.quads - 1) * sq),
-                                       (moe_lds*)(scales + (quad & 1) * SCALES + wid * 1024), 16, 0, 0);
+  mx4_i32x4 w[D][2][2];
+  auto load_w = [&](int slot, int step) {
+    const int at = min(step, a.steps - 1) * 1024;
+    #pragma unroll
+    for (int t = 0; t < 2; ++t)
+      #pragma unroll
+      for (int u = 0; u < 2; ++u) w[slot][t][u] = __builtin_amdgcn_raw_buffer_load_b128(wr[t], w_lane[t] + u * 512, at, 0);
   };
   mx4_f32x16 acc[MT][2];
   #pragma unroll
@@ -529,65 +513,68 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
     for (int t = 0; t < 2; ++t)
       #pragma unroll
       for (int i = 0; i < 16; ++i) acc[m][t][i] = 0.f;
-  fill_scales(0);
+  fill(0);
+  __builtin_amdgcn_sched_barrier(0);
   #pragma unroll
-  for (int s = 0; s < NB - 1; ++s) fill(s, s);
-  moe_wait<L * (NB - 2)>();
-  moe_barrier();
-  if (wid >= 4) moe_barrier();
+  for (int d = 0; d < D; ++d) load_w(d, d);
+  const char* const xrow = smem + r * 256;
+  const char* const srow = smem + Tile::CODES + r * 16 + h * 4;
   int xs[MT][2], ws[2][2];
-  const char* const xrow = smem + (wm * 32 + r) * 64;
-  const char* const wrow = smem + BM * 64 + (wn * 64 + r) * 64;
   auto step = [&](auto j_, int quad) {
     constexpr int J = decltype(j_)::value;
-    mx4_i32x4 xf[MT][2], wf[2][2];
-    if (J == 0) {
-      const char* sc = scales + (quad & 1) * SCALES;
-      #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          xs[m][u] = *reinterpret_cast<const int*>(sc + (m * (WM * 32) + wm * 32 + r) * 16 + u * 8 + h * 4);
-      #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          ws[t][u] = *reinterpret_cast<const int*>(sc + (BM + wn * 64 + t * 32 + r) * 16 + u * 8 + h * 4);
-    }
+    const char* x = xrow + (quad & 1) * Tile::BUFFER;
+    // this step's weights: all but the D - 1 newer steps', and what begin() started
+    // since
+    moe_wait_loads<4 * (D - 1) + (J < D ? L : 0)>();
+    mx4_i32x4 xf[MT][2];
     #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int at = J * STEP + ((2 * u + h) ^ (r >> 2 & 3)) * 16;
+      const int at = ((4 * J + 2 * u + h) ^ (r & 15)) * 16;
       #pragma unroll
-      for (int t = 0; t < 2; ++t) wf[t][u] = *reinterpret_cast<const mx4_i32x4*>(wrow + t * 2048 + at);
-      #pragma unroll
-      for (int m = 0; m < MT; ++m) xf[m][u] = *reinterpret_cast<const mx4_i32x4*>(xrow + m * (WM * 2048) + at);
+      for (int m = 0; m < MT; ++m) xf[m][u] = *reinterpret_cast<const mx4_i32x4*>(x + m * 8192 + at);
     }
-    if (J == 0) fill_scales(quad + 1);
-    fill(quad * 4 + J + NB - 1, (J + NB - 1) % NB);
-    // all but the two newest steps', and the scales' that came between
-    if (J < 2 && wid * 64 < BM + BN) moe_wait<L * (NB - 2) + 1>();
-    else moe_wait<L * (NB - 2)>();
-    moe_barrier();
-    __builtin_amdgcn_s_setprio(1);
     #pragma unroll
     for (int u = 0; u < 2; ++u)
       #pragma unroll
       for (int m = 0; m < MT; ++m)
         #pragma unroll
-        for (int t = 0; t < 2; ++t) acc[m][t] = mx4_mfma32<J>(wf[t][u], xf[m][u], acc[m][t], ws[t][u], xs[m][u]);
-    __builtin_amdgcn_s_setprio(0);
-    moe_barrier();
+        for (int t = 0; t < 2; ++t)
+          acc[m][t] = mx4_mfma32<J>(w[J % D][t][u], xf[m][u], acc[m][t], ws[t][u], xs[m][u]);
+    load_w(J % D, quad * 4 + J + D);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  for (int quad = 0; quad < a.quads; ++quad) {
+  auto begin = [&](int quad) {
+    moe_wait<4 * D>();
+    moe_barrier();
+    fill(quad + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const char* sc = srow + (quad & 1) * Tile::BUFFER;
+    #pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      #pragma unroll
+      for (int m = 0; m < MT; ++m) xs[m][u] = *reinterpret_cast<const int*>(sc + m * 512 + u * 8);
+      #pragma unroll
+      for (int t = 0; t < 2; ++t) ws[t][u] = *reinterpret_cast<const int*>(sc + 4096 + wid * 1024 + t * 512 + u * 8);
+    }
+  };
+  // Whole quads, without a condition that loads could be moved behind; the rest.
+  // (begin() counts on the loads that a whole quad's steps started.  Those above may
+  // be fewer: the compiler leaves out what a short k does not use.)
+  moe_wait<0>();
+  int quad = 0;
+  for (; quad < a.steps / 4; ++quad) {
+    begin(quad);
     step(std::integral_constant<int, 0>(), quad);
-    if (quad * 4 + 1 >= a.steps) break;
     step(std::integral_constant<int, 1>(), quad);
-    if (quad * 4 + 2 >= a.steps) break;
     step(std::integral_constant<int, 2>(), quad);
-    if (quad * 4 + 3 >= a.steps) break;
     step(std::integral_constant<int, 3>(), quad);
   }
-  if (wid < 4) moe_barrier();
+  if (quad < a.quads) {
+    begin(quad);
+    step(std::integral_constant<int, 0>(), quad);
+    if (quad * 4 + 1 < a.steps) step(std::integral_constant<int, 1>(), quad);
+    if (quad * 4 + 2 < a.steps) step(std::integral_constant<int, 2>(), quad);
+  }
   moe_wait<0>();  // no load may still write LDS when it is used again, or the workgroup ends
   moe_barrier();
   if (a.bias != nullptr) {
@@ -595,34 +582,30 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
     for (int t = 0; t < 2; ++t)
       #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int c = c0 + wn * 64 + t * 32 + i / 4 * 8 + h * 4 + i % 4;
+        const int c = c0 + t * 32 + i / 4 * 8 + h * 4 + i % 4;
         const float b = c < cols_out ? a.bias[c] : 0.f;
         #pragma unroll
         for (int m = 0; m < MT; ++m) acc[m][t][i] += b;
       }
   }
-  mx4_tile_out<MT, WM>(a, acc, smem + wid * Tile::OUT, wk.i0 + wm * 32, wk.i1, c0 + wn * (a.swiglu ? 32 : 64), cols_out,
-                       lane);
+  mx4_tile_out<MT>(a, acc, smem + wid * kMx4OutBytes, wk.i0, wk.i1, c0, cols_out, lane);
 }
 
-// WM waves share the places, every WM-th 32 of them, so a tile of fewer places
-// than BM is multiplied as one of a quarter, a half or three quarters.
-template <int BM, int BN>
-__global__ void __launch_bounds__(512) mx4_many_kernel(Mx4Args a) {
+// A tile of fewer places than its 32 MT is multiplied as one of fewer 32s.
+template <int MT>
+__global__ void __launch_bounds__(256, 2) mx4_many_kernel(Mx4Args a) {
   extern __shared__ __align__(16) char mx4_smem[];
-  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? BN / 2 : BN;
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? kMx4ManyCols / 2 : kMx4ManyCols;
   MoeWork wk;
-  if (!mx4_work<BM>(a, (cols_out + per - 1) / per, wk)) return;
-  constexpr int MT = Mx4Tile<BM, BN>::MT, WM = Mx4Tile<BM, BN>::WM;
-  const int need = (wk.i1 - wk.i0 + WM * 32 - 1) / (WM * 32);
-  if constexpr (MT == 4) {
-    if (need == 1) return mx4_many_tile<BM, BN, 1>(a, wk, mx4_smem);
-    if (need == 2) return mx4_many_tile<BM, BN, 2>(a, wk, mx4_smem);
-    if (need == 3) return mx4_many_tile<BM, BN, 3>(a, wk, mx4_smem);
-  } else if constexpr (MT == 2) {
-    if (need == 1) return mx4_many_tile<BM, BN, 1>(a, wk, mx4_smem);
-  }
-  mx4_many_tile<BM, BN, MT>(a, wk, mx4_smem);
+  if (!mx4_work<32 * MT>(a, (cols_out + per - 1) / per, wk)) return;
+  const int need = (wk.i1 - wk.i0 + 31) / 32;
+  if constexpr (MT > 1)
+    if (need == 1) return mx4_many_tile<1>(a, wk, mx4_smem);
+  if constexpr (MT > 2)
+    if (need == 2) return mx4_many_tile<2>(a, wk, mx4_smem);
+  if constexpr (MT > 3)
+    if (need == 3) return mx4_many_tile<3>(a, wk, mx4_smem);
+  mx4_many_tile<MT>(a, wk, mx4_smem);
 }
 
 int64_t mx4_grid(const Mx4Args& a, int bm, int bn) {
@@ -645,14 +628,15 @@ hipError_t launch_few(const Mx4Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int BM, int BN>
+template <int MT>
 hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
-  auto* kernel = mx4_many_kernel<BM, BN>;
-  const int64_t grid = mx4_grid(a, BM, BN);
-  if (!moe_grid_fits(grid, 512)) return hipErrorInvalidConfiguration;
-  const hipError_t e = ensure_lds((const void*)kernel, Mx4Tile<BM, BN>::BYTES);
+  auto* kernel = mx4_many_kernel<MT>;
+  constexpr int bytes = Mx4Tile<MT>::BYTES;
+  const int64_t grid = mx4_grid(a, 32 * MT, kMx4ManyCols);
+  if (!moe_grid_fits(grid, 256)) return hipErrorInvalidConfiguration;
+  const hipError_t e = ensure_lds((const void*)kernel, bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(512), (unsigned)(Mx4Tile<BM, BN>::BYTES), st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), (unsigned)bytes, st, a);
   return hipGetLastError();
 }
 
@@ -660,13 +644,9 @@ hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
   if (!codes) return launch_few<1, false>(a, st);
   const int avg = a.places / a.experts;
   if (avg <= 16) return launch_few<1, true>(a, st);
-  if (avg <= 32) return launch_few<2, true>(a, st);
-  if (avg <= 64) return launch_few<4, true>(a, st);
-  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? 64 : 128;
-  const int64_t small = (int64_t)((a.places + 127) / 128) * ((cols_out + per - 1) / per);
-  if (small <= 512) return launch_many<128, 128>(a, st);
-  if (avg <= 256) return launch_many<128, 256>(a, st);
-  return launch_many<256, 256>(a, st);
+  if (avg <= 32) return launch_many<1>(a, st);
+  if (avg <= 512) return launch_many<2>(a, st);
+  return launch_many<4>(a, st);
 }
 
 bool mx4_float(int d) { return d == HI_ROCM_DTYPE_F32 || d == HI_ROCM_DTYPE_BF16; }
