@@ -112,14 +112,12 @@ __device__ __forceinline__ uint32_t mx4_field(uint32_t pair) { return max(pair >
 // Where block b's scale lies in a row of "rows".
 __host__ __device__ __forceinline__ int mx4_scale_at(int b) { return (b >> 4) * 16 + (b & 3) * 4 + (b >> 2 & 3); }
 
-// D = A B + C over 128 values of k, both operands 4-bit; byte JA (JB) of sa (sb)
-// is the scale.
-template <int JA, int JB>
-__device__ __forceinline__ mx4_f32x4 mx4_mfma(const mx4_i32x4& a, const mx4_i32x4& b, const mx4_f32x4& c, int sa,
-                                              int sb) {
+// D = A B + C over 128 values of k, both operands 4-bit, the scales in the low bytes
+// of sa and sb.
+__device__ __forceinline__ mx4_f32x4 mx4_mfma(const mx4_i32x4& a, const mx4_i32x4& b, const mx4_f32x4& c, int sa, int sb) {
   const mx4_i32x8 wa = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
   const mx4_i32x8 wb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, c, 4, 4, JA, sa, JB, sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, c, 4, 4, 0, sa, 0, sb);
 }
 
 }  // namespace hi_rocm

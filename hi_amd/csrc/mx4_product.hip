@@ -128,7 +128,7 @@ __device__ __forceinline__ void mx4_store_codes(const Mx4Args& a, int p, bool in
 
 // Few places (decode): the weights are what is read.  The workgroup's waves take
 // the steps of k in turn; each streams 64 columns' blocks straight into registers,
-// a step ahead, and multiplies them with up to 16 MT places.  Rounded rows of x come
+// a step ahead, and multiplies them with up to 16 places.  Rounded rows of x come
 // the same way; bf16 ones are rounded into LDS first, while the first weights are on
 // their way (loads return in order: asked for in the loop, x would hold up every
 // weight asked for before it).  The waves' sums are added in wave order.
@@ -143,8 +143,8 @@ constexpr int kFewCols = 64;
 __host__ __device__ __forceinline__ int few_code_stride(int steps) { return steps * 64 + 16; }
 __host__ __device__ __forceinline__ int few_scale_stride(int quads) { return quads * 16 + 4; }
 
-template <int MT, bool CODES>
-__global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kernel(Mx4Args a) {
+template <bool CODES>
+__global__ void __launch_bounds__(64 * kFewWaves, 6) mx4_few_kernel(Mx4Args a) {
   extern __shared__ __align__(16) char few_smem[];
   constexpr int W = kFewWaves, COLS = kFewCols, NT = COLS / 16;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kerne
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols;
   const int per = a.swiglu ? COLS / 2 : COLS;
   MoeWork wk;
-  if (!mx4_work<16 * MT>(a, (cols_out + per - 1) / per, wk)) return;
+  if (!mx4_work<16>(a, (cols_out + per - 1) / per, wk)) return;
   // (all lanes' alike, which divisions in vector registers hide from the compiler)
   wk.expert = __builtin_amdgcn_readfirstlane(wk.expert);
   wk.block = __builtin_amdgcn_readfirstlane(wk.block);
@@ -187,15 +187,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kerne
       s_tile[u * HN + i] = behind * a.quads * 256;
     }
   }
-  mx4_f32x4 acc[MT][NT];
+  mx4_f32x4 acc[NT];
   #pragma unroll
-  for (int m = 0; m < MT; ++m)
-    #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[m][t] = mx4_f32x4{0.f, 0.f, 0.f, 0.f};
-  const uint8_t* xp[MT];
-  const uint8_t* xs[MT];
-  mx4_i32x4 wv[NT], xv[MT];
-  int ws[NT], xsc[MT];
+  for (int t = 0; t < NT; ++t) acc[t] = mx4_f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint8_t *xp = nullptr, *xs = nullptr;
+  mx4_i32x4 wv[NT], xv;
+  int ws[NT], xsc;
   auto load_w = [&](int step) {
     #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -207,21 +204,15 @@ __global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kerne
     if constexpr (CODES) {
       // (past k: the row's neighbours or scales, any code being finite, meet weights
       // of 0 and scales of 1)
-      #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        xv[m] = *reinterpret_cast<const mx4_i32x4*>(xp[m] + (int64_t)step * 64);
-        xsc[m] = *reinterpret_cast<const int*>(xs[m] + (step >> 2) * 16);
-      }
+      xv = *reinterpret_cast<const mx4_i32x4*>(xp + (int64_t)step * 64);
+      xsc = *reinterpret_cast<const int*>(xs + (step >> 2) * 16);
     }
   };
   load_w(min(wid, a.steps - 1));
   if constexpr (CODES) {  // (behind the weights, which need no row's number)
-    #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int64_t row = mx4_row(a, min(wk.i0 + 16 * m + r, wk.i1 - 1));
-      xp[m] = a.x + row * a.x_stride + 16 * g;
-      xs[m] = a.x_scales + row * a.x_scale_stride + 4 * g;
-    }
+    const int64_t row = mx4_row(a, min(wk.i0 + r, wk.i1 - 1));
+    xp = a.x + row * a.x_stride + 16 * g;
+    xs = a.x_scales + row * a.x_scale_stride + 4 * g;
     load_x(min(wid, a.steps - 1));
   }
   const int xc_stride = few_code_stride(a.steps), xs_stride = few_scale_stride(a.quads);
@@ -246,27 +237,23 @@ __global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kerne
     moe_wait_lds();  // (the weights stay on their way)
     moe_barrier();
   }
-  const int rr = min(r, n_places - 1);  // (MT = 1 here)
+  const int rr = min(r, n_places - 1);
   const char* const xrow = few_smem + rr * xc_stride + g * 16;
   const char* const srow = x_scales + rr * xs_stride + g * 4;
   const int shift = (wid & 3) * 8;  // every step of this wave's is the same of its quad
   auto multiply = [&](int step) {
-    #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      mx4_i32x4 xc;
-      int s;
-      if constexpr (CODES) {
-        xc = xv[m];
-        s = xsc[m];
-      } else {
-        xc = *reinterpret_cast<const mx4_i32x4*>(xrow + step * 64);
-        s = *reinterpret_cast<const int*>(srow + (step >> 2) * 16);
-      }
-      s = (int)((uint32_t)s >> shift);
-      #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        acc[m][t] = mx4_mfma<0, 0>(wv[t], xc, acc[m][t], (int)((uint32_t)ws[t] >> shift), s);
+    mx4_i32x4 xc;
+    int s;
+    if constexpr (CODES) {
+      xc = xv;
+      s = xsc;
+    } else {
+      xc = *reinterpret_cast<const mx4_i32x4*>(xrow + step * 64);
+      s = *reinterpret_cast<const int*>(srow + (step >> 2) * 16);
     }
+    s = (int)((uint32_t)s >> shift);
+    #pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = mx4_mfma(wv[t], xc, acc[t], (int)((uint32_t)ws[t] >> shift), s);
   };
   int s = wid;
   for (; s + W < a.steps; s += W) {
@@ -278,47 +265,41 @@ __global__ void __launch_bounds__(64 * kFewWaves, MT == 1 ? 6 : 2) mx4_few_kerne
   mx4_f32x4* const part = reinterpret_cast<mx4_f32x4*>(few_smem);
   if constexpr (!CODES) moe_barrier();  // (x's place; its reads are behind their products)
   #pragma unroll
-  for (int m = 0; m < MT; ++m)
-    #pragma unroll
-    for (int t = 0; t < NT; ++t) part[((m * NT + t) * W + wid) * 64 + lane] = acc[m][t];
+  for (int t = 0; t < NT; ++t) part[(t * W + wid) * 64 + lane] = acc[t];
   __syncthreads();
-  auto total = [&](int m, int t) {
-    mx4_f32x4 y = part[((m * NT + t) * W) * 64 + lane];
+  auto total = [&](int t) {
+    mx4_f32x4 y = part[t * W * 64 + lane];
     #pragma unroll
-    for (int w = 1; w < W; ++w) y += part[((m * NT + t) * W + w) * 64 + lane];
+    for (int w = 1; w < W; ++w) y += part[(t * W + w) * 64 + lane];
     return y;
   };
-  if (a.swiglu) {
-    // 32 columns at a time, two tiles of gate and two of up: a block of codes
-    for (int i = wid; i < MT * (NT / 4); i += W) {
-      const int m = i / (NT / 4), b = i % (NT / 4), c = c0 + b * 32, p = wk.i0 + 16 * m + r;
-      mx4_f32x4 y[2];
+  const int p = wk.i0 + r;
+  if (a.swiglu) {  // two tiles of gate and two of up: a block of codes
+    if (wid > 0 || c0 >= cols_out) return;
+    mx4_f32x4 y[2];
+    #pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const mx4_f32x4 gate = total(t), up = total(NT / 2 + t);
       #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const mx4_f32x4 gate = total(m, 2 * b + t), up = total(m, NT / 2 + 2 * b + t);
-        #pragma unroll
-        for (int q = 0; q < 4; ++q) y[t][q] = moe_silu_mul(gate[q], up[q]);
-      }
-      if (c >= cols_out) continue;
-      if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
-        mx4_store_codes(a, p, p < wk.i1, c, g, y[0], y[1]);
-      } else if (p < wk.i1) {
-        #pragma unroll
-        for (int t = 0; t < 2; ++t) mx4_store(a, p, c + t * 16 + 4 * g, cols_out, y[t]);
-      }
+      for (int q = 0; q < 4; ++q) y[t][q] = moe_silu_mul(gate[q], up[q]);
+    }
+    if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
+      mx4_store_codes(a, p, p < wk.i1, c0, g, y[0], y[1]);
+    } else if (p < wk.i1) {
+      #pragma unroll
+      for (int t = 0; t < 2; ++t) mx4_store(a, p, c0 + t * 16 + 4 * g, cols_out, y[t]);
     }
     return;
   }
-  for (int i = wid; i < MT * NT; i += W) {
-    const int m = i / NT, t = i % NT, p = wk.i0 + 16 * m + r, c = c0 + t * 16 + 4 * g;
-    if (p >= wk.i1 || c >= cols_out) continue;
-    mx4_f32x4 y = total(m, t);
-    if (a.bias != nullptr) {
-      #pragma unroll
-      for (int q = 0; q < 4; ++q) y[q] += c + q < cols_out ? a.bias[c + q] : 0.f;
-    }
-    mx4_store(a, p, c, cols_out, y);
+  static_assert(NT == W, "a tile a wave");
+  const int c = c0 + wid * 16 + 4 * g;
+  if (p >= wk.i1 || c >= cols_out) return;
+  mx4_f32x4 y = total(wid);
+  if (a.bias != nullptr) {
+    #pragma unroll
+    for (int q = 0; q < 4; ++q) y[q] += c + q < cols_out ? a.bias[c + q] : 0.f;
   }
+  mx4_store(a, p, c, cols_out, y);
 }
 
 // Many places (prompts, many requests): 32 MT places by 256 weight rows a workgroup
@@ -520,26 +501,35 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
   const char* const xrow = smem + r * 256;
   const char* const srow = smem + Tile::CODES + r * 16 + h * 4;
   int xs[MT][2], ws[2][2];
+  mx4_i32x4 xf[2][MT];
+  auto read_x = [&](const char* x, int half) {
+    #pragma unroll
+    for (int m = 0; m < MT; ++m)
+      xf[half & 1][m] = *reinterpret_cast<const mx4_i32x4*>(x + m * 8192 + ((2 * half + h) ^ (r & 15)) * 16);
+  };
+  auto multiply = [&](auto j_, int u) {
+    constexpr int J = decltype(j_)::value;
+    #pragma unroll
+    for (int m = 0; m < MT; ++m)
+      #pragma unroll
+      for (int t = 0; t < 2; ++t)
+        acc[m][t] = mx4_mfma32<J>(w[J % D][t][u], xf[u][m], acc[m][t], ws[t][u], xs[m][u]);
+  };
   auto step = [&](auto j_, int quad) {
     constexpr int J = decltype(j_)::value;
     const char* x = xrow + (quad & 1) * Tile::BUFFER;
     // this step's weights: all but the D - 1 newer steps', and what begin() started
     // since
     moe_wait_loads<4 * (D - 1) + (J < D ? L : 0)>();
-    mx4_i32x4 xf[MT][2];
-    #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int at = ((4 * J + 2 * u + h) ^ (r & 15)) * 16;
-      #pragma unroll
-      for (int m = 0; m < MT; ++m) xf[m][u] = *reinterpret_cast<const mx4_i32x4*>(x + m * 8192 + at);
-    }
-    #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          acc[m][t] = mx4_mfma32<J>(w[J % D][t][u], xf[m][u], acc[m][t], ws[t][u], xs[m][u]);
+    // a half's x is read while the half before it is multiplied (the first of a quad
+    // by begin)
+    read_x(x, 2 * J + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(j_, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (J < 3) read_x(x, 2 * J + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(j_, 1);
     load_w(J % D, quad * 4 + J + D);
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -556,6 +546,7 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
       #pragma unroll
       for (int t = 0; t < 2; ++t) ws[t][u] = *reinterpret_cast<const int*>(sc + 4096 + wid * 1024 + t * 512 + u * 8);
     }
+    read_x(xrow + (quad & 1) * Tile::BUFFER, 0);
   };
   // Whole quads, without a condition that loads could be moved behind; the rest.
   // (begin() counts on the loads that a whole quad's steps started.  Those above may
@@ -614,14 +605,13 @@ int64_t mx4_grid(const Mx4Args& a, int bm, int bn) {
   return (nt * (((int64_t)a.cols + bn - 1) / bn) + kXcds - 1) / kXcds * kXcds;
 }
 
-template <int MT, bool CODES>
+template <bool CODES>
 hipError_t launch_few(const Mx4Args& a, hipStream_t st) {
-  const int64_t grid = mx4_grid(a, 16 * MT, kFewCols);
+  const int64_t grid = mx4_grid(a, 16, kFewCols);
   if (!moe_grid_fits(grid, 64 * kFewWaves)) return hipErrorInvalidConfiguration;
-  int bytes = MT * (kFewCols / 16) * kFewWaves * 1024;  // the waves' sums, and before them x
-  if (!CODES)
-    bytes = std::max(bytes, std::min(a.places, 16 * MT) * (few_code_stride(a.steps) + few_scale_stride(a.quads)));
-  auto* kernel = mx4_few_kernel<MT, CODES>;
+  int bytes = kFewCols / 16 * kFewWaves * 1024;  // the waves' sums, and before them x
+  if (!CODES) bytes = std::max(bytes, std::min(a.places, 16) * (few_code_stride(a.steps) + few_scale_stride(a.quads)));
+  auto* kernel = mx4_few_kernel<CODES>;
   const hipError_t e = ensure_lds((const void*)kernel, bytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * kFewWaves), (unsigned)bytes, st, a);
@@ -640,13 +630,42 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Which kernel, and how many places a tile.  us of a product alone, 4096 inputs:
+//   16,384 outputs, rows 8, 16, 32, 64: few 8.6, 8.9, 12.4, 21.3; 32 places 10.7, 10.9, 11.1, 11.3
+//   4,096 outputs,  rows 8, 32, 64, 96: few 6.4, 7.2, 7.6, 12.1; 32 places 8.4, 9.1, 9.6, 9.7
+//   128 experts, 1536 x 2048, 4, 8, 16 places each: few 31, 40, 52; 32 places 34, 37, 42
+// so rows of a linear layer go to the first while they make no more than a
+// workgroup a CU, or are one tile of its 16; experts' places up to seven each.
+// Tiles of 32 MT places: a workgroup takes 3 MT + 4 parts of time (its weights, and
+// its places), two of them on a CU twice as long, so what counts is the workgroups
+// of the busiest CU; where there are many, their average.  16,384 outputs, tiles of
+// 32, 64, 96, 128:
+//   rows 128: 12.3, 14.0, 16.0, 19.6;  256: 19.2, 16.1, 17.5, 20.6;  320: 27, 27, 18.3, 20.8
+//   rows 512: 33, 24.8, 27.8, 23.7;   1,024: 67, 45, 43, 39;        2,048: 134, 87, 82, 72
+//   128 experts, 1536 x 2048, 48 places each: 50, 45, 47, 49; 128: 85, 69, 61, 59; 512: 242, 178, 160, 151
+// Experts fill three quarters of a tile more than their places, about.
 hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
-  if (!codes) return launch_few<1, false>(a, st);
-  const int avg = a.places / a.experts;
-  if (avg <= 16) return launch_few<1, true>(a, st);
-  if (avg <= 32) return launch_many<1>(a, st);
-  if (avg <= 512) return launch_many<2>(a, st);
-  return launch_many<4>(a, st);
+  if (!codes) return launch_few<false>(a, st);
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? kMx4ManyCols / 2 : kMx4ManyCols;
+  const int64_t blocks = (cols_out + per - 1) / per, met = std::min(a.experts, a.places);
+  if (a.offsets != nullptr ? a.places / a.experts < 8
+                           : a.places <= 16 || ((int64_t)a.places + 15) / 16 * ((a.cols + 63) / 64) <= 256)
+    return launch_few<true>(a, st);
+  auto time = [&](int mt) {
+    const int bm = 32 * mt;
+    const int64_t tiles = a.offsets != nullptr ? std::max(met, a.places / bm + met * 3 / 4) : (a.places + bm - 1) / bm;
+    const int64_t wgs = tiles * blocks;
+    return (wgs <= 1024 ? (wgs + 255) / 256 * 256 : wgs) * (3 * mt + 4);
+  };
+  int best = 4;
+  for (int mt = 3; mt >= 1; --mt)
+    if (time(mt) < time(best)) best = mt;
+  switch (best) {
+    case 1: return launch_many<1>(a, st);
+    case 2: return launch_many<2>(a, st);
+    case 3: return launch_many<3>(a, st);
+    default: return launch_many<4>(a, st);
+  }
 }
 
 bool mx4_float(int d) { return d == HI_ROCM_DTYPE_F32 || d == HI_ROCM_DTYPE_BF16; }
