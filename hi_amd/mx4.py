@@ -14,6 +14,7 @@ from .beam import _CODES, _empty, _on, _ptr, _stream
 from .moe import RowGroups
 
 BLOCK = 32
+_BYTE = torch.uint8
 
 
 def _rows_of(what: str, name: str, x: torch.Tensor, k: Optional[int] = None) -> None:
@@ -45,20 +46,26 @@ def quantize_mx4(x: torch.Tensor, out: Optional[Tuple[torch.Tensor, torch.Tensor
     """Rounds x (float32 or bfloat16 [rows][k], rows on 16 bytes): codes uint8
     [rows][k / 2] (value 2 j in byte j's low nibble) and scales uint8 [rows]
     [k / 32], as ``Mx4Linear`` takes them."""
+    # (checks written out where a call's host side takes longer than its kernel)
     what = "quantize mx4"
-    _rows_of(what, "x", x)
-    rows, k = x.shape
+    code = _CODES.get(x.dtype)
+    if code is None or x.dim() != 2 or x.numel() == 0 or x.stride(1) != 1 or x.size(1) % BLOCK != 0:
+        _rows_of(what, "x", x)
+    rows, k = x.size(0), x.size(1)
     if out is None:
-        out = (_empty((rows, k // 2), torch.uint8, x.device, stream),
-               _empty((rows, k // BLOCK), torch.uint8, x.device, stream))
+        out = (_empty((rows, k // 2), _BYTE, x.device, stream), _empty((rows, k // BLOCK), _BYTE, x.device, stream))
     codes, scales = out
-    _codes_of(what, codes, scales, 2)
-    if codes.shape != (rows, k // 2):
-        raise ValueError(f"{what}: out is for {codes.size(0)} rows of {codes.size(1) * 2}")
+    if not (codes.dtype is _BYTE and scales.dtype is _BYTE and codes.dim() == 2 and scales.dim() == 2 and
+            codes.size(0) == rows and codes.size(1) == k // 2 and scales.size(0) == rows and
+            scales.size(1) == k // BLOCK and codes.is_contiguous() and scales.is_contiguous()):
+        raise ValueError(f"{what}: out must be contiguous uint8 codes [{rows}][{k // 2}] and scales [{rows}][{k // BLOCK}]")
     dev = x.get_device()
-    _on(what, dev, codes, scales)
-    check(load().hi_rocm_mx4_quantize(x.data_ptr(), _CODES[x.dtype], rows, k, x.stride(0) if rows > 1 else k,
-                                      codes.data_ptr(), scales.data_ptr(), _stream(what, dev, stream)))
+    if dev < 0 or codes.get_device() != dev or scales.get_device() != dev:
+        _on(what, dev, codes, scales)
+    status = load().hi_rocm_mx4_quantize(x.data_ptr(), code, rows, k, x.stride(0) if rows > 1 else k, codes.data_ptr(),
+                                         scales.data_ptr(), _stream(what, dev, stream))
+    if status:
+        check(status)
     return out
 
 
@@ -67,17 +74,23 @@ def dequantize_mx4(codes: torch.Tensor, scales: torch.Tensor, out: Optional[torc
     """The values [rows][k] of codes and scales, float32 or bfloat16 (``out``'s
     type)."""
     what = "dequantize mx4"
-    _codes_of(what, codes, scales, 2)
+    if not (codes.dtype is _BYTE and scales.dtype is _BYTE and codes.dim() == 2 and scales.dim() == 2 and
+            codes.numel() > 0 and codes.size(1) == scales.size(1) * (BLOCK // 2) and scales.size(0) == codes.size(0) and
+            codes.is_contiguous() and scales.is_contiguous()):
+        _codes_of(what, codes, scales, 2)
     rows, k = codes.size(0), codes.size(1) * 2
     if out is None:
         out = _empty((rows, k), dtype, codes.device, stream)
-    _rows_of(what, "out", out, k)
-    if out.size(0) != rows:
-        raise ValueError(f"{what}: out has {out.size(0)} rows, the codes {rows}")
+    code = _CODES.get(out.dtype)
+    if code is None or out.dim() != 2 or out.size(0) != rows or out.size(1) != k or out.stride(1) != 1:
+        raise ValueError(f"{what}: out must be a float32 or bfloat16 [{rows}][{k}] tensor, values contiguous")
     dev = codes.get_device()
-    _on(what, dev, scales, out)
-    check(load().hi_rocm_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(), _CODES[out.dtype],
-                                        out.stride(0) if rows > 1 else k, _stream(what, dev, stream)))
+    if dev < 0 or scales.get_device() != dev or out.get_device() != dev:
+        _on(what, dev, scales, out)
+    status = load().hi_rocm_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), rows, k, out.data_ptr(), code,
+                                           out.stride(0) if rows > 1 else k, _stream(what, dev, stream))
+    if status:
+        check(status)
     return out
 
 
@@ -140,6 +153,7 @@ class Mx4Linear:
         self.bias = bias
         self.packed = _pack(what, codes, scales, 1, stream)
         self._bytes = self.packed.numel()
+        self._device, self._linear = self.packed.get_device(), load().hi_rocm_mx4_linear
         self._work = {}  # rows: bytes of their workspace
 
     def __call__(self, x: Union[torch.Tensor, Mx4Rows], out: Optional[torch.Tensor] = None, dtype=torch.float32,
@@ -147,9 +161,7 @@ class Mx4Linear:
         """x bfloat16 [rows][k], rows starting on 16 bytes, or ``mx4_rows`` of
         it; returns out [rows][n] (a new tensor of ``dtype`` when not given)."""
         what = "mx4 linear"
-        n, k, packed = self.n, self.k, self.packed
-        dev = packed.get_device()
-        memory, work, work_bytes = None, None, 0
+        n, k, dev, work, work_bytes = self.n, self.k, self._device, None, 0
         if isinstance(x, Mx4Rows):
             if x.k != k:
                 raise ValueError(f"{what}: rows of {x.k}, the weight's are {k}")
@@ -160,22 +172,24 @@ class Mx4Linear:
             rows, at, code_x, memory = x.size(0), x.data_ptr(), DTYPE_BF16, x
             stride = x.stride(0) if rows > 1 else k
         if out is None:
-            out = _empty((rows, n), dtype, packed.device, stream)
+            out = _empty((rows, n), dtype, self.packed.device, stream)
         code = _CODES.get(out.dtype)
         if code is None or out.dim() != 2 or out.size(0) != rows or out.size(1) != n or (n > 1 and out.stride(1) != 1):
             raise ValueError(f"{what}: out must be a float32 or bfloat16 [{rows}][{n}] tensor, outputs contiguous")
-        _on(what, dev, memory, out)
-        lib, st = load(), _stream(what, dev, stream)
+        if memory.get_device() != dev or out.get_device() != dev:
+            _on(what, dev, memory, out)
         if code_x == DTYPE_BF16:
             work_bytes = self._work.get(rows)
             if work_bytes is None:
-                work_bytes = self._work[rows] = _size(lib.hi_rocm_mx4_workspace_bytes, rows, rows, k)
+                work_bytes = self._work[rows] = _size(load().hi_rocm_mx4_workspace_bytes, rows, rows, k)
             if work_bytes:  # a call's own: calls on several streams, or captured ones, share nothing
-                work = _empty((work_bytes,), torch.uint8, packed.device, stream)
+                work = _empty((work_bytes,), _BYTE, self.packed.device, stream)
         # (a single row's stride says nothing)
-        check(lib.hi_rocm_mx4_linear(
-            at, code_x, rows, stride, packed.data_ptr(), self._bytes, n, k, _ptr(self.bias), out.data_ptr(), code,
-            out.stride(0) if rows > 1 else n, _ptr(work), work_bytes, st))
+        status = self._linear(
+            at, code_x, rows, stride, self.packed.data_ptr(), self._bytes, n, k, _ptr(self.bias), out.data_ptr(), code,
+            out.stride(0) if rows > 1 else n, _ptr(work), work_bytes, _stream(what, dev, stream))
+        if status:
+            check(status)
         return out
 
 

@@ -10,6 +10,8 @@ import torch
 from ._lib import check, load
 from .beam import _CODES, _F32, _I32, _on, _ptr, _stream, _vector
 
+_INT, _FLOAT = torch.int32, torch.float32
+
 
 class SpecVerifier:
     """The rejection rule for up to ``max_batch`` requests of ``max_draft``
@@ -24,6 +26,7 @@ class SpecVerifier:
         check(load().hi_rocm_spec_sampled_workspace_bytes(max_batch, vocab, ctypes.byref(nbytes)))
         self._bytes = nbytes.value
         self.workspace = torch.zeros(nbytes.value, dtype=torch.uint8, device=device)
+        self._device, self._verify = self.workspace.get_device(), load().hi_rocm_spec_verify_sampled
 
     def outputs(self, batch: int, stream: Optional[torch.cuda.Stream] = None) -> dict:
         """Output tensors of a call for ``batch`` requests."""
@@ -48,39 +51,44 @@ class SpecVerifier:
         [vocab], or None for drafts that were not sampled; ``draft_len`` int32
         [batch].  Returns ``tokens`` int32 [batch][max_draft + 1] (accepted
         drafts, drawn token, then -1) and ``counts`` int32 [batch]."""
+        # (each check is written out: a call takes longer on the host than its kernel)
         what = "spec verifier"
-        K, V = self.max_draft, self.vocab
-        code = _CODES.get(target_probs.dtype)
-        if code is None or target_probs.dim() != 3 or target_probs.shape[1:] != (K + 1, V) or (
-                V > 1 and target_probs.stride(2) != 1):
+        K, V, p, q, dev = self.max_draft, self.vocab, target_probs, draft_probs, self._device
+        code = _CODES.get(p.dtype)
+        if code is None or p.dim() != 3 or p.size(1) != K + 1 or p.size(2) != V or (V > 1 and p.stride(2) != 1):
             raise ValueError(f"{what}: target_probs must be a float32 or bfloat16 [batch][{K + 1}][{V}] tensor, values "
                              "contiguous")
-        batch = target_probs.size(0)
+        batch = p.size(0)
         if not 0 < batch <= self.max_batch:
             raise ValueError(f"{what}: {batch} requests, at most {self.max_batch}")
-        strides = (0, 0)
-        if draft_probs is not None:
-            if draft_probs.dtype != target_probs.dtype or draft_probs.shape != (batch, K, V) or (
-                    V > 1 and K > 0 and draft_probs.stride(2) != 1):
-                raise ValueError(f"{what}: draft_probs must be a {target_probs.dtype} [{batch}][{K}][{V}] tensor, values "
-                                 "contiguous")
-            strides = draft_probs.stride(0), draft_probs.stride(1)
-        _vector(what, "draft_tokens", draft_tokens, _I32, batch * K)
-        _vector(what, "uniforms", uniforms, _F32, batch * (K + 1))
-        if draft_len is not None:
-            _vector(what, "draft_len", draft_len, _I32, batch)
+        q_at = q_batch = q_row = 0
+        if q is not None:
+            if q.dtype is not p.dtype or q.dim() != 3 or q.size(0) != batch or q.size(1) != K or q.size(2) != V or (
+                    V > 1 and K > 0 and q.stride(2) != 1):
+                raise ValueError(f"{what}: draft_probs must be a {p.dtype} [{batch}][{K}][{V}] tensor, values contiguous")
+            q_at, q_batch, q_row = q.data_ptr(), q.stride(0), q.stride(1)
         if out is None:
             out = self.outputs(batch, stream)
         tokens, counts = out["tokens"], out["counts"]
-        _vector(what, "out tokens", tokens, _I32, batch * (K + 1))
-        _vector(what, "out counts", counts, _I32, batch)
-        workspace = self.workspace
-        dev = workspace.get_device()
-        _on(what, dev, target_probs, draft_tokens, uniforms, draft_probs, draft_len, tokens, counts)
-        check(load().hi_rocm_spec_verify_sampled(
-            target_probs.data_ptr(), code, batch, K, V, target_probs.stride(0), target_probs.stride(1),
-            _ptr(draft_probs), strides[0], strides[1], draft_tokens.data_ptr(), _ptr(draft_len), uniforms.data_ptr(),
-            tokens.data_ptr(), counts.data_ptr(), workspace.data_ptr(), self._bytes, _stream(what, dev, stream)))
+        if not (draft_tokens.dtype is _INT and tokens.dtype is _INT and counts.dtype is _INT and
+                uniforms.dtype is _FLOAT and draft_tokens.numel() == batch * K and tokens.numel() == batch * (K + 1) and
+                counts.numel() == batch and uniforms.numel() == batch * (K + 1) and draft_tokens.is_contiguous() and
+                tokens.is_contiguous() and counts.is_contiguous() and uniforms.is_contiguous()):
+            _vector(what, "draft_tokens", draft_tokens, _I32, batch * K)
+            _vector(what, "uniforms", uniforms, _F32, batch * (K + 1))
+            _vector(what, "out tokens", tokens, _I32, batch * (K + 1))
+            _vector(what, "out counts", counts, _I32, batch)
+        if draft_len is not None:
+            _vector(what, "draft_len", draft_len, _I32, batch)
+        if not (p.get_device() == draft_tokens.get_device() == uniforms.get_device() == tokens.get_device() ==
+                counts.get_device() == dev) or q is not None or draft_len is not None:
+            _on(what, dev, p, draft_tokens, uniforms, q, draft_len, tokens, counts)
+        status = self._verify(
+            p.data_ptr(), code, batch, K, V, p.stride(0), p.stride(1), q_at, q_batch, q_row, draft_tokens.data_ptr(),
+            _ptr(draft_len), uniforms.data_ptr(), tokens.data_ptr(), counts.data_ptr(), self.workspace.data_ptr(), self._bytes,
+            _stream(what, dev, stream))
+        if status:
+            check(status)
         return out
 
 
