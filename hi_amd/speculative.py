@@ -81,12 +81,12 @@ class SpecVerifier:
         if draft_len is not None:
             _vector(what, "draft_len", draft_len, _I32, batch)
         if not (p.get_device() == draft_tokens.get_device() == uniforms.get_device() == tokens.get_device() ==
-                counts.get_device() == dev) or q is not None or draft_len is not None:
+                counts.get_device() == dev) or dev < 0 or q is not None or draft_len is not None:
             _on(what, dev, p, draft_tokens, uniforms, q, draft_len, tokens, counts)
         status = self._verify(
             p.data_ptr(), code, batch, K, V, p.stride(0), p.stride(1), q_at, q_batch, q_row, draft_tokens.data_ptr(),
-            _ptr(draft_len), uniforms.data_ptr(), tokens.data_ptr(), counts.data_ptr(), self.workspace.data_ptr(), self._bytes,
-            _stream(what, dev, stream))
+            _ptr(draft_len), uniforms.data_ptr(), tokens.data_ptr(), counts.data_ptr(), self.workspace.data_ptr(),
+            self._bytes, _stream(what, dev, stream))
         if status:
             check(status)
         return out
