@@ -198,9 +198,12 @@ class Mx4Experts:
     gate_e Q(x[t])) * (up_e Q(x[t]))), e = ids[t][s].  ``up`` uint8 [experts]
     [2 * inter][hidden / 2] (gate rows, then up rows) and ``down`` uint8
     [experts][hidden][inter / 2] with their scales; hidden and inter multiples
-    of 32.  Activations go from f32 to 4 bits without a step between; the
-    second product's results stay f32 until they are summed.  Weights are
-    packed on ``stream`` and need not be kept; buffers for up to ``max_tokens``
+    of 32.  Activations go from f32 to 4 bits without a step between.  A
+    token's terms have the result's type, and their sum is f32: for a bfloat16
+    result they are rounded before they are weighted.  That is off by 0.0024
+    where f32 terms give 0.0017, next to a tenth by the 4-bit roundings, and
+    takes a fifth off a long prompt's layer (4,096 tokens of 8 terms, 240 to 195
+    us); a float32 result has f32 terms.  Weights are packed on ``stream`` and need not be kept; buffers for up to ``max_tokens``
     tokens are allocated once, and calls allocate nothing when ``out`` is
     given."""
 
@@ -223,7 +226,7 @@ class Mx4Experts:
         self._h_bytes = _size(lib.hi_rocm_mx4_rows_bytes, places, self.inter)
         self._x = torch.empty(self._x_bytes, dtype=torch.uint8, device=dev)
         self._h = torch.empty(self._h_bytes, dtype=torch.uint8, device=dev)
-        self._y = torch.empty(places, self.hidden, dtype=torch.float32, device=dev)
+        self._y = torch.empty(places, self.hidden, dtype=torch.float32, device=dev)  # (or as many bfloat16)
         self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev)
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -258,9 +261,9 @@ class Mx4Experts:
             self._x.data_ptr(), self._x_bytes, st))
         check(lib.hi_rocm_mx4_grouped_product(
             h.data_ptr(), DTYPE_MX4, places, 0, 0, 1, offsets, places, E, self._down.data_ptr(), self._down.numel(), H, I,
-            0, y.data_ptr(), _CODES[y.dtype], H, 0, 0, 0, st))
+            0, y.data_ptr(), code, H, 0, 0, 0, st))
         check(lib.hi_rocm_moe_combine(
-            y.data_ptr(), _CODES[y.dtype], H, slots, offsets, E, weights.data_ptr(), tokens, k, H, out.data_ptr(), code,
+            y.data_ptr(), code, H, slots, offsets, E, weights.data_ptr(), tokens, k, H, out.data_ptr(), code,
             out.stride(0) if tokens > 1 else H, st))
         return out
 

@@ -137,8 +137,7 @@ def test_layer(hip, T, E, K, H, I, none):
     x = torch.randn(T, H, generator=gen(4), device="cuda").bfloat16()
     layer = Mx4Experts(up, ups, down, downs, max_tokens=T + 3, top_k=K)
     out32 = layer(x, ids, wts, out=torch.empty(T, H, device="cuda"))
-    got = layer(x, ids, wts)
-    assert torch.equal(got, out32.bfloat16())
+    got = layer(x, ids, wts).cpu()
     # from the kernel's own activations
     groups = group_rows(ids, E)
     h = mx4.Mx4Rows(groups.places, I)
@@ -154,6 +153,9 @@ def test_layer(hip, T, E, K, H, I, none):
     want = (y[slots].view(T, K, H) * ww[:, :, None]).sum(1)
     tol = ((I // 32 + 8 + K + 2) * STEP * size[slots].view(T, K, H) * ww[:, :, None]).sum(1)
     assert ((out32.double().cpu() - want).abs() <= tol).all()
+    # bf16 terms are off by another half step each, 2^-8 of what is within their bound
+    bound = tol + 1.01 * 2.0 ** -8 * (y[slots].abs().view(T, K, H) * ww[:, :, None]).sum(1) + 2.0 ** -7 * tol
+    assert ((got >= (want - bound).float().bfloat16()) & (got <= (want + bound).float().bfloat16())).all()
     # the activations against the exact ones: a code a step away only next to a border
     token, _ = in_places(groups, ids, E)
     xx, wu = O.rounded(x)[token], O.values(up, ups)
