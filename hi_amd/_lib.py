@@ -94,6 +94,7 @@ SIGNATURES = {
     "hi_rocm_mx4_dequantize": (_i, [_vp, _vp, _i64, _i, _vp, _i, _i64, _vp]),
     "hi_rocm_mx4_rows_bytes": (_i, [_i64, _i, ctypes.POINTER(_sz)]),
     "hi_rocm_mx4_rows": (_i, [_vp, _i, _i64, _i, _i64, _vp, _sz, _vp]),
+    "hi_rocm_mx4_moe_prepare": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i64, _vp, _sz, _vp]),
     "hi_rocm_mx4_packed_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
     "hi_rocm_mx4_pack": (_i, [_vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
     "hi_rocm_mx4_workspace_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "hi_rocm.h"
+#include "moe_group.h"
 #include "mx4.h"
 #include "sampler_internal.h"
 #include "wave_ops.h"
@@ -30,14 +31,25 @@ __device__ __forceinline__ Mx4Unit mx4_unit(int64_t u, int64_t units, int quads,
 
 // Rounds rows of x.  ROWS: scales in the order of "rows", else [rows][k / 32].
 // Bound by the bytes: 2 or 4 read and 0.53 written a value.
+template <typename T>
+struct Mx4Quantize {
+  const T* x;
+  int64_t x_stride, units;
+  int quads, k;
+  uint8_t* codes;
+  int64_t code_stride;
+  uint8_t* scales;
+  int64_t scale_stride;
+};
 template <typename T, bool ROWS>
-__global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, int64_t x_stride, int64_t units, int quads, int k,
-                                                           uint8_t* codes, int64_t code_stride, uint8_t* scales,
-                                                           int64_t scale_stride) {
+__device__ __forceinline__ void mx4_quantize_units(const Mx4Quantize<T>& q, int64_t u0) {
+  const T* x = q.x;
+  const int64_t x_stride = q.x_stride, units = q.units, code_stride = q.code_stride, scale_stride = q.scale_stride;
+  const int quads = q.quads, k = q.k;
+  uint8_t *codes = q.codes, *scales = q.scales;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int L = F32 ? 2 : 1;
   const int lane = threadIdx.x & 63;
-  const int64_t u0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kMx4Units;
   uint4 v[kMx4Units][L];
   #pragma unroll
   for (int i = 0; i < kMx4Units; ++i) {
@@ -78,6 +90,22 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, int64_t x
       scales[un.row * scale_stride + (ROWS ? mx4_scale_at(b) : b)] = (uint8_t)(un.in ? s : 127u);
     }
   }
+}
+
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(256) mx4_quantize_kernel(Mx4Quantize<T> q) {
+  mx4_quantize_units<T, ROWS>(q, ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kMx4Units);
+}
+
+// The expert layer's first launch: workgroups 0 .. experts group the pairs, the
+// others round the tokens' rows, which need no group (200 tokens of 1440: one launch
+// MEASURED us, two MEASURED).
+template <int W, int L>
+__global__ void __launch_bounds__(64 * W) mx4_prepare_kernel(const uint32_t* ids, int pairs, int experts, int32_t* order,
+                                                             int32_t* slots, int32_t* offsets, Mx4Quantize<__bf16> q) {
+  const int b = (int)blockIdx.x - (experts + 1);
+  if (b < 0) moe_group_pairs<W, L>(ids, pairs, experts, order, slots, offsets, blockIdx.x);
+  else mx4_quantize_units<__bf16, true>(q, ((int64_t)b * W + (threadIdx.x >> 6)) * kMx4Units);
 }
 
 // Back to values, in f32 or bf16 (exact but for bf16's range: code times power
@@ -159,11 +187,11 @@ hipError_t launch_quantize(const void* x, int dtype, int64_t rows, int k, int64_
   const int64_t units = rows * quads;
   const dim3 grid((unsigned)((units + 4 * kMx4Units - 1) / (4 * kMx4Units)));
   if (dtype == HI_ROCM_DTYPE_F32)
-    hipLaunchKernelGGL((mx4_quantize_kernel<float, ROWS>), grid, dim3(256), 0, st, (const float*)x, x_stride, units,
-                       quads, k, codes, code_stride, scales, scale_stride);
+    hipLaunchKernelGGL((mx4_quantize_kernel<float, ROWS>), grid, dim3(256), 0, st,
+                       Mx4Quantize<float>{(const float*)x, x_stride, units, quads, k, codes, code_stride, scales, scale_stride});
   else
-    hipLaunchKernelGGL((mx4_quantize_kernel<__bf16, ROWS>), grid, dim3(256), 0, st, (const __bf16*)x, x_stride, units,
-                       quads, k, codes, code_stride, scales, scale_stride);
+    hipLaunchKernelGGL((mx4_quantize_kernel<__bf16, ROWS>), grid, dim3(256), 0, st,
+                       Mx4Quantize<__bf16>{(const __bf16*)x, x_stride, units, quads, k, codes, code_stride, scales, scale_stride});
   return hipGetLastError();
 }
 
@@ -247,6 +275,39 @@ int hi_rocm_mx4_rows(const void* x, int dtype, int64_t rows, int k, int64_t x_st
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_mx4_rows: out not on 16 bytes, or too small (hi_rocm_mx4_rows_bytes)");
   const hipError_t e = mx4_make_rows(x, dtype, rows, k, x_stride, out, (hipStream_t)stream);
   return e == hipSuccess ? HI_ROCM_OK : api_hip_fail(e, "mx4 rows launch");
+}
+
+int hi_rocm_mx4_moe_prepare(const uint32_t* ids, int tokens, int top_k, int experts, int32_t* order, int32_t* slots,
+                            int32_t* offsets, const void* x, int k, int64_t x_stride, void* out, size_t out_bytes,
+                            void* stream) {
+  if (ids == nullptr || order == nullptr || slots == nullptr || offsets == nullptr || x == nullptr || out == nullptr ||
+      tokens <= 0 || top_k <= 0 || experts <= 0 || k <= 0 || x_stride < k)
+    return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_mx4_moe_prepare: invalid arguments");
+  if (experts > kMoeMaxExperts || (int64_t)tokens * top_k > kMoeMaxPairs)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_mx4_moe_prepare: more than 2048 experts or 2^22 pairs");
+  if (k % kMx4Block != 0 || (uintptr_t)x % 16 != 0 || x_stride % 8 != 0)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED,
+                    "hi_rocm_mx4_moe_prepare: needs k a multiple of 32 and rows that start on 16 bytes");
+  if (k > HI_ROCM_MX4_MAX_K || !mx4_rows_fit(tokens, k))
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_mx4_moe_prepare: more than 2^24 inputs, or too many rows");
+  const Mx4Rows R = mx4_rows_layout(tokens, k);
+  if ((uintptr_t)out % 16 != 0 || out_bytes < R.total)
+    return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_mx4_moe_prepare: out not on 16 bytes, or too small (hi_rocm_mx4_rows_bytes)");
+  const int pairs = tokens * top_k, quads = (k + kMx4Quad - 1) / kMx4Quad;
+  const Mx4Quantize<__bf16> q{(const __bf16*)x, x_stride, (int64_t)tokens * quads, quads, k, (uint8_t*)out, R.code_stride,
+                              (uint8_t*)out + R.scales, R.scale_stride};
+  const int waves = pairs <= kMoeFewPairs ? 4 : 16;
+  const int64_t groups = experts + 1 + (q.units + waves * kMx4Units - 1) / (waves * kMx4Units);
+  if (groups > UINT32_MAX / (64 * waves))
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_mx4_moe_prepare: too many rows for one launch");
+  if (waves == 4)
+    hipLaunchKernelGGL((mx4_prepare_kernel<4, 4>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, ids, pairs,
+                       experts, order, slots, offsets, q);
+  else
+    hipLaunchKernelGGL((mx4_prepare_kernel<16, 8>), dim3((unsigned)groups), dim3(1024), 0, (hipStream_t)stream, ids, pairs,
+                       experts, order, slots, offsets, q);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? HI_ROCM_OK : api_hip_fail(e, "mx4 moe prepare launch");
 }
 
 int hi_rocm_mx4_packed_bytes(int experts, int n, int k, size_t* out_bytes) {

@@ -203,9 +203,9 @@ class Mx4Experts:
     result they are rounded before they are weighted.  That is off by 0.0024
     where f32 terms give 0.0017, next to a tenth by the 4-bit roundings, and
     takes a fifth off a long prompt's layer (4,096 tokens of 8 terms, 240 to 195
-    us); a float32 result has f32 terms.  Weights are packed on ``stream`` and need not be kept; buffers for up to ``max_tokens``
-    tokens are allocated once, and calls allocate nothing when ``out`` is
-    given."""
+    us); a float32 result has f32 terms.  Weights are packed on ``stream`` and
+    need not be kept; buffers for up to ``max_tokens`` tokens are allocated
+    once, and calls allocate nothing when ``out`` is given."""
 
     def __init__(self, up: torch.Tensor, up_scales: torch.Tensor, down: torch.Tensor, down_scales: torch.Tensor,
                  max_tokens: int, top_k: int, stream: Optional[torch.cuda.Stream] = None):
@@ -228,6 +228,7 @@ class Mx4Experts:
         self._h = torch.empty(self._h_bytes, dtype=torch.uint8, device=dev)
         self._y = torch.empty(places, self.hidden, dtype=torch.float32, device=dev)  # (or as many bfloat16)
         self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev)
+        self._few = {}  # tokens: whether their rows need no rounding beforehand
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, out: Optional[torch.Tensor] = None,
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
@@ -254,11 +255,18 @@ class Mx4Experts:
         _on(what, h.get_device(), x, ids, weights, out)
         places, st, lib = tokens * k, _stream(what, h.get_device(), stream), load()
         order, slots, offsets = g.order.data_ptr(), g.slots.data_ptr(), g.offsets.data_ptr()
-        check(lib.hi_rocm_moe_group(ids.data_ptr(), tokens, k, E, order, slots, offsets, st))
+        at, code_x, stride = x.data_ptr(), DTYPE_BF16, x.stride(0) if tokens > 1 else H
+        if self._few.get(tokens) is None:
+            self._few[tokens] = _size(lib.hi_rocm_mx4_workspace_bytes, tokens, places, H) == 0
+        if self._few[tokens]:  # the product rounds the rows as it reads them
+            check(lib.hi_rocm_moe_group(ids.data_ptr(), tokens, k, E, order, slots, offsets, st))
+        else:
+            check(lib.hi_rocm_mx4_moe_prepare(ids.data_ptr(), tokens, k, E, order, slots, offsets, at, H, stride,
+                                              self._x.data_ptr(), self._x_bytes, st))
+            at, code_x = self._x.data_ptr(), DTYPE_MX4
         check(lib.hi_rocm_mx4_grouped_product(
-            x.data_ptr(), DTYPE_BF16, tokens, x.stride(0) if tokens > 1 else H, order, k, offsets, places, E,
-            self._up.data_ptr(), self._up.numel(), 2 * I, H, 1, h.data_ptr(), DTYPE_MX4, I, self._h_bytes,
-            self._x.data_ptr(), self._x_bytes, st))
+            at, code_x, tokens, stride, order, k, offsets, places, E, self._up.data_ptr(), self._up.numel(), 2 * I, H, 1,
+            h.data_ptr(), DTYPE_MX4, I, self._h_bytes, 0, 0, st))
         check(lib.hi_rocm_mx4_grouped_product(
             h.data_ptr(), DTYPE_MX4, places, 0, 0, 1, offsets, places, E, self._down.data_ptr(), self._down.numel(), H, I,
             0, y.data_ptr(), code, H, 0, 0, 0, st))

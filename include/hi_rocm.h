@@ -556,6 +556,13 @@ int hi_rocm_mx4_rows_bytes(int64_t rows, int k, size_t* out_bytes);
 int hi_rocm_mx4_rows(const void* x, int dtype, int64_t rows, int k, int64_t x_stride, void* out, size_t out_bytes,
                      void* stream);
 
+/* hi_rocm_moe_group, and hi_rocm_mx4_rows of the tokens' bf16 rows x [tokens][x_stride],
+ * in one launch: what a layer's products read (x_dtype HI_ROCM_DTYPE_MX4, gathered by
+ * order). */
+int hi_rocm_mx4_moe_prepare(const uint32_t* ids, int tokens, int top_k, int experts, int32_t* order, int32_t* slots,
+                            int32_t* offsets, const void* x, int k, int64_t x_stride, void* out, size_t out_bytes,
+                            void* stream);
+
 /* Lays weights [experts][n][k] out for the products, once (experts 1 for a linear
  * layer): codes on 16 bytes and scales as above into packed, on 16 bytes. */
 int hi_rocm_mx4_packed_bytes(int experts, int n, int k, size_t* out_bytes);

@@ -23,6 +23,9 @@ GOOD = {
     "hi_rocm_mx4_quantize": dict(x=P, dtype=BF16, rows=3, k=64, x_stride=64, codes=P, scales=P, stream=None),
     "hi_rocm_mx4_dequantize": dict(codes=P, scales=P, rows=3, k=64, out=P, out_dtype=F32, out_stride=64, stream=None),
     "hi_rocm_mx4_rows": dict(x=P, dtype=BF16, rows=3, k=64, x_stride=64, out=P, out_bytes=BIG, stream=None),
+    "hi_rocm_mx4_moe_prepare": dict(
+        ids=P, tokens=20, top_k=2, experts=4, order=P, slots=P, offsets=P, x=P, k=64, x_stride=64, out=P, out_bytes=BIG,
+        stream=None),
     "hi_rocm_mx4_pack": dict(codes=P, scales=P, experts=2, n=48, k=64, packed=P, packed_bytes=BIG, stream=None),
     "hi_rocm_mx4_linear": dict(
         x=P, x_dtype=BF16, rows=20, x_stride=64, packed=P, packed_bytes=BIG, n=48, k=64, bias=0, out=P, out_dtype=F32,
@@ -55,6 +58,13 @@ REFUSED = [
     ("hi_rocm_mx4_rows", ARGS, [
         dict(x=None), dict(out=None), dict(rows=0), dict(dtype=5), dict(x_stride=32), dict(out=P + 8), dict(out_bytes=64)]),
     ("hi_rocm_mx4_rows", UNSUPPORTED, [dict(k=40), dict(x=P + 2), dict(x_stride=65), dict(rows=1 << 29)]),
+    ("hi_rocm_mx4_moe_prepare", ARGS, [
+        dict(ids=None), dict(order=None), dict(slots=None), dict(offsets=None), dict(x=None), dict(out=None),
+        dict(tokens=0), dict(top_k=0), dict(experts=0), dict(k=0), dict(x_stride=63), dict(out=P + 8),
+        dict(out_bytes=100)]),
+    ("hi_rocm_mx4_moe_prepare", UNSUPPORTED, [
+        dict(experts=2049), dict(tokens=(1 << 21) + 1), dict(k=48), dict(x=P + 8), dict(x_stride=68),
+        dict(k=(1 << 24) + 32, x_stride=1 << 25)]),
     ("hi_rocm_mx4_pack", ARGS, [
         dict(codes=None), dict(scales=None), dict(packed=None), dict(experts=0), dict(n=0), dict(k=0), dict(packed=P + 8),
         dict(packed_bytes=1000)]),
