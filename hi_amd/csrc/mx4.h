@@ -36,7 +36,7 @@ struct Mx4Rows {
 };
 inline Mx4Rows mx4_rows_layout(int64_t rows, int k) {
   Mx4Rows L;
-  L.code_stride = (((int64_t)k / 2 + 127) / 128 | 1) * 128;
+  L.code_stride = k / 2;
   L.scale_stride = ((int64_t)k + kMx4Quad - 1) / kMx4Quad * 16;
   L.scales = (size_t)rows * L.code_stride;
   L.total = L.scales + (size_t)rows * L.scale_stride + kMx4Quad / 2;  // (a last quad's codes may be read whole)

@@ -74,9 +74,16 @@ __device__ __forceinline__ bool mx4_work(const Mx4Args& a, int blocks, MoeWork& 
   return true;
 }
 
-// The row of x behind place i.
-__device__ __forceinline__ int mx4_row(const Mx4Args& a, int i) {
-  const int row = a.order ? a.order[i] / a.top_k : i;
+// The row of x behind place i: its pair, as loaded, and the pair's token.  (The
+// quotient of up to 2^22 by a float's reciprocal is off by one at most.)
+__device__ __forceinline__ int mx4_pair(const Mx4Args& a, int i) { return a.order ? a.order[i] : i; }
+__device__ __forceinline__ int mx4_row(const Mx4Args& a, int pair) {
+  int row = pair;
+  if (a.order) {
+    row = (int)((float)pair * __builtin_amdgcn_rcpf((float)a.top_k));
+    const int left = pair - row * a.top_k;
+    row += (left >= a.top_k) - (left < 0);
+  }
   return min(max(row, 0), a.x_rows - 1);
 }
 
@@ -162,7 +169,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 6) mx4_few_kernel(Mx4Args a) {
   uint4 raw[4];
   auto raw_load = [&](int b) {
     const int j = b / blocks;
-    const uint4* p = reinterpret_cast<const uint4*>(a.x + mx4_row(a, wk.i0 + j) * a.x_stride) + (b - j * blocks) * 4;
+    const uint4* p = reinterpret_cast<const uint4*>(a.x + mx4_row(a, mx4_pair(a, wk.i0 + j)) * a.x_stride) + (b - j * blocks) * 4;
     #pragma unroll
     for (int i = 0; i < 4; ++i) raw[i] = p[i];
   };
@@ -210,7 +217,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 6) mx4_few_kernel(Mx4Args a) {
   };
   load_w(min(wid, a.steps - 1));
   if constexpr (CODES) {  // (behind the weights, which need no row's number)
-    const int64_t row = mx4_row(a, min(wk.i0 + r, wk.i1 - 1));
+    const int64_t row = mx4_row(a, mx4_pair(a, min(wk.i0 + r, wk.i1 - 1)));
     xp = a.x + row * a.x_stride + 16 * g;
     xs = a.x_scales + row * a.x_scale_stride + 4 * g;
     load_x(min(wid, a.steps - 1));
@@ -457,14 +464,29 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
   const uint8_t* const wsp =
       a.w_scales +
       ((int64_t)expert * a.tiles + min(tile_s + (lane >> 4 & 1), a.tiles - 1)) * a.quads * 256 + (lane & 15) * 16;
-  // x: a round of loads takes 16 rows, this thread's chunk of one
+  // x: a round of loads takes 16 rows, this thread's chunk of one.  (The rows'
+  // numbers are asked for before the first weights, and needed behind them.)
   const int jr = tid / 16, chunk = (tid & 15) ^ jr;
+  int pair[L - 2];
+  #pragma unroll
+  for (int i = 0; i < L - 2; ++i) pair[i] = mx4_pair(a, min(wk.i0 + i * 16 + jr, wk.i1 - 1));
+  const int pair_s = mx4_pair(a, min(wk.i0 + min(tid, BM - 1), wk.i1 - 1));
+  __builtin_amdgcn_sched_barrier(0);
+  mx4_i32x4 w[D][2][2];
+  auto load_w = [&](int slot, int step) {
+    const int at = min(step, a.steps - 1) * 1024;
+    #pragma unroll
+    for (int t = 0; t < 2; ++t)
+      #pragma unroll
+      for (int u = 0; u < 2; ++u) w[slot][t][u] = __builtin_amdgcn_raw_buffer_load_b128(wr[t], w_lane[t] + u * 512, at, 0);
+  };
+  #pragma unroll
+  for (int d = 0; d < D; ++d) load_w(d, d);
+  __builtin_amdgcn_sched_barrier(0);
   const uint8_t* xp[L - 2];
   #pragma unroll
-  for (int i = 0; i < L - 2; ++i)
-    xp[i] = a.x + (int64_t)mx4_row(a, min(wk.i0 + i * 16 + jr, wk.i1 - 1)) * a.x_stride + 16 * chunk;
-  const uint8_t* const sp =
-      a.x_scales + (int64_t)mx4_row(a, min(wk.i0 + min(tid, BM - 1), wk.i1 - 1)) * a.x_scale_stride;
+  for (int i = 0; i < L - 2; ++i) xp[i] = a.x + (int64_t)mx4_row(a, pair[i]) * a.x_stride + 16 * chunk;
+  const uint8_t* const sp = a.x_scales + (int64_t)mx4_row(a, pair_s) * a.x_scale_stride;
   auto fill = [&](int quad) {  // (past the last quad, that again, for a buffer that is not read)
     char* to = smem + (quad & 1) * Tile::BUFFER;
     const int at = min(quad, a.quads - 1);
@@ -479,14 +501,6 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
     __builtin_amdgcn_global_load_lds((moe_global*)(wsp + (int64_t)at * 256),
                                      (moe_lds*)(to + Tile::CODES + 4096 + wid * 1024), 16, 0, 0);
   };
-  mx4_i32x4 w[D][2][2];
-  auto load_w = [&](int slot, int step) {
-    const int at = min(step, a.steps - 1) * 1024;
-    #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      #pragma unroll
-      for (int u = 0; u < 2; ++u) w[slot][t][u] = __builtin_amdgcn_raw_buffer_load_b128(wr[t], w_lane[t] + u * 512, at, 0);
-  };
   mx4_f32x16 acc[MT][2];
   #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -495,9 +509,6 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
       #pragma unroll
       for (int i = 0; i < 16; ++i) acc[m][t][i] = 0.f;
   fill(0);
-  __builtin_amdgcn_sched_barrier(0);
-  #pragma unroll
-  for (int d = 0; d < D; ++d) load_w(d, d);
   const char* const xrow = smem + r * 256;
   const char* const srow = smem + Tile::CODES + r * 16 + h * 4;
   int xs[MT][2], ws[2][2];

@@ -20,10 +20,11 @@ struct Mx4Unit {
   int quad, at;  // at: this lane's first value
   bool in;
 };
-__device__ __forceinline__ Mx4Unit mx4_unit(int64_t u, int64_t units, int quads, int k, int lane) {
+__device__ __forceinline__ Mx4Unit mx4_unit(uint32_t u, uint32_t units, uint32_t quads, int k, int lane) {
   Mx4Unit x;
-  x.row = (int64_t)((uint64_t)u / (uint32_t)quads);
-  x.quad = (int)(u - x.row * quads);
+  const uint32_t row = u / quads;  // (units fit 28 bits: mx4_rows_fit)
+  x.row = row;
+  x.quad = (int)(u - row * quads);
   x.at = x.quad * kMx4Quad + lane * 8;
   x.in = u < units && x.at < k;
   return x;
@@ -34,7 +35,8 @@ __device__ __forceinline__ Mx4Unit mx4_unit(int64_t u, int64_t units, int quads,
 template <typename T>
 struct Mx4Quantize {
   const T* x;
-  int64_t x_stride, units;
+  int64_t x_stride;
+  uint32_t units;
   int quads, k;
   uint8_t* codes;
   int64_t code_stride;
@@ -42,9 +44,10 @@ struct Mx4Quantize {
   int64_t scale_stride;
 };
 template <typename T, bool ROWS>
-__device__ __forceinline__ void mx4_quantize_units(const Mx4Quantize<T>& q, int64_t u0) {
+__device__ __forceinline__ void mx4_quantize_units(const Mx4Quantize<T>& q, uint32_t u0) {
   const T* x = q.x;
-  const int64_t x_stride = q.x_stride, units = q.units, code_stride = q.code_stride, scale_stride = q.scale_stride;
+  const int64_t x_stride = q.x_stride, code_stride = q.code_stride, scale_stride = q.scale_stride;
+  const uint32_t units = q.units;
   const int quads = q.quads, k = q.k;
   uint8_t *codes = q.codes, *scales = q.scales;
   constexpr bool F32 = sizeof(T) == 4;
@@ -94,27 +97,27 @@ __device__ __forceinline__ void mx4_quantize_units(const Mx4Quantize<T>& q, int6
 
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(Mx4Quantize<T> q) {
-  mx4_quantize_units<T, ROWS>(q, ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kMx4Units);
+  mx4_quantize_units<T, ROWS>(q, (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kMx4Units);
 }
 
 // The expert layer's first launch: workgroups 0 .. experts group the pairs, the
-// others round the tokens' rows, which need no group (200 tokens of 1440: one launch
-// MEASURED us, two MEASURED).
+// others round the tokens' rows, which need no group (200 tokens of 1440: 3.8 us,
+// in two launches 3.2 and 3.5).
 template <int W, int L>
 __global__ void __launch_bounds__(64 * W) mx4_prepare_kernel(const uint32_t* ids, int pairs, int experts, int32_t* order,
                                                              int32_t* slots, int32_t* offsets, Mx4Quantize<__bf16> q) {
   const int b = (int)blockIdx.x - (experts + 1);
   if (b < 0) moe_group_pairs<W, L>(ids, pairs, experts, order, slots, offsets, blockIdx.x);
-  else mx4_quantize_units<__bf16, true>(q, ((int64_t)b * W + (threadIdx.x >> 6)) * kMx4Units);
+  else mx4_quantize_units<__bf16, true>(q, ((uint32_t)b * W + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kMx4Units);
 }
 
 // Back to values, in f32 or bf16 (exact but for bf16's range: code times power
 // of two has two bits).
 template <typename T>
-__global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int64_t units,
+__global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, uint32_t units,
                                                              int quads, int k, T* out, int64_t out_stride) {
   const int lane = threadIdx.x & 63;
-  const int64_t u0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kMx4Units;
+  const uint32_t u0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kMx4Units;
   uint32_t c[kMx4Units], s[kMx4Units];
   #pragma unroll
   for (int i = 0; i < kMx4Units; ++i) {
@@ -184,7 +187,7 @@ template <bool ROWS>
 hipError_t launch_quantize(const void* x, int dtype, int64_t rows, int k, int64_t x_stride, uint8_t* codes,
                            int64_t code_stride, uint8_t* scales, int64_t scale_stride, hipStream_t st) {
   const int quads = (k + kMx4Quad - 1) / kMx4Quad;
-  const int64_t units = rows * quads;
+  const uint32_t units = (uint32_t)(rows * quads);
   const dim3 grid((unsigned)((units + 4 * kMx4Units - 1) / (4 * kMx4Units)));
   if (dtype == HI_ROCM_DTYPE_F32)
     hipLaunchKernelGGL((mx4_quantize_kernel<float, ROWS>), grid, dim3(256), 0, st,
@@ -242,7 +245,7 @@ int hi_rocm_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t 
   if (k > HI_ROCM_MX4_MAX_K || !mx4_rows_fit(rows, k))
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_mx4_dequantize: more than 2^24 inputs, or too many rows");
   const int quads = (k + kMx4Quad - 1) / kMx4Quad;
-  const int64_t units = rows * quads;
+  const uint32_t units = (uint32_t)(rows * quads);
   const dim3 grid((unsigned)((units + 4 * kMx4Units - 1) / (4 * kMx4Units)));
   if (out_dtype == HI_ROCM_DTYPE_F32)
     hipLaunchKernelGGL((mx4_dequantize_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, codes, scales, units,
@@ -294,10 +297,10 @@ int hi_rocm_mx4_moe_prepare(const uint32_t* ids, int tokens, int top_k, int expe
   if ((uintptr_t)out % 16 != 0 || out_bytes < R.total)
     return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_mx4_moe_prepare: out not on 16 bytes, or too small (hi_rocm_mx4_rows_bytes)");
   const int pairs = tokens * top_k, quads = (k + kMx4Quad - 1) / kMx4Quad;
-  const Mx4Quantize<__bf16> q{(const __bf16*)x, x_stride, (int64_t)tokens * quads, quads, k, (uint8_t*)out, R.code_stride,
+  const Mx4Quantize<__bf16> q{(const __bf16*)x, x_stride, (uint32_t)(tokens * quads), quads, k, (uint8_t*)out, R.code_stride,
                               (uint8_t*)out + R.scales, R.scale_stride};
   const int waves = pairs <= kMoeFewPairs ? 4 : 16;
-  const int64_t groups = experts + 1 + (q.units + waves * kMx4Units - 1) / (waves * kMx4Units);
+  const int64_t groups = experts + 1 + ((int64_t)q.units + waves * kMx4Units - 1) / (waves * kMx4Units);
   if (groups > UINT32_MAX / (64 * waves))
     return api_fail(HI_ROCM_ERR_UNSUPPORTED, "hi_rocm_mx4_moe_prepare: too many rows for one launch");
   if (waves == 4)

@@ -154,11 +154,29 @@ def test_large(hip, rows, n, k):
     agree(got[r][:, c], y, tol)
 
 
-@pytest.mark.parametrize("rows", [7, 16, 40, 200])
-def test_rows_do_not_mix(hip, rows):
+@pytest.mark.parametrize("k", [32, 96, 256, 384, 512, 544, 896, 1184, 1664])
+@pytest.mark.parametrize("rows,n", [(130, 16400), (250, 16380), (310, 16384), (509, 16385), (2048, 4097), (33, 70001)])
+def test_tiles(hip, rows, n, k):
+    """Every size of tile, tiles that end inside the places or the weight's last
+    rows, and every number of steps behind whole quads: the last rows and columns
+    and some between."""
+    codes, scales = weight(n, k, seed=k)
+    x = torch.randn(rows, k, generator=gen(rows), device="cuda").bfloat16()
+    bias = torch.randn(n, generator=gen(n), device="cuda")
+    lin = Mx4Linear(codes, scales, bias)
+    c = torch.cat((torch.randint(0, n, (200,), generator=gen(1), device="cuda"), torch.arange(n - 70, n, device="cuda"))).unique()
+    r = torch.cat((torch.randint(0, rows, (40,), generator=gen(2), device="cuda"),
+                   torch.arange(rows - 33, rows, device="cuda"))).unique()
+    y, tol = exact(x[r], codes[c], scales[c], bias[c])
+    for dtype in (torch.float32, torch.bfloat16):
+        agree(lin(x, dtype=dtype)[r][:, c], y, tol)
+
+
+@pytest.mark.parametrize("rows,n", [(7, 96), (16, 96), (40, 96), (200, 96), (130, 16384), (520, 16384), (2000, 4096)])
+def test_rows_do_not_mix(hip, rows, n):
     """A row's bits are the same whatever the other rows hold; a row with an
     infinity or NaN gives NaN."""
-    codes, scales = weight(96, 640, seed=1)
+    codes, scales = weight(n, 640, seed=1)
     lin = Mx4Linear(codes, scales)
     x = torch.randn(rows, 640, generator=gen(2), device="cuda").bfloat16()
     y = lin(x)
@@ -171,10 +189,10 @@ def test_rows_do_not_mix(hip, rows):
     assert torch.equal(lin(x), y)
 
 
-@pytest.mark.parametrize("rows", [3, 70, 300])
-def test_scales_at_their_ends(hip, rows):
+@pytest.mark.parametrize("rows,n", [(3, 40), (70, 40), (300, 40), (300, 1000)])
+def test_scales_at_their_ends(hip, rows, n):
     """Weights of NaN blocks, of the smallest and largest scales, and of zeros."""
-    codes, scales = weight(40, 192, seed=3)
+    codes, scales = weight(n, 192, seed=3)
     scales[7, 2] = 255
     scales[8], scales[9] = 0, 250
     codes[10] = 0
@@ -196,21 +214,21 @@ def test_scales_at_their_ends(hip, rows):
     assert (got[:, 10] == 0).all()
 
 
-@pytest.mark.parametrize("rows", [5, 40, 300])
-def test_padding_stays_out(hip, rows):
+@pytest.mark.parametrize("rows,n", [(5, 21), (40, 21), (300, 21), (300, 1013)])
+def test_padding_stays_out(hip, rows, n):
     """k that ends inside a step and n inside a tile: what lies behind the
     inputs (NaN) and the outputs (a mark) is neither used nor written."""
-    codes, scales = weight(21, 160, seed=2)
+    codes, scales = weight(n, 160, seed=2)
     big = torch.full((rows, 320), float("nan"), device="cuda").bfloat16()
     x = big[:, :160]
     x.copy_(torch.randn(rows, 160, generator=gen(6), device="cuda"))
     for dtype in (torch.float32, torch.bfloat16):
-        for pad in (40, 43):
+        for pad in (n + 19, n + 22):
             out = torch.full((rows + 1, pad), 77.0, device="cuda", dtype=dtype)
-            Mx4Linear(codes, scales)(x, out=out[:rows, :21])
+            Mx4Linear(codes, scales)(x, out=out[:rows, :n])
             y, tol = exact(x, codes, scales)
-            agree(out[:rows, :21].clone(), y, tol)
-            assert (out[:, 21:] == 77).all() and (out[rows] == 77).all()
+            agree(out[:rows, :n].clone(), y, tol)
+            assert (out[:, n:] == 77).all() and (out[rows] == 77).all()
 
 
 def test_rows_used_twice(hip):
@@ -230,10 +248,10 @@ def test_rows_used_twice(hip):
 def test_graph_replays(hip):
     """Captured calls (few rows, and rows rounded in a workspace) on new inputs,
     eager calls between the replays."""
-    lin = Mx4Linear(*weight(300, 512, seed=1))
+    lin = Mx4Linear(*weight(1000, 512, seed=1))
     for rows in (3, 50, 400):
         x = torch.randn(rows, 512, generator=gen(rows), device="cuda").bfloat16()
-        out = torch.empty(rows, 300, device="cuda")
+        out = torch.empty(rows, 1000, device="cuda")
         lin(x, out=out)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):

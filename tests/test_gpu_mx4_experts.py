@@ -64,9 +64,8 @@ def product(x, packed, groups, cols, k, swiglu=False, gather=True, dtype=torch.f
 def values_of(rows):
     """The values (float64) and scale bytes of Mx4Rows."""
     k, n = rows.k, rows.rows
-    stride, quads = (-(-k // 256) | 1) * 128, -(-k // 512)
-    codes = rows.memory[:n * stride].view(n, stride)[:, :k // 2]
-    begin = n * stride
+    quads, begin = -(-k // 512), n * (k // 2)
+    codes = rows.memory[:begin].view(n, k // 2)
     s = rows.memory[begin:begin + n * quads * 16].view(n, quads, 4, 4)  # [g][j]: block 4 j + g
     s = s.transpose(2, 3).reshape(n, quads * 16)[:, :k // 32].contiguous()
     return O.values(codes.contiguous(), s), s.cpu()
@@ -163,6 +162,48 @@ def test_layer(hip, T, E, K, H, I, none):
         g = torch.stack([wu[e] @ r for e, r in zip(expert[:n], xx[:n])])
         exact = torch.nn.functional.silu(g[:, :I]) * g[:, I:]
         assert (v[:n] != O.rounded(exact)).sum() <= 1 + n * I // 10000
+
+
+@pytest.mark.parametrize("cols", [1, 50, 300, 1000])
+@pytest.mark.parametrize("T,E,K,H", [(3, 5, 2, 96), (90, 3, 2, 384), (2, 1, 40, 160), (700, 6, 3, 896)])
+def test_any_number_of_columns(hip, T, E, K, H, cols):
+    """Columns that end inside tiles and blocks, more pairs of an expert than
+    tokens; rows of the same places in any form."""
+    g = gen(T)
+    ids = torch.randint(0, E, (T, K), generator=g, device="cuda").int()
+    w, s = weights(E, cols, H, seed=cols)
+    packed = mx4._pack("test", w, s, E, None)
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    groups = group_rows(ids, E)
+    token, expert = in_places(groups, ids, E)
+    xx, ww = O.rounded(x)[token], O.values(w, s)
+    y = torch.stack([ww[e] @ r for e, r in zip(expert, xx)])
+    tol = (H // 32 + 8) * STEP * torch.stack([ww[e].abs() @ r.abs() for e, r in zip(expert, xx)])
+    out = torch.full((T * K, cols + 5), 55.0, device="cuda")
+    product(x, packed, groups, cols, H, out=out[:, :cols])
+    assert ((out[:, :cols].double().cpu() - y).abs() <= tol).all() and (out[:, cols:] == 55).all()
+    got = product(mx4.mx4_rows(x), packed, groups, cols, H)
+    assert ((got.double().cpu() - y).abs() <= tol).all()
+
+
+def test_prepared_together(hip):
+    """Groups and rows from one launch are those of two."""
+    lib = _lib.load()
+    for T, E, K, H in ((1, 3, 1, 32), (20, 60, 4, 1440), (3000, 17, 6, 544)):
+        ids, _ = route(T, E, K, seed=T, none=0.1)
+        x = torch.randn(T, H + 32, generator=gen(T), device="cuda").bfloat16()[:, :H]
+        want, rows = group_rows(ids, E), mx4.mx4_rows(x)
+        got, out = RowGroups(T, K, E), mx4.Mx4Rows(T, H)
+        for t in (got.order, got.slots, got.offsets):
+            t.fill_(-7)
+        _lib.check(lib.hi_rocm_mx4_moe_prepare(
+            ids.data_ptr(), T, K, E, got.order.data_ptr(), got.slots.data_ptr(), got.offsets.data_ptr(), x.data_ptr(), H,
+            x.stride(0), out.memory.data_ptr(), out.memory.numel(), torch.cuda.current_stream().cuda_stream))
+        n = int(want.offsets[E])
+        assert torch.equal(got.offsets, want.offsets) and torch.equal(got.order, want.order)
+        assert torch.equal(got.slots, want.slots) and 0 <= n <= T * K
+        for a, b in zip(values_of(out), values_of(rows)):
+            assert torch.equal(a, b)
 
 
 def test_fused_rows_and_workspace_agree(hip):

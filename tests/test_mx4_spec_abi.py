@@ -116,10 +116,9 @@ def test_sizes():
         _bytes(name, *bad, status=ARGS)
     for bad in ((65536, 10), (1, (1 << 23) + 1)):
         _bytes(name, *bad, status=UNSUPPORTED)
-    # rows: whole lines, an odd number of them, then the scales of whole quads
+    # rows: codes, then the scales of whole quads
     for rows, k in ((1, 32), (3, 1184), (8192, 4096)):
-        line, quads = (-(-k // 256) | 1) * 128, -(-k // 512)
-        assert _bytes("hi_rocm_mx4_rows_bytes", rows, k) >= rows * (line + 16 * quads)
+        assert _bytes("hi_rocm_mx4_rows_bytes", rows, k) >= rows * (k // 2 + 16 * -(-k // 512))
     for e, n, k in ((1, 1, 32), (1, 151936, 4096), (60, 1000, 1184)):
         tiles, steps, quads = -(-n // 16), -(-k // 128), -(-k // 512)
         assert _bytes("hi_rocm_mx4_packed_bytes", e, n, k) >= e * tiles * (1024 * steps + 256 * quads)
