@@ -424,7 +424,16 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
       const uint4 v = *reinterpret_cast<const uint4*>(mem + j * (64 * es) + (c ^ (j & 7)) * 16);
       char* to = (char*)a.out + ((int64_t)p * a.out_stride + col) * es;
       if (col + n <= cols_out && a.out_vec) {
-        *reinterpret_cast<uint4*>(to) = v;
+        // A linear layer's rows past the caches: x and the weights stay there
+        // (8,192 x 4,096 x 16,384: 311 -> 293 us).  The experts' terms are read next
+        // (their sum 4.0 us, past the caches 4.2).
+        if (a.offsets == nullptr) {
+          typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+          const u32x4 line = {v.x, v.y, v.z, v.w};
+          __builtin_nontemporal_store(line, reinterpret_cast<u32x4*>(to));
+        } else {
+          *reinterpret_cast<uint4*>(to) = v;
+        }
       } else {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         #pragma unroll
