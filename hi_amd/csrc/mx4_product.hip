@@ -309,17 +309,20 @@ __global__ void __launch_bounds__(64 * kFewWaves, 6) mx4_few_kernel(Mx4Args a) {
   mx4_store(a, p, c, cols_out, y);
 }
 
-// Many places (prompts, many requests): 32 MT places by 256 weight rows a workgroup
-// of four waves, a wave all of the places by 64 of the rows, with MFMA 32x32x64
-// (lane 32 h + r: row r, block h of a half step; D rows 8 i + 4 h .. + 3 of column r
-// in registers 4 i .. + 3).
+// Many places (prompts, many requests): 32 MT places by 64 CW weight rows a workgroup
+// of four waves, with MFMA 32x32x64 (lane 32 h + r: row r, block h of a half step; D
+// rows 8 i + 4 h .. + 3 of column r in registers 4 i .. + 3).  CW waves have all of the
+// places by 64 of the weight rows each, and 4 / CW such groups a stretch of k each, whose
+// sums are added through LDS at the end.  Few columns a workgroup make more workgroups
+// where there would be less than one a CU: what a CU fetches takes 0.8 us a quad of
+// 256 rows (80 bytes a ns, however much is asked for ahead), with one of 64 rows 0.3.
 //
 // Weights go from memory straight to registers, where no other wave needs them,
-// kMx4Ahead steps ahead.  x goes through LDS a quad of steps at a time, filled by
+// AHEAD steps ahead.  x goes through LDS a quad of steps at a time, filled by
 // direct loads a quad ahead, with its scales; so there is a barrier a quad, and two
 // workgroups a CU work through each other's beginnings, ends and waits.  Before the
 // barrier each wave waits for its own loads of the quad that is read behind it:
-// loads return in order, and at least 4 kMx4Ahead of weights were started later.
+// loads return in order, and at least 4 AHEAD of weights were started later.
 // Behind it the other buffer is filled, whose reads all waves have waited for.
 //
 // A row of a quad is 256 bytes; its 16-byte chunk c lies at c ^ (row & 15), so that
@@ -337,34 +340,38 @@ __device__ __forceinline__ mx4_f32x16 mx4_mfma32(const mx4_i32x4& a, const mx4_i
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, J, sa, J, sb);
 }
 
-constexpr int kMx4ManyCols = 256;
 constexpr int kMx4OutBytes = 8192;  // a wave's, for 32 places of 64 columns
 
-template <int MT>
+template <int MT, int CW>
 struct Mx4Tile {
-  static constexpr int BM = 32 * MT;
+  static constexpr int BM = 32 * MT, KG = 4 / CW;
   static constexpr int AHEAD = MT > 2 ? 2 : 4;  // steps; more do not fit 256 registers
-  static constexpr int CODES = BM * 256, BUFFER = CODES + 8192;  // bytes of a quad's codes, with 256 rows' scales twice
-  static constexpr int L = BM / 16 + 2;                             // loads a thread and quad
-  static constexpr int BYTES = std::max(2 * BUFFER, 4 * kMx4OutBytes);
+  static constexpr int CODES = BM * 256, SCALES = CW * 1024;       // bytes of a quad's codes, of 64 CW rows' scales
+  static constexpr int BUFFER = CODES + 2 * SCALES;
+  static constexpr int ROWS = 4 * CW, L = BM / ROWS + 2;            // of a load, loads a thread and quad
+  static constexpr int BYTES = std::max(std::max(KG * 2 * BUFFER, 4 * kMx4OutBytes), MT * (KG - 1) * CW * kMx4OutBytes);
+  static_assert(64 * CW >= BM, "a row's scales a thread");
 };
 
 // A wave's results by way of its own LDS, 32 places at a time, written out 16
 // bytes a lane, a row's bytes next to each other.  With swiglu half 0 of acc is the
 // gate and half 1 up.
-template <int MT>
+template <int MT, int KG>
 __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
-                                             int c0, int cols_out, int lane) {
+                                             int c0, int cols_out, int lane, int group) {
   const int r = lane & 31, h = lane >> 5;
   if (a.swiglu) {
     #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m) {
+      if (m % KG != group) continue;
       #pragma unroll
       for (int i = 0; i < 16; ++i) acc[m][0][i] = moe_silu_mul(acc[m][0][i], acc[m][1][i]);
+    }
     if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
       // the 32 columns are a block; a place's other half is lane ^ 32's
       #pragma unroll
       for (int m = 0; m < MT; ++m) {
+        if (m % KG != group) continue;
         uint32_t most = 0u;
         #pragma unroll
         for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(acc[m][0][i]) & 0x7fffffffu);
@@ -400,6 +407,7 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
   typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
   #pragma unroll
   for (int m = 0; m < MT; ++m) {
+    if (m % KG != group) continue;
     if (p0 + m * 32 >= i1) return;
     // row j of 64 values: the 16-byte chunk c at c ^ (j & 7)
     #pragma unroll
@@ -448,16 +456,21 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
   }
 }
 
-template <int MT>
-__device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& wk, char* smem) {
-  typedef Mx4Tile<MT> Tile;
-  constexpr int BM = Tile::BM, D = Tile::AHEAD, L = Tile::L;
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+template <int MT, int CW>
+__device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& wk, char* smem0) {
+  typedef Mx4Tile<MT, CW> Tile;
+  constexpr int KG = Tile::KG, D = Tile::AHEAD, L = Tile::L, ROWS = Tile::ROWS, COLS = 64 * CW;
+  const int tid = threadIdx.x & (COLS - 1), lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // this group of waves: quads [quad0, quad1) of k, up to step `steps`
+  const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / COLS);
+  const int per = (a.quads + KG - 1) / KG, quad0 = min(group * per, a.quads), quad1 = min(quad0 + per, a.quads);
+  const int steps = min(quad1 * 4, a.steps);
+  char* const smem = smem0 + group * 2 * Tile::BUFFER;
   const int cols_out = a.swiglu ? a.cols / 2 : a.cols;
   const int expert = __builtin_amdgcn_readfirstlane(wk.expert), block = __builtin_amdgcn_readfirstlane(wk.block);
   // this wave's first column: with swiglu 32 of gate and the same of up
-  const int c0 = block * (a.swiglu ? kMx4ManyCols / 2 : kMx4ManyCols) + wid * (a.swiglu ? 32 : 64);
+  const int c0 = block * (a.swiglu ? COLS / 2 : COLS) + wid * (a.swiglu ? 32 : 64);
   // Its weights: two halves of 32 rows (two tiles; past the last one, that again).
   __amdgpu_buffer_rsrc_t wr[2];
   int w_lane[2];
@@ -475,40 +488,40 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
       ((int64_t)expert * a.tiles + min(tile_s + (lane >> 4 & 1), a.tiles - 1)) * a.quads * 256 + (lane & 15) * 16;
   // x: a round of loads takes 16 rows, this thread's chunk of one.  (The rows'
   // numbers are asked for before the first weights, and needed behind them.)
-  const int jr = tid / 16, chunk = (tid & 15) ^ jr;
+  const int jr = tid / 16;
   int pair[L - 2];
   #pragma unroll
-  for (int i = 0; i < L - 2; ++i) pair[i] = mx4_pair(a, min(wk.i0 + i * 16 + jr, wk.i1 - 1));
-  const int pair_s = mx4_pair(a, min(wk.i0 + min(tid, BM - 1), wk.i1 - 1));
+  for (int i = 0; i < L - 2; ++i) pair[i] = mx4_pair(a, min(wk.i0 + i * ROWS + jr, wk.i1 - 1));
+  const int pair_s = mx4_pair(a, min(wk.i0 + min(tid, Tile::BM - 1), wk.i1 - 1));
   __builtin_amdgcn_sched_barrier(0);
   mx4_i32x4 w[D][2][2];
   auto load_w = [&](int slot, int step) {
-    const int at = min(step, a.steps - 1) * 1024;
+    const int at = min(step, steps - 1) * 1024;
     #pragma unroll
     for (int t = 0; t < 2; ++t)
       #pragma unroll
       for (int u = 0; u < 2; ++u) w[slot][t][u] = __builtin_amdgcn_raw_buffer_load_b128(wr[t], w_lane[t] + u * 512, at, 0);
   };
   #pragma unroll
-  for (int d = 0; d < D; ++d) load_w(d, d);
+  for (int d = 0; d < D; ++d) load_w(d, quad0 * 4 + d);
   __builtin_amdgcn_sched_barrier(0);
   const uint8_t* xp[L - 2];
   #pragma unroll
-  for (int i = 0; i < L - 2; ++i) xp[i] = a.x + (int64_t)mx4_row(a, pair[i]) * a.x_stride + 16 * chunk;
+  for (int i = 0; i < L - 2; ++i) xp[i] = a.x + (int64_t)mx4_row(a, pair[i]) * a.x_stride + 16 * ((tid & 15) ^ ((i * ROWS + jr) & 15));
   const uint8_t* const sp = a.x_scales + (int64_t)mx4_row(a, pair_s) * a.x_scale_stride;
   auto fill = [&](int quad) {  // (past the last quad, that again, for a buffer that is not read)
     char* to = smem + (quad & 1) * Tile::BUFFER;
-    const int at = min(quad, a.quads - 1);
+    const int at = min(quad, quad1 - 1);
     #pragma unroll
     for (int i = 0; i < L - 2; ++i)
-      __builtin_amdgcn_global_load_lds((moe_global*)(xp[i] + (int64_t)at * 256), (moe_lds*)(to + i * 4096 + wid * 1024), 16,
+      __builtin_amdgcn_global_load_lds((moe_global*)(xp[i] + (int64_t)at * 256), (moe_lds*)(to + i * CW * 1024 + wid * 1024), 16,
                                        0, 0);
     // (every thread one row's scales, past the tile's the last one's: no branch, behind
     // which the compiler would not know how many loads are on their way)
     __builtin_amdgcn_global_load_lds((moe_global*)(sp + (int64_t)at * 16), (moe_lds*)(to + Tile::CODES + wid * 1024), 16, 0,
                                      0);
     __builtin_amdgcn_global_load_lds((moe_global*)(wsp + (int64_t)at * 256),
-                                     (moe_lds*)(to + Tile::CODES + 4096 + wid * 1024), 16, 0, 0);
+                                     (moe_lds*)(to + Tile::CODES + Tile::SCALES + wid * 1024), 16, 0, 0);
   };
   mx4_f32x16 acc[MT][2];
   #pragma unroll
@@ -517,7 +530,7 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
     for (int t = 0; t < 2; ++t)
       #pragma unroll
       for (int i = 0; i < 16; ++i) acc[m][t][i] = 0.f;
-  fill(0);
+  fill(quad0);
   const char* const xrow = smem + r * 256;
   const char* const srow = smem + Tile::CODES + r * 16 + h * 4;
   int xs[MT][2], ws[2][2];
@@ -564,7 +577,7 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
       #pragma unroll
       for (int m = 0; m < MT; ++m) xs[m][u] = *reinterpret_cast<const int*>(sc + m * 512 + u * 8);
       #pragma unroll
-      for (int t = 0; t < 2; ++t) ws[t][u] = *reinterpret_cast<const int*>(sc + 4096 + wid * 1024 + t * 512 + u * 8);
+      for (int t = 0; t < 2; ++t) ws[t][u] = *reinterpret_cast<const int*>(sc + Tile::SCALES + wid * 1024 + t * 512 + u * 8);
     }
     read_x(xrow + (quad & 1) * Tile::BUFFER, 0);
   };
@@ -572,22 +585,54 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
   // (begin() counts on the loads that a whole quad's steps started.  Those above may
   // be fewer: the compiler leaves out what a short k does not use.)
   moe_wait<0>();
-  int quad = 0;
-  for (; quad < a.steps / 4; ++quad) {
+  int quad = quad0;
+  for (; quad < steps / 4; ++quad) {
     begin(quad);
     step(std::integral_constant<int, 0>(), quad);
     step(std::integral_constant<int, 1>(), quad);
     step(std::integral_constant<int, 2>(), quad);
     step(std::integral_constant<int, 3>(), quad);
   }
-  if (quad < a.quads) {
+  if (quad < quad1) {
     begin(quad);
     step(std::integral_constant<int, 0>(), quad);
     if (quad * 4 + 1 < a.steps) step(std::integral_constant<int, 1>(), quad);
     if (quad * 4 + 2 < a.steps) step(std::integral_constant<int, 2>(), quad);
   }
+  if constexpr (KG > 1)  // (as many barriers as the other groups)
+    for (int i = quad1 - quad0; i < per; ++i) moe_barrier();
   moe_wait<0>();  // no load may still write LDS when it is used again, or the workgroup ends
   moe_barrier();
+  if constexpr (KG > 1) {
+    mx4_f32x4* const part = reinterpret_cast<mx4_f32x4*>(smem0);
+    auto at = [&](int m, int g, int t, int i) { return (((m * (KG - 1) + g) * CW + wid) * 8 + t * 4 + i) * 64 + lane; };
+    #pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m % KG == group) continue;
+      #pragma unroll
+      for (int t = 0; t < 2; ++t)
+        #pragma unroll
+        for (int i = 0; i < 4; ++i)
+          part[at(m, group - (group > m % KG), t, i)] =
+              mx4_f32x4{acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
+    }
+    __syncthreads();
+    #pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m % KG != group) continue;
+      #pragma unroll
+      for (int g = 0; g < KG - 1; ++g)
+        #pragma unroll
+        for (int t = 0; t < 2; ++t)
+          #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const mx4_f32x4 y = part[at(m, g, t, i)];
+            #pragma unroll
+            for (int q = 0; q < 4; ++q) acc[m][t][4 * i + q] += y[q];
+          }
+    }
+    __syncthreads();
+  }
   if (a.bias != nullptr) {
     #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -599,24 +644,24 @@ __device__ __forceinline__ void mx4_many_tile(const Mx4Args& a, const MoeWork& w
         for (int m = 0; m < MT; ++m) acc[m][t][i] += b;
       }
   }
-  mx4_tile_out<MT>(a, acc, smem + wid * kMx4OutBytes, wk.i0, wk.i1, c0, cols_out, lane);
+  mx4_tile_out<MT, KG>(a, acc, smem0 + (group * CW + wid) * kMx4OutBytes, wk.i0, wk.i1, c0, cols_out, lane, group);
 }
 
 // A tile of fewer places than its 32 MT is multiplied as one of fewer 32s.
-template <int MT>
+template <int MT, int CW>
 __global__ void __launch_bounds__(256, 2) mx4_many_kernel(Mx4Args a) {
   extern __shared__ __align__(16) char mx4_smem[];
-  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? kMx4ManyCols / 2 : kMx4ManyCols;
+  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? 32 * CW : 64 * CW;
   MoeWork wk;
   if (!mx4_work<32 * MT>(a, (cols_out + per - 1) / per, wk)) return;
   const int need = (wk.i1 - wk.i0 + 31) / 32;
   if constexpr (MT > 1)
-    if (need == 1) return mx4_many_tile<1>(a, wk, mx4_smem);
+    if (need == 1) return mx4_many_tile<1, CW>(a, wk, mx4_smem);
   if constexpr (MT > 2)
-    if (need == 2) return mx4_many_tile<2>(a, wk, mx4_smem);
+    if (need == 2) return mx4_many_tile<2, CW>(a, wk, mx4_smem);
   if constexpr (MT > 3)
-    if (need == 3) return mx4_many_tile<3>(a, wk, mx4_smem);
-  mx4_many_tile<MT>(a, wk, mx4_smem);
+    if (need == 3) return mx4_many_tile<3, CW>(a, wk, mx4_smem);
+  mx4_many_tile<MT, CW>(a, wk, mx4_smem);
 }
 
 int64_t mx4_grid(const Mx4Args& a, int bm, int bn) {
@@ -638,11 +683,11 @@ hipError_t launch_few(const Mx4Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int MT>
+template <int MT, int CW>
 hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
-  auto* kernel = mx4_many_kernel<MT>;
-  constexpr int bytes = Mx4Tile<MT>::BYTES;
-  const int64_t grid = mx4_grid(a, 32 * MT, kMx4ManyCols);
+  auto* kernel = mx4_many_kernel<MT, CW>;
+  constexpr int bytes = Mx4Tile<MT, CW>::BYTES;
+  const int64_t grid = mx4_grid(a, 32 * MT, 64 * CW);
   if (!moe_grid_fits(grid, 256)) return hipErrorInvalidConfiguration;
   const hipError_t e = ensure_lds((const void*)kernel, bytes);
   if (e != hipSuccess) return e;
@@ -650,41 +695,68 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Which kernel, and how many places a tile.  us of a product alone, 4096 inputs:
-//   16,384 outputs, rows 8, 16, 32, 64: few 8.6, 8.9, 12.4, 21.3; 32 places 10.7, 10.9, 11.1, 11.3
-//   4,096 outputs,  rows 8, 32, 64, 96: few 6.4, 7.2, 7.6, 12.1; 32 places 8.4, 9.1, 9.6, 9.7
-//   128 experts, 1536 x 2048, 4, 8, 16 places each: few 31, 40, 52; 32 places 34, 37, 42
-// so rows of a linear layer go to the first while they make no more than a
-// workgroup a CU, or are one tile of its 16; experts' places up to seven each.
-// Tiles of 32 MT places: a workgroup takes 3 MT + 4 parts of time (its weights, and
-// its places), two of them on a CU twice as long, so what counts is the workgroups
-// of the busiest CU; where there are many, their average.  16,384 outputs, tiles of
-// 32, 64, 96, 128:
-//   rows 128: 12.3, 14.0, 16.0, 19.6;  256: 19.2, 16.1, 17.5, 20.6;  320: 27, 27, 18.3, 20.8
-//   rows 512: 33, 24.8, 27.8, 23.7;   1,024: 67, 45, 43, 39;        2,048: 134, 87, 82, 72
-//   128 experts, 1536 x 2048, 48 places each: 50, 45, 47, 49; 128: 85, 69, 61, 59; 512: 242, 178, 160, 151
-// Experts fill three quarters of a tile more than their places, about.
+// Which kernel, and its tile.  The time of a linear layer is taken as
+//   max(fixed + rounds * quads * a quad's, weights at 5.8 TB/s + what is not hidden)
+// us, a round being a workgroup on each CU (two of them on one take twice as long, and
+// where there are many rounds, what counts is their average).  Measured, products
+// alone, rows as given (f: the kernel for few; places x columns):
+//   n 4,096, k 14,336   f 18.4 to 64; 32 x 256: 25, 32 x 128: 17, 32 x 64: 13 up to 128 rows;
+//                       64 x 128: 23 at 512 rows, 64 x 256: 37 at 1,024, 128 x 256: 63 at 2,048
+//   n 4,096, k 4,096    f 6.9, 8.7, 7.0, 6.4 at 32 rows; 256 rows 10.2, 9.0, 11.2 (32 x 256, 128, 64)
+//   n 1,000, k 8,192    f 11, 15, 9.8, 8.2 at 32 rows; 512 rows 16.7, 11.8, 10.4
+//   n 2,048, k 1,024    f 3.6, 4.8, 4.8, 5.2 at 32 rows
+//   n 16,384, k 4,096   rows 128: 11, 13, 15, 19 (32, 64, 96, 128 places); 320: 27, 26, 17, 21; 512: 35, 25, 28, 23
+//   n 16,384, k 8,192   f 13 to 16 rows, 20 above; 32 x 256, 128, 64: 17, 14, 15 at 16 rows
+// Rows that come as bf16 (few: mx4_needs_rows) only the first kernel takes.
+//
+// Experts have a tile or more each, and so workgroups enough: up to seven places each
+// the first kernel (128 experts, 1536 x 2048, 4, 8, 16 places: 31, 40, 52; 32 places a
+// tile 34, 37, 42), then 256 columns (128 and 64: 41, 54 against 40 at 12 places, 85, 167
+// against 60 at 128) and the places that take the least of rounds x (their
+// part of a quad's time, 3 MT + 4); 48 places each: 50, 45, 47, 49; 128: 85, 69, 61,
+// 59; 512: 242, 178, 160, 151.  They fill three quarters of a tile more than their
+// places, about.
+struct Mx4Shape {
+  int mt, cw;
+  float fixed, quad;  // us: of a launch, of a quad by a round of workgroups
+};
+constexpr Mx4Shape kMx4Shapes[] = {{4, 4, 2.5f, 2.4f}, {3, 4, 2.5f, 1.9f},  {2, 4, 2.5f, 1.35f}, {1, 4, 2.5f, 1.0f},
+                                   {2, 2, 3.5f, 0.85f}, {1, 2, 3.5f, 0.6f}, {1, 1, 3.9f, 0.4f}};
+constexpr float kFewFixed = 2.6f, kFewQuad = 0.56f, kManyHidden = 2.5f, kMx4Rate = 5.8e6f;  // bytes a us
+
+float mx4_rounds(int64_t wgs) { return wgs <= 1024 ? (float)((wgs + 255) / 256) : (float)wgs / 256.f; }
+
 hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
   if (!codes) return launch_few<false>(a, st);
-  const int cols_out = a.swiglu ? a.cols / 2 : a.cols, per = a.swiglu ? kMx4ManyCols / 2 : kMx4ManyCols;
-  const int64_t blocks = (cols_out + per - 1) / per, met = std::min(a.experts, a.places);
-  if (a.offsets != nullptr ? a.places / a.experts < 8
-                           : a.places <= 16 || ((int64_t)a.places + 15) / 16 * ((a.cols + 63) / 64) <= 256)
-    return launch_few<true>(a, st);
-  auto time = [&](int mt) {
-    const int bm = 32 * mt;
-    const int64_t tiles = a.offsets != nullptr ? std::max(met, a.places / bm + met * 3 / 4) : (a.places + bm - 1) / bm;
-    const int64_t wgs = tiles * blocks;
-    return (wgs <= 1024 ? (wgs + 255) / 256 * 256 : wgs) * (3 * mt + 4);
-  };
-  int best = 4;
-  for (int mt = 3; mt >= 1; --mt)
-    if (time(mt) < time(best)) best = mt;
-  switch (best) {
-    case 1: return launch_many<1>(a, st);
-    case 2: return launch_many<2>(a, st);
-    case 3: return launch_many<3>(a, st);
-    default: return launch_many<4>(a, st);
+  Mx4Shape best = {0, 0, 0.f, 0.f};
+  float least = 0.f;
+  if (a.offsets != nullptr) {
+    if (a.places / a.experts < 8) return launch_few<true>(a, st);
+    const int64_t blocks = ((int64_t)a.cols + 255) / 256, met = std::min(a.experts, a.places);
+    for (const Mx4Shape& s : kMx4Shapes) {
+      if (s.cw != 4) continue;
+      const float t = mx4_rounds(std::max(met, a.places / (32 * s.mt) + met * 3 / 4) * blocks) * (float)(3 * s.mt + 4);
+      if (best.mt == 0 || t < least) best = s, least = t;
+    }
+  } else {
+    const float read = (float)a.tiles * 16.f * (float)a.k * (17.f / 32.f) / kMx4Rate;
+    auto rounds = [&](int bm, int bn) {
+      return mx4_rounds(((int64_t)a.places + bm - 1) / bm * (((int64_t)a.cols + bn - 1) / bn)) * (float)a.quads;
+    };
+    for (const Mx4Shape& s : kMx4Shapes) {
+      const float t = std::max(s.fixed + rounds(32 * s.mt, 64 * s.cw) * s.quad, read + kManyHidden);
+      if (best.mt == 0 || t < least) best = s, least = t;
+    }
+    if (std::max(kFewFixed + rounds(16, kFewCols) * kFewQuad, read) < least) return launch_few<true>(a, st);
+  }
+  switch (best.mt * 8 + best.cw) {
+    case 12: return launch_many<1, 4>(a, st);
+    case 20: return launch_many<2, 4>(a, st);
+    case 28: return launch_many<3, 4>(a, st);
+    case 18: return launch_many<2, 2>(a, st);
+    case 10: return launch_many<1, 2>(a, st);
+    case 9: return launch_many<1, 1>(a, st);
+    default: return launch_many<4, 4>(a, st);
   }
 }
 
@@ -700,7 +772,7 @@ bool mx4_needs_rows(int64_t x_rows, int64_t places, int k) {
 // x as a product reads it: "rows" given, bf16 rows as they are when they are
 // few, or "rows" made of them in the workspace.
 int mx4_take_x(const char* name, Mx4Args& a, const void* x, int x_dtype, int64_t x_rows, int64_t x_stride, void* ws,
-               size_t ws_bytes, hipStream_t st, bool& codes) {
+               hipStream_t st, bool& codes) {
   const Mx4Rows L = mx4_rows_layout(x_rows, a.k);
   a.x_rows = (int)x_rows;
   codes = x_dtype == HI_ROCM_DTYPE_MX4 || mx4_needs_rows(x_rows, a.places, a.k);
@@ -796,7 +868,7 @@ int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, c
   a.places = rows;
   a.top_k = 1;
   bool codes;
-  const int rc = mx4_take_x(name, a, x, x_dtype, rows, x_stride, workspace, workspace_bytes, (hipStream_t)stream, codes);
+  const int rc = mx4_take_x(name, a, x, x_dtype, rows, x_stride, workspace, (hipStream_t)stream, codes);
   if (rc != HI_ROCM_OK) return rc;
   const hipError_t e = launch_product(a, codes, (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
@@ -846,8 +918,7 @@ int hi_rocm_mx4_grouped_product(const void* x, int x_dtype, int x_rows, int64_t 
   a.top_k = order ? top_k : 1;
   a.swiglu = swiglu != 0;
   bool codes;
-  const int rc =
-      mx4_take_x(name, a, x, x_dtype, x_rows, x_stride, workspace, workspace_bytes, (hipStream_t)stream, codes);
+  const int rc = mx4_take_x(name, a, x, x_dtype, x_rows, x_stride, workspace, (hipStream_t)stream, codes);
   if (rc != HI_ROCM_OK) return rc;
   const hipError_t e = launch_product(a, codes, (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)

@@ -211,8 +211,8 @@ int hi_rocm_spec_sampled_workspace_bytes(int max_batch, int vocab, size_t* out_b
  * token, then HI_ROCM_SPEC_NO_TOKEN) and out_count i32[batch] (n + 1); no output
  * may overlap an input.  The workspace (16-byte aligned) is zeroed once before its
  * first use and every call leaves it ready for the next, for any smaller batch or
- * vocabulary too, given the same workspace_bytes each time; one stream at a time.  No allocation and no host
- * synchronisation: graph-capturable. */
+ * vocabulary too, given the same workspace_bytes each time; one stream at a time.
+ * No allocation and no host synchronisation: graph-capturable. */
 int hi_rocm_spec_verify_sampled(const void* target_probs, int dtype, int batch, int max_draft, int vocab,
                                 int64_t target_batch_stride, int64_t target_row_stride, const void* draft_probs,
                                 int64_t draft_batch_stride, int64_t draft_row_stride, const uint32_t* draft_tokens,

@@ -172,6 +172,23 @@ def test_tiles(hip, rows, n, k):
         agree(lin(x, dtype=dtype)[r][:, c], y, tol)
 
 
+@pytest.mark.parametrize("k", [1056, 1568, 2048, 2592, 3104, 3680, 4640, 8224])
+@pytest.mark.parametrize("rows,n", [(300, 1001), (300, 2050), (330, 4090), (190, 70), (500, 4001)])
+def test_narrow_tiles(hip, rows, n, k):
+    """Few columns, whose tiles share out k: stretches of different lengths, of no
+    quad, and ones that end inside a quad."""
+    codes, scales = weight(n, k, seed=k)
+    x = torch.randn(rows, k, generator=gen(rows), device="cuda").bfloat16()
+    bias = torch.randn(n, generator=gen(n), device="cuda")
+    lin = Mx4Linear(codes, scales, bias)
+    c = torch.cat((torch.randint(0, n, (200,), generator=gen(1), device="cuda"), torch.arange(n - 70, n, device="cuda"))).unique()
+    r = torch.cat((torch.randint(0, rows, (60,), generator=gen(2), device="cuda"),
+                   torch.arange(rows - 65, rows, device="cuda"))).unique()
+    y, tol = exact(x[r], codes[c], scales[c], bias[c])
+    for dtype in (torch.float32, torch.bfloat16):
+        agree(lin(x, dtype=dtype)[r][:, c], y, tol)
+
+
 @pytest.mark.parametrize("rows,n", [(7, 96), (16, 96), (40, 96), (200, 96), (130, 16384), (520, 16384), (2000, 4096)])
 def test_rows_do_not_mix(hip, rows, n):
     """A row's bits are the same whatever the other rows hold; a row with an
