@@ -577,11 +577,12 @@ int hi_rocm_mx4_workspace_bytes(int x_rows, int places, int k, size_t* out_bytes
 /* out[m][c] = sum_k Q(x[m])[k] * w[c][k] + bias[c], Q the rounding above: x bf16
  * [rows][x_stride] (rows on 16 bytes) or rows (x_dtype HI_ROCM_DTYPE_MX4, x_stride
  * not used); bias f32[n] or NULL; out f32 or bf16 [rows][out_stride].  Sums are f32,
- * products exact.  A row's result does not depend on the other rows' values; a row
- * that holds an infinity or NaN gives NaN; where the magnitudes of a sum's terms pass
- * f32's largest, it may be an infinity or NaN.  The workspace
- * (hi_rocm_mx4_workspace_bytes; NULL where that is 0 or x is rows) is on 16 bytes, needs no
- * initial value and serves one stream at a time.  At most 2^22 rows.  No allocation: graph-capturable. */
+ * products exact.  A row's result does not depend on the other rows' values, but on
+ * their number, which decides how k is split; a row that holds an infinity or NaN
+ * gives NaN; where the magnitudes of a sum's terms pass f32's largest, it may be an
+ * infinity or NaN.  The workspace (hi_rocm_mx4_workspace_bytes; NULL where that is 0
+ * or x is rows) is on 16 bytes, needs no initial value and serves one stream at a
+ * time.  At most 2^22 rows.  No allocation: graph-capturable. */
 int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
                        int n, int k, const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                        size_t workspace_bytes, void* stream);
