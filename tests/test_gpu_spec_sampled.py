@@ -122,6 +122,17 @@ def test_strides_and_alignment(hip, dtype):
     check(one, q, t, u)
 
 
+def test_rows_far_apart(hip):
+    """Requests whose offsets pass 32 bits, in values and in bytes."""
+    B, K, V = 3, 2, 5000
+    p, q, t, u = make(B, K, V, torch.float32, True, seed=21)
+    far = 2 ** 31 + 12
+    place = torch.empty((B - 1) * far + (K + 1) * 6000, device="cuda")
+    vp = place.as_strided((B, K + 1, V), (far, 6000, 1))
+    vp.copy_(p)
+    check(vp, q, t, u)
+
+
 def test_workspace_serves_any_batch(hip):
     """Large and small batches in turn, types mixed: the counters stay ready."""
     plan = SpecVerifier(64, 3, 40000)
