@@ -350,7 +350,10 @@ constexpr int kMx4OutBytes = 8192;  // a wave's, for 32 places of 64 columns
 template <int MT, int CW>
 struct Mx4Tile {
   static constexpr int BM = 32 * MT, KG = 4 / CW;
-  static constexpr int AHEAD = MT > 2 ? 2 : 4;  // steps; more do not fit 256 registers
+  // Steps: more do not fit 256 registers where MT is 3 or 4, and with 4 fewer workgroups of
+  // 32 places share a CU (128 experts, 2048 x 768, 12 and 32 places: 21.4 and 26.4 us, with
+  // 2 20.6 and 24.8).
+  static constexpr int AHEAD = 2;
   static constexpr int CODES = BM * 256, SCALES = CW * 1024;       // bytes of a quad's codes, of 64 CW rows' scales
   static constexpr int BUFFER = CODES + 2 * SCALES;
   static constexpr int ROWS = 4 * CW, L = BM / ROWS + 2;            // of a load, loads a thread and quad
