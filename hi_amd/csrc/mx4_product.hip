@@ -361,9 +361,72 @@ struct Mx4Tile {
   static_assert(64 * CW >= BM, "a row's scales a thread");
 };
 
-// A wave's results by way of its own LDS, 32 places at a time, written out 16
-// bytes a lane, a row's bytes next to each other.  With swiglu half 0 of acc is the
-// gate and half 1 up.
+// 32 places of a wave's results at a time through its own LDS, so that 16 bytes a
+// lane and a row's bytes next to each other are written: all of the 32 places' reads,
+// then all of their stores (a read and its store after another: experts of 256 places,
+// 2048 x 768, 72 us where this takes 65).
+template <int MT, int KG, typename T, int COLS>
+__device__ __forceinline__ void mx4_tile_store(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
+                                               int c0, int cols_out, int lane, int group) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef T vec __attribute__((ext_vector_type(4)));
+  constexpr int ES = sizeof(T), N = 16 / ES;              // values of a chunk
+  constexpr int LANES = COLS / N, ROWS = 64 / LANES;      // lanes of a row, rows at a time
+  const int r = lane & 31, h = lane >> 5, c = lane % LANES, j0 = lane / LANES, col = c0 + c * N;
+  const bool whole = a.out_vec && c0 + COLS <= cols_out;  // (all lanes alike)
+  #pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (m % KG != group) continue;
+    const int first = p0 + m * 32;
+    if (first >= i1) return;
+    // row j of 64 values: the 16-byte chunk c at c ^ (j & 7)
+    #pragma unroll
+    for (int t = 0; t < COLS / 32; ++t)
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const mx4_f32x4 y = {acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
+        const int at = (t * 32 + i * 8 + h * 4) * ES;
+        *reinterpret_cast<vec*>(mem + r * (64 * ES) + (((at >> 4) ^ (r & 7)) << 4 | (at & 15))) =
+            __builtin_convertvector(y, vec);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    u32x4 v[32 / ROWS];
+    #pragma unroll
+    for (int q = 0; q < 32 / ROWS; ++q) {
+      const int j = q * ROWS + j0;
+      v[q] = *reinterpret_cast<const u32x4*>(mem + j * (64 * ES) + (c ^ (j & 7)) * 16);
+    }
+    T* to = (T*)a.out + (int64_t)(first + j0) * a.out_stride + col;
+    const int64_t step = ROWS * a.out_stride;
+    if (whole) {
+      #pragma unroll
+      for (int q = 0; q < 32 / ROWS; ++q, to += step) {
+        if (first + q * ROWS + j0 >= i1) break;
+        // A linear layer's rows past the caches: x and the weights stay there
+        // (8,192 x 4,096 x 16,384: 311 -> 293 us).  The experts' terms are read next
+        // (their sum 4.0 us, past the caches 4.2).
+        if (a.offsets == nullptr) __builtin_nontemporal_store(v[q], reinterpret_cast<u32x4*>(to));
+        else *reinterpret_cast<u32x4*>(to) = v[q];
+      }
+    } else {
+      #pragma unroll
+      for (int q = 0; q < 32 / ROWS; ++q, to += step) {
+        if (first + q * ROWS + j0 >= i1) break;
+        #pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (col + e >= cols_out) break;
+          if constexpr (ES == 2) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(v[q][e >> 1] >> (e & 1) * 16);
+          else reinterpret_cast<uint32_t*>(to)[e] = v[q][e];
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// A wave's results: with swiglu half 0 of acc is the gate and half 1 up.
 template <int MT, int KG>
 __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
                                              int c0, int cols_out, int lane, int group) {
@@ -383,20 +446,22 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
         uint32_t most = 0u;
         #pragma unroll
         for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(acc[m][0][i]) & 0x7fffffffu);
-        most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
-        const uint32_t s = mx4_scale_of(most >> 23);
-        uint32_t mine[2], theirs[2];
+        const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+        const uint32_t s = mx4_scale_of(max((uint32_t)both[0], (uint32_t)both[1]) >> 23);
+        uint32_t mine[2];
         #pragma unroll
         for (int q = 0; q < 2; ++q) {
           float v[8];
           #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = acc[m][0][q * 8 + i];
           mine[q] = mx4_codes(v, s);  // columns 16 q + 4 h .. + 3, then 8 on
-          theirs[q] = (uint32_t)__shfl_xor((int)mine[q], 32, 64);
         }
+        // lane r gets columns 0 .. 15 of the place, lane 32 + r the others: the upper
+        // lanes of the first change places with the lower ones of the second
+        const auto all = __builtin_amdgcn_permlane32_swap(mine[0], mine[1], false, false);
         const int p = p0 + m * 32 + r;
         if (p < i1 && c0 < cols_out) {
-          const uint32_t lo = h ? theirs[1] : mine[0], hi = h ? mine[1] : theirs[0];
+          const uint32_t lo = all[0], hi = all[1];
           uint2 w;
           w.x = (lo & 0xffffu) | hi << 16;
           w.y = lo >> 16 | (hi & 0xffff0000u);
@@ -407,60 +472,12 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
       return;
     }
   }
-  const bool bf16 = a.out_dtype == HI_ROCM_DTYPE_BF16;
-  const int wide = a.swiglu ? 32 : 64;            // columns of a row
-  const int es = bf16 ? 2 : 4, n = 16 / es;       // bytes of a value, values of a chunk
-  const int lanes = wide / n, rows = 64 / lanes;  // lanes of a row, rows at a time
-  const int c = lane % lanes, col = c0 + c * n;
-  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-  #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    if (m % KG != group) continue;
-    if (p0 + m * 32 >= i1) return;
-    // row j of 64 values: the 16-byte chunk c at c ^ (j & 7)
-    #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const mx4_f32x4 y = {acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
-        if (bf16)
-          *reinterpret_cast<bf16x4*>(mem + r * 128 + ((t * 4 + i) ^ (r & 7)) * 16 + h * 8) =
-              __builtin_convertvector(y, bf16x4);
-        else
-          *reinterpret_cast<mx4_f32x4*>(mem + r * 256 + ((t * 8 + i * 2 + h) ^ (r & 7)) * 16) = y;
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    #pragma unroll 1
-    for (int j = lane / lanes; j < 32; j += rows) {
-      const int p = p0 + m * 32 + j;
-      if (p >= i1) break;
-      const uint4 v = *reinterpret_cast<const uint4*>(mem + j * (64 * es) + (c ^ (j & 7)) * 16);
-      char* to = (char*)a.out + ((int64_t)p * a.out_stride + col) * es;
-      if (col + n <= cols_out && a.out_vec) {
-        // A linear layer's rows past the caches: x and the weights stay there
-        // (8,192 x 4,096 x 16,384: 311 -> 293 us).  The experts' terms are read next
-        // (their sum 4.0 us, past the caches 4.2).
-        if (a.offsets == nullptr) {
-          typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-          const u32x4 line = {v.x, v.y, v.z, v.w};
-          __builtin_nontemporal_store(line, reinterpret_cast<u32x4*>(to));
-        } else {
-          *reinterpret_cast<uint4*>(to) = v;
-        }
-      } else {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (q >= n || col + q >= cols_out) break;
-          if (bf16) ((uint16_t*)to)[q] = (uint16_t)(w[q >> 1] >> (q & 1) * 16);
-          else ((uint32_t*)to)[q] = w[q & 3];
-        }
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
+  if (a.out_dtype == HI_ROCM_DTYPE_BF16) {
+    if (a.swiglu) mx4_tile_store<MT, KG, __bf16, 32>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+    else mx4_tile_store<MT, KG, __bf16, 64>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+  } else {
+    if (a.swiglu) mx4_tile_store<MT, KG, float, 32>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+    else mx4_tile_store<MT, KG, float, 64>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
   }
 }
 
