@@ -365,7 +365,10 @@ struct Mx4Tile {
 // lane and a row's bytes next to each other are written: all of the 32 places' reads,
 // then all of their stores (a read and its store after another: experts of 256 places,
 // 2048 x 768, 72 us where this takes 65).
-template <int MT, int KG, typename T, int COLS>
+// PAST: rows past the caches.  A linear layer's, whose x and weights then stay there
+// (8,192 x 4,096 x 16,384: 307 -> 293 us); the experts' terms are read next (their sum
+// 4.0 us, past the caches 4.2).
+template <int MT, int KG, typename T, int COLS, bool PAST>
 __device__ __forceinline__ void mx4_tile_store(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
                                                int c0, int cols_out, int lane, int group) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -404,10 +407,7 @@ __device__ __forceinline__ void mx4_tile_store(const Mx4Args& a, mx4_f32x16 (&ac
       #pragma unroll
       for (int q = 0; q < 32 / ROWS; ++q, to += step) {
         if (first + q * ROWS + j0 >= i1) break;
-        // A linear layer's rows past the caches: x and the weights stay there
-        // (8,192 x 4,096 x 16,384: 311 -> 293 us).  The experts' terms are read next
-        // (their sum 4.0 us, past the caches 4.2).
-        if (a.offsets == nullptr) __builtin_nontemporal_store(v[q], reinterpret_cast<u32x4*>(to));
+        if constexpr (PAST) __builtin_nontemporal_store(v[q], reinterpret_cast<u32x4*>(to));
         else *reinterpret_cast<u32x4*>(to) = v[q];
       }
     } else {
@@ -472,13 +472,14 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
       return;
     }
   }
-  if (a.out_dtype == HI_ROCM_DTYPE_BF16) {
-    if (a.swiglu) mx4_tile_store<MT, KG, __bf16, 32>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
-    else mx4_tile_store<MT, KG, __bf16, 64>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
-  } else {
-    if (a.swiglu) mx4_tile_store<MT, KG, float, 32>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
-    else mx4_tile_store<MT, KG, float, 64>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
-  }
+  auto store = [&](auto type) {
+    using T = decltype(type);
+    if (a.swiglu) mx4_tile_store<MT, KG, T, 32, false>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+    else if (a.offsets != nullptr) mx4_tile_store<MT, KG, T, 64, false>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+    else mx4_tile_store<MT, KG, T, 64, true>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+  };
+  if (a.out_dtype == HI_ROCM_DTYPE_BF16) store(__bf16());
+  else store(float());
 }
 
 template <int MT, int CW>
