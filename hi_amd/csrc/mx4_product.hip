@@ -87,14 +87,6 @@ __device__ __forceinline__ int mx4_row(const Mx4Args& a, int pair) {
   return min(max(row, 0), a.x_rows - 1);
 }
 
-// silu(g) * u on its way to 4 bits: exp(-g) as 2^(-g log2 e), off by |g| 2^-24 for the
-// product's rounding, which is less than the sums behind g are off, and beside a
-// rounding to 2^-2 moves a value only from next to a border (moe_silu_mul's
-// correction costs 3 of 183 us, 4,096 tokens x 8 of 128 experts).
-__device__ __forceinline__ float mx4_silu_mul(float g, float u) {
-  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269502e+00f)) * u;
-}
-
 // Four columns c .. c + 3 of place p.
 __device__ __forceinline__ void mx4_store(const Mx4Args& a, int p, int c, int cols_out, const mx4_f32x4& y) {
   const int64_t at = (int64_t)p * a.out_stride + c;
@@ -291,15 +283,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, 6) mx4_few_kernel(Mx4Args a) {
   const int p = wk.i0 + r;
   if (a.swiglu) {  // two tiles of gate and two of up: a block of codes
     if (wid > 0 || c0 >= cols_out) return;
-    const bool codes = a.out_dtype == HI_ROCM_DTYPE_MX4;
     mx4_f32x4 y[2];
     #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const mx4_f32x4 gate = total(t), up = total(NT / 2 + t);
       #pragma unroll
-      for (int q = 0; q < 4; ++q) y[t][q] = codes ? mx4_silu_mul(gate[q], up[q]) : moe_silu_mul(gate[q], up[q]);
+      for (int q = 0; q < 4; ++q) y[t][q] = moe_silu_mul(gate[q], up[q]);
     }
-    if (codes) {
+    if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
       mx4_store_codes(a, p, p < wk.i1, c0, g, y[0], y[1]);
     } else if (p < wk.i1) {
       #pragma unroll
@@ -440,16 +431,14 @@ template <int MT, int KG>
 __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
                                              int c0, int cols_out, int lane, int group) {
   const int r = lane & 31, h = lane >> 5;
-  const bool codes = a.out_dtype == HI_ROCM_DTYPE_MX4;
   if (a.swiglu) {
     #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (m % KG != group) continue;
       #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        acc[m][0][i] = codes ? mx4_silu_mul(acc[m][0][i], acc[m][1][i]) : moe_silu_mul(acc[m][0][i], acc[m][1][i]);
+      for (int i = 0; i < 16; ++i) acc[m][0][i] = moe_silu_mul(acc[m][0][i], acc[m][1][i]);
     }
-    if (codes) {
+    if (a.out_dtype == HI_ROCM_DTYPE_MX4) {
       // the 32 columns are a block; a place's other half is lane ^ 32's
       #pragma unroll
       for (int m = 0; m < MT; ++m) {
