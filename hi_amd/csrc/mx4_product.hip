@@ -19,6 +19,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "hi_rocm.h"
@@ -735,46 +736,42 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
 //   n 16,384, k 8,192   f 13 to 16 rows, 20 above; 32 x 256, 128, 64: 17, 14, 15 at 16 rows
 // Rows that come as bf16 (few: mx4_needs_rows) only the first kernel takes.
 //
-// Experts have a tile or more each, and so workgroups enough: up to seven places each
-// the first kernel (128 experts, 1536 x 2048, 4, 8, 16 places: 31, 40, 52; 32 places a
-// tile 34, 37, 42), then 256 columns (128 and 64: 41, 54 against 40 at 12 places, 85, 167
-// against 60 at 128) and the places that take the least of rounds x (their
-// part of a quad's time, 3 MT + 4); 48 places each: 50, 45, 47, 49; 128: 85, 69, 61,
-// 59; 512: 242, 178, 160, 151.  They fill three quarters of a tile more than their
-// places, about.
+// Experts with up to seven places each the first kernel always takes (128 experts, 1536 x
+// 2048, 4, 8, 16 places: 31, 40, 52; 32 places a tile 34, 37, 42).  Of more the places are
+// known on the device alone: experts are taken to fill three quarters of a tile more than
+// their places, and rounds that are not whole to cost a half more.
+//   128 experts, 1536 x 2048, 48 places each: 50, 45, 47, 49 (32 to 128 places x 256);
+//     128: 85, 69, 61, 59; 512: 242, 178, 160, 151
+//   8 experts, 2048 x 4096, 24 places: 11.6, 10.2, 11.9 (32 x 256, 128, 64); f 12.7
+//   60 experts, 1408 x 1440, 48 places: 15.9, 15.8, 18.4 (32, 64, 96 x 256); f 29
 struct Mx4Shape {
   int mt, cw;
   float fixed, quad;  // us: of a launch, of a quad by a round of workgroups
 };
-constexpr Mx4Shape kMx4Shapes[] = {{4, 4, 2.5f, 2.4f}, {3, 4, 2.5f, 1.9f},  {2, 4, 2.5f, 1.35f}, {1, 4, 2.5f, 1.0f},
-                                   {2, 2, 3.5f, 0.85f}, {1, 2, 3.5f, 0.6f}, {1, 1, 3.9f, 0.4f}};
+constexpr Mx4Shape kMx4Shapes[] = {{4, 4, 2.5f, 2.29f}, {3, 4, 2.5f, 1.86f}, {2, 4, 2.5f, 1.43f}, {1, 4, 2.5f, 1.0f},
+                                   {2, 2, 3.5f, 0.85f}, {1, 2, 3.5f, 0.6f},  {1, 1, 3.9f, 0.4f}};
 constexpr float kFewFixed = 2.6f, kFewQuad = 0.56f, kManyHidden = 2.5f, kMx4Rate = 5.8e6f;  // bytes a us
-
-float mx4_rounds(int64_t wgs) { return wgs <= 1024 ? (float)((wgs + 255) / 256) : (float)wgs / 256.f; }
 
 hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
   if (!codes) return launch_few<false>(a, st);
+  const bool grouped = a.offsets != nullptr;
+  if (grouped && a.places / a.experts < 8) return launch_few<true>(a, st);
+  const float read = grouped ? 0.f : (float)a.tiles * 16.f * (float)a.k * (17.f / 32.f) / kMx4Rate;
+  auto rounds = [&](int bm, int bn) {
+    const int64_t met = std::min(a.experts, a.places);
+    const int64_t tiles = grouped ? std::max(met, a.places / bm + met * 3 / 4) : ((int64_t)a.places + bm - 1) / bm;
+    const int64_t wgs = tiles * (((int64_t)a.cols + bn - 1) / bn);
+    if (wgs <= 256) return (float)a.quads;
+    const float r = (float)wgs / 256.f;
+    return (float)a.quads * (grouped ? r + 0.5f : wgs <= 1024 ? std::ceil(r) : r);
+  };
   Mx4Shape best = {0, 0, 0.f, 0.f};
   float least = 0.f;
-  if (a.offsets != nullptr) {
-    if (a.places / a.experts < 8) return launch_few<true>(a, st);
-    const int64_t blocks = ((int64_t)a.cols + 255) / 256, met = std::min(a.experts, a.places);
-    for (const Mx4Shape& s : kMx4Shapes) {
-      if (s.cw != 4) continue;
-      const float t = mx4_rounds(std::max(met, a.places / (32 * s.mt) + met * 3 / 4) * blocks) * (float)(3 * s.mt + 4);
-      if (best.mt == 0 || t < least) best = s, least = t;
-    }
-  } else {
-    const float read = (float)a.tiles * 16.f * (float)a.k * (17.f / 32.f) / kMx4Rate;
-    auto rounds = [&](int bm, int bn) {
-      return mx4_rounds(((int64_t)a.places + bm - 1) / bm * (((int64_t)a.cols + bn - 1) / bn)) * (float)a.quads;
-    };
-    for (const Mx4Shape& s : kMx4Shapes) {
-      const float t = std::max(s.fixed + rounds(32 * s.mt, 64 * s.cw) * s.quad, read + kManyHidden);
-      if (best.mt == 0 || t < least) best = s, least = t;
-    }
-    if (std::max(kFewFixed + rounds(16, kFewCols) * kFewQuad, read) < least) return launch_few<true>(a, st);
+  for (const Mx4Shape& s : kMx4Shapes) {
+    const float t = std::max(s.fixed + rounds(32 * s.mt, 64 * s.cw) * s.quad, read + kManyHidden);
+    if (best.mt == 0 || t < least) best = s, least = t;
   }
+  if (std::max(kFewFixed + rounds(16, kFewCols) * kFewQuad, read) < least) return launch_few<true>(a, st);
   switch (best.mt * 8 + best.cw) {
     case 12: return launch_many<1, 4>(a, st);
     case 20: return launch_many<2, 4>(a, st);

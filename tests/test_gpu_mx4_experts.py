@@ -82,7 +82,12 @@ SIZES = [(1, 1, 1, 32, 32), (1, 4, 2, 64, 32), (5, 8, 2, 96, 64), (16, 3, 3, 160
          (64, 7, 2, 544, 96), (200, 16, 4, 512, 224), (300, 4, 2, 1184, 352), (700, 8, 4, 256, 128)]
 
 
-@pytest.mark.parametrize("T,E,K,H,I", SIZES)
+# Few experts with some places each: narrow tiles that share a long k out, larger tiles
+NARROW = [(30, 8, 4, 2080, 1056), (26, 4, 2, 1568, 96), (50, 5, 3, 4640, 64), (90, 16, 2, 1440, 1536), (9, 1, 1, 3680, 544),
+          (120, 8, 4, 1056, 2592), (460, 2, 2, 608, 1056), (135, 16, 2, 32, 1920), (280, 16, 3, 32, 1728)]
+
+
+@pytest.mark.parametrize("T,E,K,H,I", SIZES + NARROW)
 @pytest.mark.parametrize("none", [0.0, 0.3])
 def test_products(hip, T, E, K, H, I, none):
     """Both products on their own: gathered bf16 rows, rows in the groups' order,
@@ -126,7 +131,7 @@ def test_products(hip, T, E, K, H, I, none):
     assert (s[n:] == 0xA5).all()
 
 
-@pytest.mark.parametrize("T,E,K,H,I", SIZES)
+@pytest.mark.parametrize("T,E,K,H,I", SIZES + NARROW)
 @pytest.mark.parametrize("none", [0.0, 0.3])
 def test_layer(hip, T, E, K, H, I, none):
     K = min(K, E)
