@@ -734,7 +734,7 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
 //   n 2,048, k 1,024    f 3.6, 4.8, 4.8, 5.2 at 32 rows
 //   n 16,384, k 4,096   rows 128: 11, 13, 15, 19 (32, 64, 96, 128 places); 320: 27, 26, 17, 21; 512: 35, 25, 28, 23
 //   n 16,384, k 8,192   f 13 to 16 rows, 20 above; 32 x 256, 128, 64: 17, 14, 15 at 16 rows
-// Rows that come as bf16 (few: mx4_needs_rows) only the first kernel takes.
+// Rows that come as bf16 only the first kernel takes (mx4_needs_rows, mx4_round_on_the_way).
 //
 // Experts with up to seven places each the first kernel always takes (128 experts, 1536 x
 // 2048, 4, 8, 16 places: 31, 40, 52; 32 places a tile 34, 37, 42).  Of more the places are
@@ -752,27 +752,53 @@ constexpr Mx4Shape kMx4Shapes[] = {{4, 4, 2.5f, 2.29f}, {3, 4, 2.5f, 1.86f}, {2,
                                    {2, 2, 3.5f, 0.85f}, {1, 2, 3.5f, 0.6f},  {1, 1, 3.9f, 0.4f}};
 constexpr float kFewFixed = 2.6f, kFewQuad = 0.56f, kManyHidden = 2.5f, kMx4Rate = 5.8e6f;  // bytes a us
 
+// Quads of k by rounds of workgroups of bm places by bn columns.
+float mx4_rounds(const Mx4Args& a, int bm, int bn) {
+  const bool grouped = a.offsets != nullptr;
+  const int64_t met = std::min(a.experts, a.places);
+  const int64_t tiles = grouped ? std::max(met, a.places / bm + met * 3 / 4) : ((int64_t)a.places + bm - 1) / bm;
+  const int64_t wgs = tiles * (((int64_t)a.cols + bn - 1) / bn);
+  if (wgs <= 256) return (float)a.quads;
+  const float r = (float)wgs / 256.f;
+  return (float)a.quads * (grouped ? r + 0.5f : wgs <= 1024 ? std::ceil(r) : r);
+}
+
+struct Mx4Choice {
+  Mx4Shape shape;  // mt 0: the kernel for few
+  float us;
+};
+Mx4Choice mx4_choose(const Mx4Args& a) {
+  const Mx4Shape few = {0, 1, kFewFixed, kFewQuad};
+  const bool grouped = a.offsets != nullptr;
+  if (grouped && a.places / a.experts < 8) return {few, 0.f};
+  const float read = grouped ? 0.f : (float)a.tiles * 16.f * (float)a.k * (17.f / 32.f) / kMx4Rate;
+  Mx4Choice best = {kMx4Shapes[0], INFINITY};
+  for (const Mx4Shape& s : kMx4Shapes) {
+    const float t = std::max(s.fixed + mx4_rounds(a, 32 * s.mt, 64 * s.cw) * s.quad, read + kManyHidden);
+    if (t < best.us) best = {s, t};
+  }
+  const float t = std::max(few.fixed + mx4_rounds(a, 16, kFewCols) * few.quad, read);
+  if (t < best.us) best = {few, t};
+  return best;
+}
+
+// Whether more bf16 rows than 16 (up to 4,096 inputs: mx4_few_kernel's LDS) are rounded by
+// the workgroups that multiply them rather than beforehand, which is another launch of
+// 2.5 us: theirs take 2.8 + 0.7 a quad and round, and x from the L2s at 20 TB/s.  17 to 64
+// rows, us in a graph (eagerly another 4 for the second launch): 512 x 512 3.3 against 5.5, 2,048
+// x 1,024 4.2 and 6.3, 8,192 x 1,024 4.2 to 5.6 and 6.4 to 7.2, 4,096 x 2,048 5.7 and 7.5;
+// 4,096 x 4,096 17 rows 8.9 and 9.8, 64 rows 10.8 and 9.9; 32,000 x 1,024 64 rows 13.5 and 9.8.
+bool mx4_round_on_the_way(const Mx4Args& a) {
+  if (a.offsets != nullptr || a.k > 4096) return false;
+  const float wgs = (float)(((int64_t)a.places + 15) / 16 * (((int64_t)a.cols + kFewCols - 1) / kFewCols));
+  return 2.8f + mx4_rounds(a, 16, kFewCols) * 0.7f + wgs * 32.f * (float)a.k / 20e6f < mx4_choose(a).us + 2.5f;
+}
+
 hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
   if (!codes) return launch_few<false>(a, st);
-  const bool grouped = a.offsets != nullptr;
-  if (grouped && a.places / a.experts < 8) return launch_few<true>(a, st);
-  const float read = grouped ? 0.f : (float)a.tiles * 16.f * (float)a.k * (17.f / 32.f) / kMx4Rate;
-  auto rounds = [&](int bm, int bn) {
-    const int64_t met = std::min(a.experts, a.places);
-    const int64_t tiles = grouped ? std::max(met, a.places / bm + met * 3 / 4) : ((int64_t)a.places + bm - 1) / bm;
-    const int64_t wgs = tiles * (((int64_t)a.cols + bn - 1) / bn);
-    if (wgs <= 256) return (float)a.quads;
-    const float r = (float)wgs / 256.f;
-    return (float)a.quads * (grouped ? r + 0.5f : wgs <= 1024 ? std::ceil(r) : r);
-  };
-  Mx4Shape best = {0, 0, 0.f, 0.f};
-  float least = 0.f;
-  for (const Mx4Shape& s : kMx4Shapes) {
-    const float t = std::max(s.fixed + rounds(32 * s.mt, 64 * s.cw) * s.quad, read + kManyHidden);
-    if (best.mt == 0 || t < least) best = s, least = t;
-  }
-  if (std::max(kFewFixed + rounds(16, kFewCols) * kFewQuad, read) < least) return launch_few<true>(a, st);
-  switch (best.mt * 8 + best.cw) {
+  const Mx4Shape s = mx4_choose(a).shape;
+  switch (s.mt * 8 + s.cw) {
+    case 1: return launch_few<true>(a, st);
     case 12: return launch_many<1, 4>(a, st);
     case 20: return launch_many<2, 4>(a, st);
     case 28: return launch_many<3, 4>(a, st);
@@ -787,7 +813,7 @@ bool mx4_float(int d) { return d == HI_ROCM_DTYPE_F32 || d == HI_ROCM_DTYPE_BF16
 int mx4_size(int d) { return d == HI_ROCM_DTYPE_F32 ? 4 : 2; }
 
 // Few bf16 rows are rounded by each workgroup in LDS, at most 16 of them and 65,536
-// values (36 KB); more, beforehand in a workspace.
+// values (36 KB); more need a workspace, in which they may be rounded beforehand.
 bool mx4_needs_rows(int64_t x_rows, int64_t places, int k) {
   return x_rows > 16 || std::min<int64_t>(places, 16) * k > 65536;
 }
@@ -798,7 +824,7 @@ int mx4_take_x(const char* name, Mx4Args& a, const void* x, int x_dtype, int64_t
                hipStream_t st, bool& codes) {
   const Mx4Rows L = mx4_rows_layout(x_rows, a.k);
   a.x_rows = (int)x_rows;
-  codes = x_dtype == HI_ROCM_DTYPE_MX4 || mx4_needs_rows(x_rows, a.places, a.k);
+  codes = x_dtype == HI_ROCM_DTYPE_MX4 || (mx4_needs_rows(x_rows, a.places, a.k) && !mx4_round_on_the_way(a));
   if (!codes) {
     a.x = (const uint8_t*)x;
     a.x_stride = x_stride * 2;
