@@ -813,18 +813,23 @@ bool mx4_float(int d) { return d == HI_ROCM_DTYPE_F32 || d == HI_ROCM_DTYPE_BF16
 int mx4_size(int d) { return d == HI_ROCM_DTYPE_F32 ? 4 : 2; }
 
 // Few bf16 rows are rounded by each workgroup in LDS, at most 16 of them and 65,536
-// values (36 KB); more need a workspace, in which they may be rounded beforehand.
+// values (36 KB); more, beforehand in a workspace, but for mx4_round_on_the_way.
 bool mx4_needs_rows(int64_t x_rows, int64_t places, int k) {
   return x_rows > 16 || std::min<int64_t>(places, 16) * k > 65536;
 }
 
+// A linear layer's rows: the weight and the number of rows are in `a`.
+bool mx4_linear_needs_rows(const Mx4Args& a) {
+  return mx4_needs_rows(a.places, a.places, a.k) && !mx4_round_on_the_way(a);
+}
+
 // x as a product reads it: "rows" given, bf16 rows as they are when they are
 // few, or "rows" made of them in the workspace.
-int mx4_take_x(const char* name, Mx4Args& a, const void* x, int x_dtype, int64_t x_rows, int64_t x_stride, void* ws,
-               hipStream_t st, bool& codes) {
+int mx4_take_x(const char* name, Mx4Args& a, const void* x, int x_dtype, int64_t x_rows, int64_t x_stride, bool needs,
+               void* ws, hipStream_t st, bool& codes) {
   const Mx4Rows L = mx4_rows_layout(x_rows, a.k);
   a.x_rows = (int)x_rows;
-  codes = x_dtype == HI_ROCM_DTYPE_MX4 || (mx4_needs_rows(x_rows, a.places, a.k) && !mx4_round_on_the_way(a));
+  codes = x_dtype == HI_ROCM_DTYPE_MX4 || needs;
   if (!codes) {
     a.x = (const uint8_t*)x;
     a.x_stride = x_stride * 2;
@@ -848,9 +853,9 @@ int mx4_fail(int status, const char* name, const char* what) {
   return api_fail(status, text);
 }
 
-// What both products check of x and the weight.
+// What both products check of x, the weight and the workspace.
 int mx4_check(const char* name, const void* x, int x_dtype, int64_t x_rows, int64_t x_stride, const void* packed,
-              size_t packed_bytes, int places, int experts, int n, int k, const void* ws, size_t ws_bytes) {
+              size_t packed_bytes, int experts, int n, int k) {
   if (x == nullptr || packed == nullptr || x_rows <= 0 || n <= 0 || k <= 0 || experts <= 0 ||
       (x_dtype != HI_ROCM_DTYPE_BF16 && x_dtype != HI_ROCM_DTYPE_MX4) || (x_dtype == HI_ROCM_DTYPE_BF16 && x_stride < k))
     return mx4_fail(HI_ROCM_ERR_ARGS, name, "invalid arguments");
@@ -861,7 +866,10 @@ int mx4_check(const char* name, const void* x, int x_dtype, int64_t x_rows, int6
     return mx4_fail(HI_ROCM_ERR_ARGS, name, "packed not on 16 bytes, or too small (hi_rocm_mx4_packed_bytes)");
   if ((uintptr_t)x % 16 != 0 || (x_dtype == HI_ROCM_DTYPE_BF16 && x_stride % 8 != 0))
     return mx4_fail(HI_ROCM_ERR_UNSUPPORTED, name, "needs rows that start on 16 bytes");
-  if (x_dtype == HI_ROCM_DTYPE_BF16 && mx4_needs_rows(x_rows, places, k) &&
+  return HI_ROCM_OK;
+}
+int mx4_check_workspace(const char* name, int x_dtype, bool needs, int64_t x_rows, int k, const void* ws, size_t ws_bytes) {
+  if (x_dtype == HI_ROCM_DTYPE_BF16 && needs &&
       (ws == nullptr || (uintptr_t)ws % 16 != 0 || ws_bytes < mx4_rows_layout(x_rows, k).total))
     return mx4_fail(HI_ROCM_ERR_ARGS, name, "workspace not on 16 bytes, or too small (hi_rocm_mx4_workspace_bytes)");
   return HI_ROCM_OK;
@@ -896,12 +904,26 @@ int hi_rocm_mx4_workspace_bytes(int x_rows, int places, int k, size_t* out_bytes
   return HI_ROCM_OK;
 }
 
+int hi_rocm_mx4_linear_workspace_bytes(int rows, int n, int k, size_t* out_bytes) {
+  if (rows <= 0 || n <= 0 || k <= 0 || out_bytes == nullptr)
+    return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_mx4_linear_workspace_bytes: invalid arguments");
+  if (!mx4_weight_fits(1, n, k) || rows > HI_ROCM_MX4_MAX_ROWS)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED,
+                    "hi_rocm_mx4_linear_workspace_bytes: needs k a multiple of 32 up to 2^24, at most 2^24 outputs, 2^35 "
+                    "weights, 2^22 rows");
+  Mx4Args a;
+  memset(&a, 0, sizeof(a));
+  mx4_take_weight(a, nullptr, 1, n, k);
+  a.places = rows;
+  *out_bytes = mx4_linear_needs_rows(a) ? mx4_rows_layout(rows, k).total : 0;
+  return HI_ROCM_OK;
+}
+
 int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
                        int n, int k, const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                        size_t workspace_bytes, void* stream) {
   const char* name = "hi_rocm_mx4_linear";
-  const int bad = mx4_check(name, x, x_dtype, rows, x_stride, packed, packed_bytes, rows, 1, n, k, workspace,
-                            workspace_bytes);
+  int bad = mx4_check(name, x, x_dtype, rows, x_stride, packed, packed_bytes, 1, n, k);
   if (bad != HI_ROCM_OK) return bad;
   if (out == nullptr || !mx4_float(out_dtype) || out_stride < n || (uintptr_t)out % mx4_size(out_dtype) != 0 ||
       (uintptr_t)bias % 4 != 0)
@@ -909,15 +931,18 @@ int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, c
   Mx4Args a;
   memset(&a, 0, sizeof(a));
   mx4_take_weight(a, packed, 1, n, k);
+  a.places = rows;
+  const bool needs = mx4_linear_needs_rows(a);
+  bad = mx4_check_workspace(name, x_dtype, needs, rows, k, workspace, workspace_bytes);
+  if (bad != HI_ROCM_OK) return bad;
   a.bias = bias;
   a.out = out;
   a.out_stride = out_stride;
   a.out_dtype = out_dtype;
   a.out_vec = (uintptr_t)out % 16 == 0 && out_stride * mx4_size(out_dtype) % 16 == 0;
-  a.places = rows;
   a.top_k = 1;
   bool codes;
-  const int rc = mx4_take_x(name, a, x, x_dtype, rows, x_stride, workspace, (hipStream_t)stream, codes);
+  const int rc = mx4_take_x(name, a, x, x_dtype, rows, x_stride, needs, workspace, (hipStream_t)stream, codes);
   if (rc != HI_ROCM_OK) return rc;
   const hipError_t e = launch_product(a, codes, (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
@@ -931,9 +956,10 @@ int hi_rocm_mx4_grouped_product(const void* x, int x_dtype, int x_rows, int64_t 
                                 int64_t out_stride, size_t out_bytes, void* workspace, size_t workspace_bytes,
                                 void* stream) {
   const char* name = "hi_rocm_mx4_grouped_product";
-  const int bad =
-      mx4_check(name, x, x_dtype, x_rows, x_stride, packed, packed_bytes, places, experts, cols, k, workspace,
-                workspace_bytes);
+  int bad = mx4_check(name, x, x_dtype, x_rows, x_stride, packed, packed_bytes, experts, cols, k);
+  if (bad != HI_ROCM_OK) return bad;
+  const bool needs = mx4_needs_rows(x_rows, places, k);
+  bad = mx4_check_workspace(name, x_dtype, needs, x_rows, k, workspace, workspace_bytes);
   if (bad != HI_ROCM_OK) return bad;
   const int wide = swiglu ? cols / 2 : cols;
   const bool to_rows = out_dtype == HI_ROCM_DTYPE_MX4;
@@ -967,7 +993,7 @@ int hi_rocm_mx4_grouped_product(const void* x, int x_dtype, int x_rows, int64_t 
   a.top_k = order ? top_k : 1;
   a.swiglu = swiglu != 0;
   bool codes;
-  const int rc = mx4_take_x(name, a, x, x_dtype, x_rows, x_stride, workspace, (hipStream_t)stream, codes);
+  const int rc = mx4_take_x(name, a, x, x_dtype, x_rows, x_stride, needs, workspace, (hipStream_t)stream, codes);
   if (rc != HI_ROCM_OK) return rc;
   const hipError_t e = launch_product(a, codes, (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)

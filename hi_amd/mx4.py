@@ -181,7 +181,7 @@ class Mx4Linear:
         if code_x == DTYPE_BF16:
             work_bytes = self._work.get(rows)
             if work_bytes is None:
-                work_bytes = self._work[rows] = _size(load().hi_rocm_mx4_workspace_bytes, rows, rows, k)
+                work_bytes = self._work[rows] = _size(load().hi_rocm_mx4_linear_workspace_bytes, rows, n, k)
             if work_bytes:  # a call's own: calls on several streams, or captured ones, share nothing
                 work = _empty((work_bytes,), _BYTE, self.packed.device, stream)
         # (a single row's stride says nothing)

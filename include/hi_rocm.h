@@ -571,8 +571,10 @@ int hi_rocm_mx4_pack(const uint8_t* codes, const uint8_t* scales, int experts, i
 
 /* Bytes of the workspace that the products below need for bf16 x: 0 where the rows
  * are few enough to be rounded on the way, else those of hi_rocm_mx4_rows.  places:
- * the rows of a linear layer, tokens * top_k of a grouped product. */
+ * tokens * top_k of a grouped product, the rows of a linear layer; a linear layer of
+ * n outputs may need none of it (hi_rocm_mx4_linear_workspace_bytes). */
 int hi_rocm_mx4_workspace_bytes(int x_rows, int places, int k, size_t* out_bytes);
+int hi_rocm_mx4_linear_workspace_bytes(int rows, int n, int k, size_t* out_bytes);
 
 /* out[m][c] = sum_k Q(x[m])[k] * w[c][k] + bias[c], Q the rounding above: x bf16
  * [rows][x_stride] (rows on 16 bytes) or rows (x_dtype HI_ROCM_DTYPE_MX4, x_stride
@@ -580,7 +582,7 @@ int hi_rocm_mx4_workspace_bytes(int x_rows, int places, int k, size_t* out_bytes
  * products exact.  A row's result does not depend on the other rows' values, but on
  * their number, which decides how k is split; a row that holds an infinity or NaN
  * gives NaN; where the magnitudes of a sum's terms pass f32's largest, it may be an
- * infinity or NaN.  The workspace (hi_rocm_mx4_workspace_bytes; NULL where that is 0
+ * infinity or NaN.  The workspace (of either call's bytes; NULL where those are 0
  * or x is rows) is on 16 bytes, needs no initial value and serves one stream at a
  * time.  At most 2^22 rows.  No allocation: graph-capturable. */
 int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,

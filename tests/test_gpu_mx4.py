@@ -189,6 +189,23 @@ def test_narrow_tiles(hip, rows, n, k):
         agree(lin(x, dtype=dtype)[r][:, c], y, tol)
 
 
+@pytest.mark.parametrize("k", [32, 160, 512, 1184, 2080, 4096])
+@pytest.mark.parametrize("rows,n", [(17, 48), (40, 1000), (100, 130), (500, 65), (1999, 48), (64, 2048), (30, 8190)])
+def test_more_rows_without_a_workspace(hip, rows, n, k):
+    """Rows rounded by the workgroups that multiply them, whatever their number: the
+    result of rows rounded beforehand, up to the order of the sums."""
+    codes, scales = weight(n, k, seed=n + k)
+    x = torch.randn(rows, k, generator=gen(rows), device="cuda").bfloat16()
+    bias = torch.randn(n, generator=gen(n), device="cuda")
+    lin = Mx4Linear(codes, scales, bias)
+    r = torch.cat((torch.randint(0, rows, (40,), generator=gen(2), device="cuda"),
+                   torch.arange(max(rows - 20, 0), rows, device="cuda"))).unique()
+    y, tol = exact(x[r], codes, scales, bias)
+    for given in (x, mx4_rows(x)):
+        for dtype in (torch.float32, torch.bfloat16):
+            agree(lin(given, dtype=dtype)[r], y, tol)
+
+
 @pytest.mark.parametrize("rows,n", [(7, 96), (16, 96), (40, 96), (200, 96), (130, 16384), (520, 16384), (2000, 4096)])
 def test_rows_do_not_mix(hip, rows, n):
     """A row's bits are the same whatever the other rows hold; a row with an

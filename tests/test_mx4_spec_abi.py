@@ -74,8 +74,8 @@ REFUSED = [
     ("hi_rocm_mx4_linear", ARGS, [
         dict(x=None), dict(packed=None), dict(out=None), dict(rows=0), dict(n=0), dict(k=0), dict(x_dtype=F32),
         dict(x_stride=32), dict(out_dtype=MX4), dict(out_stride=47), dict(out=P + 2), dict(out=P + 1, out_dtype=BF16),
-        dict(bias=P + 2), dict(packed=P + 8), dict(packed_bytes=100), dict(workspace=None), dict(workspace=P + 8),
-        dict(workspace_bytes=100)]),
+        dict(bias=P + 2), dict(packed=P + 8), dict(packed_bytes=100), dict(k=4128, x_stride=4128, workspace=None),
+        dict(k=4128, x_stride=4128, workspace=P + 8), dict(k=4128, x_stride=4128, workspace_bytes=100)]),
     ("hi_rocm_mx4_linear", UNSUPPORTED, [
         dict(k=48), dict(rows=(1 << 22) + 1), dict(x=P + 8), dict(x_stride=68), dict(n=(1 << 24) + 1, out_stride=1 << 25),
         dict(x=P + 8, x_dtype=MX4)]),
@@ -128,7 +128,13 @@ def test_sizes():
     assert _bytes(name, 17, 17, 64) == _bytes("hi_rocm_mx4_rows_bytes", 17, 64)
     assert _bytes(name, 16, 16, 8192) == _bytes("hi_rocm_mx4_rows_bytes", 16, 8192)
     assert _bytes(name, 2, 64, 65536) == _bytes("hi_rocm_mx4_rows_bytes", 2, 65536)
+    # a linear layer of few columns rounds more rows on the way, of no more than 4,096 inputs
+    name = "hi_rocm_mx4_linear_workspace_bytes"
+    assert _bytes(name, 1, 151936, 65536) == 0 and _bytes(name, 16, 48, 4096) == 0 and _bytes(name, 64, 1000, 1184) == 0
+    for rows, n, k in ((500, 16384, 512), (17, 48, 4128), (64, 32000, 1024), (16, 48, 8192)):
+        assert _bytes(name, rows, n, k) == _bytes("hi_rocm_mx4_rows_bytes", rows, k)
     for name, good in (("hi_rocm_mx4_rows_bytes", (4, 64)), ("hi_rocm_mx4_packed_bytes", (1, 4, 64)),
+                       ("hi_rocm_mx4_linear_workspace_bytes", (4, 4, 64)),
                        ("hi_rocm_mx4_workspace_bytes", (4, 4, 64))):
         assert getattr(lib, name)(*good, None) == ARGS
         _bytes(name, *good[:-1], 48, status=UNSUPPORTED)
