@@ -741,15 +741,16 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
 // known on the device alone: experts are taken to fill three quarters of a tile more than
 // their places, and rounds that are not whole to cost a half more.
 //   128 experts, 1536 x 2048, 48 places each: 50, 45, 47, 49 (32 to 128 places x 256);
-//     128: 85, 69, 61, 59; 512: 242, 178, 160, 151
+//     128: 85, 69, 61, 59; 256 (4,096 tokens x 8, with 2048 x 768): 161 for both in 96 places,
+//     150 in 128; 512: 242, 178, 160, 151
 //   8 experts, 2048 x 4096, 24 places: 11.6, 10.2, 11.9 (32 x 256, 128, 64); f 12.7
 //   60 experts, 1408 x 1440, 48 places: 15.9, 15.8, 18.4 (32, 64, 96 x 256); f 29
 struct Mx4Shape {
   int mt, cw;
   float fixed, quad;  // us: of a launch, of a quad by a round of workgroups
 };
-constexpr Mx4Shape kMx4Shapes[] = {{4, 4, 2.5f, 2.29f}, {3, 4, 2.5f, 1.86f}, {2, 4, 2.5f, 1.43f}, {1, 4, 2.5f, 1.0f},
-                                   {2, 2, 3.5f, 0.85f}, {1, 2, 3.5f, 0.6f},  {1, 1, 3.9f, 0.4f}};
+constexpr Mx4Shape kMx4Shapes[] = {{4, 4, 2.5f, 2.25f}, {3, 4, 2.5f, 1.9f}, {2, 4, 2.5f, 1.5f}, {1, 4, 2.5f, 1.05f},
+                                   {2, 2, 3.5f, 0.85f}, {1, 2, 3.5f, 0.6f}, {1, 1, 3.9f, 0.4f}};
 constexpr float kFewFixed = 2.6f, kFewQuad = 0.56f, kManyHidden = 2.5f, kMx4Rate = 5.8e6f;  // bytes a us
 
 // Quads of k by rounds of workgroups of bm places by bn columns.
