@@ -199,16 +199,19 @@ class Mx4Experts:
     [2 * inter][hidden / 2] (gate rows, then up rows) and ``down`` uint8
     [experts][hidden][inter / 2] with their scales; hidden and inter multiples
     of 32.  Activations go from f32 to 4 bits without a step between.  A
-    token's terms have the result's type, and their sum is f32: for a bfloat16
-    result they are rounded before they are weighted.  That is off by 0.0024
-    where f32 terms give 0.0017, next to a tenth by the 4-bit roundings, and
-    takes a fifth off a long prompt's layer (4,096 tokens of 8 terms, 240 to 195
-    us); a float32 result has f32 terms.  Weights are packed on ``stream`` and
-    need not be kept; buffers for up to ``max_tokens`` tokens are allocated
-    once, and calls allocate nothing when ``out`` is given."""
+    token's terms are ``terms``, float32 or bfloat16, whatever the result's
+    type, and their sum is f32.  float32 terms leave a bfloat16 result the one
+    rounding at its end (0.0017 of its norm).  bfloat16 ones are rounded before
+    they are weighted, each by up to 2^-8 of itself, which where a token's terms
+    cancel is more than the result's own rounding (0.0024 of the norm for random
+    ones), and halve what is written and read between the last two launches (8
+    terms of 2048: 1,024 tokens 111 -> 101 us, 4,096 225 -> 185).  Weights are
+    packed on ``stream`` and need not be kept; buffers for up to ``max_tokens``
+    tokens are allocated once, and calls allocate nothing when ``out`` is
+    given."""
 
     def __init__(self, up: torch.Tensor, up_scales: torch.Tensor, down: torch.Tensor, down_scales: torch.Tensor,
-                 max_tokens: int, top_k: int, stream: Optional[torch.cuda.Stream] = None):
+                 max_tokens: int, top_k: int, stream: Optional[torch.cuda.Stream] = None, terms=torch.float32):
         what = "mx4 experts"
         _codes_of(what, up, up_scales, 3)
         _codes_of(what, down, down_scales, 3)
@@ -217,6 +220,8 @@ class Mx4Experts:
             raise ValueError(f"{what}: up [experts][2 * inter][hidden / 2] and down [experts][hidden][inter / 2]")
         if max_tokens <= 0 or top_k <= 0:
             raise ValueError(f"{what}: {max_tokens} tokens, top {top_k}")
+        if terms not in _CODES:
+            raise ValueError(f"{what}: terms must be float32 or bfloat16")
         _on(what, up.get_device(), down)
         self.max_tokens, self.top_k = max_tokens, top_k
         self._up = _pack(what, up, up_scales, self.experts, stream)
@@ -226,7 +231,7 @@ class Mx4Experts:
         self._h_bytes = _size(lib.hi_rocm_mx4_rows_bytes, places, self.inter)
         self._x = torch.empty(self._x_bytes, dtype=torch.uint8, device=dev)
         self._h = torch.empty(self._h_bytes, dtype=torch.uint8, device=dev)
-        self._y = torch.empty(places, self.hidden, dtype=torch.float32, device=dev)  # (or as many bfloat16)
+        self._y = torch.empty(places, self.hidden, dtype=terms, device=dev)
         self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev)
         self._few = {}  # tokens: whether their rows need no rounding beforehand
 
@@ -269,9 +274,9 @@ class Mx4Experts:
             h.data_ptr(), DTYPE_MX4, I, self._h_bytes, 0, 0, st))
         check(lib.hi_rocm_mx4_grouped_product(
             h.data_ptr(), DTYPE_MX4, places, 0, 0, 1, offsets, places, E, self._down.data_ptr(), self._down.numel(), H, I,
-            0, y.data_ptr(), code, H, 0, 0, 0, st))
+            0, y.data_ptr(), _CODES[y.dtype], H, 0, 0, 0, st))
         check(lib.hi_rocm_moe_combine(
-            y.data_ptr(), code, H, slots, offsets, E, weights.data_ptr(), tokens, k, H, out.data_ptr(), code,
+            y.data_ptr(), _CODES[y.dtype], H, slots, offsets, E, weights.data_ptr(), tokens, k, H, out.data_ptr(), code,
             out.stride(0) if tokens > 1 else H, st))
         return out
 
