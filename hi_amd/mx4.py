@@ -207,8 +207,9 @@ class Mx4Experts:
     ones), and halve what is written and read between the last two launches (8
     terms of 2048: 1,024 tokens 111 -> 101 us, 4,096 225 -> 185).  Weights are
     packed on ``stream`` and need not be kept; buffers for up to ``max_tokens``
-    tokens are allocated once, and calls allocate nothing when ``out`` is
-    given."""
+    tokens are allocated once, of that stream too, and calls allocate nothing
+    when ``out`` is given.  Calls on another stream must come after what was on
+    ``stream`` when the layer was made, and end before the layer is dropped."""
 
     def __init__(self, up: torch.Tensor, up_scales: torch.Tensor, down: torch.Tensor, down_scales: torch.Tensor,
                  max_tokens: int, top_k: int, stream: Optional[torch.cuda.Stream] = None, terms=torch.float32):
@@ -229,10 +230,12 @@ class Mx4Experts:
         dev, lib, places = up.device, load(), max_tokens * top_k
         self._x_bytes = _size(lib.hi_rocm_mx4_rows_bytes, max_tokens, self.hidden)
         self._h_bytes = _size(lib.hi_rocm_mx4_rows_bytes, places, self.inter)
-        self._x = torch.empty(self._x_bytes, dtype=torch.uint8, device=dev)
-        self._h = torch.empty(self._h_bytes, dtype=torch.uint8, device=dev)
-        self._y = torch.empty(places, self.hidden, dtype=terms, device=dev)
-        self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev)
+        # (of the stream that packed the weights: another's allocator may hand out memory
+        # that its own work still uses, and take it back while this one's does)
+        self._x = _empty((self._x_bytes,), _BYTE, dev, stream)
+        self._h = _empty((self._h_bytes,), _BYTE, dev, stream)
+        self._y = _empty((places, self.hidden), terms, dev, stream)
+        self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev, stream=stream)
         self._few = {}  # tokens: whether their rows need no rounding beforehand
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, out: Optional[torch.Tensor] = None,

@@ -1,0 +1,89 @@
+"""Whose memory an operator with buffers of its own takes: the given stream's,
+as its work there is ordered behind what the memory held before, and the
+allocator gives it back in that stream's order.  On the CPU, by an allocator
+that notes the stream; on the GPU, beside a stream that is busy."""
+import contextlib
+import types
+
+import pytest
+import torch
+
+from hi_amd import beam, mx4
+from hi_amd.mx4 import Mx4Experts, Mx4Linear, quantize_mx4
+
+SIDE = types.SimpleNamespace(name="side")
+
+
+@pytest.fixture
+def allocations(monkeypatch):
+    """The stream (None: the current one) of every torch.empty and torch.zeros."""
+    at, made = [None], []
+
+    @contextlib.contextmanager
+    def on(stream):
+        at.append(stream)
+        yield
+        at.pop()
+
+    def noting(fn):
+        def new(*a, **kw):
+            made.append(at[-1])
+            return fn(*a, **kw)
+        return new
+
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch, "empty", noting(torch.empty))
+    monkeypatch.setattr(torch, "zeros", noting(torch.zeros))
+    return made
+
+
+def _codes(*shape):
+    return torch.full((*shape[:-1], shape[-1] // 2), 1, dtype=torch.uint8), torch.full(
+        (*shape[:-1], shape[-1] // 32), 127, dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("stream", [None, SIDE])
+def test_experts_buffers(monkeypatch, allocations, stream):
+    monkeypatch.setattr(mx4, "_on", lambda *a: None)
+    monkeypatch.setattr(mx4, "_pack", lambda *a: beam._empty((16,), torch.uint8, "cpu", a[-1]))
+    layer = Mx4Experts(*_codes(3, 128, 96), *_codes(3, 96, 64), max_tokens=5, top_k=2, stream=stream)
+    # weights twice, rows, activations, terms, the groups' three
+    assert allocations == [stream] * 8
+    assert layer._y.shape == (10, 96) and layer._groups.order.numel() == 10
+
+
+def _busy(x, ms):
+    """Some milliseconds of work on the current stream."""
+    y = x @ x
+    for _ in range(ms):
+        y = x @ y
+    return y
+
+
+@pytest.mark.gpu
+def test_layer_of_a_side_stream(hip, new_stream):
+    """Made and called on a stream while the current one is busy with memory that it
+    has given back: the results of the same layer alone."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    E, H, I, T, K = 6, 256, 96, 300, 2
+    up = quantize_mx4(torch.randn(E * 2 * I, H, generator=g, device="cuda") * H ** -0.5)
+    down = quantize_mx4(torch.randn(E * H, I, generator=g, device="cuda") * I ** -0.5)
+    args = (up[0].view(E, 2 * I, -1), up[1].view(E, 2 * I, -1), down[0].view(E, H, -1), down[1].view(E, H, -1))
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    ids = torch.rand(T, E, generator=g, device="cuda").topk(K, 1).indices.int()
+    wts = torch.rand(T, K, generator=g, device="cuda")
+    want = Mx4Experts(*args, max_tokens=T, top_k=K)(x, ids, wts)
+    a = torch.randn(4096, 4096, generator=g, device="cuda").bfloat16()
+    side = new_stream()
+    torch.cuda.synchronize()
+    for size in (T * K * H, T * H, E * 2 * I * H):
+        _busy(a, 4)
+        late = torch.empty(size, device="cuda")
+        late.fill_(float("nan"))  # (runs behind the products, in memory that is free at once)
+        del late
+    got = Mx4Experts(*args, max_tokens=T, top_k=K, stream=side)(x, ids, wts, stream=side)
+    lin = Mx4Linear(*up, stream=side)(x, stream=side)
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert torch.equal(lin, Mx4Linear(*up)(x))
