@@ -45,6 +45,25 @@ def _empty(shape, dtype, device, stream: Optional[torch.cuda.Stream]) -> torch.T
         return torch.empty(shape, dtype=dtype, device=device)
 
 
+def _zeroed(nbytes: int, device, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
+    """A workspace whose bytes are 0, of ``stream``.  The fill has ended when this
+    returns, as a first call on another stream would not wait for it (in a
+    capture it is the graph's, whose calls come after it)."""
+    if stream is None:
+        made = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        if made.get_device() >= 0:
+            stream = torch.cuda.current_stream(made.get_device())
+    else:
+        with torch.cuda.stream(stream):
+            made = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing:
+            stream.synchronize()
+    return made
+
+
 def _on(what: str, dev: int, *tensors: Optional[torch.Tensor]) -> None:
     """All tensors on CUDA device ``dev``."""
     if dev < 0:

@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from ._lib import check, load
-from .beam import _CODES, _F32, _I32, _on, _ptr, _stream, _vector
+from .beam import _CODES, _F32, _I32, _on, _ptr, _stream, _vector, _zeroed
 
 _INT, _FLOAT = torch.int32, torch.float32
 
@@ -16,16 +16,18 @@ _INT, _FLOAT = torch.int32, torch.float32
 class SpecVerifier:
     """The rejection rule for up to ``max_batch`` requests of ``max_draft``
     drafts over ``vocab`` tokens, with its own workspace (one stream at a
-    time)."""
+    time), which is allocated and zeroed on ``stream`` and ready for any when
+    this returns."""
 
-    def __init__(self, max_batch: int, max_draft: int, vocab: int, device="cuda"):
+    def __init__(self, max_batch: int, max_draft: int, vocab: int, device="cuda",
+                 stream: Optional[torch.cuda.Stream] = None):
         if max_draft < 0:
             raise ValueError(f"spec verifier: {max_draft} drafts")
         self.max_batch, self.max_draft, self.vocab = max_batch, max_draft, vocab
         nbytes = ctypes.c_size_t()
         check(load().hi_rocm_spec_sampled_workspace_bytes(max_batch, vocab, ctypes.byref(nbytes)))
         self._bytes = nbytes.value
-        self.workspace = torch.zeros(nbytes.value, dtype=torch.uint8, device=device)
+        self.workspace = _zeroed(nbytes.value, device, stream)
         self._device, self._verify = self.workspace.get_device(), load().hi_rocm_spec_verify_sampled
 
     def outputs(self, batch: int, stream: Optional[torch.cuda.Stream] = None) -> dict:

@@ -10,6 +10,8 @@ import torch
 
 from hi_amd import beam, mx4
 from hi_amd.mx4 import Mx4Experts, Mx4Linear, quantize_mx4
+from hi_amd.speculative import SpecVerifier
+from oracle import spec_sampled_oracle
 
 SIDE = types.SimpleNamespace(name="side")
 
@@ -52,6 +54,45 @@ def test_experts_buffers(monkeypatch, allocations, stream):
     assert layer._y.shape == (10, 96) and layer._groups.order.numel() == 10
 
 
+@pytest.mark.parametrize("capturing", [False, True])
+@pytest.mark.parametrize("stream", [None, "side"])
+def test_verifier_workspace(monkeypatch, stream, capturing):
+    """Zeroed on the given stream, and waited for there: a first call on any other
+    finds the zeros.  (A capture cannot wait, and orders the fill itself.)"""
+    done, at = [], []
+
+    class Stream:
+        def __init__(self, name):
+            self.name = name
+
+        def synchronize(self):
+            done.append(("waited", self.name))
+
+    class Zeros:
+        device = torch.device("cuda:0")
+
+        def get_device(self):
+            return 0
+
+    def zeros(*a, **kw):
+        done.append(("filled", at[-1].name if at else "current"))
+        return Zeros()
+
+    @contextlib.contextmanager
+    def on(s):
+        at.append(s)
+        yield
+        at.pop()
+
+    monkeypatch.setattr(torch, "zeros", zeros)
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: Stream("current"))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    SpecVerifier(4, 2, 1000, **({"stream": Stream("side")} if stream else {}))
+    name = stream or "current"
+    assert done == [("filled", name)] + [("waited", name)] * (not capturing)
+
+
 def _busy(x, ms):
     """Some milliseconds of work on the current stream."""
     y = x @ x
@@ -87,3 +128,52 @@ def test_layer_of_a_side_stream(hip, new_stream):
     torch.cuda.synchronize()
     assert torch.equal(got, want)
     assert torch.equal(lin, Mx4Linear(*up)(x))
+
+
+@pytest.mark.gpu
+def test_verifier_on_another_stream(hip, new_stream):
+    """A verifier made while the current stream is busy, called on another at once."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    B, K, V = 5, 3, 9000
+    p = torch.softmax(torch.randn(B, K + 1, V, generator=g, device="cuda") * 2, 2)
+    q = torch.softmax(torch.randn(B, K, V, generator=g, device="cuda") * 2, 2)
+    t = torch.randint(0, V, (B, K), generator=g, device="cuda").int()
+    u = torch.rand(B, K + 1, generator=g, device="cuda")
+    a = torch.randn(4096, 4096, generator=g, device="cuda").bfloat16()
+    side, own = new_stream(), new_stream()
+    f64 = lambda x: x.double().cpu().numpy()
+    want, counts = spec_sampled_oracle.verify(f64(p), t.cpu().numpy(), u.cpu().numpy(), f64(q))
+    torch.cuda.synchronize()
+    for kw in ({}, {"stream": own}):
+        _busy(a, 8)
+        verifier = SpecVerifier(B, K, V, **kw)
+        for _ in range(3):
+            out = verifier(p, t, u, draft_probs=q, stream=side)
+            side.synchronize()
+            assert (out["tokens"].cpu().numpy() == want).all() and (out["counts"].cpu().numpy() == counts).all()
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_verifier_made_in_a_capture(hip):
+    """The fill is the graph's then: every replay begins with a workspace of zeros."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    B, K, V = 3, 2, 20000
+    p = torch.softmax(torch.randn(B, K + 1, V, generator=g, device="cuda") * 2, 2)
+    t = torch.randint(0, V, (B, K), generator=g, device="cuda").int()
+    u = torch.rand(B, K + 1, generator=g, device="cuda")
+    eager = SpecVerifier(B, K, V)
+    eager(p, t, u)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        verifier = SpecVerifier(B, K, V)
+        out = verifier(p, t, u)
+    for i in range(4):
+        p.copy_(torch.softmax(torch.randn(B, K + 1, V, generator=g, device="cuda") * 2, 2))
+        u.copy_(torch.rand(B, K + 1, generator=g, device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = eager(p, t, u)
+        assert torch.equal(out["tokens"], want["tokens"]) and torch.equal(out["counts"], want["counts"])
