@@ -8,9 +8,15 @@ from typing import Optional
 import torch
 
 from ._lib import check, load
-from .beam import _CODES, _F32, _I32, _on, _ptr, _stream, _vector, _zeroed
+from .beam import _CODES, _on, _ptr, _stream, _zeroed
 
 _INT, _FLOAT = torch.int32, torch.float32
+
+
+def _shaped(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, *shape: int) -> None:
+    # (by shape, not by number: [drafts][batch] has as many values as [batch][drafts])
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} {''.join(f'[{n}]' for n in shape)} tensor")
 
 
 class SpecVerifier:
@@ -73,15 +79,15 @@ class SpecVerifier:
             out = self.outputs(batch, stream)
         tokens, counts = out["tokens"], out["counts"]
         if not (draft_tokens.dtype is _INT and tokens.dtype is _INT and counts.dtype is _INT and
-                uniforms.dtype is _FLOAT and draft_tokens.numel() == batch * K and tokens.numel() == batch * (K + 1) and
-                counts.numel() == batch and uniforms.numel() == batch * (K + 1) and draft_tokens.is_contiguous() and
+                uniforms.dtype is _FLOAT and draft_tokens.shape == (batch, K) and tokens.shape == (batch, K + 1) and
+                counts.shape == (batch,) and uniforms.shape == (batch, K + 1) and draft_tokens.is_contiguous() and
                 tokens.is_contiguous() and counts.is_contiguous() and uniforms.is_contiguous()):
-            _vector(what, "draft_tokens", draft_tokens, _I32, batch * K)
-            _vector(what, "uniforms", uniforms, _F32, batch * (K + 1))
-            _vector(what, "out tokens", tokens, _I32, batch * (K + 1))
-            _vector(what, "out counts", counts, _I32, batch)
+            _shaped(what, "draft_tokens", draft_tokens, _INT, batch, K)
+            _shaped(what, "uniforms", uniforms, _FLOAT, batch, K + 1)
+            _shaped(what, "out tokens", tokens, _INT, batch, K + 1)
+            _shaped(what, "out counts", counts, _INT, batch)
         if draft_len is not None:
-            _vector(what, "draft_len", draft_len, _I32, batch)
+            _shaped(what, "draft_len", draft_len, _INT, batch)
         if not (p.get_device() == draft_tokens.get_device() == uniforms.get_device() == tokens.get_device() ==
                 counts.get_device() == dev) or dev < 0 or q is not None or draft_len is not None:
             _on(what, dev, p, draft_tokens, uniforms, q, draft_len, tokens, counts)
