@@ -100,6 +100,7 @@ SIGNATURES = {
     "hi_rocm_mx4_workspace_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
     "hi_rocm_mx4_linear_workspace_bytes": (_i, [_i, _i, _i, ctypes.POINTER(_sz)]),
     "hi_rocm_mx4_linear": (_i, [_vp, _i, _i, _i64, _vp, _sz, _i, _i, _vp, _vp, _i, _i64, _vp, _sz, _vp]),
+    "hi_rocm_debug_mx4_linear": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "hi_rocm_mx4_grouped_product": (_i, [_vp, _i, _i, _i64, _vp, _i, _vp, _i, _i, _vp, _sz, _i, _i, _i, _vp, _i, _i64,
                                          _sz, _vp, _sz, _vp]),
     "hi_rocm_last_error": (ctypes.c_char_p, []),

@@ -51,6 +51,7 @@ struct Mx4Args {
   int x_rows, top_k, places, experts, cols, k, swiglu, out_dtype;
   int tiles, steps, quads;   // of an expert's packed weight
   int out_vec;               // rows of out start on 16 bytes
+  int past;                  // results are stored past the caches (mx4_past)
 };
 
 // This workgroup's tile of BM places and block of columns.
@@ -366,9 +367,7 @@ struct Mx4Tile {
 // lane and a row's bytes next to each other are written: all of the 32 places' reads,
 // then all of their stores (a read and its store after another: experts of 256 places,
 // 2048 x 768, 72 us where this takes 65).
-// PAST: rows past the caches.  A linear layer's, whose x and weights then stay there
-// (8,192 x 4,096 x 16,384: 307 -> 293 us); the experts' terms are read next (their sum
-// 4.0 us, past the caches 4.2).
+// PAST: rows past the caches (mx4_past).
 template <int MT, int KG, typename T, int COLS, bool PAST>
 __device__ __forceinline__ void mx4_tile_store(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
                                                int c0, int cols_out, int lane, int group) {
@@ -476,8 +475,8 @@ __device__ __forceinline__ void mx4_tile_out(const Mx4Args& a, mx4_f32x16 (&acc)
   auto store = [&](auto type) {
     using T = decltype(type);
     if (a.swiglu) mx4_tile_store<MT, KG, T, 32, false>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
-    else if (a.offsets != nullptr) mx4_tile_store<MT, KG, T, 64, false>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
-    else mx4_tile_store<MT, KG, T, 64, true>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+    else if (a.past) mx4_tile_store<MT, KG, T, 64, true>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
+    else mx4_tile_store<MT, KG, T, 64, false>(a, acc, mem, p0, i1, c0, cols_out, lane, group);
   };
   if (a.out_dtype == HI_ROCM_DTYPE_BF16) store(__bf16());
   else store(float());
@@ -810,6 +809,30 @@ hipError_t launch_product(const Mx4Args& a, bool codes, hipStream_t st) {
   }
 }
 
+// Whether a linear layer's tiles store their results past the caches: where the last-level
+// cache does not hold them (256 MB), so that x and the weights stay there, and between one
+// L2 and all eight, whose dirty lines a launch's end writes back.  Elsewhere what reads the
+// result next loses more than the product gains.  us with and without, layers of k 4,096 on
+// end, alone and each with the rounding of its result:
+//   1.0 MB (128 x 4,096 bf16)      7.3 and 7.2, 10.5 and 10.1
+//   2.6 MB (320 x 4,096 bf16)      10.1 and 10.2, 13.4 and 13.2
+//   5.2 MB (320 x 4,096 f32)       10.5 and 10.5, 14.3 and 14.4
+//   10.5 MB (320 x 16,384 bf16)    16.9 and 17.9, 21.8 and 22.0
+//   16.8 MB (2,048 x 4,096 bf16)   19.8 and 21.1, 25.5 and 26.2
+//   33.6 MB (2,048 x 4,096 f32)    22.6 and 23.4, 30.8 and 30.7
+//   67 MB (1,024 x 16,384 f32)     45.8 and 44.8, 60.4 and 57.1
+//   134 MB (8,192 x 4,096 f32)     72.8 and 76.8, 104 and 99.6
+//   197 MB (6,000 x 16,384 bf16)   206 and 207, 245 and 240
+//   249 MB (7,600 x 16,384 bf16)   260 and 261, 307 and 309
+//   268 MB (8,192 x 16,384 bf16)   283 and 290, 337 and 343
+//   537 MB (8,192 x 16,384 f32)    321 and 342, 425 and 460
+// (The experts' terms, 67 and 134 MB at 4,096 tokens, are read next.)
+constexpr double kMx4PastOne = 4e6, kMx4PastAll = 32e6, kMx4PastLast = 240e6;
+bool mx4_past(int64_t rows, int n, int size) {
+  const double bytes = (double)rows * n * size;
+  return (bytes > kMx4PastOne && bytes <= kMx4PastAll) || bytes > kMx4PastLast;
+}
+
 bool mx4_float(int d) { return d == HI_ROCM_DTYPE_F32 || d == HI_ROCM_DTYPE_BF16; }
 int mx4_size(int d) { return d == HI_ROCM_DTYPE_F32 ? 4 : 2; }
 
@@ -920,6 +943,28 @@ int hi_rocm_mx4_linear_workspace_bytes(int rows, int n, int k, size_t* out_bytes
   return HI_ROCM_OK;
 }
 
+int hi_rocm_debug_mx4_linear(int rows, int n, int k, int x_dtype, int out_dtype, int* out_places, int* out_cols,
+                             int* out_past) {
+  if (rows <= 0 || n <= 0 || k <= 0 || (x_dtype != HI_ROCM_DTYPE_BF16 && x_dtype != HI_ROCM_DTYPE_MX4) ||
+      !mx4_float(out_dtype) || out_places == nullptr || out_cols == nullptr || out_past == nullptr)
+    return api_fail(HI_ROCM_ERR_ARGS, "hi_rocm_debug_mx4_linear: invalid arguments");
+  if (!mx4_weight_fits(1, n, k) || rows > HI_ROCM_MX4_MAX_ROWS)
+    return api_fail(HI_ROCM_ERR_UNSUPPORTED,
+                    "hi_rocm_debug_mx4_linear: needs k a multiple of 32 up to 2^24, at most 2^24 outputs, 2^35 weights, "
+                    "2^22 rows");
+  Mx4Args a;
+  memset(&a, 0, sizeof(a));
+  mx4_take_weight(a, nullptr, 1, n, k);
+  a.places = rows;
+  const bool codes = x_dtype == HI_ROCM_DTYPE_MX4 || mx4_linear_needs_rows(a);
+  const Mx4Shape s = mx4_choose(a).shape;
+  const bool many = codes && s.mt > 0;
+  *out_places = many ? 32 * s.mt : 16;
+  *out_cols = many ? 64 * s.cw : kFewCols;
+  *out_past = many && mx4_past(rows, n, mx4_size(out_dtype));
+  return HI_ROCM_OK;
+}
+
 int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, const void* packed, size_t packed_bytes,
                        int n, int k, const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                        size_t workspace_bytes, void* stream) {
@@ -941,6 +986,7 @@ int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, c
   a.out_stride = out_stride;
   a.out_dtype = out_dtype;
   a.out_vec = (uintptr_t)out % 16 == 0 && out_stride * mx4_size(out_dtype) % 16 == 0;
+  a.past = mx4_past(rows, n, mx4_size(out_dtype));
   a.top_k = 1;
   bool codes;
   const int rc = mx4_take_x(name, a, x, x_dtype, rows, x_stride, needs, workspace, (hipStream_t)stream, codes);

@@ -589,6 +589,12 @@ int hi_rocm_mx4_linear(const void* x, int x_dtype, int rows, int64_t x_stride, c
                        int n, int k, const float* bias, void* out, int out_dtype, int64_t out_stride, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* How hi_rocm_mx4_linear takes a call of these sizes: the rows and outputs of a
+ * workgroup (16 x 64 is the kernel for few rows, which rounds bf16 ones on the
+ * way), and whether its results are stored past the caches.  Host only. */
+int hi_rocm_debug_mx4_linear(int rows, int n, int k, int x_dtype, int out_dtype, int* out_places, int* out_cols,
+                             int* out_past);
+
 /* hi_rocm_moe_grouped_product with such weights: x, x_rows and workspace as above,
  * order, top_k, offsets, places and swiglu as there (with swiglu halves of a
  * multiple of 32 columns).  out f32 or bf16 [places][out_stride], or with swiglu
