@@ -23,6 +23,7 @@ import torch
 
 from . import _lib
 from ._lib import ROW_PARAMS_DTYPE, HiRocmError, check, load
+from .beam import _empty, _zeroed
 
 
 class SamplerError(RuntimeError):
@@ -181,15 +182,17 @@ class Sampler:
     """The extended decode-step sampler (``hi_rocm_sample``) with its own workspace.
 
     The workspace is allocated once, for up to ``max_batch`` rows of ``vocab``
-    logits; ``sample`` allocates nothing and only enqueues kernels.
+    logits, and zeroed on ``stream``, ready for any stream when this returns;
+    ``sample`` allocates nothing when ``out`` is given and only enqueues kernels.
     """
 
-    def __init__(self, max_batch: int, vocab: int, n_logprobs: int = 0, device="cuda"):
+    def __init__(self, max_batch: int, vocab: int, n_logprobs: int = 0, device="cuda",
+                 stream: Optional[torch.cuda.Stream] = None):
         lib = load()
         nbytes = ctypes.c_size_t()
         check(lib.hi_rocm_sampler_workspace_bytes(max_batch, vocab, n_logprobs, ctypes.byref(nbytes)))
         self.max_batch, self.vocab, self.n_logprobs = max_batch, vocab, n_logprobs
-        self.workspace = torch.zeros(nbytes.value, dtype=torch.uint8, device=device)
+        self.workspace = _zeroed(nbytes.value, device, stream)
 
     def sample(self, logits: torch.Tensor, params: torch.Tensor, uniforms: torch.Tensor,
                hist_offsets: Optional[torch.Tensor] = None, hist_ids: Optional[torch.Tensor] = None,
@@ -210,12 +213,12 @@ class Sampler:
             raise ValueError("shape exceeds the workspace this Sampler was built for")
         dev = logits.device
         if out is None:
-            out = {"tokens": torch.empty(B, dtype=torch.int32, device=dev)}
+            out = {"tokens": _empty((B,), torch.int32, dev, stream)}
             if n_logprobs > 0:
-                out["logprobs"] = torch.empty(B, n_logprobs, dtype=torch.float32, device=dev)
-                out["logprob_ids"] = torch.empty(B, n_logprobs, dtype=torch.int32, device=dev)
+                out["logprobs"] = _empty((B, n_logprobs), torch.float32, dev, stream)
+                out["logprob_ids"] = _empty((B, n_logprobs), torch.int32, dev, stream)
             if token_logprobs:
-                out["token_logprobs"] = torch.empty(B, dtype=torch.float32, device=dev)
+                out["token_logprobs"] = _empty((B,), torch.float32, dev, stream)
 
         def p(t):
             return 0 if t is None else t.data_ptr()

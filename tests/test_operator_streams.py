@@ -8,7 +8,7 @@ import types
 import pytest
 import torch
 
-from hi_amd import beam, mx4
+from hi_amd import beam, mx4, sampler
 from hi_amd.mx4 import Mx4Experts, Mx4Linear, quantize_mx4
 from hi_amd.speculative import SpecVerifier
 from oracle import spec_sampled_oracle
@@ -54,9 +54,22 @@ def test_experts_buffers(monkeypatch, allocations, stream):
     assert layer._y.shape == (10, 96) and layer._groups.order.numel() == 10
 
 
+@pytest.mark.parametrize("stream", [None, SIDE])
+def test_sampler_outputs(monkeypatch, allocations, stream):
+    monkeypatch.setattr(sampler, "_zeroed", lambda *a: beam._empty((16,), torch.uint8, "cpu", a[-1]))
+    monkeypatch.setattr(sampler, "_stream_ptr", lambda s: 0)
+    one = sampler.Sampler(2, 50, n_logprobs=3, stream=stream)
+    monkeypatch.setattr(sampler, "load", lambda: types.SimpleNamespace(hi_rocm_sample=lambda *a: 0))
+    x = torch.ones(2, 50)
+    out = one.sample(x, x, x, n_logprobs=3, token_logprobs=True, stream=stream)
+    assert allocations == [stream] * 5 and out["logprob_ids"].shape == (2, 3)
+
+
+@pytest.mark.parametrize("make", [lambda **kw: SpecVerifier(4, 2, 1000, **kw), lambda **kw: sampler.Sampler(4, 1000, **kw)],
+                         ids=["verifier", "sampler"])
 @pytest.mark.parametrize("capturing", [False, True])
 @pytest.mark.parametrize("stream", [None, "side"])
-def test_verifier_workspace(monkeypatch, stream, capturing):
+def test_zeroed_workspace(monkeypatch, make, stream, capturing):
     """Zeroed on the given stream, and waited for there: a first call on any other
     finds the zeros.  (A capture cannot wait, and orders the fill itself.)"""
     done, at = [], []
@@ -88,7 +101,7 @@ def test_verifier_workspace(monkeypatch, stream, capturing):
     monkeypatch.setattr(torch.cuda, "stream", on)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: Stream("current"))
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
-    SpecVerifier(4, 2, 1000, **({"stream": Stream("side")} if stream else {}))
+    make(**({"stream": Stream("side")} if stream else {}))
     name = stream or "current"
     assert done == [("filled", name)] + [("waited", name)] * (not capturing)
 
@@ -177,3 +190,24 @@ def test_verifier_made_in_a_capture(hip):
         torch.cuda.synchronize()
         want = eager(p, t, u)
         assert torch.equal(out["tokens"], want["tokens"]) and torch.equal(out["counts"], want["counts"])
+
+
+@pytest.mark.gpu
+def test_sampler_on_another_stream(hip, new_stream):
+    """As above for the sampler, whose workspace begins as zeros too."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    B, V = 6, 50000
+    x, u = torch.randn(B, V, generator=g, device="cuda") * 3, torch.rand(B, generator=g, device="cuda")
+    params = sampler.params_to_device(sampler.row_params(B, temperature=0.8, top_p=0.9), "cuda")
+    a = torch.randn(4096, 4096, generator=g, device="cuda").bfloat16()
+    side, own = new_stream(), new_stream()
+    want = sampler.Sampler(B, V).sample(x, params, u)["tokens"].clone()
+    torch.cuda.synchronize()
+    for kw in ({}, {"stream": own}):
+        _busy(a, 8)
+        one = sampler.Sampler(B, V, **kw)
+        for _ in range(3):
+            got = one.sample(x, params, u, stream=side)["tokens"]
+            side.synchronize()
+            assert torch.equal(got, want)
+        torch.cuda.synchronize()
