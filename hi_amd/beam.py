@@ -85,15 +85,16 @@ _F32, _I32, _FLAG = (torch.float32,), (torch.int32,), (torch.uint8, torch.bool)
 class BeamSearch:
     """Selection for up to ``max_batch`` requests of ``beams`` beams over
     ``vocab`` tokens, ``n_out`` candidates each, with its own workspace (one
-    stream at a time)."""
+    stream at a time), of ``stream``."""
 
-    def __init__(self, max_batch: int, beams: int, vocab: int, n_out: Optional[int] = None, device="cuda"):
+    def __init__(self, max_batch: int, beams: int, vocab: int, n_out: Optional[int] = None, device="cuda",
+                 stream: Optional[torch.cuda.Stream] = None):
         self.max_batch, self.beams, self.vocab = max_batch, beams, vocab
         self.n_out = beams if n_out is None else n_out
         nbytes = ctypes.c_size_t()
         check(load().hi_rocm_beam_workspace_bytes(max_batch, beams, vocab, self.n_out, ctypes.byref(nbytes)))
         self._bytes = nbytes.value
-        self.workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+        self.workspace = _empty((nbytes.value,), torch.uint8, device, stream)
 
     def outputs(self, batch: int, stream: Optional[torch.cuda.Stream] = None) -> dict:
         """Output tensors of ``select`` for ``batch`` requests."""

@@ -106,10 +106,11 @@ class MoeExperts:
     The activations between the two products are rounded to bfloat16, as in a
     bfloat16 model (a relative error of 0.0023 of a bfloat16 result, 0.0017
     with them in f32); all sums are f32.
-    Buffers for up to ``max_tokens`` tokens are allocated once; calls allocate
-    nothing when ``out`` is given."""
+    Buffers for up to ``max_tokens`` tokens are allocated once, of ``stream``;
+    calls allocate nothing when ``out`` is given."""
 
-    def __init__(self, w_up: torch.Tensor, w_down: torch.Tensor, max_tokens: int, top_k: int):
+    def __init__(self, w_up: torch.Tensor, w_down: torch.Tensor, max_tokens: int, top_k: int,
+                 stream: Optional[torch.cuda.Stream] = None):
         if (w_up.dim() != 3 or w_down.dim() != 3 or w_up.shape[1] % 2 or
                 w_down.shape != (w_up.shape[0], w_up.shape[2], w_up.shape[1] // 2) or
                 w_up.dtype is not torch.bfloat16 or w_down.dtype is not torch.bfloat16 or
@@ -123,9 +124,9 @@ class MoeExperts:
         # The activations between the products are what the second product's
         # matrix instructions take, bf16; its results stay f32 until they are
         # summed.
-        self._h = torch.empty(max_tokens * top_k, self.inter, dtype=torch.bfloat16, device=dev)
-        self._y = torch.empty(max_tokens * top_k, self.hidden, dtype=torch.float32, device=dev)
-        self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev)
+        self._h = _empty((max_tokens * top_k, self.inter), torch.bfloat16, dev, stream)
+        self._y = _empty((max_tokens * top_k, self.hidden), torch.float32, dev, stream)
+        self._groups = RowGroups(max_tokens, top_k, self.experts, device=dev, stream=stream)
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, out: Optional[torch.Tensor] = None,
                  stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:

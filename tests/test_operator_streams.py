@@ -8,7 +8,7 @@ import types
 import pytest
 import torch
 
-from hi_amd import beam, mx4, sampler
+from hi_amd import beam, moe, mx4, sampler
 from hi_amd.mx4 import Mx4Experts, Mx4Linear, quantize_mx4
 from hi_amd.speculative import SpecVerifier
 from oracle import spec_sampled_oracle
@@ -52,6 +52,14 @@ def test_experts_buffers(monkeypatch, allocations, stream):
     # weights twice, rows, activations, terms, the groups' three
     assert allocations == [stream] * 8
     assert layer._y.shape == (10, 96) and layer._groups.order.numel() == 10
+
+
+@pytest.mark.parametrize("stream", [None, SIDE])
+def test_beam_and_bf16_experts_buffers(monkeypatch, allocations, stream):
+    beam.BeamSearch(2, 4, 1000, device="cpu", stream=stream)
+    monkeypatch.setattr(moe, "_on", lambda *a: None)
+    moe.MoeExperts(torch.ones(3, 128, 96).bfloat16(), torch.ones(3, 96, 64).bfloat16(), 5, 2, stream=stream)
+    assert allocations == [stream] * 6
 
 
 @pytest.mark.parametrize("stream", [None, SIDE])
