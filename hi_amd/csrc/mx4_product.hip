@@ -366,7 +366,7 @@ struct Mx4Tile {
 // 32 places of a wave's results at a time through its own LDS, so that 16 bytes a
 // lane and a row's bytes next to each other are written: all of the 32 places' reads,
 // then all of their stores (a read and its store after another: experts of 256 places,
-// 2048 x 768, 72 us where this takes 65).
+// 2048 x 768, bf16 terms, 72 us where this takes 65).
 // PAST: rows past the caches (mx4_past).
 template <int MT, int KG, typename T, int COLS, bool PAST>
 __device__ __forceinline__ void mx4_tile_store(const Mx4Args& a, mx4_f32x16 (&acc)[MT][2], char* mem, int p0, int i1,
@@ -740,8 +740,8 @@ hipError_t launch_many(const Mx4Args& a, hipStream_t st) {
 // known on the device alone: experts are taken to fill three quarters of a tile more than
 // their places, and rounds that are not whole to cost a half more.
 //   128 experts, 1536 x 2048, 48 places each: 50, 45, 47, 49 (32 to 128 places x 256);
-//     128: 85, 69, 61, 59; 256 (4,096 tokens x 8, with 2048 x 768): 161 for both in 96 places,
-//     150 in 128; 512: 242, 178, 160, 151
+//     128: 85, 69, 61, 59; 256 (4,096 tokens x 8, with 2048 x 768, bf16 terms): 161 for both in
+//     96 places, 150 in 128; 512: 242, 178, 160, 151
 //   8 experts, 2048 x 4096, 24 places: 11.6, 10.2, 11.9 (32 x 256, 128, 64); f 12.7
 //   60 experts, 1408 x 1440, 48 places: 15.9, 15.8, 18.4 (32, 64, 96 x 256); f 29
 struct Mx4Shape {
