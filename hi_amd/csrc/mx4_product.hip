@@ -333,9 +333,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, 6) mx4_few_kernel(Mx4Args a) {
 // there.  Chunks of x past k hold what follows in memory (the next row, or the
 // scales): any code is finite, and meets weights of 0 and scales of 1.
 //
-// 8,192 x 4,096 x 16,384: 273 to 283 us, 4.0 PFLOP/s, the matrix cores busy half the
-// time at some 1.65 GHz.  These instructions alone, on random data in registers, reach
-// 6.1 (the card's power; 8.4 on zeros).  With weights through LDS too 344 (eight waves in
+// 8,192 x 4,096 x 16,384: 264 to 299 us by the card, 3.7 to 4.2 PFLOP/s, the matrix cores
+// busy half the time at some 1.65 GHz.  These instructions alone, on random data in
+// registers, reach 6.1 (the card's power; 8.4 on zeros), 180 us, and the loop without them
+// takes 207: the two overlap by about half.  With weights through LDS too 344 (eight waves in
 // two phases) and 396 (256 x 256 a workgroup).
 typedef float mx4_f32x16 __attribute__((ext_vector_type(16)));
 
