@@ -11,7 +11,9 @@
 // (16 + q), and the rows' sums over the group, e = sum x (a product with ones,
 // in the same layout), give
 //     y += s * (d - (16 + z) * e)
-// in f32: the weights are never rounded.  (An offset of 128, which needs no
+// in f32: the weights are never rounded.  Without zeros (z = 8) 24 e is itself a
+// product, with 24s: a group of weights of 0 makes d the same one, rounding for
+// rounding, and adds nothing (24 times a rounded e would be a step off d).  (An offset of 128, which needs no
 // shift for the first pair, would lose three more bits to the difference.)
 //
 // hi_rocm_w4_pack lays the weights out once: blocks of 16 outputs x 128 inputs
@@ -140,7 +142,7 @@ struct W4Scales<ST, 1> {
 // a group to add their sums, in wave order, through LDS.
 //
 // A group's e does not depend on the output: each wave makes it once a pass (a
-// product with ones) and keeps -24 e (-e with zeros) in LDS.  What goes into the
+// product with ones or 24s) and keeps -24 e (-e with zeros) in LDS.  What goes into the
 // sum, s (d - (16 + z) e), follows one group behind, while the next group's
 // product runs.  (Products that start from -24 e would save an addition, but
 // weights of 0 would then not give 0.)
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
     }
     w4_bf16x8 ones;
     #pragma unroll
-    for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.0f;
+    for (int i = 0; i < 8; ++i) ones[i] = (__bf16)(ZEROS ? 1.0f : 24.0f);
     #pragma unroll
     for (int i = 0; i < BPW; ++i) {
       #pragma unroll
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(64 * kW4Waves) w4_linear_kernel(W4Args a) {
           #pragma unroll
           for (int c = j * CH; c < (j + 1) * CH; ++c)
             e = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[i][c][m], ones, e, 0, 0, 0);
-          if (r == 0) ex[((i * GPB + j) * MT + m) * 4] = ZEROS ? -e : -24.f * e;
+          if (r == 0) ex[((i * GPB + j) * MT + m) * 4] = -e;
         }
       }
     }
