@@ -56,6 +56,8 @@ def _zeroed(nbytes: int, device, stream: Optional[torch.cuda.Stream]) -> torch.T
     else:
         with torch.cuda.stream(stream):
             made = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        if made.get_device() != stream.device_index:
+            raise ValueError(f"a workspace on {made.device}, its stream on cuda:{stream.device_index}")
     if stream is not None:
         with torch.cuda.stream(stream):
             capturing = torch.cuda.is_current_stream_capturing()

@@ -83,6 +83,8 @@ def test_zeroed_workspace(monkeypatch, make, stream, capturing):
     done, at = [], []
 
     class Stream:
+        device_index = 0
+
         def __init__(self, name):
             self.name = name
 
@@ -112,6 +114,11 @@ def test_zeroed_workspace(monkeypatch, make, stream, capturing):
     make(**({"stream": Stream("side")} if stream else {}))
     name = stream or "current"
     assert done == [("filled", name)] + [("waited", name)] * (not capturing)
+    if stream:
+        elsewhere = Stream("elsewhere")
+        elsewhere.device_index = 1
+        with pytest.raises(ValueError, match="cuda:1"):
+            make(stream=elsewhere)
 
 
 def _busy(x, ms):
